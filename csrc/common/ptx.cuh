@@ -40,6 +40,8 @@ enum StatusCode : int {
   kWaitFlagTimeout = 105,    // flag written by another CTA / another GPU never arrived
   kWaitDrainTimeout = 106,
   kBadArgument = 201,
+  kBadPage = 202,            // a page number outside the pool, or a place outside the table (paged_attention.cu, pages.cu)
+  kPoolFull = 203,           // no free page left for a row that grows (pages.cu)
 };
 
 __device__ __forceinline__ void report_error(int code) {

@@ -237,6 +237,11 @@ def check(rc: int, what: str) -> None:
     raise KernelError(f"{what}: {names.get(rc, 'library error')} ({rc})")
 
 
+# What a kernel found in device memory and passed over (csrc/common/ptx.cuh); other codes are bounded waits.
+STATUS_TEXT = {202: "a page number outside the pool, or a row or position outside the table; what belonged there was left out",
+               203: "the pool has no free page left for a row that grows; the row has none there"}
+
+
 def read_status() -> tuple:
     """(code, block, waits_timed_out, reserved) of the device status word; synchronises the device."""
     lib = load()
@@ -254,5 +259,7 @@ def raise_on_device_error() -> None:
     code, block, waits, _ = read_status()
     if code != 0:
         clear_status()
+        if code in STATUS_TEXT:
+            raise KernelError(f"device status {code} (block {block}, {waits} times): {STATUS_TEXT[code]}")
         raise KernelError(f"device status {code} (block {block}, {waits} waits ran out): a bounded wait inside a kernel "
                           f"gave up; the results of that launch are invalid")

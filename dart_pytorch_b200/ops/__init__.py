@@ -12,6 +12,8 @@ import torch
 
 from . import cpu_fast as fast
 from . import reference as ref
+from .beam import beam_step  # noqa: F401  (re-exported)
+from .paged import compact_pages, copy_pages, fork_pages, paged_append, paged_attention  # noqa: F401  (re-exported)
 from .reference import causal_mask, sample_from_logits  # noqa: F401  (re-exported)
 
 

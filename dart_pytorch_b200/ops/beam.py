@@ -1,0 +1,112 @@
+"""Beam search's selection over beams and vocabulary (``csrc/beam.cu``).  CPU tensors run reference formulas."""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional, Tuple
+
+import torch
+
+from .. import _native as N
+from .paged import _here, _no_grad
+
+c_void_p, c_int, c_ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
+
+MAX_BEAMS = 32
+MAX_ROWS = 1 << 20
+
+
+class BeamArgs(ctypes.Structure):
+    _fields_ = [(n, c_void_p) for n in ("logits", "scores", "finished", "out_scores", "out_parents", "out_tokens", "out_finished",
+                                        "ws")] + \
+        [(n, c_ll) for n in ("ld", "ws_bytes")] + [(n, c_int) for n in ("items", "beams", "vocab", "eos", "f32")]
+
+
+_declared = False
+
+
+def _lib():
+    global _declared
+    lib = N.load()
+    if not _declared:
+        lib.dptb_beam_step.argtypes, lib.dptb_beam_step.restype = [ctypes.POINTER(BeamArgs), c_void_p], c_int
+        lib.dptb_beam_ws_bytes.argtypes, lib.dptb_beam_ws_bytes.restype = [c_int, c_int], c_ll
+        _declared = True
+    return lib
+
+
+def beam_step_reference(logits, scores, finished=None, eos=-1):
+    """64-bit formulas over all continuations, sorted by value and then by place."""
+    items, beams = scores.shape
+    x = logits.double().view(items, beams, -1)
+    vocab = x.shape[-1]
+    lp = torch.log_softmax(x, -1)
+    lp = torch.where(lp.isfinite().any(-1, keepdim=True) & ~lp.isnan().any(-1, keepdim=True), lp, -math.inf)
+    start = scores.double()[..., None]
+    total = torch.where(start > -math.inf, start + lp, -math.inf)
+    if finished is not None:
+        only = torch.where(torch.arange(vocab, device=x.device) == eos, start, -math.inf)
+        total = torch.where(finished[..., None], only, total)
+    total = torch.where(total.isnan(), -math.inf, total).view(items, -1)
+    total, order = torch.sort(total, dim=-1, descending=True, stable=True)
+    total, order = total[:, :beams], order[:, :beams]
+    beam, token = order // vocab, order % vocab
+    done = token == eos
+    if finished is not None:
+        done = done | finished.gather(1, beam)
+    parents = beam + beams * torch.arange(items, device=x.device)[:, None]
+    return total.float(), parents.int(), token, done
+
+
+def beam_step(logits: torch.Tensor, scores: torch.Tensor, finished: Optional[torch.Tensor] = None,
+              eos: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """One step of beam search for ``items`` searches of ``beams`` beams: of all ``beams * vocab`` continuations of an item the
+    best ``beams``, by ``scores [items, beams]`` (fp32) plus the log-probability that ``logits [items * beams, vocab]`` (bf16 or
+    fp32) gives the token; equal ones in the order of beam and token.
+
+    A beam of ``finished [items, beams]`` (bool) goes on with ``eos`` alone, at its old score.  A beam of score -inf (or NaN) and a
+    row of logits that is no distribution (a NaN, an infinity, nothing but -inf) have continuations worth -inf only, so a search starts
+    with the scores ``0, -inf, -inf, ...``.
+
+    Returns ``(scores, parents, tokens, finished)``, each ``[items, beams]``, best first: ``parents`` (int32) are rows of ``logits``,
+    as ``fork_pages`` takes them, ``tokens`` int64.  Up to 32 beams."""
+    what = "beam_step"
+    if scores.dim() != 2 or scores.dtype != torch.float32:
+        raise ValueError(f"{what}: scores must be fp32 [items, beams], got {scores.dtype} {list(scores.shape)}")
+    items, beams = scores.shape
+    if logits.dim() != 2 or logits.shape[0] != items * beams or logits.shape[1] == 0:
+        raise ValueError(f"{what}: logits {list(logits.shape)} are not [{items} * {beams}, vocab]")
+    if logits.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"{what}: logits must be float32 or bfloat16, got {logits.dtype}")
+    if not 0 < beams <= MAX_BEAMS or items * beams > MAX_ROWS or logits.shape[1] >= 1 << 31:
+        raise ValueError(f"{what}: 1 to {MAX_BEAMS} beams, at most {MAX_ROWS} rows, got {items} x {beams}")
+    if finished is not None and (finished.shape != scores.shape or finished.dtype != torch.bool):
+        raise ValueError(f"{what}: finished must be bool {list(scores.shape)}")
+    if eos is not None and not 0 <= eos < logits.shape[1]:
+        raise ValueError(f"{what}: eos {eos} is no token of {logits.shape[1]}")
+    if finished is not None and eos is None:
+        raise ValueError(f"{what}: finished beams need an eos to go on with")
+    _here(what, logits, scores, finished)
+    _no_grad(what, logits, scores)
+    last = -1 if eos is None else eos
+    if not logits.is_cuda:
+        return beam_step_reference(logits, scores, finished, last)
+    from .kernels import splitk_workspace
+    if logits.stride(1) != 1 and logits.shape[1] > 1:
+        logits = logits.contiguous()
+    scores = scores.contiguous()
+    finished = None if finished is None else finished.contiguous()
+    dev = logits.device
+    out_scores = torch.empty(items, beams, dtype=torch.float32, device=dev)
+    out_parents = torch.empty(items, beams, dtype=torch.int32, device=dev)
+    out_tokens = torch.empty(items, beams, dtype=torch.long, device=dev)
+    out_finished = torch.empty(items, beams, dtype=torch.bool, device=dev)
+    lib = _lib()
+    ws = splitk_workspace(dev)[0]
+    if lib.dptb_beam_ws_bytes(items, beams) > ws.numel():
+        ws = torch.empty(lib.dptb_beam_ws_bytes(items, beams), dtype=torch.uint8, device=dev)
+    a = BeamArgs(logits.data_ptr(), scores.data_ptr(), N.ptr(finished), out_scores.data_ptr(), out_parents.data_ptr(),
+                 out_tokens.data_ptr(), out_finished.data_ptr(), ws.data_ptr(), logits.stride(0), ws.numel(), items, beams,
+                 logits.shape[1], last, logits.dtype == torch.float32)
+    N.check(lib.dptb_beam_step(a, N.stream_ptr()), what)
+    return out_scores, out_parents, out_tokens, out_finished

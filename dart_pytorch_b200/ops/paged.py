@@ -1,0 +1,381 @@
+"""A key / value cache in pages: attention over it, the append to it and the operations on who holds which page
+(``csrc/paged_attention.cu``, ``csrc/pages.cu``).
+
+``k_pages`` / ``v_pages`` are ``[pages, kv_heads, page, head_dim]`` (any strides, features contiguous), ``table [rows, width]``
+lists the pages of every sequence in order, with -1 behind the last, and ``lens [rows]`` counts its tokens; both are int32.  A
+page may stand in several rows.  It is free when no row lists it.
+
+The operations on pages run on the device and return new tables; nothing is read back.  What only the device can see, a page
+number outside the pool or a pool without a free page, is recorded in the status word: the kernels skip such a page, and
+``_native.raise_on_device_error`` raises.  CPU tensors run reference formulas with the same contracts, which raise at once.
+
+None of this has gradients: tensors that want them are refused.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional, Tuple, Union
+
+import torch
+
+from .. import _native as N
+
+c_void_p, c_int, c_ll, c_float = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
+c_double = ctypes.c_double
+
+MAX_HEAD_DIM = 256
+MAX_ROWS = 4096           # rows of a table in one call
+MAX_PAGES = 1 << 19
+
+
+class PagedAttnArgs(ctypes.Structure):
+    _fields_ = [(n, c_void_p) for n in ("q", "k", "v", "o", "table", "lens")] + \
+        [(n, c_ll) for n in ("q_row", "q_head", "o_row", "o_head", "k_page", "k_head", "k_tok", "v_page", "v_head", "v_tok",
+                             "table_row")] + \
+        [(n, c_int) for n in ("rows", "heads", "kv_heads", "hd", "page", "width", "pages", "f32")] + [("scale", c_float)]
+
+
+class AppendArgs(ctypes.Structure):
+    _fields_ = [(n, c_void_p) for n in ("qkv", "q", "keys", "k", "v", "table", "positions", "rows")] + \
+        [(n, c_ll) for n in ("ld", "k_page", "k_head", "k_tok", "v_page", "v_head", "v_tok", "table_row")] + \
+        [(n, c_int) for n in ("tokens", "heads", "kv_heads", "hd", "rotary", "page", "width", "pages", "table_rows", "f32")] + \
+        [("base", c_double)]
+
+
+class ForkArgs(ctypes.Structure):
+    _fields_ = [(n, c_void_p) for n in ("table", "lens", "parents", "grow", "new_table", "new_lens", "src", "dst", "free_list")] + \
+        [("table_row", c_ll)] + [(n, c_int) for n in ("rows_in", "rows", "width", "pages", "page", "grow_all")]
+
+
+class CompactArgs(ctypes.Structure):
+    _fields_ = [(n, c_void_p) for n in ("table", "new_table", "src", "dst", "live")] + \
+        [("table_row", c_ll)] + [(n, c_int) for n in ("rows", "width", "pages")]
+
+
+_declared = False
+
+
+def _lib():
+    global _declared
+    lib = N.load()
+    if not _declared:
+        for name, args in (("dptb_paged_attention", PagedAttnArgs), ("dptb_paged_append", AppendArgs),
+                           ("dptb_fork_pages", ForkArgs), ("dptb_compact_pages", CompactArgs)):
+            fn = getattr(lib, name)
+            fn.argtypes, fn.restype = [ctypes.POINTER(args), c_void_p], c_int
+        lib.dptb_copy_pages.argtypes = [c_void_p, c_void_p, c_void_p, c_int, c_ll, c_int, c_ll, c_void_p]
+        lib.dptb_copy_pages.restype = c_int
+        _declared = True
+    return lib
+
+
+# ------------------------------------------------------------------------------------------------------------ checks
+def _here(what: str, first: torch.Tensor, *others) -> None:
+    """One device for all, and the current one if it is a CUDA device: kernels go to its current stream."""
+    dev = first.device
+    for t in others:
+        if t is not None and t.device != dev:
+            raise ValueError(f"{what}: tensors on different devices ({dev} and {t.device})")
+    if first.is_cuda and dev.index != torch.cuda.current_device():
+        raise ValueError(f"{what}: tensors are on {dev}, the current device is {torch.cuda.current_device()}")
+
+
+def _no_grad(what: str, *tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError(f"{what} has no gradients; call it under torch.no_grad()")
+
+
+def _ints(what: str, name: str, t: torch.Tensor, *shape) -> None:
+    if t.dtype != torch.int32:
+        raise TypeError(f"{what}: {name} must be int32, got {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{what}: {name} must be {list(shape)}, got {list(t.shape)}")
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        raise ValueError(f"{what}: {name} must have a contiguous last axis")
+
+
+def _table(what: str, table: torch.Tensor) -> None:
+    if table.dim() != 2:
+        raise ValueError(f"{what}: the table must be [rows, width], got {list(table.shape)}")
+    _ints(what, "the table", table, *table.shape)
+    if table.shape[0] > MAX_ROWS:
+        raise ValueError(f"{what}: at most {MAX_ROWS} rows, got {table.shape[0]}")
+
+
+def _pages(what: str, k: torch.Tensor, v: torch.Tensor) -> None:
+    if k.dim() != 4 or k.shape != v.shape:
+        raise ValueError(f"{what}: k_pages and v_pages must be [pages, kv_heads, page, head_dim] both, got {list(k.shape)} "
+                         f"and {list(v.shape)}")
+    if k.dtype not in (torch.bfloat16, torch.float32) or v.dtype != k.dtype:
+        raise TypeError(f"{what}: pages must be float32 or bfloat16 both, got {k.dtype} and {v.dtype}")
+    pages, heads, page, hd = k.shape
+    if not 0 < hd <= MAX_HEAD_DIM or heads == 0 or page == 0 or pages > MAX_PAGES:
+        raise ValueError(f"{what}: pages of {list(k.shape)}: heads of 1 to {MAX_HEAD_DIM} features, at most {MAX_PAGES} pages")
+    for t in (k, v):
+        if t.stride(3) != 1 and hd > 1:
+            raise ValueError(f"{what}: the features of a page must be contiguous")
+
+
+# ------------------------------------------------------------------------------------------------------------ attention
+def paged_attention_reference(q, k_pages, v_pages, table, lens, scale=None):
+    """fp32 formulas, a row at a time."""
+    rows, heads, hd = q.shape
+    pages, hkv, page, _ = k_pages.shape
+    scale = 1.0 / math.sqrt(hd) if scale is None else scale
+    out = torch.zeros(rows, heads, hd, dtype=torch.float32, device=q.device)
+    for r, n in enumerate(lens.tolist()):
+        if n <= 0:
+            continue
+        held = table[r, :-(-n // page)].long()
+        if n > table.shape[1] * page or bool((held < 0).any()) or bool((held >= pages).any()):
+            raise ValueError(f"paged_attention: row {r} of {n} tokens lists a page that is not in the pool")
+        k, v = (t[held].transpose(0, 1).reshape(hkv, -1, hd)[:, :n].float() for t in (k_pages, v_pages))
+        s = q[r].float().view(hkv, heads // hkv, hd) @ k.transpose(1, 2) * scale
+        out[r] = (torch.softmax(s, -1) @ v).view(heads, hd)
+    return out.to(q.dtype)
+
+
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
+                    scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of one new token per row, ``q [rows, heads, head_dim]``, over the ``lens[r]`` tokens of its pages (the new one
+    among them).  Query heads share key heads in groups of ``heads // kv_heads``; a row of no tokens gives zeros.  bf16 or fp32, one type for all; sums in
+    fp32.  ``scale`` is ``head_dim ** -0.5`` unless given.  Returns ``[rows, heads, head_dim]``."""
+    what = "paged_attention"
+    _pages(what, k_pages, v_pages)
+    _table(what, table)
+    if q.dim() != 3 or q.shape[0] != table.shape[0] or q.shape[2] != k_pages.shape[3] or q.shape[1] % k_pages.shape[1]:
+        raise ValueError(f"{what}: queries {list(q.shape)} do not go with a table of {list(table.shape)} and pages of "
+                         f"{list(k_pages.shape)}")
+    if q.dtype != k_pages.dtype:
+        raise TypeError(f"{what}: queries are {q.dtype}, pages {k_pages.dtype}")
+    rows, heads, hd = q.shape
+    _ints(what, "lens", lens, rows)
+    _here(what, q, k_pages, v_pages, table, lens, out)
+    _no_grad(what, q, k_pages, v_pages)
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 and hd > 1):
+        raise ValueError(f"{what}: out must be {list(q.shape)} {q.dtype} with contiguous features")
+    if not q.is_cuda:
+        o = paged_attention_reference(q, k_pages, v_pages, table, lens, scale)
+        return o if out is None else out.copy_(o)
+    if q.stride(2) != 1 and hd > 1:
+        q = q.contiguous()
+    if out is None:
+        out = torch.empty(rows, heads, hd, dtype=q.dtype, device=q.device)
+    (q_row, q_head, _), (o_row, o_head, _) = q.stride(), out.stride()
+    kp, kh, kt, _ = k_pages.stride()
+    vp, vh, vt, _ = v_pages.stride()
+    pages, hkv, page, _ = k_pages.shape
+    a = PagedAttnArgs(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), table.data_ptr(), lens.data_ptr(),
+                      q_row, q_head, o_row, o_head, kp, kh, kt, vp, vh, vt, table.stride(0),
+                      rows, heads, hkv, hd, page, table.shape[1], pages, q.dtype == torch.float32,
+                      1.0 / math.sqrt(hd) if scale is None else scale)
+    N.check(_lib().dptb_paged_attention(a, N.stream_ptr()), what)
+    return out
+
+
+# ------------------------------------------------------------------------------------------------------------ append
+def paged_append_reference(qkv, k_pages, v_pages, table, positions, heads, rows, rotary_dim, rope_base):
+    pages, hkv, page, hd = k_pages.shape
+    x = qkv.reshape(-1, heads + 2 * hkv, hd)
+    half = rotary_dim // 2
+    pos = positions.double()
+    angle = pos[:, None] * rope_base ** (-2.0 * torch.arange(half, dtype=torch.float64, device=x.device) / max(rotary_dim, 1))
+    angle = torch.where(pos[:, None] >= 0, angle, 0.0)
+    cos, sin = torch.cos(angle).float()[:, None], torch.sin(angle).float()[:, None]
+    y = x.clone()
+    a, b = x[:, :heads + hkv, :half].float(), x[:, :heads + hkv, half:rotary_dim].float()
+    y[:, :heads + hkv, :half] = (a * cos - b * sin).to(x.dtype)
+    y[:, :heads + hkv, half:rotary_dim] = (b * cos + a * sin).to(x.dtype)
+    for t, p in enumerate(positions.tolist()):
+        if p < 0:
+            continue
+        r = t if rows is None else int(rows[t])
+        at = int(table[r, p // page]) if 0 <= r < table.shape[0] and p // page < table.shape[1] else -1
+        if not 0 <= at < pages:
+            raise ValueError(f"paged_append: token {t} has no page at position {p} of row {r}")
+        k_pages[at, :, p % page] = y[t, heads:heads + hkv]
+        v_pages[at, :, p % page] = y[t, heads + hkv:]
+    return y[:, :heads].contiguous(), y[:, heads:heads + hkv].contiguous()
+
+
+def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, positions: torch.Tensor,
+                 heads: int, rows: Optional[torch.Tensor] = None, rotary_dim: Optional[int] = None, rope_base: float = 10000.0,
+                 keys: bool = False) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """Keys and values of a projection output ``qkv [tokens, (heads + 2 kv_heads) head_dim]`` to their places in the pages: token
+    ``t`` is token ``positions[t]`` of row ``rows[t]`` (of row ``t`` without ``rows``); int32.  A negative position is padding
+    and writes nothing.  Queries and keys are turned by the half-split rotary embedding over ``rotary_dim`` features (all of
+    them unless given; 0: not at all).  Returns the turned queries ``[tokens, heads, head_dim]``, and with ``keys`` the turned keys
+    too; ``qkv`` stays as it is.  No two tokens may have one place."""
+    what = "paged_append"
+    _pages(what, k_pages, v_pages)
+    _table(what, table)
+    pages, hkv, page, hd = k_pages.shape
+    rotary = hd if rotary_dim is None else rotary_dim
+    if rotary < 0 or rotary % 2 or rotary > hd:
+        raise ValueError(f"{what}: rotary_dim must be even and in [0, {hd}], got {rotary}")
+    if heads <= 0 or qkv.dim() != 2 or qkv.shape[1] != (heads + 2 * hkv) * hd:
+        raise ValueError(f"{what}: qkv {list(qkv.shape)} is not [tokens, ({heads} + 2 * {hkv}) * {hd}]")
+    if qkv.dtype != k_pages.dtype:
+        raise TypeError(f"{what}: qkv is {qkv.dtype}, pages {k_pages.dtype}")
+    if not rope_base > 0:
+        raise ValueError(f"{what}: rope_base must be positive")
+    tokens = qkv.shape[0]
+    _ints(what, "positions", positions, tokens)
+    if rows is not None:
+        _ints(what, "rows", rows, tokens)
+    elif tokens != table.shape[0]:
+        raise ValueError(f"{what}: {tokens} tokens without `rows` for a table of {table.shape[0]} rows")
+    _here(what, qkv, k_pages, v_pages, table, positions, rows)
+    _no_grad(what, qkv, k_pages, v_pages)
+    if not qkv.is_cuda:
+        q, k = paged_append_reference(qkv, k_pages, v_pages, table, positions, heads, rows, rotary, rope_base)
+        return (q, k) if keys else q
+    if qkv.stride(1) != 1:
+        qkv = qkv.contiguous()
+    q = torch.empty(tokens, heads, hd, dtype=qkv.dtype, device=qkv.device)
+    k = torch.empty(tokens, hkv, hd, dtype=qkv.dtype, device=qkv.device) if keys else None
+    kp, kh, kt, _ = k_pages.stride()
+    vp, vh, vt, _ = v_pages.stride()
+    a = AppendArgs(qkv.data_ptr(), q.data_ptr(), N.ptr(k), k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(),
+                   positions.data_ptr(), N.ptr(rows), qkv.stride(0), kp, kh, kt, vp, vh, vt, table.stride(0),
+                   tokens, heads, hkv, hd, rotary, page, table.shape[1], pages, table.shape[0], qkv.dtype == torch.float32,
+                   rope_base)
+    N.check(_lib().dptb_paged_append(a, N.stream_ptr()), what)
+    torch.autograd.graph.increment_version((k_pages, v_pages))
+    return (q, k) if keys else q
+
+
+# ------------------------------------------------------------------------------------------------------------ pages
+def fork_pages_reference(table, lens, pages, page, parents, grow):
+    t_in, l_in, width = table.tolist(), lens.tolist(), table.shape[1]
+    who = list(range(len(t_in))) if parents is None else parents.tolist()
+    more = grow.tolist() if isinstance(grow, torch.Tensor) else [grow if p >= 0 else 0 for p in who]
+    held, old, new = [], [], []
+    for p, g in zip(who, more):
+        if p >= len(t_in):
+            raise ValueError(f"fork_pages: parent {p} of {len(t_in)} rows")
+        n = max(0, l_in[p]) if p >= 0 else 0
+        row = t_in[p][:-(-n // page)] if n else []
+        if n + max(g, 0) > width * page or any(not 0 <= x < pages for x in row) or len(row) < -(-n // page):
+            raise ValueError(f"fork_pages: a row of {n} tokens, {g} more, in {width} pages of {page}: {row}")
+        held.append(row)
+        old.append(n)
+        new.append(n + max(g, 0))
+    grows = [b > a and a % page != 0 for a, b in zip(old, new)]
+    used = {x for row in held for x in row}
+    others = {x for row, g in zip(held, grows) for x in (row[:-1] if g else row)}
+    free = iter([x for x in range(pages) if x not in used])
+    keeper, src, dst = {}, [-1] * len(who), [-1] * len(who)
+    try:
+        for r, row in enumerate(held):
+            row = list(row)
+            if grows[r] and (row[-1] in others or keeper.setdefault(row[-1], r) != r):
+                src[r], row[-1] = row[-1], next(free)
+                dst[r] = row[-1]
+            while len(row) * page < new[r]:
+                row.append(next(free))
+            held[r] = row + [-1] * (width - len(row))
+    except StopIteration:
+        raise ValueError(f"fork_pages: a pool of {pages} pages has no free one left") from None
+    make = lambda x, *shape: torch.tensor(x, dtype=torch.int32, device=table.device).view(*shape)  # noqa: E731
+    return make(held, len(who), width), make(new, -1), make(src, -1), make(dst, -1)
+
+
+def fork_pages(table: torch.Tensor, lens: torch.Tensor, pages: int, page: int, parents: Optional[torch.Tensor] = None,
+               grow: Union[int, torch.Tensor] = 0) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The rows of a cache anew: row ``r`` becomes row ``parents[r]`` (itself without ``parents``; -1: empty, which frees its
+    pages), longer by ``grow`` tokens: an int for every row that has a parent, or int32 ``[rows]``, which starts empty rows as well.
+    Pages of a ``pages``-page pool (``page`` tokens each) are taken for them, free ones of the lowest numbers first, row by row;
+    a part-filled last page that others list too is replaced by a copy of the row's own, except for the first row that grows into it.
+    Returns ``(table, lens, src, dst)``: the new table and lengths, and for every row the page to copy and its copy (-1: none), which
+    ``copy_pages`` takes before anything is appended.  The old table is left as it is."""
+    what = "fork_pages"
+    _table(what, table)
+    rows_in, width = table.shape
+    _ints(what, "lens", lens, rows_in)
+    rows = rows_in if parents is None else parents.numel()
+    if parents is not None:
+        _ints(what, "parents", parents, rows)
+    each = isinstance(grow, torch.Tensor)
+    if each:
+        _ints(what, "grow", grow, rows)
+    elif grow < 0:
+        raise ValueError(f"{what}: rows grow by 0 or more tokens, got {grow}")
+    if rows > MAX_ROWS or not 0 <= pages <= MAX_PAGES or page <= 0:
+        raise ValueError(f"{what}: {rows} rows (at most {MAX_ROWS}), {pages} pages (at most {MAX_PAGES}) of {page} tokens")
+    _here(what, table, lens, parents, grow if each else None)
+    if not table.is_cuda:
+        return fork_pages_reference(table, lens, pages, page, parents, grow)
+    new_table = torch.empty(rows, width, dtype=torch.int32, device=table.device)
+    new_lens, src, dst = torch.empty(3, rows, dtype=torch.int32, device=table.device).unbind(0)
+    free = torch.empty(max(pages, 1), dtype=torch.int32, device=table.device)
+    a = ForkArgs(table.data_ptr(), lens.data_ptr(), N.ptr(parents), grow.data_ptr() if each else None, new_table.data_ptr(),
+                 new_lens.data_ptr(), src.data_ptr(), dst.data_ptr(), free.data_ptr(), table.stride(0), rows_in, rows, width,
+                 pages, page, 0 if each else grow)
+    N.check(_lib().dptb_fork_pages(a, N.stream_ptr()), what)
+    return new_table, new_lens, src, dst
+
+
+def compact_pages_reference(table, pages):
+    held = sorted({p for p in table.flatten().tolist() if p >= 0})
+    if held and held[-1] >= pages:
+        raise ValueError(f"compact_pages: page {held[-1]} of a pool of {pages}")
+    live, on = len(held), set(held)
+    moves = dict(zip([p for p in held if p >= live], [p for p in range(live) if p not in on]))
+    make = lambda x: torch.tensor(x, dtype=torch.int32, device=table.device)  # noqa: E731
+    new = make([moves.get(p, p) if p >= 0 else -1 for p in table.flatten().tolist()]).view(table.shape)
+    blank = [-1] * (pages // 2 - len(moves))
+    return new, make(list(moves) + blank), make(list(moves.values()) + blank), make([live])
+
+
+def compact_pages(table: torch.Tensor, pages: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The ``n`` listed pages of a pool numbered 0 to ``n - 1``: those numbered ``n`` and above move, in order, to the unlisted
+    numbers below.  Returns ``(table, src, dst, live)``: the table in the new numbers, the moves (``[pages // 2]``, -1 behind
+    the last) for ``copy_pages``, and ``n`` as an int32 ``[1]``."""
+    what = "compact_pages"
+    _table(what, table)
+    if not 0 <= pages <= MAX_PAGES:
+        raise ValueError(f"{what}: a pool of {pages} pages (at most {MAX_PAGES})")
+    _here(what, table)
+    if not table.is_cuda:
+        return compact_pages_reference(table, pages)
+    new = torch.empty(table.shape, dtype=torch.int32, device=table.device)
+    src, dst = torch.empty(2, pages // 2, dtype=torch.int32, device=table.device).unbind(0)
+    live = torch.empty(1, dtype=torch.int32, device=table.device)
+    a = CompactArgs(table.data_ptr(), new.data_ptr(), src.data_ptr(), dst.data_ptr(), live.data_ptr(), table.stride(0),
+                    *table.shape, pages)
+    N.check(_lib().dptb_compact_pages(a, N.stream_ptr()), what)
+    return new, src, dst, live
+
+
+def copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None:
+    """In place: page ``dst[i]`` of ``pool [..., pages, kv_heads, page, head_dim]`` (contiguous; every layer's keys and values at
+    once) becomes a copy of page ``src[i]``; pairs with a -1 are passed over.  A page that is copied to must be in no other pair."""
+    what = "copy_pages"
+    if pool.dim() < 4 or not pool.is_contiguous():
+        raise ValueError(f"{what}: the pool must be a contiguous [..., pages, kv_heads, page, head_dim], got {list(pool.shape)}")
+    if pool.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"{what}: pages must be float32 or bfloat16, got {pool.dtype}")
+    _ints(what, "src", src, *src.shape)
+    _ints(what, "dst", dst, *src.shape)
+    if src.dim() != 1:
+        raise ValueError(f"{what}: src and dst must be lists of pages")
+    _here(what, pool, src, dst)
+    _no_grad(what, pool)
+    pages = pool.shape[-4]
+    outer = math.prod(pool.shape[:-4])
+    if not pool.is_cuda:
+        real = (src >= 0) & (dst >= 0)
+        x, y = src[real].long(), dst[real].long()
+        if bool((x >= pages).any()) or bool((y >= pages).any()):
+            raise ValueError(f"{what}: a page outside the pool of {pages}")
+        flat = pool.view(outer, pages, -1)
+        flat[:, y] = flat[:, x]
+        return
+    if outer > 65535:
+        raise ValueError(f"{what}: at most 65535 pools at once, got {outer}")
+    size = math.prod(pool.shape[-3:]) * pool.element_size()
+    N.check(_lib().dptb_copy_pages(pool.data_ptr(), src.data_ptr(), dst.data_ptr(), src.numel(), outer, pages, size,
+                                   N.stream_ptr()), what)
+    torch.autograd.graph.increment_version(pool)
