@@ -6,8 +6,24 @@
 // length zero gives zeros.  Positions from lens[r] on are never read as numbers: what lies there may be anything.  A page number
 // outside the pool hides its keys and records kBadPage in the status word, which the host turns into an exception.
 //
-// paged_attention_simple_kernel: a CTA per (row, query head); tiles of 128 keys, a thread a key for the scores and a thread a feature for
-// the weighted sum; fp32 throughout.
+// paged_attention_kernel reads every key and value once for all heads of its group.  The keys of all (row, kv head) pairs, "jobs", are one
+// sequence of rounds (16 keys in bf16, 8 in fp32) that is dealt out evenly: a CTA an SM takes a contiguous range, each of its warps a contiguous
+// part of that, so lengths from one token to the longest mix without an idle SM and without the host knowing them.  A warp keeps the running
+// maximum, sum and weighted values of its job in registers.  Parts of a job that fell to several warps are joined in shared memory, and
+// of several CTAs through a workspace by the last of them to finish (a counter, no waiting; parts are added in order, so results
+// repeat to the bit).
+//
+// Loads: a lane copies the 16-byte pieces that it will itself need, in the layout of the matrix instructions' fragments, to slots of its
+// own in shared memory (cp.async, several rounds ahead, across jobs too) and reads them back alone: no barrier, no bank conflict, and any
+// strides.  The features of a fragment are dealt to the lanes in another order than the instruction's, in queries and keys alike, which a sum
+// does not notice.
+//
+// bf16: S^T = K Q^T and O^T = V^T P^T by mma.sync, the group's heads as the 8 columns (two tiles of them for 9 to 16 heads); the bound is
+// the cache stream, and a tcgen05 tile of 128 rows would be padding for the most part.  The weights enter as two bf16 parts (16 bits).
+// fp32: multiply-adds, 8 lanes a key.
+//
+// paged_attention_simple_kernel takes what 16-byte pieces do not fit (head sizes, strides or addresses off them): a CTA per (row, query
+// head), a thread a key for the scores and a thread a feature for the weighted sum.
 #include <cuda_bf16.h>
 
 #include "common/host.h"
@@ -28,8 +44,694 @@ struct PagedAttnArgs {
   long long table_row;
   int rows, heads, kv_heads, hd, page, width, pages, f32;
   float scale;
+  float* ws;           // parts of jobs that several CTAs share
+  long long ws_floats;
+  unsigned* counters;  // zeroed words, one per CTA; zero again afterwards
+  int num_counters;
 };
 
+// ------------------------------------------------------------------------------------------------------------ pieces
+__device__ __forceinline__ void copy_piece(uint32_t smem_dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ uint4 read_piece(uint32_t addr) {
+  uint4 u;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(addr) : "memory");
+  return u;
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// What of a round a lane looks up: the page of a position, from a window of 32 table entries that the lanes hold.
+struct PageWindow {
+  int row = -1, first = 0, entry = -1;
+  __device__ __forceinline__ void cover(const PagedAttnArgs& a, int r, int slot, int last, int held, int lane) {
+    if (r != row || slot < first || last >= first + 32) {
+      row = r;
+      first = slot;
+      entry = slot + lane < held ? a.table[r * a.table_row + slot + lane] : -1;
+    }
+  }
+  __device__ __forceinline__ int at(int slot) const { return __shfl_sync(0xffffffffu, entry, (slot - first) & 31); }
+};
+
+// A place in the sequence of rounds: round k of the n rounds of job (row, vh).
+struct Cursor {
+  int row, vh, k, n;
+};
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kTiny = 1.2e-38f;
+
+// ------------------------------------------------------------------------------------------------------------ bf16
+// HD: features of a head, padded with zeros; NT: tiles of 8 query heads.
+template <int HD, int NT>
+struct Bf16Round {
+  using T = __nv_bfloat16;
+  static constexpr int kKeys = 16, kHeads = 8 * NT, kHD = HD;
+  static constexpr int kKeyPieces = 2 * (HD / 32), kValuePieces = 4 * (HD / 64);       // per lane and round
+  static constexpr int kBytes = (kKeyPieces + kValuePieces) * 512;
+  static constexpr int kQueryBytes = 0;
+
+  uint4 q[NT][HD / 32];       // head lane / 4, pieces (lane % 4) + 4 i
+  float m[NT][2], l[NT][2];   // heads (lane % 4) * 2 and the next; l: of this lane's keys
+  float o[NT][HD / 64][4][4]; // features 8 (lane / 4 + 8 b) + 2 i and the next, of those heads
+
+  static __device__ __forceinline__ unsigned issue(const PagedAttnArgs& a, PageWindow& win, const Cursor& c, int kv, int len, uint32_t ring, int lane) {
+    const T* kb = static_cast<const T*>(a.k) + kv * a.k_head;
+    const T* vb = static_cast<const T*>(a.v) + kv * a.v_head;
+    const int p0 = c.k * kKeys, g = lane >> 2, t = lane & 3;
+    win.cover(a, c.row, p0 / a.page, (min(p0 + kKeys, len) - 1) / a.page, (len + a.page - 1) / a.page, lane);
+    unsigned live = 0;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int pos = p0 + g + 8 * j, slot = pos / a.page;
+      const int page = win.at(slot);
+      bool ok = pos < len;
+      if (ok && (unsigned)page >= (unsigned)a.pages) {
+        report_error(kBadPage);
+        ok = false;
+      }
+      live |= (unsigned)ok << j;
+      const T* src = kb + (ok ? page * a.k_page + (pos - slot * a.page) * a.k_tok : 0);
+#pragma unroll
+      for (int i = 0; i < HD / 32; ++i) {
+        const int f = (t + 4 * i) * 8;
+        const bool in = ok && f < a.hd;
+        copy_piece(ring + (j * (HD / 32) + i) * 512 + lane * 16, in ? src + f : kb, in);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int pos = p0 + 2 * t + (j & 1) + 8 * (j >> 1), slot = pos / a.page;
+      const int page = win.at(slot);
+      const bool ok = pos < len && (unsigned)page < (unsigned)a.pages;
+      const T* src = vb + (ok ? page * a.v_page + (pos - slot * a.page) * a.v_tok : 0);
+#pragma unroll
+      for (int b = 0; b < HD / 64; ++b) {
+        const int f = (g + 8 * b) * 8;
+        const bool in = ok && f < a.hd;
+        copy_piece(ring + (kKeyPieces + j * (HD / 64) + b) * 512 + lane * 16, in ? src + f : vb, in);
+      }
+    }
+    return live;
+  }
+
+  // The queries of heads head0 .. head0 + count of a row.
+  __device__ __forceinline__ void start(const PagedAttnArgs& a, int row, int head0, int count, bool vec, float*, int lane) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int h = n * 8 + (lane >> 2);
+      const T* src = static_cast<const T*>(a.q) + row * a.q_row + (long long)(head0 + min(h, count - 1)) * a.q_head;
+#pragma unroll
+      for (int i = 0; i < HD / 32; ++i) {
+        const int f = ((lane & 3) + 4 * i) * 8;
+        uint4 u = make_uint4(0, 0, 0, 0);
+        if (h < count && f < a.hd) {
+          if (vec) {
+            u = *reinterpret_cast<const uint4*>(src + f);
+          } else {
+            const unsigned short* e = reinterpret_cast<const unsigned short*>(src + f);
+            u.x = e[0] | e[1] << 16;
+            u.y = e[2] | e[3] << 16;
+            u.z = e[4] | e[5] << 16;
+            u.w = e[6] | e[7] << 16;
+          }
+        }
+        q[n][i] = u;
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        m[n][e] = -INFINITY;
+        l[n][e] = 0.0f;
+      }
+#pragma unroll
+      for (int b = 0; b < HD / 64; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[n][b][i][e] = 0.0f;
+    }
+  }
+
+  __device__ __forceinline__ void compute(const PagedAttnArgs& a, uint32_t ring, unsigned live, float scale2, const float*, int lane) {
+    float sc[NT][2][4] = {};
+#pragma unroll
+    for (int i = 0; i < HD / 32; ++i) {
+      const uint4 k0 = read_piece(ring + i * 512 + lane * 16), k1 = read_piece(ring + (HD / 32 + i) * 512 + lane * 16);
+      const uint32_t fa[4] = {k0.x, k1.x, k0.y, k1.y}, fb[4] = {k0.z, k1.z, k0.w, k1.w};
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        mma_bf16_16816(sc[n][0], fa, q[n][i].x, q[n][i].y);
+        mma_bf16_16816(sc[n][1], fb, q[n][i].z, q[n][i].w);
+      }
+    }
+    uint32_t pp[NT][2][2];      // [part][keys, keys + 8]: pairs of keys of head lane / 4
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float p[2][2], corr[2];   // [key, key + 8][head]
+      bool moved = false;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float s[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) s[r] = live >> r & 1 ? (sc[n][0][2 * r + e] + sc[n][1][2 * r + e]) * scale2 : -INFINITY;
+        float mx = fmaxf(s[0], s[1]);
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+        const float nm = fmaxf(m[n][e], mx), sub = nm == -INFINITY ? 0.0f : nm;
+        moved |= nm != m[n][e];
+        corr[e] = exp2_fast(m[n][e] - sub);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) p[r][e] = live >> r & 1 ? exp2_fast(s[r] - sub) : 0.0f;
+        l[n][e] = l[n][e] * corr[e] + (p[0][e] + p[1][e]);
+        m[n][e] = nm;
+      }
+      // Leading 8 bits and the rest.  Parts of a positive weight stay positive: its product with an infinite value is infinite in each.
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const uint32_t u0 = __float_as_uint(p[r][0]), u1 = __float_as_uint(p[r][1]);
+        pp[n][0][r] = movmatrix_trans((u0 >> 16) | (u1 & 0xffff0000u));
+        const float r0 = p[r][0] > 0.0f ? fmaxf(p[r][0] - __uint_as_float(u0 & 0xffff0000u), kTiny) : 0.0f;
+        const float r1 = p[r][1] > 0.0f ? fmaxf(p[r][1] - __uint_as_float(u1 & 0xffff0000u), kTiny) : 0.0f;
+        pp[n][1][r] = movmatrix_trans(pack_bf16x2(r0, r1));
+      }
+      if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+        for (int b = 0; b < HD / 64; ++b)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[n][b][i][e] *= corr[e & 1];
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < HD / 64; ++b) {
+      uint32_t v[4][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint4 u = read_piece(ring + (kKeyPieces + j * (HD / 64) + b) * 512 + lane * 16);
+        v[j][0] = u.x; v[j][1] = u.y; v[j][2] = u.z; v[j][3] = u.w;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t f[4] = {__byte_perm(v[0][i], v[1][i], 0x5410), __byte_perm(v[0][i], v[1][i], 0x7632),
+                               __byte_perm(v[2][i], v[3][i], 0x5410), __byte_perm(v[2][i], v[3][i], 0x7632)};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          mma_bf16_16816(o[n][b][i], f, pp[n][0][0], pp[n][0][1]);
+          mma_bf16_16816(o[n][b][i], f, pp[n][1][0], pp[n][1][1]);
+        }
+      }
+    }
+  }
+
+  __device__ __forceinline__ void finish(int lane) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], off);
+  }
+  // Eight consecutive features at a time: put(head, first feature, values, maximum, sum).
+  template <typename F>
+  __device__ __forceinline__ void each(int lane, F put) const {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int b = 0; b < HD / 64; ++b) {
+          float f[8];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            f[2 * i] = o[n][b][i][e];
+            f[2 * i + 1] = o[n][b][i][2 + e];
+          }
+          put(n * 8 + (lane & 3) * 2 + e, 8 * ((lane >> 2) + 8 * b), f, m[n][e], l[n][e]);
+        }
+  }
+};
+
+// ------------------------------------------------------------------------------------------------------------ fp32
+// GP: query heads at a time.  Lane s of the 8 lanes of a key holds pieces s + 8 i of it; four keys go by at once, two steps a round.  The
+// scaled queries lie in shared memory, a copy for every warp.
+template <int HD, int GP>
+struct F32Round {
+  using T = float;
+  static constexpr int kKeys = 8, kHeads = GP, kHD = HD;
+  static constexpr int P = HD / 32;                      // pieces of a key per lane
+  static constexpr int kBytes = 4 * P * 512;
+  static constexpr int kQueryBytes = GP * HD * 4;
+
+  float m[GP], l[GP];
+  float4 o[GP][P];
+
+  static __device__ __forceinline__ unsigned issue(const PagedAttnArgs& a, PageWindow& win, const Cursor& c, int kv, int len, uint32_t ring, int lane) {
+    const T* kb = static_cast<const T*>(a.k) + kv * a.k_head;
+    const T* vb = static_cast<const T*>(a.v) + kv * a.v_head;
+    const int p0 = c.k * kKeys, g = lane >> 3, t = lane & 7;
+    win.cover(a, c.row, p0 / a.page, (min(p0 + kKeys, len) - 1) / a.page, (len + a.page - 1) / a.page, lane);
+    unsigned live = 0;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int pos = p0 + g + 4 * j, slot = pos / a.page;
+      const int page = win.at(slot);
+      bool ok = pos < len;
+      if (ok && (unsigned)page >= (unsigned)a.pages) {
+        report_error(kBadPage);
+        ok = false;
+      }
+      live |= (unsigned)ok << j;
+      const T* ks = kb + (ok ? page * a.k_page + (pos - slot * a.page) * a.k_tok : 0);
+      const T* vs = vb + (ok ? page * a.v_page + (pos - slot * a.page) * a.v_tok : 0);
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const int f = (t + 8 * i) * 4;
+        const bool in = ok && f < a.hd;
+        copy_piece(ring + (j * P + i) * 512 + lane * 16, in ? ks + f : kb, in);
+        copy_piece(ring + ((2 + j) * P + i) * 512 + lane * 16, in ? vs + f : vb, in);
+      }
+    }
+    return live;
+  }
+
+  __device__ __forceinline__ void start(const PagedAttnArgs& a, int row, int head0, int count, bool, float* queries, int lane) {
+    __syncwarp();
+    for (int x = lane; x < GP * HD; x += 32) {
+      const int h = x / HD, f = x % HD;
+      queries[x] = h < count && f < a.hd ? static_cast<const T*>(a.q)[row * a.q_row + (long long)(head0 + h) * a.q_head + f] : 0.0f;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int h = 0; h < GP; ++h) {
+      m[h] = -INFINITY;
+      l[h] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < P; ++i) o[h][i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+  }
+
+  __device__ __forceinline__ void compute(const PagedAttnArgs& a, uint32_t ring, unsigned live, float scale2, const float* queries, int lane) {
+    const float4* q4 = reinterpret_cast<const float4*>(queries) + (lane & 7);
+    float p[GP][2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float4 k[P];
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const uint4 u = read_piece(ring + (j * P + i) * 512 + lane * 16);
+        k[i] = make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w));
+      }
+#pragma unroll
+      for (int h = 0; h < GP; ++h) {
+        float s = 0.0f, s1 = 0.0f;
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          const float4 w = q4[h * (HD / 4) + 8 * i];
+          s = fmaf(k[i].x, w.x, s);
+          s1 = fmaf(k[i].y, w.y, s1);
+          s = fmaf(k[i].z, w.z, s);
+          s1 = fmaf(k[i].w, w.w, s1);
+        }
+        p[h][j] = s + s1;
+      }
+    }
+    bool moved = false;
+    float corr[GP];
+#pragma unroll
+    for (int h = 0; h < GP; ++h) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float s = p[h][j];
+#pragma unroll
+        for (int off = 1; off < 8; off <<= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+        p[h][j] = live >> j & 1 ? s * scale2 : -INFINITY;
+      }
+      float mx = fmaxf(p[h][0], p[h][1]);
+#pragma unroll
+      for (int off = 8; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+      const float nm = fmaxf(m[h], mx), sub = nm == -INFINITY ? 0.0f : nm;
+      moved |= nm != m[h];
+      corr[h] = exp2_fast(m[h] - sub);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) p[h][j] = live >> j & 1 ? exp2_fast(p[h][j] - sub) : 0.0f;
+      l[h] = l[h] * corr[h] + (p[h][0] + p[h][1]);
+      m[h] = nm;
+    }
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+      for (int h = 0; h < GP; ++h)
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          o[h][i].x *= corr[h];
+          o[h][i].y *= corr[h];
+          o[h][i].z *= corr[h];
+          o[h][i].w *= corr[h];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const uint4 u = read_piece(ring + ((2 + j) * P + i) * 512 + lane * 16);
+#pragma unroll
+        for (int h = 0; h < GP; ++h) {
+          o[h][i].x = fmaf(p[h][j], __uint_as_float(u.x), o[h][i].x);
+          o[h][i].y = fmaf(p[h][j], __uint_as_float(u.y), o[h][i].y);
+          o[h][i].z = fmaf(p[h][j], __uint_as_float(u.z), o[h][i].z);
+          o[h][i].w = fmaf(p[h][j], __uint_as_float(u.w), o[h][i].w);
+        }
+      }
+  }
+
+  __device__ __forceinline__ void finish(int) {
+#pragma unroll
+    for (int h = 0; h < GP; ++h)
+#pragma unroll
+      for (int off = 8; off < 32; off <<= 1) {
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], off);
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          o[h][i].x += __shfl_xor_sync(0xffffffffu, o[h][i].x, off);
+          o[h][i].y += __shfl_xor_sync(0xffffffffu, o[h][i].y, off);
+          o[h][i].z += __shfl_xor_sync(0xffffffffu, o[h][i].z, off);
+          o[h][i].w += __shfl_xor_sync(0xffffffffu, o[h][i].w, off);
+        }
+      }
+  }
+  template <typename F>
+  __device__ __forceinline__ void each(int lane, F put) const {
+    if (lane >= 8) return;
+#pragma unroll
+    for (int h = 0; h < GP; ++h)
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const float f[4] = {o[h][i].x, o[h][i].y, o[h][i].z, o[h][i].w};
+        put(h, 4 * (lane + 8 * i), f, m[h], l[h]);
+      }
+  }
+};
+
+// ------------------------------------------------------------------------------------------------------------ the kernel
+// A part of a job in memory: [heads][HD] weighted values, then the heads' maxima and sums.
+template <typename R>
+struct Part {
+  static constexpr int kFloats = (R::kHeads * (R::kHD + 2) + 3) / 4 * 4;
+};
+
+template <typename T, int N>
+__device__ __forceinline__ void store_out(T* dst, const float (&f)[N], float by, int valid, bool vec) {
+  T e[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) e[i] = from_f32<T>(f[i] * by);
+  if constexpr (N * sizeof(T) == 16) {
+    if (vec && valid >= N) {
+      *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(e);
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i < valid) dst[i] = e[i];
+}
+
+// W warps, S rounds of a warp in flight or in use.
+template <typename R, int W, int S>
+__global__ void __launch_bounds__(W * 32, 1)
+paged_attention_kernel(const PagedAttnArgs a, int head_tiles, int tile_heads, int q_vec, int o_vec) {
+  using T = typename R::T;
+  constexpr int kPart = Part<R>::kFloats;
+  static_assert(S * R::kBytes >= kPart * 4, "a warp's ring holds its last part");
+  extern __shared__ __align__(16) unsigned char smem[];
+  unsigned char* rings = smem;                                              // [W][S] rounds
+  float* leads = reinterpret_cast<float*>(rings + W * S * R::kBytes);       // [W] parts
+  float* queries = leads + W * kPart;                                       // [W] copies of the queries
+  int* before = reinterpret_cast<int*>(queries + W * (R::kQueryBytes / 4)); // [rows + 1]: rounds of a kv head ahead of a row
+  __shared__ int scan[W + 1];
+  __shared__ int part_job[2 * W];
+  __shared__ int shared_job[2], shared_slot[2], merges[2];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tiles = a.kv_heads * head_tiles;                                // jobs of a row
+  const int room = (int)min((long long)a.width * a.page, 0x7fffffffLL);
+  const int group = a.heads / a.kv_heads;
+
+  // Rounds ahead of every row.
+  auto length = [&](int r) { return max(0, min(a.lens[r], room)); };
+  {
+    const int each = (a.rows + W * 32 - 1) / (W * 32), r0 = min(a.rows, tid * each), r1 = min(a.rows, r0 + each);
+    int mine = 0;
+    for (int r = r0; r < r1; ++r) {
+      const int n = a.lens[r];
+      if (n > room && blockIdx.x == 0) report_error(kBadPage);
+      mine += (max(0, min(n, room)) + R::kKeys - 1) / R::kKeys;
+    }
+    int s = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += u;
+    }
+    if (lane == 31) scan[warp] = s;
+    __syncthreads();
+    int at = s - mine;
+    for (int w = 0; w < warp; ++w) at += scan[w];
+    for (int r = r0; r < r1; ++r) {
+      before[r] = at;
+      at += (length(r) + R::kKeys - 1) / R::kKeys;
+    }
+    if (tid == 0) {
+      int t = 0;
+      for (int w = 0; w < W; ++w) t += scan[w];
+      before[a.rows] = t;
+    }
+    if (tid < 2 * W) part_job[tid] = -1;
+    if (tid < 2) shared_job[tid] = -1;
+    __syncthreads();
+  }
+  const long long total = (long long)before[a.rows] * tiles;
+  // A CTA takes a round for each of its warps at least: parts of one CTA are joined sooner than those of several.
+  const long long share = max((long long)W, (total + gridDim.x - 1) / gridDim.x);
+  const long long begin = min(total, share * blockIdx.x), end = min(total, begin + share);
+  for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {       // rows of no tokens
+    if (before[r + 1] > before[r]) continue;
+    for (int x = tid; x < a.heads * a.hd; x += W * 32) static_cast<T*>(a.o)[r * a.o_row + x / a.hd * a.o_head + x % a.hd] = from_f32<T>(0.0f);
+  }
+  if (begin >= end) return;
+
+  const long long quota = (end - begin + W - 1) / W;
+  const long long w0 = min(end, begin + quota * warp), w1 = min(end, w0 + quota);
+  int todo = (int)(w1 - w0);
+  if (todo > 0) {
+    const uint32_t ring = smem_u32(rings) + warp * S * R::kBytes;
+    float* my_queries = queries + warp * (R::kQueryBytes / 4);
+    int row = 0;
+    {
+      int hi = a.rows - 1;                                     // the last row with no more rounds ahead than w0, which has some itself
+      while (row < hi) {
+        const int mid = (row + hi + 1) / 2;
+        if ((long long)before[mid] * tiles <= w0) row = mid;
+        else hi = mid - 1;
+      }
+    }
+    const int n0 = before[row + 1] - before[row];
+    const int rem = (int)(w0 - (long long)before[row] * tiles);
+    Cursor c{row, rem / n0, rem % n0, n0}, ahead = c;
+    auto advance = [&](Cursor& x) {
+      if (++x.k < x.n) return;
+      x.k = 0;
+      if (++x.vh < tiles) return;
+      x.vh = 0;
+      do {
+        ++x.row;
+      } while (x.row < a.rows && before[x.row + 1] == before[x.row]);
+      if (x.row < a.rows) x.n = before[x.row + 1] - before[x.row];
+    };
+    PageWindow win;
+    unsigned lives = 0;                                        // two bits for each round of the ring
+    int left = todo, put = 0, take = 0, len = length(row), len_row = row;
+    auto fetch = [&] {
+      if (left > 0) {
+        if (ahead.row != len_row) {
+          len_row = ahead.row;
+          len = length(len_row);
+        }
+        const unsigned live = R::issue(a, win, ahead, ahead.vh / head_tiles, len, ring + put * R::kBytes, lane);
+        lives = (lives & ~(3u << (2 * put))) | live << (2 * put);
+        put = put + 1 == S ? 0 : put + 1;
+        --left;
+        if (left > 0) advance(ahead);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int s = 0; s < S - 1; ++s) fetch();
+    const float scale2 = a.scale * kLog2e;
+    R x;
+    int from = c.k;
+    bool fresh = true, first = true;
+    for (; todo > 0; --todo) {
+      fetch();
+      const int head0 = c.vh / head_tiles * group + c.vh % head_tiles * tile_heads;
+      const int count = min(tile_heads, group - c.vh % head_tiles * tile_heads);
+      if (fresh) {
+        x.start(a, c.row, head0, count, q_vec, my_queries, lane);
+        from = c.k;
+        fresh = false;
+      }
+      asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory");
+      x.compute(a, ring + take * R::kBytes, lives >> (2 * take) & 3, scale2, my_queries, lane);
+      take = take + 1 == S ? 0 : take + 1;
+      const bool last = c.k + 1 == c.n;
+      if (last || todo == 1) {
+        x.finish(lane);
+        if (from == 0 && last) {
+          T* out = static_cast<T*>(a.o) + c.row * a.o_row + (long long)head0 * a.o_head;
+          x.each(lane, [&](int h, int f, const auto& v, float, float l) {
+            if (h < count) store_out(out + h * a.o_head + f, v, 1.0f / l, a.hd - f, o_vec);
+          });
+        } else {
+          const int at = 2 * warp + (first ? 0 : 1);
+          float* part = first ? leads + warp * kPart : reinterpret_cast<float*>(rings + warp * S * R::kBytes);
+          if (!first) asm volatile("cp.async.wait_all;" ::: "memory");
+          __syncwarp();
+          x.each(lane, [&](int h, int f, const auto& v, float m, float l) {
+            if (h >= count) return;
+            constexpr int N = sizeof(v) / sizeof(float);
+#pragma unroll
+            for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(part + h * R::kHD + f + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+            if (f == 0) {
+              part[R::kHeads * R::kHD + h] = m;
+              part[R::kHeads * (R::kHD + 1) + h] = l;
+            }
+          });
+          if (lane == 0) part_job[at] = c.row * tiles + c.vh;
+        }
+        fresh = true;
+        first = false;
+      }
+      if (todo > 1) advance(c);
+    }
+  }
+  __syncthreads();
+
+  // Parts of a job in this CTA are neighbours.  A job that lies within the CTA is written out, another's part goes to the workspace: place 0
+  // of the CTA for the job of its first round, 1 for one that begins later.
+  constexpr int kPer = R::kHD / 32;                            // features of a lane
+  auto part_at = [&](int i) { return i & 1 ? reinterpret_cast<const float*>(rings + (i >> 1) * S * R::kBytes) : leads + (i >> 1) * kPart; };
+  auto write = [&](int job, int h, const float (&f)[kPer], float l) {
+    const int row = job / tiles, vh = job % tiles;
+    T* out = static_cast<T*>(a.o) + row * a.o_row + (long long)(vh / head_tiles * group + vh % head_tiles * tile_heads + h) * a.o_head;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (lane * kPer + i < a.hd) out[lane * kPer + i] = from_f32<T>(f[i] / l);
+  };
+  auto heads_of = [&](int job) { return min(tile_heads, group - job % tiles % head_tiles * tile_heads); };
+  auto job_begin = [&](int job) {
+    const int row = job / tiles;
+    return (long long)before[row] * tiles + (long long)(job % tiles) * (before[row + 1] - before[row]);
+  };
+  auto job_end = [&](int job) { return job_begin(job) + (before[job / tiles + 1] - before[job / tiles]); };
+  int unit = 0;
+  for (int i = 0; i < 2 * W;) {
+    const int job = part_job[i];
+    if (job < 0) {
+      ++i;
+      continue;
+    }
+    int stop = i + 1;
+    while (stop < 2 * W && (part_job[stop] == job || part_job[stop] < 0)) ++stop;
+    const long long jb = job_begin(job);
+    const bool whole = jb >= begin && job_end(job) <= end;
+    const int place = jb > begin;
+    float* dst = a.ws + (blockIdx.x * 2LL + place) * kPart;
+    if (!whole && tid == 0) {
+      shared_job[place] = job;
+      shared_slot[place] = (int)(jb / share);
+    }
+    for (int h = 0; h < heads_of(job); ++h, ++unit) {
+      if (unit % W != warp) continue;
+      float m = -INFINITY;
+      for (int j = i; j < stop; ++j)
+        if (part_job[j] == job) m = fmaxf(m, part_at(j)[R::kHeads * R::kHD + h]);
+      const float sub = m == -INFINITY ? 0.0f : m;
+      float l = 0.0f, f[kPer] = {};
+      for (int j = i; j < stop; ++j) {
+        if (part_job[j] != job) continue;
+        const float* part = part_at(j);
+        const float w = exp2_fast(part[R::kHeads * R::kHD + h] - sub);
+        l += w * part[R::kHeads * (R::kHD + 1) + h];
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) f[e] += w * part[h * R::kHD + lane * kPer + e];
+      }
+      if (whole) {
+        write(job, h, f, l);
+      } else {
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) dst[h * R::kHD + lane * kPer + e] = f[e];
+        if (lane == 0) {
+          dst[R::kHeads * R::kHD + h] = m;
+          dst[R::kHeads * (R::kHD + 1) + h] = l;
+        }
+      }
+    }
+    i = stop;
+  }
+  __threadfence();
+  __syncthreads();
+  if (tid < 2) {
+    int last = 0;
+    const int job = shared_job[tid];
+    if (job >= 0) {
+      const int first = shared_slot[tid], n = (int)((job_end(job) - 1) / share) - first + 1;
+      last = atomicAdd(a.counters + first, 1u) == (unsigned)n - 1;
+      if (last) a.counters[first] = 0;
+    }
+    merges[tid] = last;
+  }
+  __syncthreads();
+  for (int p = 0; p < 2; ++p) {
+    if (!merges[p]) continue;
+    __threadfence();
+    const int job = shared_job[p], first = shared_slot[p], n = (int)((job_end(job) - 1) / share) - first + 1;
+    const int place = job_begin(job) > first * share;
+    for (int h = warp; h < heads_of(job); h += W) {
+      auto part = [&](int j) { return a.ws + ((first + j) * 2LL + (j == 0 ? place : 0)) * kPart; };
+      float m = -INFINITY;
+      for (int j = lane; j < n; j += 32) m = fmaxf(m, __ldcg(part(j) + R::kHeads * R::kHD + h));
+      m = warp_max(m);
+      const float sub = m == -INFINITY ? 0.0f : m;
+      float l = 0.0f, f[kPer] = {};
+#pragma unroll 4
+      for (int j = 0; j < n; ++j) {
+        const float* src = part(j);
+        const float w = exp2_fast(__ldcg(src + R::kHeads * R::kHD + h) - sub);
+        l += w * __ldcg(src + R::kHeads * (R::kHD + 1) + h);
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) f[e] += w * __ldcg(src + h * R::kHD + lane * kPer + e);
+      }
+      write(job, h, f, l);
+    }
+  }
+}
+
+template <typename R, int W, int S>
+static int launch_paged(const PagedAttnArgs& a, int head_tiles, int tile_heads, bool q_vec, bool o_vec, cudaStream_t st) {
+  const size_t smem = (size_t)W * S * R::kBytes + W * (Part<R>::kFloats * 4 + R::kQueryBytes) + (a.rows + 1) * 4;
+  constexpr int kLimit = 226 << 10;
+  static SmemLimit limit;
+  const int grid = sm_count();
+  if (smem > kLimit || a.ws_floats < grid * 2LL * Part<R>::kFloats || a.num_counters < grid) return kErrTooLarge;
+  DPTB_CUDA_OK(limit.raise((const void*)paged_attention_kernel<R, W, S>, kLimit));
+  paged_attention_kernel<R, W, S><<<grid, W * 32, smem, st>>>(a, head_tiles, tile_heads, q_vec, o_vec);
+  return counted(1, (int)cudaGetLastError());
+}
+
+// ------------------------------------------------------------------------------------------------------------ any layout
 constexpr int kSimpleTile = 128;
 constexpr int kMaxHeadDim = 256;
 
@@ -106,8 +808,34 @@ extern "C" int dptb_paged_attention(const PagedAttnArgs* args, void* stream) {
   if (a.rows < 0 || a.rows > 65535 || a.heads < 0 || a.kv_heads <= 0 || a.heads % a.kv_heads || a.hd <= 0 || a.hd > kMaxHeadDim ||
       a.page <= 0 || a.width < 0 || a.pages < 0)
     return kErrBadShape;
-  const dim3 grid(a.heads, a.rows);
   auto st = static_cast<cudaStream_t>(stream);
+  const int per = a.f32 ? 4 : 8;                       // elements of a piece
+  auto whole = [&](const void* p, long long s0, long long s1, long long s2) {
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && s0 % per == 0 && s1 % per == 0 && s2 % per == 0;
+  };
+  if (a.hd % per == 0 && whole(a.k, a.k_page, a.k_head, a.k_tok) && whole(a.v, a.v_page, a.v_head, a.v_tok)) {
+    const bool qv = whole(a.q, a.q_row, a.q_head, 0), ov = whole(a.o, a.o_row, a.o_head, 0);
+    const int group = a.heads / a.kv_heads;
+    if ((long long)a.rows * ((long long)a.width * a.page / 8 + 1) >= 1LL << 31 || (long long)a.rows * a.heads >= 1LL << 31) return kErrTooLarge;
+#define DPTB_PAGED(R, W, S) return launch_paged<R, W, S>(a, (group + R::kHeads - 1) / R::kHeads, R::kHeads, qv, ov, st)
+    if (!a.f32) {
+      using B64 = Bf16Round<64, 1>; using C64 = Bf16Round<64, 2>;
+      using B128 = Bf16Round<128, 1>; using C128 = Bf16Round<128, 2>;
+      using B256 = Bf16Round<256, 1>;
+      if (a.hd <= 64) { if (group <= 8) DPTB_PAGED(B64, 8, 4); DPTB_PAGED(C64, 8, 4); }
+      if (a.hd <= 128) { if (group <= 8) DPTB_PAGED(B128, 8, 2); DPTB_PAGED(C128, 8, 2); }
+      DPTB_PAGED(B256, 4, 2);
+    }
+    using F1_64 = F32Round<64, 1>; using F4_64 = F32Round<64, 4>; using F8_64 = F32Round<64, 8>;
+    using F1_128 = F32Round<128, 1>; using F4_128 = F32Round<128, 4>; using F8_128 = F32Round<128, 8>;
+    using F1_256 = F32Round<256, 1>; using F4_256 = F32Round<256, 4>;
+    if (a.hd <= 64) { if (group == 1) DPTB_PAGED(F1_64, 8, 4); if (group <= 4) DPTB_PAGED(F4_64, 8, 4); DPTB_PAGED(F8_64, 8, 4); }
+    if (a.hd <= 128) { if (group == 1) DPTB_PAGED(F1_128, 8, 2); if (group <= 4) DPTB_PAGED(F4_128, 8, 2); DPTB_PAGED(F8_128, 8, 2); }
+    if (group == 1) DPTB_PAGED(F1_256, 4, 2);
+    DPTB_PAGED(F4_256, 4, 2);
+#undef DPTB_PAGED
+  }
+  const dim3 grid(a.heads, a.rows);
   if (a.f32) paged_attention_simple_kernel<float><<<grid, kSimpleTile, 0, st>>>(a);
   else       paged_attention_simple_kernel<__nv_bfloat16><<<grid, kSimpleTile, 0, st>>>(a);
   return counted(1, (int)cudaGetLastError());

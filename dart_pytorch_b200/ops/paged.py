@@ -20,6 +20,7 @@ from typing import Optional, Tuple, Union
 import torch
 
 from .. import _native as N
+from .kernels import splitk_workspace
 
 c_void_p, c_int, c_ll, c_float = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
 c_double = ctypes.c_double
@@ -33,7 +34,8 @@ class PagedAttnArgs(ctypes.Structure):
     _fields_ = [(n, c_void_p) for n in ("q", "k", "v", "o", "table", "lens")] + \
         [(n, c_ll) for n in ("q_row", "q_head", "o_row", "o_head", "k_page", "k_head", "k_tok", "v_page", "v_head", "v_tok",
                              "table_row")] + \
-        [(n, c_int) for n in ("rows", "heads", "kv_heads", "hd", "page", "width", "pages", "f32")] + [("scale", c_float)]
+        [(n, c_int) for n in ("rows", "heads", "kv_heads", "hd", "page", "width", "pages", "f32")] + [("scale", c_float)] + \
+        [("ws", c_void_p), ("ws_floats", c_ll), ("counters", c_void_p), ("num_counters", c_int)]
 
 
 class AppendArgs(ctypes.Structure):
@@ -166,10 +168,12 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     kp, kh, kt, _ = k_pages.stride()
     vp, vh, vt, _ = v_pages.stride()
     pages, hkv, page, _ = k_pages.shape
+    ws, counters = splitk_workspace(q.device)
     a = PagedAttnArgs(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), table.data_ptr(), lens.data_ptr(),
                       q_row, q_head, o_row, o_head, kp, kh, kt, vp, vh, vt, table.stride(0),
                       rows, heads, hkv, hd, page, table.shape[1], pages, q.dtype == torch.float32,
-                      1.0 / math.sqrt(hd) if scale is None else scale)
+                      1.0 / math.sqrt(hd) if scale is None else scale, ws.data_ptr(), ws.numel() // 4, counters.data_ptr(),
+                      counters.numel())
     N.check(_lib().dptb_paged_attention(a, N.stream_ptr()), what)
     return out
 
