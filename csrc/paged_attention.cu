@@ -48,6 +48,7 @@ struct PagedAttnArgs {
   long long ws_floats;
   unsigned* counters;  // zeroed words, one per CTA; zero again afterwards
   int num_counters;
+  int page_shift;      // of a power of two; -1 otherwise (set by the launcher)
 };
 
 // ------------------------------------------------------------------------------------------------------------ pieces
@@ -78,6 +79,9 @@ struct PageWindow {
   __device__ __forceinline__ int at(int slot) const { return __shfl_sync(0xffffffffu, entry, (slot - first) & 31); }
 };
 
+struct Yes { static constexpr bool value = true; };
+struct No { static constexpr bool value = false; };
+
 // A place in the sequence of rounds: round k of the n rounds of job (row, vh).
 struct Cursor {
   int row, vh, k, n;
@@ -91,7 +95,7 @@ constexpr float kTiny = 1.2e-38f;
 template <int HD, int NT>
 struct Bf16Round {
   using T = __nv_bfloat16;
-  static constexpr int kKeys = 16, kHeads = 8 * NT, kHD = HD;
+  static constexpr int kKeys = 16, kShift = 4, kHeads = 8 * NT, kHD = HD;
   static constexpr int kKeyPieces = 2 * (HD / 32), kValuePieces = 4 * (HD / 64);       // per lane and round
   static constexpr int kBytes = (kKeyPieces + kValuePieces) * 512;
   static constexpr int kQueryBytes = 0;
@@ -100,10 +104,43 @@ struct Bf16Round {
   float m[NT][2], l[NT][2];   // heads (lane % 4) * 2 and the next; l: of this lane's keys
   float o[NT][HD / 64][4][4]; // features 8 (lane / 4 + 8 b) + 2 i and the next, of those heads
 
+  // Requests the keys and values of a round; bit j: whether key g + 8 j is one.
   static __device__ __forceinline__ unsigned issue(const PagedAttnArgs& a, PageWindow& win, const Cursor& c, int kv, int len, uint32_t ring, int lane) {
     const T* kb = static_cast<const T*>(a.k) + kv * a.k_head;
     const T* vb = static_cast<const T*>(a.v) + kv * a.v_head;
     const int p0 = c.k * kKeys, g = lane >> 2, t = lane & 3;
+    ring += lane * 16;
+    if (a.page_shift >= kShift && p0 + kKeys <= len) {
+      // A round of one page: addresses are the page's and offsets that no round changes.  With the general form below for every
+      // round a round was 840 instructions, twice the arithmetic, and bound the kernel.
+      const int slot = p0 >> a.page_shift;
+      win.cover(a, c.row, slot, slot, (len - 1 >> a.page_shift) + 1, lane);
+      const int page = win.at(slot);
+      if ((unsigned)page < (unsigned)a.pages) {
+        const int off = p0 & ((1 << a.page_shift) - 1);
+        const T* ks = kb + page * a.k_page + off * a.k_tok + (g * a.k_tok + t * 8);
+        const T* vs = vb + page * a.v_page + off * a.v_tok + (2 * t * a.v_tok + g * 8);
+        auto pieces = [&](auto whole) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int i = 0; i < HD / 32; ++i) {
+              const bool in = decltype(whole)::value || (t + 4 * i) * 8 < a.hd;
+              copy_piece(ring + (j * (HD / 32) + i) * 512, in ? ks + j * 8 * a.k_tok + 32 * i : kb, in);
+            }
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int b = 0; b < HD / 64; ++b) {
+              const bool in = decltype(whole)::value || (g + 8 * b) * 8 < a.hd;
+              copy_piece(ring + (kKeyPieces + j * (HD / 64) + b) * 512, in ? vs + ((j & 1) + 8 * (j >> 1)) * a.v_tok + 64 * b : vb, in);
+            }
+        };
+        if (a.hd == HD) pieces(Yes{});
+        else pieces(No{});
+        return 3;
+      }
+    }
     win.cover(a, c.row, p0 / a.page, (min(p0 + kKeys, len) - 1) / a.page, (len + a.page - 1) / a.page, lane);
     unsigned live = 0;
 #pragma unroll
@@ -121,7 +158,7 @@ struct Bf16Round {
       for (int i = 0; i < HD / 32; ++i) {
         const int f = (t + 4 * i) * 8;
         const bool in = ok && f < a.hd;
-        copy_piece(ring + (j * (HD / 32) + i) * 512 + lane * 16, in ? src + f : kb, in);
+        copy_piece(ring + (j * (HD / 32) + i) * 512, in ? src + f : kb, in);
       }
     }
 #pragma unroll
@@ -134,7 +171,7 @@ struct Bf16Round {
       for (int b = 0; b < HD / 64; ++b) {
         const int f = (g + 8 * b) * 8;
         const bool in = ok && f < a.hd;
-        copy_piece(ring + (kKeyPieces + j * (HD / 64) + b) * 512 + lane * 16, in ? src + f : vb, in);
+        copy_piece(ring + (kKeyPieces + j * (HD / 64) + b) * 512, in ? src + f : vb, in);
       }
     }
     return live;
@@ -283,7 +320,7 @@ struct Bf16Round {
 template <int HD, int GP>
 struct F32Round {
   using T = float;
-  static constexpr int kKeys = 8, kHeads = GP, kHD = HD;
+  static constexpr int kKeys = 8, kShift = 3, kHeads = GP, kHD = HD;
   static constexpr int P = HD / 32;                      // pieces of a key per lane
   static constexpr int kBytes = 4 * P * 512;
   static constexpr int kQueryBytes = GP * HD * 4;
@@ -295,6 +332,30 @@ struct F32Round {
     const T* kb = static_cast<const T*>(a.k) + kv * a.k_head;
     const T* vb = static_cast<const T*>(a.v) + kv * a.v_head;
     const int p0 = c.k * kKeys, g = lane >> 3, t = lane & 7;
+    ring += lane * 16;
+    if (a.page_shift >= kShift && p0 + kKeys <= len) {       // (as in bf16)
+      const int slot = p0 >> a.page_shift;
+      win.cover(a, c.row, slot, slot, (len - 1 >> a.page_shift) + 1, lane);
+      const int page = win.at(slot);
+      if ((unsigned)page < (unsigned)a.pages) {
+        const int off = p0 & ((1 << a.page_shift) - 1);
+        const T* ks = kb + page * a.k_page + off * a.k_tok + (g * a.k_tok + t * 4);
+        const T* vs = vb + page * a.v_page + off * a.v_tok + (g * a.v_tok + t * 4);
+        auto pieces = [&](auto whole) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+              const bool in = decltype(whole)::value || (t + 8 * i) * 4 < a.hd;
+              copy_piece(ring + (j * P + i) * 512, in ? ks + j * 4 * a.k_tok + 32 * i : kb, in);
+              copy_piece(ring + ((2 + j) * P + i) * 512, in ? vs + j * 4 * a.v_tok + 32 * i : vb, in);
+            }
+        };
+        if (a.hd == HD) pieces(Yes{});
+        else pieces(No{});
+        return 3;
+      }
+    }
     win.cover(a, c.row, p0 / a.page, (min(p0 + kKeys, len) - 1) / a.page, (len + a.page - 1) / a.page, lane);
     unsigned live = 0;
 #pragma unroll
@@ -313,8 +374,8 @@ struct F32Round {
       for (int i = 0; i < P; ++i) {
         const int f = (t + 8 * i) * 4;
         const bool in = ok && f < a.hd;
-        copy_piece(ring + (j * P + i) * 512 + lane * 16, in ? ks + f : kb, in);
-        copy_piece(ring + ((2 + j) * P + i) * 512 + lane * 16, in ? vs + f : vb, in);
+        copy_piece(ring + (j * P + i) * 512, in ? ks + f : kb, in);
+        copy_piece(ring + ((2 + j) * P + i) * 512, in ? vs + f : vb, in);
       }
     }
     return live;
@@ -803,11 +864,14 @@ paged_attention_simple_kernel(const PagedAttnArgs a) {
 using namespace dptb;
 
 extern "C" int dptb_paged_attention(const PagedAttnArgs* args, void* stream) {
-  const PagedAttnArgs& a = *args;
+  PagedAttnArgs a = *args;
   if (a.rows == 0 || a.heads == 0) return 0;
   if (a.rows < 0 || a.rows > 65535 || a.heads < 0 || a.kv_heads <= 0 || a.heads % a.kv_heads || a.hd <= 0 || a.hd > kMaxHeadDim ||
       a.page <= 0 || a.width < 0 || a.pages < 0)
     return kErrBadShape;
+  a.page_shift = -1;
+  if ((a.page & (a.page - 1)) == 0)
+    for (a.page_shift = 0; 1 << a.page_shift < a.page;) ++a.page_shift;
   auto st = static_cast<cudaStream_t>(stream);
   const int per = a.f32 ? 4 : 8;                       // elements of a piece
   auto whole = [&](const void* p, long long s0, long long s1, long long s2) {
