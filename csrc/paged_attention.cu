@@ -13,10 +13,10 @@
 // of several CTAs through a workspace by the last of them to finish (a counter, no waiting; parts are added in order, so results
 // repeat to the bit).
 //
-// Loads: a lane copies the 16-byte pieces that it will itself need, in the layout of the matrix instructions' fragments, to slots of its
-// own in shared memory (cp.async, several rounds ahead, across jobs too) and reads them back alone: no barrier, no bank conflict, and any
-// strides.  The features of a fragment are dealt to the lanes in another order than the instruction's, in queries and keys alike, which a sum
-// does not notice.
+// Loads: TMA tiles of 128-byte rows, 128-byte swizzled, a ring of rounds for every warp that runs on across jobs; a few instructions a round
+// for any strides and page sizes (a page that a round does not fit into is fetched in several boxes).  The features of a fragment are dealt to
+// the lanes in another order than the matrix instruction's, and the keys of a round too, in all its operands alike, which a sum does not
+// notice: so a lane reads 16 bytes at a time, and the eight lanes of a read fall on different banks.
 //
 // bf16: S^T = K Q^T and O^T = V^T P^T by mma.sync, the group's heads as the 8 columns (two tiles of them for 9 to 16 heads); the bound is
 // the cache stream, and a tcgen05 tile of 128 rows would be padding for the most part.  The weights enter as two bf16 parts (16 bits).
@@ -52,9 +52,6 @@ struct PagedAttnArgs {
 };
 
 // ------------------------------------------------------------------------------------------------------------ pieces
-__device__ __forceinline__ void copy_piece(uint32_t smem_dst, const void* src, bool valid) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
-}
 __device__ __forceinline__ uint4 read_piece(uint32_t addr) {
   uint4 u;
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(addr) : "memory");
@@ -76,11 +73,9 @@ struct PageWindow {
       entry = slot + lane < held ? a.table[r * a.table_row + slot + lane] : -1;
     }
   }
+  // (every lane of the warp calls it)
   __device__ __forceinline__ int at(int slot) const { return __shfl_sync(0xffffffffu, entry, (slot - first) & 31); }
 };
-
-struct Yes { static constexpr bool value = true; };
-struct No { static constexpr bool value = false; };
 
 // A place in the sequence of rounds: round k of the n rounds of job (row, vh).
 struct Cursor {
@@ -95,87 +90,16 @@ constexpr float kTiny = 1.2e-38f;
 template <int HD, int NT>
 struct Bf16Round {
   using T = __nv_bfloat16;
-  static constexpr int kKeys = 16, kShift = 4, kHeads = 8 * NT, kHD = HD;
-  static constexpr int kKeyPieces = 2 * (HD / 32), kValuePieces = 4 * (HD / 64);       // per lane and round
-  static constexpr int kBytes = (kKeyPieces + kValuePieces) * 512;
+  static constexpr int kKeys = 16, kHeads = 8 * NT, kHD = HD;
+  static constexpr int kSegs = HD / 64, kSeg = kKeys * 128, kBytes = 2 * kSegs * kSeg;   // keys, then values: a tile for every 64 features
   static constexpr int kQueryBytes = 0;
 
   uint4 q[NT][HD / 32];       // head lane / 4, pieces (lane % 4) + 4 i
   float m[NT][2], l[NT][2];   // heads (lane % 4) * 2 and the next; l: of this lane's keys
-  float o[NT][HD / 64][4][4]; // features 8 (lane / 4 + 8 b) + 2 i and the next, of those heads
+  float o[NT][HD / 64][4][4]; // features 8 (order(lane / 4) + 8 b) + 2 i and the next, of those heads
 
-  // Requests the keys and values of a round; bit j: whether key g + 8 j is one.
-  static __device__ __forceinline__ unsigned issue(const PagedAttnArgs& a, PageWindow& win, const Cursor& c, int kv, int len, uint32_t ring, int lane) {
-    const T* kb = static_cast<const T*>(a.k) + kv * a.k_head;
-    const T* vb = static_cast<const T*>(a.v) + kv * a.v_head;
-    const int p0 = c.k * kKeys, g = lane >> 2, t = lane & 3;
-    ring += lane * 16;
-    if (a.page_shift >= kShift && p0 + kKeys <= len) {
-      // A round of one page: addresses are the page's and offsets that no round changes.  With the general form below for every
-      // round a round was 840 instructions, twice the arithmetic, and bound the kernel.
-      const int slot = p0 >> a.page_shift;
-      win.cover(a, c.row, slot, slot, (len - 1 >> a.page_shift) + 1, lane);
-      const int page = win.at(slot);
-      if ((unsigned)page < (unsigned)a.pages) {
-        const int off = p0 & ((1 << a.page_shift) - 1);
-        const T* ks = kb + page * a.k_page + off * a.k_tok + (g * a.k_tok + t * 8);
-        const T* vs = vb + page * a.v_page + off * a.v_tok + (2 * t * a.v_tok + g * 8);
-        auto pieces = [&](auto whole) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int i = 0; i < HD / 32; ++i) {
-              const bool in = decltype(whole)::value || (t + 4 * i) * 8 < a.hd;
-              copy_piece(ring + (j * (HD / 32) + i) * 512, in ? ks + j * 8 * a.k_tok + 32 * i : kb, in);
-            }
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int b = 0; b < HD / 64; ++b) {
-              const bool in = decltype(whole)::value || (g + 8 * b) * 8 < a.hd;
-              copy_piece(ring + (kKeyPieces + j * (HD / 64) + b) * 512, in ? vs + ((j & 1) + 8 * (j >> 1)) * a.v_tok + 64 * b : vb, in);
-            }
-        };
-        if (a.hd == HD) pieces(Yes{});
-        else pieces(No{});
-        return 3;
-      }
-    }
-    win.cover(a, c.row, p0 / a.page, (min(p0 + kKeys, len) - 1) / a.page, (len + a.page - 1) / a.page, lane);
-    unsigned live = 0;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int pos = p0 + g + 8 * j, slot = pos / a.page;
-      const int page = win.at(slot);
-      bool ok = pos < len;
-      if (ok && (unsigned)page >= (unsigned)a.pages) {
-        report_error(kBadPage);
-        ok = false;
-      }
-      live |= (unsigned)ok << j;
-      const T* src = kb + (ok ? page * a.k_page + (pos - slot * a.page) * a.k_tok : 0);
-#pragma unroll
-      for (int i = 0; i < HD / 32; ++i) {
-        const int f = (t + 4 * i) * 8;
-        const bool in = ok && f < a.hd;
-        copy_piece(ring + (j * (HD / 32) + i) * 512, in ? src + f : kb, in);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int pos = p0 + 2 * t + (j & 1) + 8 * (j >> 1), slot = pos / a.page;
-      const int page = win.at(slot);
-      const bool ok = pos < len && (unsigned)page < (unsigned)a.pages;
-      const T* src = vb + (ok ? page * a.v_page + (pos - slot * a.page) * a.v_tok : 0);
-#pragma unroll
-      for (int b = 0; b < HD / 64; ++b) {
-        const int f = (g + 8 * b) * 8;
-        const bool in = ok && f < a.hd;
-        copy_piece(ring + (kKeyPieces + j * (HD / 64) + b) * 512, in ? src + f : vb, in);
-      }
-    }
-    return live;
-  }
+  // Which key of a half round is row i of a fragment, and which piece of 8 features a lane takes: neighbours in a read differ in bit 2.
+  static __device__ __forceinline__ int order(int i) { return i >> 1 | (i & 1) << 2; }
 
   // The queries of heads head0 .. head0 + count of a row.
   __device__ __forceinline__ void start(const PagedAttnArgs& a, int row, int head0, int count, bool vec, float*, int lane) {
@@ -214,11 +138,17 @@ struct Bf16Round {
     }
   }
 
-  __device__ __forceinline__ void compute(const PagedAttnArgs& a, uint32_t ring, unsigned live, float scale2, const float*, int lane) {
+  // `keys`: bit j, whether key j of the round is one.
+  __device__ __forceinline__ void compute(uint32_t ring, unsigned keys, float scale2, const float*, int lane) {
+    const int t = lane & 3, mine = order(lane >> 2);
+    const uint32_t swz = (mine ^ t) << 4;              // piece t of row `mine`, and piece `mine` of row t
+    const uint32_t kr = ring + mine * 128, vr = ring + kSegs * kSeg + t * 128;
+    const unsigned live = keys >> mine & 1 | (keys >> (mine + 8) & 1) << 1;
     float sc[NT][2][4] = {};
 #pragma unroll
     for (int i = 0; i < HD / 32; ++i) {
-      const uint4 k0 = read_piece(ring + i * 512 + lane * 16), k1 = read_piece(ring + (HD / 32 + i) * 512 + lane * 16);
+      const uint32_t at = kr + (i >> 1) * kSeg + (swz ^ (i & 1) << 6);
+      const uint4 k0 = read_piece(at), k1 = read_piece(at + 1024);
       const uint32_t fa[4] = {k0.x, k1.x, k0.y, k1.y}, fb[4] = {k0.z, k1.z, k0.w, k1.w};
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -270,7 +200,7 @@ struct Bf16Round {
       uint32_t v[4][4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint4 u = read_piece(ring + (kKeyPieces + j * (HD / 64) + b) * 512 + lane * 16);
+        const uint4 u = read_piece(vr + b * kSeg + j * 512 + (swz ^ (j & 1) << 6));       // keys t, t + 4, t + 8, t + 12
         v[j][0] = u.x; v[j][1] = u.y; v[j][2] = u.z; v[j][3] = u.w;
       }
 #pragma unroll
@@ -309,7 +239,7 @@ struct Bf16Round {
             f[2 * i] = o[n][b][i][e];
             f[2 * i + 1] = o[n][b][i][2 + e];
           }
-          put(n * 8 + (lane & 3) * 2 + e, 8 * ((lane >> 2) + 8 * b), f, m[n][e], l[n][e]);
+          put(n * 8 + (lane & 3) * 2 + e, 8 * (order(lane >> 2) + 8 * b), f, m[n][e], l[n][e]);
         }
   }
 };
@@ -320,66 +250,13 @@ struct Bf16Round {
 template <int HD, int GP>
 struct F32Round {
   using T = float;
-  static constexpr int kKeys = 8, kShift = 3, kHeads = GP, kHD = HD;
+  static constexpr int kKeys = 8, kHeads = GP, kHD = HD;
   static constexpr int P = HD / 32;                      // pieces of a key per lane
-  static constexpr int kBytes = 4 * P * 512;
+  static constexpr int kSegs = P, kSeg = kKeys * 128, kBytes = 2 * kSegs * kSeg;         // a tile for every 32 features
   static constexpr int kQueryBytes = GP * HD * 4;
 
   float m[GP], l[GP];
   float4 o[GP][P];
-
-  static __device__ __forceinline__ unsigned issue(const PagedAttnArgs& a, PageWindow& win, const Cursor& c, int kv, int len, uint32_t ring, int lane) {
-    const T* kb = static_cast<const T*>(a.k) + kv * a.k_head;
-    const T* vb = static_cast<const T*>(a.v) + kv * a.v_head;
-    const int p0 = c.k * kKeys, g = lane >> 3, t = lane & 7;
-    ring += lane * 16;
-    if (a.page_shift >= kShift && p0 + kKeys <= len) {       // (as in bf16)
-      const int slot = p0 >> a.page_shift;
-      win.cover(a, c.row, slot, slot, (len - 1 >> a.page_shift) + 1, lane);
-      const int page = win.at(slot);
-      if ((unsigned)page < (unsigned)a.pages) {
-        const int off = p0 & ((1 << a.page_shift) - 1);
-        const T* ks = kb + page * a.k_page + off * a.k_tok + (g * a.k_tok + t * 4);
-        const T* vs = vb + page * a.v_page + off * a.v_tok + (g * a.v_tok + t * 4);
-        auto pieces = [&](auto whole) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int i = 0; i < P; ++i) {
-              const bool in = decltype(whole)::value || (t + 8 * i) * 4 < a.hd;
-              copy_piece(ring + (j * P + i) * 512, in ? ks + j * 4 * a.k_tok + 32 * i : kb, in);
-              copy_piece(ring + ((2 + j) * P + i) * 512, in ? vs + j * 4 * a.v_tok + 32 * i : vb, in);
-            }
-        };
-        if (a.hd == HD) pieces(Yes{});
-        else pieces(No{});
-        return 3;
-      }
-    }
-    win.cover(a, c.row, p0 / a.page, (min(p0 + kKeys, len) - 1) / a.page, (len + a.page - 1) / a.page, lane);
-    unsigned live = 0;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int pos = p0 + g + 4 * j, slot = pos / a.page;
-      const int page = win.at(slot);
-      bool ok = pos < len;
-      if (ok && (unsigned)page >= (unsigned)a.pages) {
-        report_error(kBadPage);
-        ok = false;
-      }
-      live |= (unsigned)ok << j;
-      const T* ks = kb + (ok ? page * a.k_page + (pos - slot * a.page) * a.k_tok : 0);
-      const T* vs = vb + (ok ? page * a.v_page + (pos - slot * a.page) * a.v_tok : 0);
-#pragma unroll
-      for (int i = 0; i < P; ++i) {
-        const int f = (t + 8 * i) * 4;
-        const bool in = ok && f < a.hd;
-        copy_piece(ring + (j * P + i) * 512, in ? ks + f : kb, in);
-        copy_piece(ring + ((2 + j) * P + i) * 512, in ? vs + f : vb, in);
-      }
-    }
-    return live;
-  }
 
   __device__ __forceinline__ void start(const PagedAttnArgs& a, int row, int head0, int count, bool, float* queries, int lane) {
     __syncwarp();
@@ -397,7 +274,13 @@ struct F32Round {
     }
   }
 
-  __device__ __forceinline__ void compute(const PagedAttnArgs& a, uint32_t ring, unsigned live, float scale2, const float* queries, int lane) {
+  __device__ __forceinline__ void compute(uint32_t ring, unsigned keys, float scale2, const float* queries, int lane) {
+    const int g = lane >> 3, t = lane & 7;
+    const unsigned live = keys >> g & 1 | (keys >> (g + 4) & 1) << 1;
+    auto piece = [&](int seg, int j) {                   // of key g + 4 j
+      const int key = g + 4 * j;
+      return read_piece(ring + seg * kSeg + key * 128 + ((t ^ key) << 4));
+    };
     const float4* q4 = reinterpret_cast<const float4*>(queries) + (lane & 7);
     float p[GP][2];
 #pragma unroll
@@ -405,7 +288,7 @@ struct F32Round {
       float4 k[P];
 #pragma unroll
       for (int i = 0; i < P; ++i) {
-        const uint4 u = read_piece(ring + (j * P + i) * 512 + lane * 16);
+        const uint4 u = piece(i, j);
         k[i] = make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w));
       }
 #pragma unroll
@@ -459,7 +342,7 @@ struct F32Round {
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int i = 0; i < P; ++i) {
-        const uint4 u = read_piece(ring + ((2 + j) * P + i) * 512 + lane * 16);
+        const uint4 u = piece(kSegs + i, j);
 #pragma unroll
         for (int h = 0; h < GP; ++h) {
           o[h][i].x = fmaf(p[h][j], __uint_as_float(u.x), o[h][i].x);
@@ -505,6 +388,40 @@ struct Part {
   static constexpr int kFloats = (R::kHeads * (R::kHD + 2) + 3) / 4 * 4;
 };
 
+struct PageMaps {
+  CUtensorMap k, v;      // (feature, token of the page, head, page)
+};
+
+// Requests the keys and values of round c; returns which of its keys there are.
+template <typename R>
+__device__ __forceinline__ unsigned issue_round(const PagedAttnArgs& a, const PageMaps& maps, PageWindow& win, const Cursor& c, int kv, int len, int box_shift,
+                                                unsigned char* ring, uint64_t* bar, int lane) {
+  const int p0 = c.k * R::kKeys, end = min(p0 + R::kKeys, len);
+  const bool pow2 = a.page_shift >= 0;
+  auto slot_of = [&](int pos) { return pow2 ? pos >> a.page_shift : pos / a.page; };
+  win.cover(a, c.row, slot_of(p0), slot_of(end - 1), slot_of(len - 1) + 1, lane);
+  if (lane == 0) mbar_arrive_expect_tx(bar, R::kBytes);
+  const int pos = p0 + (lane & (R::kKeys - 1));
+  const unsigned mine = win.at(slot_of(pos));
+  const bool bad = pos < end && mine >= (unsigned)a.pages;
+  if (bad) report_error(kBadPage);
+  const unsigned keys = __ballot_sync(0xffffffffu, pos < end && !bad) & ((1u << R::kKeys) - 1);      // (orders the lanes before the copies too)
+  const int per = (R::kKeys >> box_shift), boxes = per * 2 * R::kSegs;
+  for (int b0 = 0; b0 < boxes; b0 += 32) {
+    const int b = b0 + lane, first = (b & (per - 1)) << box_shift, tile = b / per;
+    const int slot = slot_of(p0 + first);
+    int page = win.at(slot);
+    if ((unsigned)page >= (unsigned)a.pages) page = a.pages;                                            // beyond the pool: zeros
+    if (b < boxes) {
+      const int tok = pow2 ? (p0 + first) & (a.page - 1) : p0 + first - slot * a.page;
+      const bool is_v = tile >= R::kSegs;
+      const int x = (is_v ? tile - R::kSegs : tile) * (128 / (int)sizeof(typename R::T));
+      tma_load_4d(ring + tile * R::kSeg + first * 128, is_v ? &maps.v : &maps.k, bar, x, tok, kv, page);
+    }
+  }
+  return keys;
+}
+
 template <typename T, int N>
 __device__ __forceinline__ void store_out(T* dst, const float (&f)[N], float by, int valid, bool vec) {
   T e[N];
@@ -524,18 +441,20 @@ __device__ __forceinline__ void store_out(T* dst, const float (&f)[N], float by,
 // W warps, S rounds of a warp in flight or in use.
 template <typename R, int W, int S>
 __global__ void __launch_bounds__(W * 32, 1)
-paged_attention_kernel(const PagedAttnArgs a, int head_tiles, int tile_heads, int q_vec, int o_vec) {
+paged_attention_kernel(const PagedAttnArgs a, const __grid_constant__ PageMaps maps, int box_shift, int head_tiles, int tile_heads, int q_vec, int o_vec) {
   using T = typename R::T;
   constexpr int kPart = Part<R>::kFloats;
   static_assert(S * R::kBytes >= kPart * 4, "a warp's ring holds its last part");
-  extern __shared__ __align__(16) unsigned char smem[];
-  unsigned char* rings = smem;                                              // [W][S] rounds
+  extern __shared__ unsigned char smem[];
+  unsigned char* rings = smem + (1024 - (smem_u32(smem) & 1023) & 1023);      // [W][S] rounds
   float* leads = reinterpret_cast<float*>(rings + W * S * R::kBytes);       // [W] parts
   float* queries = leads + W * kPart;                                       // [W] copies of the queries
   int* before = reinterpret_cast<int*>(queries + W * (R::kQueryBytes / 4)); // [rows + 1]: rounds of a kv head ahead of a row
   __shared__ int scan[W + 1];
   __shared__ int part_job[2 * W];
   __shared__ int shared_job[2], shared_slot[2], merges[2];
+  __shared__ uint64_t landed[W * S];
+  __shared__ int aborted;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int tiles = a.kv_heads * head_tiles;                                // jobs of a row
   const int room = (int)min((long long)a.width * a.page, 0x7fffffffLL);
@@ -572,6 +491,9 @@ paged_attention_kernel(const PagedAttnArgs a, int head_tiles, int tile_heads, in
     }
     if (tid < 2 * W) part_job[tid] = -1;
     if (tid < 2) shared_job[tid] = -1;
+    if (tid < W * S) mbar_init(landed + tid, 1);
+    if (tid == 0) aborted = 0;
+    mbar_fence_init();
     __syncthreads();
   }
   const long long total = (long long)before[a.rows] * tiles;
@@ -588,7 +510,8 @@ paged_attention_kernel(const PagedAttnArgs a, int head_tiles, int tile_heads, in
   const long long w0 = min(end, begin + quota * warp), w1 = min(end, w0 + quota);
   int todo = (int)(w1 - w0);
   if (todo > 0) {
-    const uint32_t ring = smem_u32(rings) + warp * S * R::kBytes;
+    unsigned char* ring = rings + warp * S * R::kBytes;
+    uint64_t* bars = landed + warp * S;
     float* my_queries = queries + warp * (R::kQueryBytes / 4);
     int row = 0;
     {
@@ -613,7 +536,7 @@ paged_attention_kernel(const PagedAttnArgs a, int head_tiles, int tile_heads, in
       if (x.row < a.rows) x.n = before[x.row + 1] - before[x.row];
     };
     PageWindow win;
-    unsigned lives = 0;                                        // two bits for each round of the ring
+    unsigned long long there = 0;                              // 16 bits for each round of the ring: its keys
     int left = todo, put = 0, take = 0, len = length(row), len_row = row;
     auto fetch = [&] {
       if (left > 0) {
@@ -621,19 +544,19 @@ paged_attention_kernel(const PagedAttnArgs a, int head_tiles, int tile_heads, in
           len_row = ahead.row;
           len = length(len_row);
         }
-        const unsigned live = R::issue(a, win, ahead, ahead.vh / head_tiles, len, ring + put * R::kBytes, lane);
-        lives = (lives & ~(3u << (2 * put))) | live << (2 * put);
+        const unsigned keys = issue_round<R>(a, maps, win, ahead, ahead.vh / head_tiles, len, box_shift, ring + put * R::kBytes, bars + put, lane);
+        there = (there & ~(0xffffull << (16 * put))) | (unsigned long long)keys << (16 * put);
         put = put + 1 == S ? 0 : put + 1;
         --left;
         if (left > 0) advance(ahead);
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
     };
 #pragma unroll
     for (int s = 0; s < S - 1; ++s) fetch();
     const float scale2 = a.scale * kLog2e;
     R x;
     int from = c.k;
+    uint32_t phase = 0;
     bool fresh = true, first = true;
     for (; todo > 0; --todo) {
       fetch();
@@ -644,9 +567,22 @@ paged_attention_kernel(const PagedAttnArgs a, int head_tiles, int tile_heads, in
         from = c.k;
         fresh = false;
       }
-      asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory");
-      x.compute(a, ring + take * R::kBytes, lives >> (2 * take) & 3, scale2, my_queries, lane);
-      take = take + 1 == S ? 0 : take + 1;
+      mbar_wait(bars + take, phase, &aborted, kWaitFullTimeout);
+      const unsigned keys = (unsigned)(there >> (16 * take)) & 0xffffu;
+      if (keys != (1u << R::kKeys) - 1) {
+        // What lies where no key is may be NaN: a weight of zero times a value of zero instead.
+        unsigned char* values = ring + take * R::kBytes + R::kSegs * R::kSeg;
+        for (int i = lane; i < R::kSegs * R::kKeys * 8; i += 32)
+          if (!(keys >> (i >> 3 & (R::kKeys - 1)) & 1)) reinterpret_cast<uint4*>(values)[i] = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();                              // ahead of the copy that reuses the place
+        __syncwarp();
+      }
+      x.compute(smem_u32(ring) + take * R::kBytes, keys, scale2, my_queries, lane);
+      __syncwarp();
+      if (++take == S) {
+        take = 0;
+        phase ^= 1;
+      }
       const bool last = c.k + 1 == c.n;
       if (last || todo == 1) {
         x.finish(lane);
@@ -658,7 +594,6 @@ paged_attention_kernel(const PagedAttnArgs a, int head_tiles, int tile_heads, in
         } else {
           const int at = 2 * warp + (first ? 0 : 1);
           float* part = first ? leads + warp * kPart : reinterpret_cast<float*>(rings + warp * S * R::kBytes);
-          if (!first) asm volatile("cp.async.wait_all;" ::: "memory");
           __syncwarp();
           x.each(lane, [&](int h, int f, const auto& v, float m, float l) {
             if (h >= count) return;
@@ -780,15 +715,26 @@ paged_attention_kernel(const PagedAttnArgs a, int head_tiles, int tile_heads, in
   }
 }
 
+// Map of the pages [pages, kv_heads, page, hd]: tiles of 128 bytes of `box` tokens.
+static int map_pages(CUtensorMap* map, const PagedAttnArgs& a, const void* base, long long page, long long head, long long tok, int box) {
+  const uint64_t e = a.f32 ? 4 : 2;
+  const uint64_t dims[4] = {(uint64_t)a.hd, (uint64_t)a.page, (uint64_t)a.kv_heads, (uint64_t)a.pages};
+  const uint64_t strides[3] = {tok * e, head * e, page * e};
+  const uint32_t boxes[4] = {(uint32_t)(128 / e), (uint32_t)box, 1, 1};
+  return encode_tmap_nd(map, a.f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, 4, dims, strides, boxes);
+}
+
 template <typename R, int W, int S>
-static int launch_paged(const PagedAttnArgs& a, int head_tiles, int tile_heads, bool q_vec, bool o_vec, cudaStream_t st) {
-  const size_t smem = (size_t)W * S * R::kBytes + W * (Part<R>::kFloats * 4 + R::kQueryBytes) + (a.rows + 1) * 4;
+static int launch_paged(const PagedAttnArgs& a, const PageMaps& maps, int head_tiles, int tile_heads, bool q_vec, bool o_vec, cudaStream_t st) {
+  const size_t smem = 1024 + (size_t)W * S * R::kBytes + W * (Part<R>::kFloats * 4 + R::kQueryBytes) + (a.rows + 1) * 4;
   constexpr int kLimit = 226 << 10;
   static SmemLimit limit;
   const int grid = sm_count();
   if (smem > kLimit || a.ws_floats < grid * 2LL * Part<R>::kFloats || a.num_counters < grid) return kErrTooLarge;
   DPTB_CUDA_OK(limit.raise((const void*)paged_attention_kernel<R, W, S>, kLimit));
-  paged_attention_kernel<R, W, S><<<grid, W * 32, smem, st>>>(a, head_tiles, tile_heads, q_vec, o_vec);
+  int box_shift = 0;
+  while (2 << box_shift <= R::kKeys && a.page % (2 << box_shift) == 0) ++box_shift;
+  paged_attention_kernel<R, W, S><<<grid, W * 32, smem, st>>>(a, maps, box_shift, head_tiles, tile_heads, q_vec, o_vec);
   return counted(1, (int)cudaGetLastError());
 }
 
@@ -877,11 +823,15 @@ extern "C" int dptb_paged_attention(const PagedAttnArgs* args, void* stream) {
   auto whole = [&](const void* p, long long s0, long long s1, long long s2) {
     return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && s0 % per == 0 && s1 % per == 0 && s2 % per == 0;
   };
-  if (a.hd % per == 0 && whole(a.k, a.k_page, a.k_head, a.k_tok) && whole(a.v, a.v_page, a.v_head, a.v_tok)) {
+  PageMaps maps;
+  int box = 1;
+  while (2 * box <= (a.f32 ? 8 : 16) && a.page % (2 * box) == 0) box *= 2;
+  if (a.hd % per == 0 && whole(a.k, a.k_page, a.k_head, a.k_tok) && whole(a.v, a.v_page, a.v_head, a.v_tok) &&
+      map_pages(&maps.k, a, a.k, a.k_page, a.k_head, a.k_tok, box) == 0 && map_pages(&maps.v, a, a.v, a.v_page, a.v_head, a.v_tok, box) == 0) {
     const bool qv = whole(a.q, a.q_row, a.q_head, 0), ov = whole(a.o, a.o_row, a.o_head, 0);
     const int group = a.heads / a.kv_heads;
     if ((long long)a.rows * ((long long)a.width * a.page / 8 + 1) >= 1LL << 31 || (long long)a.rows * a.heads >= 1LL << 31) return kErrTooLarge;
-#define DPTB_PAGED(R, W, S) return launch_paged<R, W, S>(a, (group + R::kHeads - 1) / R::kHeads, R::kHeads, qv, ov, st)
+#define DPTB_PAGED(R, W, S) return launch_paged<R, W, S>(a, maps, (group + R::kHeads - 1) / R::kHeads, R::kHeads, qv, ov, st)
     if (!a.f32) {
       using B64 = Bf16Round<64, 1>; using C64 = Bf16Round<64, 2>;
       using B128 = Bf16Round<128, 1>; using C128 = Bf16Round<128, 2>;
