@@ -48,8 +48,12 @@ struct PagedAttnArgs {
   long long ws_floats;
   unsigned* counters;  // zeroed words, one per CTA; zero again afterwards
   int num_counters;
-  int page_shift;      // of a power of two; -1 otherwise (set by the launcher)
+  // pos / page = pos * page_mul >> page_shift for 0 <= pos < 2^31 (set by the launcher): page_mul = ceil(2^page_shift / page) with
+  // 2^(page_shift - 31) >= page, so the excess of page_mul adds less than 2^31 * page / 2^page_shift <= 1 quotient's last place.
+  unsigned page_mul, page_shift;
 };
+
+__device__ __forceinline__ int slot_of(const PagedAttnArgs& a, int pos) { return (int)((unsigned long long)pos * a.page_mul >> a.page_shift); }
 
 // ------------------------------------------------------------------------------------------------------------ pieces
 __device__ __forceinline__ uint4 read_piece(uint32_t addr) {
@@ -66,20 +70,20 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // What of a round a lane looks up: the page of a position, from a window of 32 table entries that the lanes hold.
 struct PageWindow {
   int row = -1, first = 0, entry = -1;
-  __device__ __forceinline__ void cover(const PagedAttnArgs& a, int r, int slot, int last, int held, int lane) {
+  __device__ __forceinline__ void cover(const PagedAttnArgs& a, int r, int slot, int last, int len, int lane) {
     if (r != row || slot < first || last >= first + 32) {
       row = r;
       first = slot;
-      entry = slot + lane < held ? a.table[r * a.table_row + slot + lane] : -1;
+      entry = slot + lane <= slot_of(a, len - 1) ? a.table[r * a.table_row + slot + lane] : -1;
     }
   }
   // (every lane of the warp calls it)
   __device__ __forceinline__ int at(int slot) const { return __shfl_sync(0xffffffffu, entry, (slot - first) & 31); }
 };
 
-// A place in the sequence of rounds: round k of the n rounds of job (row, vh).
+// A place in the sequence of rounds: round k of the n rounds of job (row, vh); vh counts kv heads and within them tiles of query heads.
 struct Cursor {
-  int row, vh, k, n;
+  int row, vh, k, n, kv;
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -90,7 +94,7 @@ constexpr float kTiny = 1.2e-38f;
 template <int HD, int NT>
 struct Bf16Round {
   using T = __nv_bfloat16;
-  static constexpr int kKeys = 16, kHeads = 8 * NT, kHD = HD;
+  static constexpr int kKeys = 16, kKeyShift = 4, kHeads = 8 * NT, kHD = HD;
   static constexpr int kSegs = HD / 64, kSeg = kKeys * 128, kBytes = 2 * kSegs * kSeg;   // keys, then values: a tile for every 64 features
   static constexpr int kQueryBytes = 0;
 
@@ -250,7 +254,7 @@ struct Bf16Round {
 template <int HD, int GP>
 struct F32Round {
   using T = float;
-  static constexpr int kKeys = 8, kHeads = GP, kHD = HD;
+  static constexpr int kKeys = 8, kKeyShift = 3, kHeads = GP, kHD = HD;
   static constexpr int P = HD / 32;                      // pieces of a key per lane
   static constexpr int kSegs = P, kSeg = kKeys * 128, kBytes = 2 * kSegs * kSeg;         // a tile for every 32 features
   static constexpr int kQueryBytes = GP * HD * 4;
@@ -394,29 +398,40 @@ struct PageMaps {
 
 // Requests the keys and values of round c; returns which of its keys there are.
 template <typename R>
-__device__ __forceinline__ unsigned issue_round(const PagedAttnArgs& a, const PageMaps& maps, PageWindow& win, const Cursor& c, int kv, int len, int box_shift,
+__device__ __forceinline__ unsigned issue_round(const PagedAttnArgs& a, const PageMaps& maps, PageWindow& win, const Cursor& c, int len, int box_shift,
                                                 unsigned char* ring, uint64_t* bar, int lane) {
-  const int p0 = c.k * R::kKeys, end = min(p0 + R::kKeys, len);
-  const bool pow2 = a.page_shift >= 0;
-  auto slot_of = [&](int pos) { return pow2 ? pos >> a.page_shift : pos / a.page; };
-  win.cover(a, c.row, slot_of(p0), slot_of(end - 1), slot_of(len - 1) + 1, lane);
+  const int p0 = c.k * R::kKeys, slot0 = slot_of(a, p0);
+  if (2 << box_shift > R::kKeys && p0 + R::kKeys <= len) {       // a full round of one page, a box for each tile
+    win.cover(a, c.row, slot0, slot0, len, lane);
+    const int page = win.at(slot0);
+    if ((unsigned)page < (unsigned)a.pages) {
+      if (lane == 0) mbar_arrive_expect_tx(bar, R::kBytes);
+      __syncwarp();
+      if (lane < 2 * R::kSegs) {
+        const bool is_v = lane >= R::kSegs;
+        tma_load_4d(ring + lane * R::kSeg, is_v ? &maps.v : &maps.k, bar, (lane & (R::kSegs - 1)) * (128 / (int)sizeof(typename R::T)), p0 - slot0 * a.page, c.kv, page);
+      }
+      return (1u << R::kKeys) - 1;
+    }
+  }
+  const int end = min(p0 + R::kKeys, len);
+  win.cover(a, c.row, slot0, slot_of(a, end - 1), len, lane);
   if (lane == 0) mbar_arrive_expect_tx(bar, R::kBytes);
   const int pos = p0 + (lane & (R::kKeys - 1));
-  const unsigned mine = win.at(slot_of(pos));
+  const unsigned mine = win.at(slot_of(a, pos));
   const bool bad = pos < end && mine >= (unsigned)a.pages;
   if (bad) report_error(kBadPage);
   const unsigned keys = __ballot_sync(0xffffffffu, pos < end && !bad) & ((1u << R::kKeys) - 1);      // (orders the lanes before the copies too)
-  const int per = (R::kKeys >> box_shift), boxes = per * 2 * R::kSegs;
+  const int per_shift = R::kKeyShift - box_shift, boxes = 2 * R::kSegs << per_shift;
   for (int b0 = 0; b0 < boxes; b0 += 32) {
-    const int b = b0 + lane, first = (b & (per - 1)) << box_shift, tile = b / per;
-    const int slot = slot_of(p0 + first);
+    const int b = b0 + lane, first = (b & ((1 << per_shift) - 1)) << box_shift, tile = b >> per_shift;
+    const int slot = slot_of(a, p0 + first);
     int page = win.at(slot);
     if ((unsigned)page >= (unsigned)a.pages) page = a.pages;                                            // beyond the pool: zeros
     if (b < boxes) {
-      const int tok = pow2 ? (p0 + first) & (a.page - 1) : p0 + first - slot * a.page;
       const bool is_v = tile >= R::kSegs;
-      const int x = (is_v ? tile - R::kSegs : tile) * (128 / (int)sizeof(typename R::T));
-      tma_load_4d(ring + tile * R::kSeg + first * 128, is_v ? &maps.v : &maps.k, bar, x, tok, kv, page);
+      tma_load_4d(ring + tile * R::kSeg + first * 128, is_v ? &maps.v : &maps.k, bar, (tile & (R::kSegs - 1)) * (128 / (int)sizeof(typename R::T)),
+                  p0 + first - slot * a.page, c.kv, page);
     }
   }
   return keys;
@@ -438,6 +453,21 @@ __device__ __forceinline__ void store_out(T* dst, const float (&f)[N], float by,
     if (i < valid) dst[i] = e[i];
 }
 
+// Values that other CTAs have written.
+template <int N>
+__device__ __forceinline__ void load_l2(const float* p, float (&v)[N]) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const float4 u = __ldcg(reinterpret_cast<const float4*>(p + i));
+      v[i] = u.x; v[i + 1] = u.y; v[i + 2] = u.z; v[i + 3] = u.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = __ldcg(p + i);
+  }
+}
+
 // W warps, S rounds of a warp in flight or in use.
 template <typename R, int W, int S>
 __global__ void __launch_bounds__(W * 32, 1)
@@ -451,8 +481,9 @@ paged_attention_kernel(const PagedAttnArgs a, const __grid_constant__ PageMaps m
   float* queries = leads + W * kPart;                                       // [W] copies of the queries
   int* before = reinterpret_cast<int*>(queries + W * (R::kQueryBytes / 4)); // [rows + 1]: rounds of a kv head ahead of a row
   __shared__ int scan[W + 1];
-  __shared__ int part_job[2 * W];
-  __shared__ int shared_job[2], shared_slot[2], merges[2];
+  __shared__ int part_job[2 * W], part_row[2 * W], part_head[2 * W], part_count[2 * W], part_rounds[2 * W];
+  __shared__ long long part_begin[2 * W];
+  __shared__ int shared_part[2], merges[2];      // jobs of several CTAs: one of their parts here, or -1
   __shared__ uint64_t landed[W * S];
   __shared__ int aborted;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -462,13 +493,17 @@ paged_attention_kernel(const PagedAttnArgs a, const __grid_constant__ PageMaps m
 
   // Rounds ahead of every row.
   auto length = [&](int r) { return max(0, min(a.lens[r], room)); };
+  bool equal = true;
+  int rounds0;
   {
     const int each = (a.rows + W * 32 - 1) / (W * 32), r0 = min(a.rows, tid * each), r1 = min(a.rows, r0 + each);
     int mine = 0;
+    rounds0 = (length(0) + R::kKeys - 1) / R::kKeys;
     for (int r = r0; r < r1; ++r) {
-      const int n = a.lens[r];
+      const int n = a.lens[r], k = (max(0, min(n, room)) + R::kKeys - 1) / R::kKeys;
       if (n > room && blockIdx.x == 0) report_error(kBadPage);
-      mine += (max(0, min(n, room)) + R::kKeys - 1) / R::kKeys;
+      mine += k;
+      equal = equal && k == rounds0;
     }
     int s = mine;
 #pragma unroll
@@ -490,15 +525,18 @@ paged_attention_kernel(const PagedAttnArgs a, const __grid_constant__ PageMaps m
       before[a.rows] = t;
     }
     if (tid < 2 * W) part_job[tid] = -1;
-    if (tid < 2) shared_job[tid] = -1;
+    if (tid < 2) shared_part[tid] = -1;
     if (tid < W * S) mbar_init(landed + tid, 1);
     if (tid == 0) aborted = 0;
     mbar_fence_init();
-    __syncthreads();
+    equal = __syncthreads_and(equal);
   }
   const long long total = (long long)before[a.rows] * tiles;
-  // A CTA takes a round for each of its warps at least: parts of one CTA are joined sooner than those of several.
-  const long long share = max((long long)W, (total + gridDim.x - 1) / gridDim.x);
+  // A CTA takes a round for each of its warps at least: parts of one CTA are joined sooner than those of several.  Whole jobs, where all
+  // are as long and short enough that each CTA still has its own at once.
+  long long share = total < 1LL << 31 ? (long long)((unsigned)(total + gridDim.x - 1) / gridDim.x) : (total + gridDim.x - 1) / gridDim.x;
+  if (equal && rounds0 > 0 && rounds0 <= 2 * W && (long long)a.rows * tiles <= gridDim.x) share = rounds0 < W / 2 && share < W ? W / rounds0 * rounds0 : rounds0;
+  else share = max((long long)W, share);
   const long long begin = min(total, share * blockIdx.x), end = min(total, begin + share);
   for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {       // rows of no tokens
     if (before[r + 1] > before[r]) continue;
@@ -524,12 +562,14 @@ paged_attention_kernel(const PagedAttnArgs a, const __grid_constant__ PageMaps m
     }
     const int n0 = before[row + 1] - before[row];
     const int rem = (int)(w0 - (long long)before[row] * tiles);
-    Cursor c{row, rem / n0, rem % n0, n0}, ahead = c;
+    Cursor c{row, rem / n0, rem % n0, n0, rem / n0 / head_tiles}, ahead = c;
     auto advance = [&](Cursor& x) {
       if (++x.k < x.n) return;
       x.k = 0;
-      if (++x.vh < tiles) return;
-      x.vh = 0;
+      ++x.vh;
+      x.kv = head_tiles == 1 ? x.vh : x.vh / head_tiles;
+      if (x.vh < tiles) return;
+      x.vh = x.kv = 0;
       do {
         ++x.row;
       } while (x.row < a.rows && before[x.row + 1] == before[x.row]);
@@ -544,7 +584,7 @@ paged_attention_kernel(const PagedAttnArgs a, const __grid_constant__ PageMaps m
           len_row = ahead.row;
           len = length(len_row);
         }
-        const unsigned keys = issue_round<R>(a, maps, win, ahead, ahead.vh / head_tiles, len, box_shift, ring + put * R::kBytes, bars + put, lane);
+        const unsigned keys = issue_round<R>(a, maps, win, ahead, len, box_shift, ring + put * R::kBytes, bars + put, lane);
         there = (there & ~(0xffffull << (16 * put))) | (unsigned long long)keys << (16 * put);
         put = put + 1 == S ? 0 : put + 1;
         --left;
@@ -555,14 +595,15 @@ paged_attention_kernel(const PagedAttnArgs a, const __grid_constant__ PageMaps m
     for (int s = 0; s < S - 1; ++s) fetch();
     const float scale2 = a.scale * kLog2e;
     R x;
-    int from = c.k;
+    int from = c.k, head0 = 0, count = 0;
     uint32_t phase = 0;
     bool fresh = true, first = true;
     for (; todo > 0; --todo) {
       fetch();
-      const int head0 = c.vh / head_tiles * group + c.vh % head_tiles * tile_heads;
-      const int count = min(tile_heads, group - c.vh % head_tiles * tile_heads);
       if (fresh) {
+        const int tile = c.vh - c.kv * head_tiles;
+        head0 = c.kv * group + tile * tile_heads;
+        count = min(tile_heads, group - tile * tile_heads);
         x.start(a, c.row, head0, count, q_vec, my_queries, lane);
         from = c.k;
         fresh = false;
@@ -605,7 +646,14 @@ paged_attention_kernel(const PagedAttnArgs a, const __grid_constant__ PageMaps m
               part[R::kHeads * (R::kHD + 1) + h] = l;
             }
           });
-          if (lane == 0) part_job[at] = c.row * tiles + c.vh;
+          if (lane == 0) {
+            part_job[at] = c.row * tiles + c.vh;
+            part_row[at] = c.row;
+            part_head[at] = head0;
+            part_count[at] = count;
+            part_begin[at] = (long long)before[c.row] * tiles + (long long)c.vh * c.n;
+            part_rounds[at] = c.n;
+          }
         }
         fresh = true;
         first = false;
@@ -615,102 +663,103 @@ paged_attention_kernel(const PagedAttnArgs a, const __grid_constant__ PageMaps m
   }
   __syncthreads();
 
-  // Parts of a job in this CTA are neighbours.  A job that lies within the CTA is written out, another's part goes to the workspace: place 0
-  // of the CTA for the job of its first round, 1 for one that begins later.
+  // Parts of a job that lies within the CTA are joined and written out; another's go to the workspace as one: place 0 of the CTA for the
+  // job of its first round, 1 for one that begins later.  Warps take turns at (job, head).
   constexpr int kPer = R::kHD / 32;                            // features of a lane
-  auto part_at = [&](int i) { return i & 1 ? reinterpret_cast<const float*>(rings + (i >> 1) * S * R::kBytes) : leads + (i >> 1) * kPart; };
-  auto write = [&](int job, int h, const float (&f)[kPer], float l) {
-    const int row = job / tiles, vh = job % tiles;
-    T* out = static_cast<T*>(a.o) + row * a.o_row + (long long)(vh / head_tiles * group + vh % head_tiles * tile_heads + h) * a.o_head;
+  constexpr int kMax = R::kHeads * R::kHD, kSum = kMax + R::kHeads;
+  auto write = [&](int row, int head, const float (&f)[kPer], float l) {
+    T* out = static_cast<T*>(a.o) + row * a.o_row + (long long)head * a.o_head;
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
       if (lane * kPer + i < a.hd) out[lane * kPer + i] = from_f32<T>(f[i] / l);
   };
-  auto heads_of = [&](int job) { return min(tile_heads, group - job % tiles % head_tiles * tile_heads); };
-  auto job_begin = [&](int job) {
-    const int row = job / tiles;
-    return (long long)before[row] * tiles + (long long)(job % tiles) * (before[row + 1] - before[row]);
-  };
-  auto job_end = [&](int job) { return job_begin(job) + (before[job / tiles + 1] - before[job / tiles]); };
-  int unit = 0;
-  for (int i = 0; i < 2 * W;) {
-    const int job = part_job[i];
-    if (job < 0) {
-      ++i;
-      continue;
-    }
-    int stop = i + 1;
-    while (stop < 2 * W && (part_job[stop] == job || part_job[stop] < 0)) ++stop;
-    const long long jb = job_begin(job);
-    const bool whole = jb >= begin && job_end(job) <= end;
-    const int place = jb > begin;
-    float* dst = a.ws + (blockIdx.x * 2LL + place) * kPart;
-    if (!whole && tid == 0) {
-      shared_job[place] = job;
-      shared_slot[place] = (int)(jb / share);
-    }
-    for (int h = 0; h < heads_of(job); ++h, ++unit) {
-      if (unit % W != warp) continue;
-      float m = -INFINITY;
-      for (int j = i; j < stop; ++j)
-        if (part_job[j] == job) m = fmaxf(m, part_at(j)[R::kHeads * R::kHD + h]);
-      const float sub = m == -INFINITY ? 0.0f : m;
-      float l = 0.0f, f[kPer] = {};
-      for (int j = i; j < stop; ++j) {
-        if (part_job[j] != job) continue;
-        const float* part = part_at(j);
-        const float w = exp2_fast(part[R::kHeads * R::kHD + h] - sub);
-        l += w * part[R::kHeads * (R::kHD + 1) + h];
+  {
+    const int job = lane < 2 * W ? part_job[lane] : -1;
+    const unsigned same = __match_any_sync(0xffffffffu, job);
+    unsigned leaders = __ballot_sync(0xffffffffu, job >= 0 && (same & ((1u << lane) - 1)) == 0);
+    const float* part = lane & 1 ? reinterpret_cast<const float*>(rings + (lane >> 1) * S * R::kBytes) : leads + (lane >> 1) * kPart;
+    for (int unit = 0; leaders; leaders &= leaders - 1) {
+      const int i = __ffs(leaders) - 1;
+      const unsigned group_of = __shfl_sync(0xffffffffu, same, i);
+      const long long jb = part_begin[i];
+      const bool whole = jb >= begin && jb + part_rounds[i] <= end;
+      const int place = jb > begin;
+      if (!whole && tid == 0) shared_part[place] = i;
+      for (int h = 0; h < part_count[i]; ++h, ++unit) {
+        if (unit % W != warp) continue;
+        const bool in = group_of >> lane & 1;
+        const float mine = in ? part[kMax + h] : -INFINITY, m = warp_max(mine), sub = m == -INFINITY ? 0.0f : m;
+        const float w = in ? exp2_fast(mine - sub) : 0.0f;     // (NaN where the maximum is: +inf)
+        const float l = warp_sum(in ? w * part[kSum + h] : 0.0f);
+        float f[kPer] = {};
+        for (unsigned g = group_of; g; g &= g - 1) {
+          const int j = __ffs(g) - 1;
+          const float* src = j & 1 ? reinterpret_cast<const float*>(rings + (j >> 1) * S * R::kBytes) : leads + (j >> 1) * kPart;
+          const float wj = __shfl_sync(0xffffffffu, w, j);
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) f[e] += w * part[h * R::kHD + lane * kPer + e];
-      }
-      if (whole) {
-        write(job, h, f, l);
-      } else {
+          for (int e = 0; e < kPer; ++e) f[e] += wj * src[h * R::kHD + lane * kPer + e];
+        }
+        if (whole) {
+          write(part_row[i], part_head[i] + h, f, l);
+        } else {
+          float* dst = a.ws + (blockIdx.x * 2LL + place) * kPart;
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) dst[h * R::kHD + lane * kPer + e] = f[e];
-        if (lane == 0) {
-          dst[R::kHeads * R::kHD + h] = m;
-          dst[R::kHeads * (R::kHD + 1) + h] = l;
+          for (int e = 0; e < kPer; ++e) dst[h * R::kHD + lane * kPer + e] = f[e];
+          if (lane == 0) {
+            dst[kMax + h] = m;
+            dst[kSum + h] = l;
+          }
         }
       }
     }
-    i = stop;
   }
+  // A job of several CTAs: the last of them to get here joins their parts, in their order.
+  __syncthreads();
+  if (shared_part[0] < 0 && shared_part[1] < 0) return;
   __threadfence();
   __syncthreads();
   if (tid < 2) {
     int last = 0;
-    const int job = shared_job[tid];
-    if (job >= 0) {
-      const int first = shared_slot[tid], n = (int)((job_end(job) - 1) / share) - first + 1;
-      last = atomicAdd(a.counters + first, 1u) == (unsigned)n - 1;
+    const int i = shared_part[tid];
+    if (i >= 0) {
+      const long long first = part_begin[i] / share, stop = (part_begin[i] + part_rounds[i] - 1) / share;
+      last = atomicAdd(a.counters + first, 1u) == (unsigned)(stop - first);
       if (last) a.counters[first] = 0;
+      merges[tid] = last ? (int)(stop - first) + 1 : 0;
+    } else {
+      merges[tid] = 0;
     }
-    merges[tid] = last;
   }
   __syncthreads();
   for (int p = 0; p < 2; ++p) {
-    if (!merges[p]) continue;
+    const int n = merges[p];
+    if (n == 0) continue;
     __threadfence();
-    const int job = shared_job[p], first = shared_slot[p], n = (int)((job_end(job) - 1) / share) - first + 1;
-    const int place = job_begin(job) > first * share;
-    for (int h = warp; h < heads_of(job); h += W) {
-      auto part = [&](int j) { return a.ws + ((first + j) * 2LL + (j == 0 ? place : 0)) * kPart; };
+    const int i = shared_part[p];
+    const long long first = part_begin[i] / share;
+    const int place = part_begin[i] > first * share;
+    auto part = [&](int j) { return a.ws + ((first + j) * 2 + (j == 0 ? place : 0)) * kPart; };
+    for (int h = warp; h < part_count[i]; h += W) {
       float m = -INFINITY;
-      for (int j = lane; j < n; j += 32) m = fmaxf(m, __ldcg(part(j) + R::kHeads * R::kHD + h));
+      for (int j = lane; j < n; j += 32) m = fmaxf(m, __ldcg(part(j) + kMax + h));
       m = warp_max(m);
       const float sub = m == -INFINITY ? 0.0f : m;
       float l = 0.0f, f[kPer] = {};
-#pragma unroll 4
-      for (int j = 0; j < n; ++j) {
-        const float* src = part(j);
-        const float w = exp2_fast(__ldcg(src + R::kHeads * R::kHD + h) - sub);
-        l += w * __ldcg(src + R::kHeads * (R::kHD + 1) + h);
+      for (int j0 = 0; j0 < n; j0 += 32) {
+        const int j = j0 + lane;
+        const float w = j < n ? exp2_fast(__ldcg(part(j) + kMax + h) - sub) : 0.0f;
+        l += j < n ? w * __ldcg(part(j) + kSum + h) : 0.0f;
+        const int some = min(32, n - j0);
+#pragma unroll 8
+        for (int x = 0; x < some; ++x) {
+          const float wx = __shfl_sync(0xffffffffu, w, x);
+          float v[kPer];
+          load_l2(part(j0 + x) + h * R::kHD + lane * kPer, v);
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) f[e] += w * __ldcg(src + h * R::kHD + lane * kPer + e);
+          for (int e = 0; e < kPer; ++e) f[e] += wx * v[e];
+        }
       }
-      write(job, h, f, l);
+      write(part_row[i], part_head[i] + h, f, warp_sum(l));
     }
   }
 }
@@ -815,9 +864,9 @@ extern "C" int dptb_paged_attention(const PagedAttnArgs* args, void* stream) {
   if (a.rows < 0 || a.rows > 65535 || a.heads < 0 || a.kv_heads <= 0 || a.heads % a.kv_heads || a.hd <= 0 || a.hd > kMaxHeadDim ||
       a.page <= 0 || a.width < 0 || a.pages < 0)
     return kErrBadShape;
-  a.page_shift = -1;
-  if ((a.page & (a.page - 1)) == 0)
-    for (a.page_shift = 0; 1 << a.page_shift < a.page;) ++a.page_shift;
+  a.page_shift = 31;
+  while (1LL << (a.page_shift - 31) < a.page) ++a.page_shift;
+  a.page_mul = (unsigned)(((1ULL << a.page_shift) + a.page - 1) / a.page);
   auto st = static_cast<cudaStream_t>(stream);
   const int per = a.f32 ? 4 : 8;                       // elements of a piece
   auto whole = [&](const void* p, long long s0, long long s1, long long s2) {

@@ -35,7 +35,8 @@ class PagedAttnArgs(ctypes.Structure):
         [(n, c_ll) for n in ("q_row", "q_head", "o_row", "o_head", "k_page", "k_head", "k_tok", "v_page", "v_head", "v_tok",
                              "table_row")] + \
         [(n, c_int) for n in ("rows", "heads", "kv_heads", "hd", "page", "width", "pages", "f32")] + [("scale", c_float)] + \
-        [("ws", c_void_p), ("ws_floats", c_ll), ("counters", c_void_p), ("num_counters", c_int), ("page_shift", c_int)]
+        [("ws", c_void_p), ("ws_floats", c_ll), ("counters", c_void_p), ("num_counters", c_int), ("page_mul", ctypes.c_uint),
+         ("page_shift", ctypes.c_uint)]
 
 
 class AppendArgs(ctypes.Structure):
