@@ -396,45 +396,52 @@ struct PageMaps {
   CUtensorMap k, v;      // (feature, token of the page, head, page)
 };
 
+// A round that is not full, or spans pages: in boxes of as many tokens as fit a page.  Out of line: the kernel's code is fetched anew at every
+// launch, and most rounds do not come here.
+template <typename R>
+__device__ __noinline__ unsigned issue_boxes(const PagedAttnArgs& a, const PageMaps& maps, int entry, int first_slot, int kv, int p0, int len, int box_shift,
+                                             unsigned char* ring, uint64_t* bar, int lane) {
+  const int end = min(p0 + R::kKeys, len);
+  auto page_of = [&](int slot) { return __shfl_sync(0xffffffffu, entry, slot - first_slot & 31); };
+  if (lane == 0) mbar_arrive_expect_tx(bar, R::kBytes);
+  const int pos = p0 + (lane & (R::kKeys - 1));
+  const unsigned mine = page_of(slot_of(a, pos));
+  const bool bad = pos < end && mine >= (unsigned)a.pages;
+  if (bad) report_error(kBadPage);
+  const unsigned keys = __ballot_sync(0xffffffffu, pos < end && !bad) & ((1u << R::kKeys) - 1);      // (orders the lanes before the copies too)
+  const int per_shift = R::kKeyShift - box_shift, boxes = 2 * R::kSegs << per_shift;
+#pragma unroll 1
+  for (int b0 = 0; b0 < boxes; b0 += 32) {
+    const int b = b0 + lane, first = (b & ((1 << per_shift) - 1)) << box_shift, tile = b >> per_shift;
+    const int slot = slot_of(a, p0 + first);
+    int page = page_of(slot);
+    if ((unsigned)page >= (unsigned)a.pages) page = a.pages;                                            // beyond the pool: zeros
+    if (b < boxes) {
+      const bool is_v = tile >= R::kSegs;
+      tma_load_4d(ring + tile * R::kSeg + first * 128, is_v ? &maps.v : &maps.k, bar, (is_v ? tile - R::kSegs : tile) * (128 / (int)sizeof(typename R::T)),
+                  p0 + first - slot * a.page, kv, page);
+    }
+  }
+  return keys;
+}
+
 // Requests the keys and values of round c; returns which of its keys there are.
 template <typename R>
 __device__ __forceinline__ unsigned issue_round(const PagedAttnArgs& a, const PageMaps& maps, PageWindow& win, const Cursor& c, int len, int box_shift,
                                                 unsigned char* ring, uint64_t* bar, int lane) {
   const int p0 = c.k * R::kKeys, slot0 = slot_of(a, p0);
-  if (2 << box_shift > R::kKeys && p0 + R::kKeys <= len) {       // a full round of one page, a box for each tile
-    win.cover(a, c.row, slot0, slot0, len, lane);
-    const int page = win.at(slot0);
-    if ((unsigned)page < (unsigned)a.pages) {
-      if (lane == 0) mbar_arrive_expect_tx(bar, R::kBytes);
-      __syncwarp();
-      if (lane < 2 * R::kSegs) {
-        const bool is_v = lane >= R::kSegs;
-        tma_load_4d(ring + lane * R::kSeg, is_v ? &maps.v : &maps.k, bar, (lane & (R::kSegs - 1)) * (128 / (int)sizeof(typename R::T)), p0 - slot0 * a.page, c.kv, page);
-      }
-      return (1u << R::kKeys) - 1;
-    }
-  }
-  const int end = min(p0 + R::kKeys, len);
-  win.cover(a, c.row, slot0, slot_of(a, end - 1), len, lane);
+  win.cover(a, c.row, slot0, slot_of(a, min(p0 + R::kKeys, len) - 1), len, lane);
+  const int page = win.at(slot0);
+  if (1 << box_shift != R::kKeys || p0 + R::kKeys > len || (unsigned)page >= (unsigned)a.pages)
+    return issue_boxes<R>(a, maps, win.entry, win.first, c.kv, p0, len, box_shift, ring, bar, lane);
   if (lane == 0) mbar_arrive_expect_tx(bar, R::kBytes);
-  const int pos = p0 + (lane & (R::kKeys - 1));
-  const unsigned mine = win.at(slot_of(a, pos));
-  const bool bad = pos < end && mine >= (unsigned)a.pages;
-  if (bad) report_error(kBadPage);
-  const unsigned keys = __ballot_sync(0xffffffffu, pos < end && !bad) & ((1u << R::kKeys) - 1);      // (orders the lanes before the copies too)
-  const int per_shift = R::kKeyShift - box_shift, boxes = 2 * R::kSegs << per_shift;
-  for (int b0 = 0; b0 < boxes; b0 += 32) {
-    const int b = b0 + lane, first = (b & ((1 << per_shift) - 1)) << box_shift, tile = b >> per_shift;
-    const int slot = slot_of(a, p0 + first);
-    int page = win.at(slot);
-    if ((unsigned)page >= (unsigned)a.pages) page = a.pages;                                            // beyond the pool: zeros
-    if (b < boxes) {
-      const bool is_v = tile >= R::kSegs;
-      tma_load_4d(ring + tile * R::kSeg + first * 128, is_v ? &maps.v : &maps.k, bar, (tile & (R::kSegs - 1)) * (128 / (int)sizeof(typename R::T)),
-                  p0 + first - slot * a.page, c.kv, page);
-    }
+  __syncwarp();
+  if (lane < 2 * R::kSegs) {                       // a full round of one page: a box for each tile
+    const bool is_v = lane >= R::kSegs;
+    tma_load_4d(ring + lane * R::kSeg, is_v ? &maps.v : &maps.k, bar, (is_v ? lane - R::kSegs : lane) * (128 / (int)sizeof(typename R::T)),
+                p0 - slot0 * a.page, c.kv, page);
   }
-  return keys;
+  return (1u << R::kKeys) - 1;
 }
 
 template <typename T, int N>
@@ -442,36 +449,20 @@ __device__ __forceinline__ void store_out(T* dst, const float (&f)[N], float by,
   T e[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) e[i] = from_f32<T>(f[i] * by);
-  if constexpr (N * sizeof(T) == 16) {
-    if (vec && valid >= N) {
-      *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(e);
-      return;
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (i < valid) dst[i] = e[i];
-}
-
-// Values that other CTAs have written.
-template <int N>
-__device__ __forceinline__ void load_l2(const float* p, float (&v)[N]) {
-  if constexpr (N % 4 == 0) {
-#pragma unroll
-    for (int i = 0; i < N; i += 4) {
-      const float4 u = __ldcg(reinterpret_cast<const float4*>(p + i));
-      v[i] = u.x; v[i + 1] = u.y; v[i + 2] = u.z; v[i + 3] = u.w;
-    }
+  static_assert(N * sizeof(T) == 16, "a piece");
+  if (vec && valid >= N) {
+    *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(e);
   } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = __ldcg(p + i);
+    for (int i = 0; i < N; ++i)
+      if (i < valid) dst[i] = e[i];
   }
 }
 
 // W warps, S rounds of a warp in flight or in use.
 template <typename R, int W, int S>
 __global__ void __launch_bounds__(W * 32, 1)
-paged_attention_kernel(const PagedAttnArgs a, const __grid_constant__ PageMaps maps, int box_shift, int head_tiles, int tile_heads, int q_vec, int o_vec) {
+paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_constant__ PageMaps maps, int box_shift, int head_tiles, int tile_heads, int q_vec, int o_vec) {
   using T = typename R::T;
   constexpr int kPart = Part<R>::kFloats;
   static_assert(S * R::kBytes >= kPart * 4, "a warp's ring holds its last part");
@@ -481,8 +472,7 @@ paged_attention_kernel(const PagedAttnArgs a, const __grid_constant__ PageMaps m
   float* queries = leads + W * kPart;                                       // [W] copies of the queries
   int* before = reinterpret_cast<int*>(queries + W * (R::kQueryBytes / 4)); // [rows + 1]: rounds of a kv head ahead of a row
   __shared__ int scan[W + 1];
-  __shared__ int part_job[2 * W], part_row[2 * W], part_head[2 * W], part_count[2 * W], part_rounds[2 * W];
-  __shared__ long long part_begin[2 * W];
+  __shared__ int part_job[2 * W], part_row[2 * W], part_head[2 * W], part_count[2 * W], part_begin[2 * W], part_rounds[2 * W];
   __shared__ int shared_part[2], merges[2];      // jobs of several CTAs: one of their parts here, or -1
   __shared__ uint64_t landed[W * S];
   __shared__ int aborted;
@@ -531,22 +521,20 @@ paged_attention_kernel(const PagedAttnArgs a, const __grid_constant__ PageMaps m
     mbar_fence_init();
     equal = __syncthreads_and(equal);
   }
-  const long long total = (long long)before[a.rows] * tiles;
+  const int total = before[a.rows] * tiles;                    // (below 2^31: the launcher sees to it)
   // A CTA takes a round for each of its warps at least: parts of one CTA are joined sooner than those of several.  Whole jobs, where all
   // are as long and short enough that each CTA still has its own at once.
-  long long share = total < 1LL << 31 ? (long long)((unsigned)(total + gridDim.x - 1) / gridDim.x) : (total + gridDim.x - 1) / gridDim.x;
-  if (equal && rounds0 > 0 && rounds0 <= 2 * W && (long long)a.rows * tiles <= gridDim.x) share = rounds0 < W / 2 && share < W ? W / rounds0 * rounds0 : rounds0;
-  else share = max((long long)W, share);
-  const long long begin = min(total, share * blockIdx.x), end = min(total, begin + share);
+  int share = max(W, (int)((unsigned)(total + gridDim.x - 1) / gridDim.x));
+  if (equal && rounds0 > 0 && rounds0 <= 2 * W && a.rows * tiles <= gridDim.x) share = rounds0;
+  const int begin = (int)min((long long)total, (long long)share * blockIdx.x), end = min(total, begin + share);
   for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {       // rows of no tokens
     if (before[r + 1] > before[r]) continue;
     for (int x = tid; x < a.heads * a.hd; x += W * 32) static_cast<T*>(a.o)[r * a.o_row + x / a.hd * a.o_head + x % a.hd] = from_f32<T>(0.0f);
   }
   if (begin >= end) return;
 
-  const long long quota = (end - begin + W - 1) / W;
-  const long long w0 = min(end, begin + quota * warp), w1 = min(end, w0 + quota);
-  int todo = (int)(w1 - w0);
+  const int quota = (end - begin + W - 1) / W, w0 = min(end, begin + quota * warp), w1 = min(end, w0 + quota);
+  int todo = w1 - w0;
   if (todo > 0) {
     unsigned char* ring = rings + warp * S * R::kBytes;
     uint64_t* bars = landed + warp * S;
@@ -556,13 +544,13 @@ paged_attention_kernel(const PagedAttnArgs a, const __grid_constant__ PageMaps m
       int hi = a.rows - 1;                                     // the last row with no more rounds ahead than w0, which has some itself
       while (row < hi) {
         const int mid = (row + hi + 1) / 2;
-        if ((long long)before[mid] * tiles <= w0) row = mid;
+        if (before[mid] * tiles <= w0) row = mid;
         else hi = mid - 1;
       }
     }
     const int n0 = before[row + 1] - before[row];
-    const int rem = (int)(w0 - (long long)before[row] * tiles);
-    Cursor c{row, rem / n0, rem % n0, n0, rem / n0 / head_tiles}, ahead = c;
+    const int rem = w0 - before[row] * tiles, vh0 = rem / n0;
+    Cursor c{row, vh0, rem - vh0 * n0, n0, head_tiles == 1 ? vh0 : vh0 / head_tiles}, ahead = c;
     auto advance = [&](Cursor& x) {
       if (++x.k < x.n) return;
       x.k = 0;
@@ -591,15 +579,19 @@ paged_attention_kernel(const PagedAttnArgs a, const __grid_constant__ PageMaps m
         if (left > 0) advance(ahead);
       }
     };
-#pragma unroll
-    for (int s = 0; s < S - 1; ++s) fetch();
     const float scale2 = a.scale * kLog2e;
     R x;
     int from = c.k, head0 = 0, count = 0;
     uint32_t phase = 0;
     bool fresh = true, first = true;
-    for (; todo > 0; --todo) {
+    todo += S - 1;
+#pragma unroll 1
+    for (int lead = S - 1; todo > 0; --todo) {
       fetch();
+      if (lead > 0) {        // the first rounds are on their way before any is waited for
+        --lead;
+        continue;
+      }
       if (fresh) {
         const int tile = c.vh - c.kv * head_tiles;
         head0 = c.kv * group + tile * tile_heads;
@@ -651,7 +643,7 @@ paged_attention_kernel(const PagedAttnArgs a, const __grid_constant__ PageMaps m
             part_row[at] = c.row;
             part_head[at] = head0;
             part_count[at] = count;
-            part_begin[at] = (long long)before[c.row] * tiles + (long long)c.vh * c.n;
+            part_begin[at] = before[c.row] * tiles + c.vh * c.n;
             part_rounds[at] = c.n;
           }
         }
@@ -663,103 +655,92 @@ paged_attention_kernel(const PagedAttnArgs a, const __grid_constant__ PageMaps m
   }
   __syncthreads();
 
-  // Parts of a job that lies within the CTA are joined and written out; another's go to the workspace as one: place 0 of the CTA for the
-  // job of its first round, 1 for one that begins later.  Warps take turns at (job, head).
+  // Parts of a job are joined, first those of this CTA (stage 0): of a job that lies within it, to the output; of another's, to the workspace, place 0
+  // of the CTA for the job of its first round, 1 for one that begins later.  The last CTA that gets so far with a job joins what the
+  // workspace holds of it (stage 1), in the order of the CTAs.  Warps take turns at (job, head); lane j has part j.  One loop for both: this code
+  // runs once a launch, and what counts is how much of it there is to fetch.
   constexpr int kPer = R::kHD / 32;                            // features of a lane
   constexpr int kMax = R::kHeads * R::kHD, kSum = kMax + R::kHeads;
-  auto write = [&](int row, int head, const float (&f)[kPer], float l) {
-    T* out = static_cast<T*>(a.o) + row * a.o_row + (long long)head * a.o_head;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      if (lane * kPer + i < a.hd) out[lane * kPer + i] = from_f32<T>(f[i] / l);
-  };
-  {
-    const int job = lane < 2 * W ? part_job[lane] : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, job);
-    unsigned leaders = __ballot_sync(0xffffffffu, job >= 0 && (same & ((1u << lane) - 1)) == 0);
-    const float* part = lane & 1 ? reinterpret_cast<const float*>(rings + (lane >> 1) * S * R::kBytes) : leads + (lane >> 1) * kPart;
-    for (int unit = 0; leaders; leaders &= leaders - 1) {
-      const int i = __ffs(leaders) - 1;
-      const unsigned group_of = __shfl_sync(0xffffffffu, same, i);
-      const long long jb = part_begin[i];
-      const bool whole = jb >= begin && jb + part_rounds[i] <= end;
-      const int place = jb > begin;
-      if (!whole && tid == 0) shared_part[place] = i;
-      for (int h = 0; h < part_count[i]; ++h, ++unit) {
-        if (unit % W != warp) continue;
-        const bool in = group_of >> lane & 1;
-        const float mine = in ? part[kMax + h] : -INFINITY, m = warp_max(mine), sub = m == -INFINITY ? 0.0f : m;
-        const float w = in ? exp2_fast(mine - sub) : 0.0f;     // (NaN where the maximum is: +inf)
-        const float l = warp_sum(in ? w * part[kSum + h] : 0.0f);
-        float f[kPer] = {};
-        for (unsigned g = group_of; g; g &= g - 1) {
-          const int j = __ffs(g) - 1;
-          const float* src = j & 1 ? reinterpret_cast<const float*>(rings + (j >> 1) * S * R::kBytes) : leads + (j >> 1) * kPart;
-          const float wj = __shfl_sync(0xffffffffu, w, j);
-#pragma unroll
-          for (int e = 0; e < kPer; ++e) f[e] += wj * src[h * R::kHD + lane * kPer + e];
+#pragma unroll 1
+  for (int stage = 0; stage < 2; ++stage) {
+    unsigned jobs, same = 0;                                   // the jobs at hand: one of their parts in this CTA each
+    if (stage == 0) {
+      const int job = lane < 2 * W ? part_job[lane] : -1;
+      same = __match_any_sync(0xffffffffu, job);
+      jobs = __ballot_sync(0xffffffffu, job >= 0 && (same & ((1u << lane) - 1)) == 0);
+    } else {
+      __syncthreads();
+      if (shared_part[0] < 0 && shared_part[1] < 0) return;
+      __threadfence();
+      __syncthreads();
+      if (tid < 2) {
+        const int i = shared_part[tid];
+        int last = 0;
+        if (i >= 0) {
+          const int first = part_begin[i] / share, n = (part_begin[i] + part_rounds[i] - 1) / share - first;
+          last = atomicAdd(a.counters + first, 1u) == (unsigned)n;
+          if (last) a.counters[first] = 0;
         }
-        if (whole) {
-          write(part_row[i], part_head[i] + h, f, l);
-        } else {
-          float* dst = a.ws + (blockIdx.x * 2LL + place) * kPart;
+        merges[tid] = last;
+      }
+      __syncthreads();
+      __threadfence();
+      jobs = (merges[0] ? 1u << shared_part[0] : 0) | (merges[1] ? 1u << shared_part[1] : 0);
+    }
+    int unit = 0;
+#pragma unroll 1
+    for (; jobs; jobs &= jobs - 1) {
+      const int i = __ffs(jobs) - 1, jb = part_begin[i], stop = jb + part_rounds[i], heads = part_count[i];
+      const bool whole = jb >= begin && stop <= end;
+      const unsigned group_of = __shfl_sync(0xffffffffu, same, i);
+      if (stage == 0 && !whole && tid == 0) shared_part[jb > begin] = i;
+      const int first = stage ? jb / share : 0, n = stage ? (stop - 1) / share - first + 1 : 32;
+#pragma unroll 1
+      for (int h = 0; h < heads; ++h, ++unit) {
+        if (unit % W != warp) continue;
+        float m = -INFINITY, l = 0.0f, f[kPer] = {};
+#pragma unroll 1
+        for (int j0 = 0; j0 < n; j0 += 32) {
+          const int j = j0 + lane;
+          const float* part = nullptr;
+          if (stage == 0) {
+            if (group_of >> lane & 1) part = lane & 1 ? reinterpret_cast<const float*>(rings + (lane >> 1) * S * R::kBytes) : leads + (lane >> 1) * kPart;
+          } else if (j < n) {
+            part = a.ws + ((first + j) * 2LL + (j == 0 && jb > first * share)) * kPart;
+          }
+          const float mine = part ? *(const volatile float*)(part + kMax + h) : -INFINITY;
+          const float nm = fmaxf(m, warp_max(mine)), sub = nm == -INFINITY ? 0.0f : nm, corr = exp2_fast(m - sub);
+          const float w = part ? exp2_fast(mine - sub) : 0.0f;
+          l = l * corr + warp_sum(part ? w * *(const volatile float*)(part + kSum + h) : 0.0f);
+          m = nm;
 #pragma unroll
-          for (int e = 0; e < kPer; ++e) dst[h * R::kHD + lane * kPer + e] = f[e];
+          for (int e = 0; e < kPer; ++e) f[e] *= corr;
+          unsigned parts = __ballot_sync(0xffffffffu, part != nullptr);
+#pragma unroll 4
+          for (; parts; parts &= parts - 1) {
+            const int x = __ffs(parts) - 1;
+            const volatile float* src = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(part), x)) + h * R::kHD + lane;
+            const float wx = __shfl_sync(0xffffffffu, w, x);
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) f[e] += wx * src[32 * e];
+          }
+        }
+        if (stage || whole) {
+          T* out = static_cast<T*>(a.o) + part_row[i] * a.o_row + (long long)(part_head[i] + h) * a.o_head;
+          const float by = 1.0f / l;
+#pragma unroll
+          for (int e = 0; e < kPer; ++e)
+            if (lane + 32 * e < a.hd) out[lane + 32 * e] = from_f32<T>(f[e] * by);
+        } else {
+          float* dst = a.ws + (blockIdx.x * 2LL + (jb > begin)) * kPart;
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) dst[h * R::kHD + lane + 32 * e] = f[e];
           if (lane == 0) {
             dst[kMax + h] = m;
             dst[kSum + h] = l;
           }
         }
       }
-    }
-  }
-  // A job of several CTAs: the last of them to get here joins their parts, in their order.
-  __syncthreads();
-  if (shared_part[0] < 0 && shared_part[1] < 0) return;
-  __threadfence();
-  __syncthreads();
-  if (tid < 2) {
-    int last = 0;
-    const int i = shared_part[tid];
-    if (i >= 0) {
-      const long long first = part_begin[i] / share, stop = (part_begin[i] + part_rounds[i] - 1) / share;
-      last = atomicAdd(a.counters + first, 1u) == (unsigned)(stop - first);
-      if (last) a.counters[first] = 0;
-      merges[tid] = last ? (int)(stop - first) + 1 : 0;
-    } else {
-      merges[tid] = 0;
-    }
-  }
-  __syncthreads();
-  for (int p = 0; p < 2; ++p) {
-    const int n = merges[p];
-    if (n == 0) continue;
-    __threadfence();
-    const int i = shared_part[p];
-    const long long first = part_begin[i] / share;
-    const int place = part_begin[i] > first * share;
-    auto part = [&](int j) { return a.ws + ((first + j) * 2 + (j == 0 ? place : 0)) * kPart; };
-    for (int h = warp; h < part_count[i]; h += W) {
-      float m = -INFINITY;
-      for (int j = lane; j < n; j += 32) m = fmaxf(m, __ldcg(part(j) + kMax + h));
-      m = warp_max(m);
-      const float sub = m == -INFINITY ? 0.0f : m;
-      float l = 0.0f, f[kPer] = {};
-      for (int j0 = 0; j0 < n; j0 += 32) {
-        const int j = j0 + lane;
-        const float w = j < n ? exp2_fast(__ldcg(part(j) + kMax + h) - sub) : 0.0f;
-        l += j < n ? w * __ldcg(part(j) + kSum + h) : 0.0f;
-        const int some = min(32, n - j0);
-#pragma unroll 8
-        for (int x = 0; x < some; ++x) {
-          const float wx = __shfl_sync(0xffffffffu, w, x);
-          float v[kPer];
-          load_l2(part(j0 + x) + h * R::kHD + lane * kPer, v);
-#pragma unroll
-          for (int e = 0; e < kPer; ++e) f[e] += wx * v[e];
-        }
-      }
-      write(part_row[i], part_head[i] + h, f, warp_sum(l));
     }
   }
 }
@@ -879,7 +860,8 @@ extern "C" int dptb_paged_attention(const PagedAttnArgs* args, void* stream) {
       map_pages(&maps.k, a, a.k, a.k_page, a.k_head, a.k_tok, box) == 0 && map_pages(&maps.v, a, a.v, a.v_page, a.v_head, a.v_tok, box) == 0) {
     const bool qv = whole(a.q, a.q_row, a.q_head, 0), ov = whole(a.o, a.o_row, a.o_head, 0);
     const int group = a.heads / a.kv_heads;
-    if ((long long)a.rows * ((long long)a.width * a.page / 8 + 1) >= 1LL << 31 || (long long)a.rows * a.heads >= 1LL << 31) return kErrTooLarge;
+    // rounds, and all else that is counted, in 32 bits
+    if ((double)a.rows * ((double)a.width * a.page / (a.f32 ? 8 : 16) + 1) * a.heads >= 2147483000.0) return kErrTooLarge;
 #define DPTB_PAGED(R, W, S) return launch_paged<R, W, S>(a, maps, (group + R::kHeads - 1) / R::kHeads, R::kHeads, qv, ov, st)
     if (!a.f32) {
       using B64 = Bf16Round<64, 1>; using C64 = Bf16Round<64, 2>;
