@@ -56,6 +56,15 @@ struct PagedAttnArgs {
 __device__ __forceinline__ int slot_of(const PagedAttnArgs& a, int pos) { return (int)((unsigned long long)pos * a.page_mul >> a.page_shift); }
 
 // ------------------------------------------------------------------------------------------------------------ pieces
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+// `bytes`, a multiple of 16, between 16-byte boundaries; they count on `bar`.
+__device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(smem_dst)), "l"(src), "r"(bytes),
+               "r"(smem_u32(bar))
+               : "memory");
+}
 __device__ __forceinline__ uint4 read_piece(uint32_t addr) {
   uint4 u;
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(addr) : "memory");
@@ -67,15 +76,23 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-// What of a round a lane looks up: the page of a position, from a window of 32 table entries that the lanes hold.
+// What of a round a lane looks up: the page of a position, from a window of 32 table entries that the lanes hold.  The first window of the
+// row after is loaded a row ahead, so that rows of a few rounds do not wait for their table.
 struct PageWindow {
-  int row = -1, first = 0, entry = -1;
+  int row = -1, first = 0, entry = -1, next_row = -1, next_entry = -1;
+  __device__ __forceinline__ int load(const PagedAttnArgs& a, int r, int slot, int len, int lane) const {
+    return slot + lane <= slot_of(a, len - 1) ? a.table[r * a.table_row + slot + lane] : -1;
+  }
   __device__ __forceinline__ void cover(const PagedAttnArgs& a, int r, int slot, int last, int len, int lane) {
     if (r != row || slot < first || last >= first + 32) {
+      entry = r == next_row && slot == 0 ? next_entry : load(a, r, slot, len, lane);
       row = r;
       first = slot;
-      entry = slot + lane <= slot_of(a, len - 1) ? a.table[r * a.table_row + slot + lane] : -1;
     }
+  }
+  __device__ __forceinline__ void ahead(const PagedAttnArgs& a, int r, int len, int lane) {
+    next_row = r;
+    next_entry = load(a, r, 0, len, lane);
   }
   // (every lane of the warp calls it)
   __device__ __forceinline__ int at(int slot) const { return __shfl_sync(0xffffffffu, entry, (slot - first) & 31); }
@@ -96,7 +113,7 @@ struct Bf16Round {
   using T = __nv_bfloat16;
   static constexpr int kKeys = 16, kKeyShift = 4, kHeads = 8 * NT, kHD = HD;
   static constexpr int kSegs = HD / 64, kSeg = kKeys * 128, kBytes = 2 * kSegs * kSeg;   // keys, then values: a tile for every 64 features
-  static constexpr int kQueryBytes = 0;
+  static constexpr int kQueryBytes = kHeads * HD * 2;
 
   uint4 q[NT][HD / 32];       // head lane / 4, pieces (lane % 4) + 4 i
   float m[NT][2], l[NT][2];   // heads (lane % 4) * 2 and the next; l: of this lane's keys
@@ -105,28 +122,15 @@ struct Bf16Round {
   // Which key of a half round is row i of a fragment, and which piece of 8 features a lane takes: neighbours in a read differ in bit 2.
   static __device__ __forceinline__ int order(int i) { return i >> 1 | (i & 1) << 2; }
 
-  // The queries of heads head0 .. head0 + count of a row.
-  __device__ __forceinline__ void start(const PagedAttnArgs& a, int row, int head0, int count, bool vec, float*, int lane) {
+  // `queries`: those of the job, [kHeads][HD]; beyond `count` heads and a.hd features it holds anything.
+  __device__ __forceinline__ void start(const PagedAttnArgs& a, const unsigned char* queries, int count, int lane) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int h = n * 8 + (lane >> 2);
-      const T* src = static_cast<const T*>(a.q) + row * a.q_row + (long long)(head0 + min(h, count - 1)) * a.q_head;
 #pragma unroll
       for (int i = 0; i < HD / 32; ++i) {
         const int f = ((lane & 3) + 4 * i) * 8;
-        uint4 u = make_uint4(0, 0, 0, 0);
-        if (h < count && f < a.hd) {
-          if (vec) {
-            u = *reinterpret_cast<const uint4*>(src + f);
-          } else {
-            const unsigned short* e = reinterpret_cast<const unsigned short*>(src + f);
-            u.x = e[0] | e[1] << 16;
-            u.y = e[2] | e[3] << 16;
-            u.z = e[4] | e[5] << 16;
-            u.w = e[6] | e[7] << 16;
-          }
-        }
-        q[n][i] = u;
+        q[n][i] = h < count && f < a.hd ? *reinterpret_cast<const uint4*>(queries + (h * HD + f) * 2) : make_uint4(0, 0, 0, 0);
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -143,7 +147,7 @@ struct Bf16Round {
   }
 
   // `keys`: bit j, whether key j of the round is one.
-  __device__ __forceinline__ void compute(uint32_t ring, unsigned keys, float scale2, const float*, int lane) {
+  __device__ __forceinline__ void compute(uint32_t ring, unsigned keys, float scale2, const unsigned char*, int lane) {
     const int t = lane & 3, mine = order(lane >> 2);
     const uint32_t swz = (mine ^ t) << 4;              // piece t of row `mine`, and piece `mine` of row t
     const uint32_t kr = ring + mine * 128, vr = ring + kSegs * kSeg + t * 128;
@@ -250,7 +254,7 @@ struct Bf16Round {
 
 // ------------------------------------------------------------------------------------------------------------ fp32
 // GP: query heads at a time.  Lane s of the 8 lanes of a key holds pieces s + 8 i of it; four keys go by at once, two steps a round.  The
-// scaled queries lie in shared memory, a copy for every warp.
+// queries are read from shared memory where they are needed (features beyond the head's are zeros there).
 template <int HD, int GP>
 struct F32Round {
   using T = float;
@@ -262,13 +266,7 @@ struct F32Round {
   float m[GP], l[GP];
   float4 o[GP][P];
 
-  __device__ __forceinline__ void start(const PagedAttnArgs& a, int row, int head0, int count, bool, float* queries, int lane) {
-    __syncwarp();
-    for (int x = lane; x < GP * HD; x += 32) {
-      const int h = x / HD, f = x % HD;
-      queries[x] = h < count && f < a.hd ? static_cast<const T*>(a.q)[row * a.q_row + (long long)(head0 + h) * a.q_head + f] : 0.0f;
-    }
-    __syncwarp();
+  __device__ __forceinline__ void start(const PagedAttnArgs&, const unsigned char*, int, int) {
 #pragma unroll
     for (int h = 0; h < GP; ++h) {
       m[h] = -INFINITY;
@@ -278,7 +276,7 @@ struct F32Round {
     }
   }
 
-  __device__ __forceinline__ void compute(uint32_t ring, unsigned keys, float scale2, const float* queries, int lane) {
+  __device__ __forceinline__ void compute(uint32_t ring, unsigned keys, float scale2, const unsigned char* queries, int lane) {
     const int g = lane >> 3, t = lane & 7;
     const unsigned live = keys >> g & 1 | (keys >> (g + 4) & 1) << 1;
     auto piece = [&](int seg, int j) {                   // of key g + 4 j
@@ -459,241 +457,55 @@ __device__ __forceinline__ void store_out(T* dst, const float (&f)[N], float by,
   }
 }
 
-// W warps, S rounds of a warp in flight or in use.
+// Parts of a job are joined, first those of this CTA (stage 0): of a job that lies within it, to the output; of another's, to the workspace, place 0
+// of the CTA for the job of its first round, 1 for one that begins later.  The last CTA that gets so far with a job joins what the
+// workspace holds of it (stage 1), in the order of the CTAs.  Warps take turns at (job, head); lane j has part j.  One loop for both.
+template <int W>
+struct Parts {
+  int job[2 * W], row[2 * W], head[2 * W], count[2 * W], begin[2 * W], rounds[2 * W];
+  int shared[2], merges[2];      // jobs of several CTAs: one of their parts here, or -1; whether this CTA is the last
+};
+
 template <typename R, int W, int S>
-__global__ void __launch_bounds__(W * 32, 1)
-paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_constant__ PageMaps maps, int box_shift, int head_tiles, int tile_heads, int q_vec, int o_vec) {
+__device__ __noinline__ void join_parts(const PagedAttnArgs& a, Parts<W>& sh, const unsigned char* rings, const float* leads, int begin, int end, int share) {
   using T = typename R::T;
   constexpr int kPart = Part<R>::kFloats;
-  static_assert(S * R::kBytes >= kPart * 4, "a warp's ring holds its last part");
-  extern __shared__ unsigned char smem[];
-  unsigned char* rings = smem + (1024 - (smem_u32(smem) & 1023) & 1023);      // [W][S] rounds
-  float* leads = reinterpret_cast<float*>(rings + W * S * R::kBytes);       // [W] parts
-  float* queries = leads + W * kPart;                                       // [W] copies of the queries
-  int* before = reinterpret_cast<int*>(queries + W * (R::kQueryBytes / 4)); // [rows + 1]: rounds of a kv head ahead of a row
-  __shared__ int scan[W + 1];
-  __shared__ int part_job[2 * W], part_row[2 * W], part_head[2 * W], part_count[2 * W], part_begin[2 * W], part_rounds[2 * W];
-  __shared__ int shared_part[2], merges[2];      // jobs of several CTAs: one of their parts here, or -1
-  __shared__ uint64_t landed[W * S];
-  __shared__ int aborted;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int tiles = a.kv_heads * head_tiles;                                // jobs of a row
-  const int room = (int)min((long long)a.width * a.page, 0x7fffffffLL);
-  const int group = a.heads / a.kv_heads;
-
-  // Rounds ahead of every row.
-  auto length = [&](int r) { return max(0, min(a.lens[r], room)); };
-  bool equal = true;
-  int rounds0;
-  {
-    const int each = (a.rows + W * 32 - 1) / (W * 32), r0 = min(a.rows, tid * each), r1 = min(a.rows, r0 + each);
-    int mine = 0;
-    rounds0 = (length(0) + R::kKeys - 1) / R::kKeys;
-    for (int r = r0; r < r1; ++r) {
-      const int n = a.lens[r], k = (max(0, min(n, room)) + R::kKeys - 1) / R::kKeys;
-      if (n > room && blockIdx.x == 0) report_error(kBadPage);
-      mine += k;
-      equal = equal && k == rounds0;
-    }
-    int s = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += u;
-    }
-    if (lane == 31) scan[warp] = s;
-    __syncthreads();
-    int at = s - mine;
-    for (int w = 0; w < warp; ++w) at += scan[w];
-    for (int r = r0; r < r1; ++r) {
-      before[r] = at;
-      at += (length(r) + R::kKeys - 1) / R::kKeys;
-    }
-    if (tid == 0) {
-      int t = 0;
-      for (int w = 0; w < W; ++w) t += scan[w];
-      before[a.rows] = t;
-    }
-    if (tid < 2 * W) part_job[tid] = -1;
-    if (tid < 2) shared_part[tid] = -1;
-    if (tid < W * S) mbar_init(landed + tid, 1);
-    if (tid == 0) aborted = 0;
-    mbar_fence_init();
-    equal = __syncthreads_and(equal);
-  }
-  const int total = before[a.rows] * tiles;                    // (below 2^31: the launcher sees to it)
-  // A CTA takes a round for each of its warps at least: parts of one CTA are joined sooner than those of several.  Whole jobs, where all
-  // are as long and short enough that each CTA still has its own at once.
-  int share = max(W, (int)((unsigned)(total + gridDim.x - 1) / gridDim.x));
-  if (equal && rounds0 > 0 && rounds0 <= 2 * W && a.rows * tiles <= gridDim.x) share = rounds0;
-  const int begin = (int)min((long long)total, (long long)share * blockIdx.x), end = min(total, begin + share);
-  for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {       // rows of no tokens
-    if (before[r + 1] > before[r]) continue;
-    for (int x = tid; x < a.heads * a.hd; x += W * 32) static_cast<T*>(a.o)[r * a.o_row + x / a.hd * a.o_head + x % a.hd] = from_f32<T>(0.0f);
-  }
-  if (begin >= end) return;
-
-  const int quota = (end - begin + W - 1) / W, w0 = min(end, begin + quota * warp), w1 = min(end, w0 + quota);
-  int todo = w1 - w0;
-  if (todo > 0) {
-    unsigned char* ring = rings + warp * S * R::kBytes;
-    uint64_t* bars = landed + warp * S;
-    float* my_queries = queries + warp * (R::kQueryBytes / 4);
-    int row = 0;
-    {
-      int hi = a.rows - 1;                                     // the last row with no more rounds ahead than w0, which has some itself
-      while (row < hi) {
-        const int mid = (row + hi + 1) / 2;
-        if (before[mid] * tiles <= w0) row = mid;
-        else hi = mid - 1;
-      }
-    }
-    const int n0 = before[row + 1] - before[row];
-    const int rem = w0 - before[row] * tiles, vh0 = rem / n0;
-    Cursor c{row, vh0, rem - vh0 * n0, n0, head_tiles == 1 ? vh0 : vh0 / head_tiles}, ahead = c;
-    auto advance = [&](Cursor& x) {
-      if (++x.k < x.n) return;
-      x.k = 0;
-      ++x.vh;
-      x.kv = head_tiles == 1 ? x.vh : x.vh / head_tiles;
-      if (x.vh < tiles) return;
-      x.vh = x.kv = 0;
-      do {
-        ++x.row;
-      } while (x.row < a.rows && before[x.row + 1] == before[x.row]);
-      if (x.row < a.rows) x.n = before[x.row + 1] - before[x.row];
-    };
-    PageWindow win;
-    unsigned long long there = 0;                              // 16 bits for each round of the ring: its keys
-    int left = todo, put = 0, take = 0, len = length(row), len_row = row;
-    auto fetch = [&] {
-      if (left > 0) {
-        if (ahead.row != len_row) {
-          len_row = ahead.row;
-          len = length(len_row);
-        }
-        const unsigned keys = issue_round<R>(a, maps, win, ahead, len, box_shift, ring + put * R::kBytes, bars + put, lane);
-        there = (there & ~(0xffffull << (16 * put))) | (unsigned long long)keys << (16 * put);
-        put = put + 1 == S ? 0 : put + 1;
-        --left;
-        if (left > 0) advance(ahead);
-      }
-    };
-    const float scale2 = a.scale * kLog2e;
-    R x;
-    int from = c.k, head0 = 0, count = 0;
-    uint32_t phase = 0;
-    bool fresh = true, first = true;
-    todo += S - 1;
-#pragma unroll 1
-    for (int lead = S - 1; todo > 0; --todo) {
-      fetch();
-      if (lead > 0) {        // the first rounds are on their way before any is waited for
-        --lead;
-        continue;
-      }
-      if (fresh) {
-        const int tile = c.vh - c.kv * head_tiles;
-        head0 = c.kv * group + tile * tile_heads;
-        count = min(tile_heads, group - tile * tile_heads);
-        x.start(a, c.row, head0, count, q_vec, my_queries, lane);
-        from = c.k;
-        fresh = false;
-      }
-      mbar_wait(bars + take, phase, &aborted, kWaitFullTimeout);
-      const unsigned keys = (unsigned)(there >> (16 * take)) & 0xffffu;
-      if (keys != (1u << R::kKeys) - 1) {
-        // What lies where no key is may be NaN: a weight of zero times a value of zero instead.
-        unsigned char* values = ring + take * R::kBytes + R::kSegs * R::kSeg;
-        for (int i = lane; i < R::kSegs * R::kKeys * 8; i += 32)
-          if (!(keys >> (i >> 3 & (R::kKeys - 1)) & 1)) reinterpret_cast<uint4*>(values)[i] = make_uint4(0, 0, 0, 0);
-        fence_proxy_async_smem();                              // ahead of the copy that reuses the place
-        __syncwarp();
-      }
-      x.compute(smem_u32(ring) + take * R::kBytes, keys, scale2, my_queries, lane);
-      __syncwarp();
-      if (++take == S) {
-        take = 0;
-        phase ^= 1;
-      }
-      const bool last = c.k + 1 == c.n;
-      if (last || todo == 1) {
-        x.finish(lane);
-        if (from == 0 && last) {
-          T* out = static_cast<T*>(a.o) + c.row * a.o_row + (long long)head0 * a.o_head;
-          x.each(lane, [&](int h, int f, const auto& v, float, float l) {
-            if (h < count) store_out(out + h * a.o_head + f, v, 1.0f / l, a.hd - f, o_vec);
-          });
-        } else {
-          const int at = 2 * warp + (first ? 0 : 1);
-          float* part = first ? leads + warp * kPart : reinterpret_cast<float*>(rings + warp * S * R::kBytes);
-          __syncwarp();
-          x.each(lane, [&](int h, int f, const auto& v, float m, float l) {
-            if (h >= count) return;
-            constexpr int N = sizeof(v) / sizeof(float);
-#pragma unroll
-            for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(part + h * R::kHD + f + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-            if (f == 0) {
-              part[R::kHeads * R::kHD + h] = m;
-              part[R::kHeads * (R::kHD + 1) + h] = l;
-            }
-          });
-          if (lane == 0) {
-            part_job[at] = c.row * tiles + c.vh;
-            part_row[at] = c.row;
-            part_head[at] = head0;
-            part_count[at] = count;
-            part_begin[at] = before[c.row] * tiles + c.vh * c.n;
-            part_rounds[at] = c.n;
-          }
-        }
-        fresh = true;
-        first = false;
-      }
-      if (todo > 1) advance(c);
-    }
-  }
-  __syncthreads();
-
-  // Parts of a job are joined, first those of this CTA (stage 0): of a job that lies within it, to the output; of another's, to the workspace, place 0
-  // of the CTA for the job of its first round, 1 for one that begins later.  The last CTA that gets so far with a job joins what the
-  // workspace holds of it (stage 1), in the order of the CTAs.  Warps take turns at (job, head); lane j has part j.  One loop for both: this code
-  // runs once a launch, and what counts is how much of it there is to fetch.
   constexpr int kPer = R::kHD / 32;                            // features of a lane
   constexpr int kMax = R::kHeads * R::kHD, kSum = kMax + R::kHeads;
 #pragma unroll 1
   for (int stage = 0; stage < 2; ++stage) {
     unsigned jobs, same = 0;                                   // the jobs at hand: one of their parts in this CTA each
     if (stage == 0) {
-      const int job = lane < 2 * W ? part_job[lane] : -1;
+      const int job = lane < 2 * W ? sh.job[lane] : -1;
       same = __match_any_sync(0xffffffffu, job);
       jobs = __ballot_sync(0xffffffffu, job >= 0 && (same & ((1u << lane) - 1)) == 0);
     } else {
       __syncthreads();
-      if (shared_part[0] < 0 && shared_part[1] < 0) return;
+      if (sh.shared[0] < 0 && sh.shared[1] < 0) return;
       __threadfence();
       __syncthreads();
       if (tid < 2) {
-        const int i = shared_part[tid];
+        const int i = sh.shared[tid];
         int last = 0;
         if (i >= 0) {
-          const int first = part_begin[i] / share, n = (part_begin[i] + part_rounds[i] - 1) / share - first;
+          const int first = sh.begin[i] / share, n = (sh.begin[i] + sh.rounds[i] - 1) / share - first;
           last = atomicAdd(a.counters + first, 1u) == (unsigned)n;
           if (last) a.counters[first] = 0;
         }
-        merges[tid] = last;
+        sh.merges[tid] = last;
       }
       __syncthreads();
       __threadfence();
-      jobs = (merges[0] ? 1u << shared_part[0] : 0) | (merges[1] ? 1u << shared_part[1] : 0);
+      jobs = (sh.merges[0] ? 1u << sh.shared[0] : 0) | (sh.merges[1] ? 1u << sh.shared[1] : 0);
     }
     int unit = 0;
 #pragma unroll 1
     for (; jobs; jobs &= jobs - 1) {
-      const int i = __ffs(jobs) - 1, jb = part_begin[i], stop = jb + part_rounds[i], heads = part_count[i];
+      const int i = __ffs(jobs) - 1, jb = sh.begin[i], stop = jb + sh.rounds[i], heads = sh.count[i];
       const bool whole = jb >= begin && stop <= end;
       const unsigned group_of = __shfl_sync(0xffffffffu, same, i);
-      if (stage == 0 && !whole && tid == 0) shared_part[jb > begin] = i;
+      if (stage == 0 && !whole && tid == 0) sh.shared[jb > begin] = i;
       const int first = stage ? jb / share : 0, n = stage ? (stop - 1) / share - first + 1 : 32;
 #pragma unroll 1
       for (int h = 0; h < heads; ++h, ++unit) {
@@ -726,7 +538,7 @@ paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_con
           }
         }
         if (stage || whole) {
-          T* out = static_cast<T*>(a.o) + part_row[i] * a.o_row + (long long)(part_head[i] + h) * a.o_head;
+          T* out = static_cast<T*>(a.o) + sh.row[i] * a.o_row + (long long)(sh.head[i] + h) * a.o_head;
           const float by = 1.0f / l;
 #pragma unroll
           for (int e = 0; e < kPer; ++e)
@@ -745,6 +557,239 @@ paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_con
   }
 }
 
+// W warps, S rounds of a warp in flight or in use.
+template <typename R, int W, int S>
+__global__ void __launch_bounds__(W * 32, 1)
+paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_constant__ PageMaps maps, int box_shift, int head_tiles, int tile_heads, int q_vec, int o_vec) {
+  using T = typename R::T;
+  constexpr int kPart = Part<R>::kFloats;
+  static_assert(S * R::kBytes >= kPart * 4, "a warp's ring holds its last part");
+  extern __shared__ unsigned char smem[];
+  unsigned char* rings = smem + (1024 - (smem_u32(smem) & 1023) & 1023);      // [W][S] rounds
+  float* leads = reinterpret_cast<float*>(rings + W * S * R::kBytes);       // [W] parts
+  unsigned char* queries = reinterpret_cast<unsigned char*>(leads + W * kPart);   // [W][S] jobs' queries
+  int* before = reinterpret_cast<int*>(queries + W * S * R::kQueryBytes);   // [rows + 1]: rounds of a kv head ahead of a row
+  unsigned char* tails = reinterpret_cast<unsigned char*>(before + a.rows + 1);   // [rows]: tokens of a row's last round
+  __shared__ int scan[W + 1];
+  __shared__ Parts<W> sh;
+  __shared__ uint64_t landed[W * S];
+  __shared__ int aborted;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tiles = a.kv_heads * head_tiles;                                // jobs of a row
+  const int room = (int)min((long long)a.width * a.page, 0x7fffffffLL);
+  const int group = a.heads / a.kv_heads;
+
+  // Rounds ahead of every row.
+  auto length = [&](int r) { return max(0, min(a.lens[r], room)); };
+  bool equal = true;
+  int rounds0;
+  {
+    const int each = (a.rows + W * 32 - 1) / (W * 32), r0 = min(a.rows, tid * each), r1 = min(a.rows, r0 + each);
+    int mine = 0;
+    rounds0 = (length(0) + R::kKeys - 1) / R::kKeys;
+    for (int r = r0; r < r1; ++r) {
+      const int n = a.lens[r], k = (max(0, min(n, room)) + R::kKeys - 1) / R::kKeys;
+      if (n > room && blockIdx.x == 0) report_error(kBadPage);
+      mine += k;
+      equal = equal && k == rounds0;
+    }
+    int s = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += u;
+    }
+    if (lane == 31) scan[warp] = s;
+    __syncthreads();
+    int at = s - mine;
+    for (int w = 0; w < warp; ++w) at += scan[w];
+    for (int r = r0; r < r1; ++r) {
+      const int n = length(r);
+      before[r] = at;
+      tails[r] = n - (n - 1) / R::kKeys * R::kKeys;
+      at += (n + R::kKeys - 1) / R::kKeys;
+    }
+    if (tid == 0) {
+      int t = 0;
+      for (int w = 0; w < W; ++w) t += scan[w];
+      before[a.rows] = t;
+    }
+    if (tid < 2 * W) sh.job[tid] = -1;
+    if (tid < 2) sh.shared[tid] = -1;
+    if (a.hd < R::kHD)
+      for (int i = tid; i < W * S * R::kQueryBytes / 16; i += W * 32) reinterpret_cast<uint4*>(queries)[i] = make_uint4(0, 0, 0, 0);
+    fence_proxy_async_smem();
+    if (tid < W * S) mbar_init(landed + tid, 1);
+    if (tid == 0) aborted = 0;
+    mbar_fence_init();
+    equal = __syncthreads_and(equal);
+  }
+  const int total = before[a.rows] * tiles;                    // (below 2^31: the launcher sees to it)
+  // A CTA takes a round for each of its warps at least: parts of one CTA are joined sooner than those of several.  Whole jobs, where all
+  // are as long and short enough that each CTA still has its own at once.
+  int share = max(W, (int)((unsigned)(total + gridDim.x - 1) / gridDim.x));
+  if (equal && rounds0 > 0 && rounds0 <= 2 * W && a.rows * tiles <= gridDim.x) share = rounds0;
+  const int begin = (int)min((long long)total, (long long)share * blockIdx.x), end = min(total, begin + share);
+  for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {       // rows of no tokens
+    if (before[r + 1] > before[r]) continue;
+    for (int x = tid; x < a.heads * a.hd; x += W * 32) static_cast<T*>(a.o)[r * a.o_row + x / a.hd * a.o_head + x % a.hd] = from_f32<T>(0.0f);
+  }
+  if (begin >= end) return;
+
+  const int quota = (end - begin + W - 1) / W, w0 = min(end, begin + quota * warp), w1 = min(end, w0 + quota);
+  int todo = w1 - w0;
+  if (todo > 0) {
+    unsigned char* ring = rings + warp * S * R::kBytes;
+    uint64_t* bars = landed + warp * S;
+    unsigned char* my_queries = queries + warp * S * R::kQueryBytes;
+    int row = 0;
+    {
+      int hi = a.rows - 1;                                     // the last row with no more rounds ahead than w0, which has some itself
+      while (row < hi) {
+        const int mid = (row + hi + 1) / 2;
+        if (before[mid] * tiles <= w0) row = mid;
+        else hi = mid - 1;
+      }
+    }
+    const int n0 = before[row + 1] - before[row];
+    const int rem = w0 - before[row] * tiles, vh0 = rem / n0;
+    Cursor c{row, vh0, rem - vh0 * n0, n0, head_tiles == 1 ? vh0 : vh0 / head_tiles}, ahead = c;
+    auto advance = [&](Cursor& x) {
+      if (++x.k < x.n) return;
+      x.k = 0;
+      ++x.vh;
+      x.kv = head_tiles == 1 ? x.vh : x.vh / head_tiles;
+      if (x.vh < tiles) return;
+      x.vh = x.kv = 0;
+      do {
+        ++x.row;
+      } while (x.row < a.rows && before[x.row + 1] == before[x.row]);
+      if (x.row < a.rows) x.n = before[x.row + 1] - before[x.row];
+    };
+    PageWindow win;
+    unsigned long long there = 0;                              // 16 bits for each round of the ring: its keys
+    int left = todo, put = 0, take = 0, len = 0, len_row = -1, put_job = 0, take_job = 0;
+    bool new_job = true;
+    auto length_of = [&](int r) { return (before[r + 1] - before[r] - 1) * R::kKeys + tails[r]; };
+    auto fetch = [&] {
+      if (left == 0) return;
+      if (ahead.row != len_row) {
+        len_row = ahead.row;
+        len = length_of(len_row);
+      }
+      uint64_t* bar = bars + put;
+      if (new_job) {
+        // The job's queries come with its first round: loaded when the job starts, they cost each job the latency of the memory.  A place is free
+        // again when the job S before is done: a fetch is at most S - 1 rounds ahead.
+        const int tile = ahead.vh - ahead.kv * head_tiles, heads = min(tile_heads, group - tile * tile_heads);
+        const T* src = static_cast<const T*>(a.q) + ahead.row * a.q_row + (long long)(ahead.kv * group + tile * tile_heads + lane) * a.q_head;
+        unsigned char* dst = my_queries + put_job * R::kQueryBytes + lane * (R::kHD * (int)sizeof(T));
+        const int bytes = a.hd * (int)sizeof(T);
+        if (q_vec) {
+          if (lane == 0) mbar_expect_tx(bar, heads * bytes);
+          __syncwarp();
+          if (lane < heads) bulk_load(dst, src, bytes, bar);
+        } else if (lane < heads) {
+          for (int f = 0; f < a.hd; ++f) reinterpret_cast<T*>(dst)[f] = src[f];
+        }
+        __syncwarp();
+        put_job = put_job + 1 == S ? 0 : put_job + 1;
+      }
+      const unsigned keys = issue_round<R>(a, maps, win, ahead, len, box_shift, ring + put * R::kBytes, bar, lane);
+      there = (there & ~(0xffffull << (16 * put))) | (unsigned long long)keys << (16 * put);
+      put = put + 1 == S ? 0 : put + 1;
+      if (--left == 0) return;
+      const int was = ahead.row;
+      if (new_job && win.next_row <= was) {                    // the row after this one
+        int r = was + 1;
+        while (r < a.rows && before[r + 1] == before[r]) ++r;
+        if (r < a.rows) win.ahead(a, r, length_of(r), lane);
+      }
+      advance(ahead);
+      new_job = ahead.k == 0;
+    };
+    const float scale2 = a.scale * kLog2e;
+    R x;
+    int from = c.k, head0 = 0, count = 0;
+    uint32_t phase = 0;
+    bool fresh = true, first = true;
+    todo += S - 1;
+#pragma unroll 1
+    for (int lead = S - 1; todo > 0; --todo) {
+      fetch();
+      if (lead > 0) {        // the first rounds are on their way before any is waited for
+        --lead;
+        continue;
+      }
+      if (fresh) {
+        const int tile = c.vh - c.kv * head_tiles;
+        head0 = c.kv * group + tile * tile_heads;
+        count = min(tile_heads, group - tile * tile_heads);
+        from = c.k;
+      }
+      mbar_wait(bars + take, phase, &aborted, kWaitFullTimeout);
+      if (fresh) {
+        x.start(a, my_queries + take_job * R::kQueryBytes, count, lane);
+        fresh = false;
+      }
+      const unsigned keys = (unsigned)(there >> (16 * take)) & 0xffffu;
+      if (keys != (1u << R::kKeys) - 1) {
+        // What lies where no key is may be NaN: a weight of zero times a value of zero instead.
+        unsigned char* values = ring + take * R::kBytes + R::kSegs * R::kSeg;
+        for (int i = lane; i < R::kSegs * R::kKeys * 8; i += 32)
+          if (!(keys >> (i >> 3 & (R::kKeys - 1)) & 1)) reinterpret_cast<uint4*>(values)[i] = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();                              // ahead of the copy that reuses the place
+        __syncwarp();
+      }
+      x.compute(smem_u32(ring) + take * R::kBytes, keys, scale2, my_queries + take_job * R::kQueryBytes, lane);
+      __syncwarp();
+      if (++take == S) {
+        take = 0;
+        phase ^= 1;
+      }
+      const bool last = c.k + 1 == c.n;
+      if (last || todo == 1) {
+        x.finish(lane);
+        if (from == 0 && last) {
+          T* out = static_cast<T*>(a.o) + c.row * a.o_row + (long long)head0 * a.o_head;
+          x.each(lane, [&](int h, int f, const auto& v, float, float l) {
+            if (h < count) store_out(out + h * a.o_head + f, v, 1.0f / l, a.hd - f, o_vec);
+          });
+        } else {
+          const int at = 2 * warp + (first ? 0 : 1);
+          float* part = first ? leads + warp * kPart : reinterpret_cast<float*>(rings + warp * S * R::kBytes);
+          __syncwarp();
+          x.each(lane, [&](int h, int f, const auto& v, float m, float l) {
+            if (h >= count) return;
+            constexpr int N = sizeof(v) / sizeof(float);
+#pragma unroll
+            for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(part + h * R::kHD + f + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+            if (f == 0) {
+              part[R::kHeads * R::kHD + h] = m;
+              part[R::kHeads * (R::kHD + 1) + h] = l;
+            }
+          });
+          if (lane == 0) {
+            sh.job[at] = c.row * tiles + c.vh;
+            sh.row[at] = c.row;
+            sh.head[at] = head0;
+            sh.count[at] = count;
+            sh.begin[at] = before[c.row] * tiles + c.vh * c.n;
+            sh.rounds[at] = c.n;
+          }
+        }
+        fresh = true;
+        first = false;
+        take_job = take_job + 1 == S ? 0 : take_job + 1;
+      }
+      if (todo > 1) advance(c);
+    }
+  }
+  __syncthreads();
+
+  join_parts<R, W, S>(a, sh, rings, leads, begin, end, share);
+}
+
 // Map of the pages [pages, kv_heads, page, hd]: tiles of 128 bytes of `box` tokens.
 static int map_pages(CUtensorMap* map, const PagedAttnArgs& a, const void* base, long long page, long long head, long long tok, int box) {
   const uint64_t e = a.f32 ? 4 : 2;
@@ -756,7 +801,7 @@ static int map_pages(CUtensorMap* map, const PagedAttnArgs& a, const void* base,
 
 template <typename R, int W, int S>
 static int launch_paged(const PagedAttnArgs& a, const PageMaps& maps, int head_tiles, int tile_heads, bool q_vec, bool o_vec, cudaStream_t st) {
-  const size_t smem = 1024 + (size_t)W * S * R::kBytes + W * (Part<R>::kFloats * 4 + R::kQueryBytes) + (a.rows + 1) * 4;
+  const size_t smem = 1024 + (size_t)W * S * (R::kBytes + R::kQueryBytes) + W * Part<R>::kFloats * 4 + (a.rows + 1) * 4 + a.rows;
   constexpr int kLimit = 226 << 10;
   static SmemLimit limit;
   const int grid = sm_count();
@@ -867,15 +912,15 @@ extern "C" int dptb_paged_attention(const PagedAttnArgs* args, void* stream) {
       using B64 = Bf16Round<64, 1>; using C64 = Bf16Round<64, 2>;
       using B128 = Bf16Round<128, 1>; using C128 = Bf16Round<128, 2>;
       using B256 = Bf16Round<256, 1>;
-      if (a.hd <= 64) { if (group <= 8) DPTB_PAGED(B64, 8, 4); DPTB_PAGED(C64, 8, 4); }
-      if (a.hd <= 128) { if (group <= 8) DPTB_PAGED(B128, 8, 2); DPTB_PAGED(C128, 8, 2); }
+      if (a.hd <= 64) { if (group <= 8) DPTB_PAGED(B64, 8, 4); DPTB_PAGED(C64, 8, 3); }
+      if (a.hd <= 128) { if (group <= 8) DPTB_PAGED(B128, 8, 2); DPTB_PAGED(C128, 6, 2); }
       DPTB_PAGED(B256, 4, 2);
     }
     using F1_64 = F32Round<64, 1>; using F4_64 = F32Round<64, 4>; using F8_64 = F32Round<64, 8>;
     using F1_128 = F32Round<128, 1>; using F4_128 = F32Round<128, 4>; using F8_128 = F32Round<128, 8>;
     using F1_256 = F32Round<256, 1>; using F4_256 = F32Round<256, 4>;
     if (a.hd <= 64) { if (group == 1) DPTB_PAGED(F1_64, 8, 4); if (group <= 4) DPTB_PAGED(F4_64, 8, 4); DPTB_PAGED(F8_64, 8, 4); }
-    if (a.hd <= 128) { if (group == 1) DPTB_PAGED(F1_128, 8, 2); if (group <= 4) DPTB_PAGED(F4_128, 8, 2); DPTB_PAGED(F8_128, 8, 2); }
+    if (a.hd <= 128) { if (group == 1) DPTB_PAGED(F1_128, 8, 2); if (group <= 4) DPTB_PAGED(F4_128, 8, 2); DPTB_PAGED(F8_128, 7, 2); }
     if (group == 1) DPTB_PAGED(F1_256, 4, 2);
     DPTB_PAGED(F4_256, 4, 2);
 #undef DPTB_PAGED
