@@ -101,6 +101,7 @@ struct PageWindow {
 // A place in the sequence of rounds: round k of the n rounds of job (row, vh); vh counts kv heads and within them tiles of query heads.
 struct Cursor {
   int row, vh, k, n, kv;
+  int unit;      // its number in the sequence
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -568,7 +569,7 @@ paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_con
   unsigned char* rings = smem + (1024 - (smem_u32(smem) & 1023) & 1023);      // [W][S] rounds
   float* leads = reinterpret_cast<float*>(rings + W * S * R::kBytes);       // [W] parts
   unsigned char* queries = reinterpret_cast<unsigned char*>(leads + W * kPart);   // [W][S] jobs' queries
-  int* before = reinterpret_cast<int*>(queries + W * S * R::kQueryBytes);   // [rows + 1]: rounds of a kv head ahead of a row
+  int* before = reinterpret_cast<int*>(queries + W * S * R::kQueryBytes);   // [rows + 1]: units of a kv head ahead of a row
   unsigned char* tails = reinterpret_cast<unsigned char*>(before + a.rows + 1);   // [rows]: tokens of a row's last round
   __shared__ int scan[W + 1];
   __shared__ Parts<W> sh;
@@ -579,7 +580,8 @@ paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_con
   const int room = (int)min((long long)a.width * a.page, 0x7fffffffLL);
   const int group = a.heads / a.kv_heads;
 
-  // Rounds ahead of every row.
+  // Units ahead of every row: a job is its rounds and, before them, one unit for what it costs to begin and end it (2100 cycles where a round took
+  // 2500; without it the warps of the shortest rows came last by a quarter).
   auto length = [&](int r) { return max(0, min(a.lens[r], room)); };
   bool equal = true;
   int rounds0;
@@ -590,7 +592,7 @@ paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_con
     for (int r = r0; r < r1; ++r) {
       const int n = a.lens[r], k = (max(0, min(n, room)) + R::kKeys - 1) / R::kKeys;
       if (n > room && blockIdx.x == 0) report_error(kBadPage);
-      mine += k;
+      mine += k + (k > 0);
       equal = equal && k == rounds0;
     }
     int s = mine;
@@ -607,7 +609,7 @@ paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_con
       const int n = length(r);
       before[r] = at;
       tails[r] = n - (n - 1) / R::kKeys * R::kKeys;
-      at += (n + R::kKeys - 1) / R::kKeys;
+      at += (n + R::kKeys - 1) / R::kKeys + (n > 0);
     }
     if (tid == 0) {
       int t = 0;
@@ -625,10 +627,10 @@ paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_con
     equal = __syncthreads_and(equal);
   }
   const int total = before[a.rows] * tiles;                    // (below 2^31: the launcher sees to it)
-  // A CTA takes a round for each of its warps at least: parts of one CTA are joined sooner than those of several.  Whole jobs, where all
+  // A CTA takes a unit for each of its warps at least: parts of one CTA are joined sooner than those of several.  Whole jobs, where all
   // are as long and short enough that each CTA still has its own at once.
   int share = max(W, (int)((unsigned)(total + gridDim.x - 1) / gridDim.x));
-  if (equal && rounds0 > 0 && rounds0 <= 2 * W && a.rows * tiles <= gridDim.x) share = rounds0;
+  if (equal && rounds0 > 0 && rounds0 <= 2 * W && a.rows * tiles <= gridDim.x) share = rounds0 + 1;
   const int begin = (int)min((long long)total, (long long)share * blockIdx.x), end = min(total, begin + share);
   for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {       // rows of no tokens
     if (before[r + 1] > before[r]) continue;
@@ -637,25 +639,25 @@ paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_con
   if (begin >= end) return;
 
   const int quota = (end - begin + W - 1) / W, w0 = min(end, begin + quota * warp), w1 = min(end, w0 + quota);
-  int todo = w1 - w0;
-  if (todo > 0) {
+  if (w0 < w1) {
     unsigned char* ring = rings + warp * S * R::kBytes;
     uint64_t* bars = landed + warp * S;
     unsigned char* my_queries = queries + warp * S * R::kQueryBytes;
     int row = 0;
     {
-      int hi = a.rows - 1;                                     // the last row with no more rounds ahead than w0, which has some itself
+      int hi = a.rows - 1;                                     // the last row with no more units ahead than w0, which has some itself
       while (row < hi) {
         const int mid = (row + hi + 1) / 2;
         if (before[mid] * tiles <= w0) row = mid;
         else hi = mid - 1;
       }
     }
-    const int n0 = before[row + 1] - before[row];
-    const int rem = w0 - before[row] * tiles, vh0 = rem / n0;
-    Cursor c{row, vh0, rem - vh0 * n0, n0, head_tiles == 1 ? vh0 : vh0 / head_tiles}, ahead = c;
+    const int n0 = before[row + 1] - before[row] - 1, rem = w0 - before[row] * tiles, vh0 = rem / (n0 + 1), u0 = rem - vh0 * (n0 + 1);
+    Cursor c{row, vh0, max(u0 - 1, 0), n0, head_tiles == 1 ? vh0 : vh0 / head_tiles, w0 + (u0 == 0)}, ahead = c;
     auto advance = [&](Cursor& x) {
+      ++x.unit;
       if (++x.k < x.n) return;
+      ++x.unit;
       x.k = 0;
       ++x.vh;
       x.kv = head_tiles == 1 ? x.vh : x.vh / head_tiles;
@@ -664,15 +666,15 @@ paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_con
       do {
         ++x.row;
       } while (x.row < a.rows && before[x.row + 1] == before[x.row]);
-      if (x.row < a.rows) x.n = before[x.row + 1] - before[x.row];
+      if (x.row < a.rows) x.n = before[x.row + 1] - before[x.row] - 1;
     };
     PageWindow win;
     unsigned long long there = 0;                              // 16 bits for each round of the ring: its keys
-    int left = todo, put = 0, take = 0, len = 0, len_row = -1, put_job = 0, take_job = 0;
+    int put = 0, take = 0, len = 0, len_row = -1, put_job = 0, take_job = 0;
     bool new_job = true;
-    auto length_of = [&](int r) { return (before[r + 1] - before[r] - 1) * R::kKeys + tails[r]; };
+    auto length_of = [&](int r) { return (before[r + 1] - before[r] - 2) * R::kKeys + tails[r]; };
     auto fetch = [&] {
-      if (left == 0) return;
+      if (ahead.unit >= w1) return;
       if (ahead.row != len_row) {
         len_row = ahead.row;
         len = length_of(len_row);
@@ -698,7 +700,6 @@ paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_con
       const unsigned keys = issue_round<R>(a, maps, win, ahead, len, box_shift, ring + put * R::kBytes, bar, lane);
       there = (there & ~(0xffffull << (16 * put))) | (unsigned long long)keys << (16 * put);
       put = put + 1 == S ? 0 : put + 1;
-      if (--left == 0) return;
       const int was = ahead.row;
       if (new_job && win.next_row <= was) {                    // the row after this one
         int r = was + 1;
@@ -713,14 +714,14 @@ paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_con
     int from = c.k, head0 = 0, count = 0;
     uint32_t phase = 0;
     bool fresh = true, first = true;
-    todo += S - 1;
 #pragma unroll 1
-    for (int lead = S - 1; todo > 0; --todo) {
+    for (int lead = S - 1;;) {
       fetch();
       if (lead > 0) {        // the first rounds are on their way before any is waited for
         --lead;
         continue;
       }
+      if (c.unit >= w1) break;
       if (fresh) {
         const int tile = c.vh - c.kv * head_tiles;
         head0 = c.kv * group + tile * tile_heads;
@@ -748,10 +749,13 @@ paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_con
         phase ^= 1;
       }
       const bool last = c.k + 1 == c.n;
-      if (last || todo == 1) {
+      const int job_begin = c.unit - c.k;
+      const Cursor was = c;
+      advance(c);
+      if (last || c.unit >= w1) {
         x.finish(lane);
         if (from == 0 && last) {
-          T* out = static_cast<T*>(a.o) + c.row * a.o_row + (long long)head0 * a.o_head;
+          T* out = static_cast<T*>(a.o) + was.row * a.o_row + (long long)head0 * a.o_head;
           x.each(lane, [&](int h, int f, const auto& v, float, float l) {
             if (h < count) store_out(out + h * a.o_head + f, v, 1.0f / l, a.hd - f, o_vec);
           });
@@ -770,19 +774,18 @@ paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_con
             }
           });
           if (lane == 0) {
-            sh.job[at] = c.row * tiles + c.vh;
-            sh.row[at] = c.row;
+            sh.job[at] = was.row * tiles + was.vh;
+            sh.row[at] = was.row;
             sh.head[at] = head0;
             sh.count[at] = count;
-            sh.begin[at] = before[c.row] * tiles + c.vh * c.n;
-            sh.rounds[at] = c.n;
+            sh.begin[at] = job_begin;
+            sh.rounds[at] = was.n;
           }
         }
         fresh = true;
         first = false;
         take_job = take_job + 1 == S ? 0 : take_job + 1;
       }
-      if (todo > 1) advance(c);
     }
   }
   __syncthreads();
