@@ -31,6 +31,7 @@ struct BeamArgs {
   long long ld, ws_bytes;
   int items, beams, vocab, eos, f32;
 };
+static_assert(sizeof(BeamArgs) == 104, "packed by the caller");
 
 // Larger for a larger value, then for a lower index; zeros of both signs are one value.
 __device__ __forceinline__ unsigned long long rank_key(float x, int index) {

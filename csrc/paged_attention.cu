@@ -52,6 +52,7 @@ struct PagedAttnArgs {
   // 2^(page_shift - 31) >= page, so the excess of page_mul adds less than 2^31 * page / 2^page_shift <= 1 quotient's last place.
   unsigned page_mul, page_shift;
 };
+static_assert(sizeof(PagedAttnArgs) == 216, "packed by the caller");
 
 __device__ __forceinline__ int slot_of(const PagedAttnArgs& a, int pos) { return (int)((unsigned long long)pos * a.page_mul >> a.page_shift); }
 

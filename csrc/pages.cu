@@ -33,6 +33,7 @@ struct AppendArgs {
   int tokens, heads, kv_heads, hd, rotary, page, width, pages, table_rows, f32;
   double base;
 };
+static_assert(sizeof(AppendArgs) == 176, "packed by the caller");
 
 constexpr int kAppendThreads = 256;
 constexpr int kAppendPairs = 128;    // of a head of 256 features
@@ -194,6 +195,7 @@ struct ForkArgs {
   long long table_row;
   int rows_in, rows, width, pages, page, grow_all;
 };
+static_assert(sizeof(ForkArgs) == 104, "packed by the caller");
 
 struct ForkRow {
   int parent, old_len, new_len, held, want;
@@ -332,6 +334,7 @@ struct CompactArgs {
   long long table_row;
   int rows, width, pages;
 };
+static_assert(sizeof(CompactArgs) == 64, "packed by the caller");
 
 __global__ void __launch_bounds__(kPageThreads)
 compact_pages_kernel(const CompactArgs a, int words) {

@@ -3,12 +3,14 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from typing import Optional, Tuple
 
 import torch
 
 from .. import _native as N
-from .paged import _here, _no_grad
+from .kernels import SPLITK_WS_BYTES as WS_BYTES
+from .paged import _BF16, _F32, _current_device, _here, _no_grad, _raw_stream, _scratch
 
 c_void_p, c_int, c_ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
 
@@ -16,11 +18,8 @@ MAX_BEAMS = 32
 MAX_ROWS = 1 << 20
 
 
-class BeamArgs(ctypes.Structure):
-    _fields_ = [(n, c_void_p) for n in ("logits", "scores", "finished", "out_scores", "out_parents", "out_tokens", "out_finished",
-                                        "ws")] + \
-        [(n, c_ll) for n in ("ld", "ws_bytes")] + [(n, c_int) for n in ("items", "beams", "vocab", "eos", "f32")]
-
+# The C struct's fields in order (see ops/paged.py).
+_BEAM_ARGS = struct.Struct("8P 2q 5i4x")
 
 _declared = False
 
@@ -29,7 +28,7 @@ def _lib():
     global _declared
     lib = N.load()
     if not _declared:
-        lib.dptb_beam_step.argtypes, lib.dptb_beam_step.restype = [ctypes.POINTER(BeamArgs), c_void_p], c_int
+        lib.dptb_beam_step.argtypes, lib.dptb_beam_step.restype = [ctypes.c_char_p, c_void_p], c_int
         lib.dptb_beam_ws_bytes.argtypes, lib.dptb_beam_ws_bytes.restype = [c_int, c_int], c_ll
         _declared = True
     return lib
@@ -70,6 +69,46 @@ def beam_step(logits: torch.Tensor, scores: torch.Tensor, finished: Optional[tor
 
     Returns ``(scores, parents, tokens, finished)``, each ``[items, beams]``, best first: ``parents`` (int32) are rows of ``logits``,
     as ``fork_pages`` takes them, ``tokens`` int64.  Up to 32 beams."""
+    dev, last = logits.get_device(), -1 if eos is None else eos
+    if not (dev >= 0 and scores.dim() == 2 and logits.dim() == 2) or _beam_is_off(logits, scores, finished, eos, dev):
+        _check_beam(logits, scores, finished, eos)
+        if dev < 0:
+            return beam_step_reference(logits, scores, finished, last)
+        if logits.stride(1) != 1 and logits.shape[1] > 1:
+            logits = logits.contiguous()
+        scores = scores.contiguous()
+        finished = None if finished is None else finished.contiguous()
+    (items, beams), vocab = scores.shape, logits.shape[1]
+    out_scores = scores.new_empty((items, beams))
+    out_parents = torch.empty((items, beams), dtype=torch.int32, device=logits.device)
+    out_tokens = torch.empty((items, beams), dtype=torch.long, device=logits.device)
+    out_finished = torch.empty((items, beams), dtype=torch.bool, device=logits.device)
+    lib, stream = _lib(), _raw_stream(dev)
+    ws = _scratch(dev, stream)[0]
+    room = WS_BYTES
+    if lib.dptb_beam_ws_bytes(items, beams) > room:
+        room = lib.dptb_beam_ws_bytes(items, beams)
+        ws = torch.empty(room, dtype=torch.uint8, device=logits.device)
+    N.check(lib.dptb_beam_step(_BEAM_ARGS.pack(
+        logits.data_ptr(), scores.data_ptr(), 0 if finished is None else finished.data_ptr(), out_scores.data_ptr(),
+        out_parents.data_ptr(), out_tokens.data_ptr(), out_finished.data_ptr(), ws.data_ptr(), logits.stride(0), room, items, beams,
+        vocab, last, logits.dtype is _F32), stream), "beam_step")
+    return out_scores, out_parents, out_tokens, out_finished
+
+
+def _beam_is_off(logits, scores, finished, eos, dev) -> bool:
+    """Whether ``_check_beam`` has to look: everything it asks for, at the price of a call on each step."""
+    (items, beams), (rows, vocab) = scores.shape, logits.shape
+    return not (
+        scores.dtype is _F32 and (logits.dtype is _BF16 or logits.dtype is _F32) and rows == items * beams and 0 < vocab < 1 << 31 and
+        0 < beams <= MAX_BEAMS and rows <= MAX_ROWS and scores.is_contiguous() and logits.stride(1) == 1 and
+        (eos is None or 0 <= eos < vocab) and scores.get_device() == dev and _current_device() == dev and
+        (finished is None or eos is not None and finished.dtype is torch.bool and finished.shape == scores.shape and
+         finished.get_device() == dev and finished.is_contiguous()) and
+        not ((logits.requires_grad or scores.requires_grad) and torch.is_grad_enabled()))
+
+
+def _check_beam(logits, scores, finished, eos) -> None:
     what = "beam_step"
     if scores.dim() != 2 or scores.dtype != torch.float32:
         raise ValueError(f"{what}: scores must be fp32 [items, beams], got {scores.dtype} {list(scores.shape)}")
@@ -88,25 +127,3 @@ def beam_step(logits: torch.Tensor, scores: torch.Tensor, finished: Optional[tor
         raise ValueError(f"{what}: finished beams need an eos to go on with")
     _here(what, logits, scores, finished)
     _no_grad(what, logits, scores)
-    last = -1 if eos is None else eos
-    if not logits.is_cuda:
-        return beam_step_reference(logits, scores, finished, last)
-    from .kernels import splitk_workspace
-    if logits.stride(1) != 1 and logits.shape[1] > 1:
-        logits = logits.contiguous()
-    scores = scores.contiguous()
-    finished = None if finished is None else finished.contiguous()
-    dev = logits.device
-    out_scores = torch.empty(items, beams, dtype=torch.float32, device=dev)
-    out_parents = torch.empty(items, beams, dtype=torch.int32, device=dev)
-    out_tokens = torch.empty(items, beams, dtype=torch.long, device=dev)
-    out_finished = torch.empty(items, beams, dtype=torch.bool, device=dev)
-    lib = _lib()
-    ws = splitk_workspace(dev)[0]
-    if lib.dptb_beam_ws_bytes(items, beams) > ws.numel():
-        ws = torch.empty(lib.dptb_beam_ws_bytes(items, beams), dtype=torch.uint8, device=dev)
-    a = BeamArgs(logits.data_ptr(), scores.data_ptr(), N.ptr(finished), out_scores.data_ptr(), out_parents.data_ptr(),
-                 out_tokens.data_ptr(), out_finished.data_ptr(), ws.data_ptr(), logits.stride(0), ws.numel(), items, beams,
-                 logits.shape[1], last, logits.dtype == torch.float32)
-    N.check(lib.dptb_beam_step(a, N.stream_ptr()), what)
-    return out_scores, out_parents, out_tokens, out_finished

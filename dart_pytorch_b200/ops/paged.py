@@ -15,46 +15,32 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from typing import Optional, Tuple, Union
 
 import torch
 
 from .. import _native as N
-from .kernels import splitk_workspace
+from . import kernels
 
-c_void_p, c_int, c_ll, c_float = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
-c_double = ctypes.c_double
+c_void_p, c_int, c_ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
+_current_device, _raw_stream, _increment_version = None, None, torch._C._increment_version
+if torch.cuda.is_available():
+    _current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+_F32, _BF16, _I32 = torch.float32, torch.bfloat16, torch.int32
 
 MAX_HEAD_DIM = 256
 MAX_ROWS = 4096           # rows of a table in one call
 MAX_PAGES = 1 << 19
+TOO_LARGE = -4
 
 
-class PagedAttnArgs(ctypes.Structure):
-    _fields_ = [(n, c_void_p) for n in ("q", "k", "v", "o", "table", "lens")] + \
-        [(n, c_ll) for n in ("q_row", "q_head", "o_row", "o_head", "k_page", "k_head", "k_tok", "v_page", "v_head", "v_tok",
-                             "table_row")] + \
-        [(n, c_int) for n in ("rows", "heads", "kv_heads", "hd", "page", "width", "pages", "f32")] + [("scale", c_float)] + \
-        [("ws", c_void_p), ("ws_floats", c_ll), ("counters", c_void_p), ("num_counters", c_int), ("page_mul", ctypes.c_uint),
-         ("page_shift", ctypes.c_uint)]
-
-
-class AppendArgs(ctypes.Structure):
-    _fields_ = [(n, c_void_p) for n in ("qkv", "q", "keys", "k", "v", "table", "positions", "rows")] + \
-        [(n, c_ll) for n in ("ld", "k_page", "k_head", "k_tok", "v_page", "v_head", "v_tok", "table_row")] + \
-        [(n, c_int) for n in ("tokens", "heads", "kv_heads", "hd", "rotary", "page", "width", "pages", "table_rows", "f32")] + \
-        [("base", c_double)]
-
-
-class ForkArgs(ctypes.Structure):
-    _fields_ = [(n, c_void_p) for n in ("table", "lens", "parents", "grow", "new_table", "new_lens", "src", "dst", "free_list")] + \
-        [("table_row", c_ll)] + [(n, c_int) for n in ("rows_in", "rows", "width", "pages", "page", "grow_all")]
-
-
-class CompactArgs(ctypes.Structure):
-    _fields_ = [(n, c_void_p) for n in ("table", "new_table", "src", "dst", "live")] + \
-        [("table_row", c_ll)] + [(n, c_int) for n in ("rows", "width", "pages")]
-
+# Arguments of the entry points, in the order and with the padding of their C structs (a ctypes.Structure takes 1.6 us to fill, a
+# packed one 0.25; a step of decoding makes a call or two a layer).
+_ATTN_ARGS = struct.Struct("6P 11q 8i f4x Pq P iII4x")
+_APPEND_ARGS = struct.Struct("8P 8q 10i d")
+_FORK_ARGS = struct.Struct("9P q 6i")
+_COMPACT_ARGS = struct.Struct("5P q 3i4x")
 
 _declared = False
 
@@ -63,14 +49,22 @@ def _lib():
     global _declared
     lib = N.load()
     if not _declared:
-        for name, args in (("dptb_paged_attention", PagedAttnArgs), ("dptb_paged_append", AppendArgs),
-                           ("dptb_fork_pages", ForkArgs), ("dptb_compact_pages", CompactArgs)):
+        for name in ("dptb_paged_attention", "dptb_paged_append", "dptb_fork_pages", "dptb_compact_pages"):
             fn = getattr(lib, name)
-            fn.argtypes, fn.restype = [ctypes.POINTER(args), c_void_p], c_int
+            fn.argtypes, fn.restype = [ctypes.c_char_p, c_void_p], c_int
         lib.dptb_copy_pages.argtypes = [c_void_p, c_void_p, c_void_p, c_int, c_ll, c_int, c_ll, c_void_p]
         lib.dptb_copy_pages.restype = c_int
         _declared = True
     return lib
+
+
+def _scratch(dev: int, stream: int):
+    """``splitk_workspace`` of the stream, which is what it is looked up by."""
+    if not torch._C._cuda_isCurrentStreamCapturing():
+        held = kernels._SPLITK_WS.get((dev, stream))
+        if held is not None:
+            return held[0], held[1]
+    return kernels.splitk_workspace(torch.device("cuda", dev))
 
 
 # ------------------------------------------------------------------------------------------------------------ checks
@@ -144,6 +138,48 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     """Attention of one new token per row, ``q [rows, heads, head_dim]``, over the ``lens[r]`` tokens of its pages (the new one
     among them).  Query heads share key heads in groups of ``heads // kv_heads``; a row of no tokens gives zeros.  bf16 or fp32, one type for all; sums in
     fp32.  ``scale`` is ``head_dim ** -0.5`` unless given.  Returns ``[rows, heads, head_dim]``."""
+    dev = q.get_device()
+    if not (dev >= 0 and q.dim() == 3 and k_pages.dim() == 4 and table.dim() == 2):
+        return _attention_on_cpu(q, k_pages, v_pages, table, lens, scale, out)
+    (rows, heads, hd), (pages, hkv, page, _), (_, width) = q.shape, k_pages.shape, table.shape
+    (q_row, q_head, q_one), (kp, kh, kt, k_one), (vp, vh, vt, v_one) = q.stride(), k_pages.stride(), v_pages.stride()
+    if q_one != 1 or out is not None or _attention_is_off(q, k_pages, v_pages, table, lens, dev, q.dtype, k_one, v_one):
+        _check_attention(q, k_pages, v_pages, table, lens, out)
+        if q_one != 1 and hd > 1:
+            q = q.contiguous()
+            q_row, q_head, _ = q.stride()
+    if out is None:
+        out = q.new_empty((rows, heads, hd))
+        o_row, o_head = heads * hd, hd
+    else:
+        o_row, o_head, _ = out.stride()
+    stream = _raw_stream(dev)
+    ws, counters = _scratch(dev, stream)
+    rc = _lib().dptb_paged_attention(_ATTN_ARGS.pack(
+        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), table.data_ptr(), lens.data_ptr(),
+        q_row, q_head, o_row, o_head, kp, kh, kt, vp, vh, vt, table.stride(0),
+        rows, heads, hkv, hd, page, width, pages, q.dtype is _F32, hd ** -0.5 if scale is None else scale,
+        ws.data_ptr(), kernels.SPLITK_WS_BYTES // 4, counters.data_ptr(), kernels.SPLITK_COUNTERS, 0, 0), stream)
+    if rc == TOO_LARGE:
+        raise ValueError(f"paged_attention: {rows} rows of up to {width * page} tokens and {heads} heads in one call are too many")
+    N.check(rc, "paged_attention")
+    return out
+
+
+def _attention_is_off(q, k, v, table, lens, dev, dtype, k_one, v_one) -> bool:
+    """Whether ``_check_attention`` has to look: everything it asks for, at the price of a call on each step."""
+    rows, heads, hd = q.shape
+    pages, hkv, page, k_hd = k.shape
+    return not (
+        (dtype is _BF16 or dtype is _F32) and k.dtype is dtype and v.dtype is dtype and table.dtype is _I32 and lens.dtype is _I32 and
+        v.shape == k.shape and k_hd == hd and table.shape[0] == rows and lens.shape == (rows,) and 0 < hd <= MAX_HEAD_DIM and
+        0 < hkv and heads % hkv == 0 and 0 < page and pages <= MAX_PAGES and rows <= MAX_ROWS and k_one == 1 and v_one == 1 and
+        (table.stride(1) == 1 or table.shape[1] <= 1) and (rows <= 1 or lens.stride(0) == 1) and
+        k.get_device() == dev and v.get_device() == dev and table.get_device() == dev and lens.get_device() == dev and
+        _current_device() == dev and not ((q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled()))
+
+
+def _check_attention(q, k_pages, v_pages, table, lens, out) -> None:
     what = "paged_attention"
     _pages(what, k_pages, v_pages)
     _table(what, table)
@@ -158,25 +194,12 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     _no_grad(what, q, k_pages, v_pages)
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 and hd > 1):
         raise ValueError(f"{what}: out must be {list(q.shape)} {q.dtype} with contiguous features")
-    if not q.is_cuda:
-        o = paged_attention_reference(q, k_pages, v_pages, table, lens, scale)
-        return o if out is None else out.copy_(o)
-    if q.stride(2) != 1 and hd > 1:
-        q = q.contiguous()
-    if out is None:
-        out = torch.empty(rows, heads, hd, dtype=q.dtype, device=q.device)
-    (q_row, q_head, _), (o_row, o_head, _) = q.stride(), out.stride()
-    kp, kh, kt, _ = k_pages.stride()
-    vp, vh, vt, _ = v_pages.stride()
-    pages, hkv, page, _ = k_pages.shape
-    ws, counters = splitk_workspace(q.device)
-    a = PagedAttnArgs(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), table.data_ptr(), lens.data_ptr(),
-                      q_row, q_head, o_row, o_head, kp, kh, kt, vp, vh, vt, table.stride(0),
-                      rows, heads, hkv, hd, page, table.shape[1], pages, q.dtype == torch.float32,
-                      1.0 / math.sqrt(hd) if scale is None else scale, ws.data_ptr(), ws.numel() // 4, counters.data_ptr(),
-                      counters.numel())
-    N.check(_lib().dptb_paged_attention(a, N.stream_ptr()), what)
-    return out
+
+
+def _attention_on_cpu(q, k_pages, v_pages, table, lens, scale, out):
+    _check_attention(q, k_pages, v_pages, table, lens, out)
+    o = paged_attention_reference(q, k_pages, v_pages, table, lens, scale)
+    return o if out is None else out.copy_(o)
 
 
 # ------------------------------------------------------------------------------------------------------------ append
@@ -212,11 +235,50 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     and writes nothing.  Queries and keys are turned by the half-split rotary embedding over ``rotary_dim`` features (all of
     them unless given; 0: not at all).  Returns the turned queries ``[tokens, heads, head_dim]``, and with ``keys`` the turned keys
     too; ``qkv`` stays as it is.  No two tokens may have one place."""
+    rotary = k_pages.shape[-1] if rotary_dim is None else rotary_dim
+    dev = qkv.get_device()
+    if dev < 0 or _append_is_off(qkv, k_pages, v_pages, table, positions, heads, rows, rotary, rope_base, dev, qkv.dtype):
+        _check_append(qkv, k_pages, v_pages, table, positions, heads, rows, rotary, rope_base)
+        if dev < 0:
+            q, k = paged_append_reference(qkv, k_pages, v_pages, table, positions, heads, rows, rotary, rope_base)
+            return (q, k) if keys else q
+        if qkv.stride(1) != 1:
+            qkv = qkv.contiguous()
+    tokens, (pages, hkv, page, hd) = qkv.shape[0], k_pages.shape
+    q = qkv.new_empty((tokens, heads, hd))
+    k = qkv.new_empty((tokens, hkv, hd)) if keys else None
+    (kp, kh, kt, _), (vp, vh, vt, _) = k_pages.stride(), v_pages.stride()
+    table_rows, width = table.shape
+    N.check(_lib().dptb_paged_append(_APPEND_ARGS.pack(
+        qkv.data_ptr(), q.data_ptr(), k.data_ptr() if keys else 0, k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(),
+        positions.data_ptr(), 0 if rows is None else rows.data_ptr(), qkv.stride(0), kp, kh, kt, vp, vh, vt, table.stride(0),
+        tokens, heads, hkv, hd, rotary, page, width, pages, table_rows, qkv.dtype is _F32, rope_base), _raw_stream(dev)), "paged_append")
+    _increment_version((k_pages, v_pages))
+    return (q, k) if keys else q
+
+
+def _append_is_off(qkv, k, v, table, positions, heads, rows, rotary, rope_base, dev, dtype) -> bool:
+    """Whether ``_check_append`` has to look (see ``_attention_is_off``)."""
+    if qkv.dim() != 2 or k.dim() != 4 or v.dim() != 4 or table.dim() != 2:
+        return True
+    tokens, pages, hkv, page, hd = qkv.shape[0], *k.shape
+    return not (
+        (dtype is _BF16 or dtype is _F32) and k.dtype is dtype and v.dtype is dtype and v.shape == k.shape and table.dtype is _I32 and
+        positions.dtype is _I32 and positions.shape == (tokens,) and (tokens <= 1 or positions.stride(0) == 1) and
+        0 < hd <= MAX_HEAD_DIM and 0 < hkv and 0 < page and pages <= MAX_PAGES and table.shape[0] <= MAX_ROWS and
+        heads > 0 and qkv.shape[1] == (heads + 2 * hkv) * hd and 0 <= rotary <= hd and rotary % 2 == 0 and rope_base > 0 and
+        qkv.stride(1) == 1 and k.stride(3) == 1 and v.stride(3) == 1 and (table.stride(1) == 1 or table.shape[1] <= 1) and
+        k.get_device() == dev and v.get_device() == dev and table.get_device() == dev and positions.get_device() == dev and
+        (table.shape[0] == tokens if rows is None else rows.dtype is _I32 and rows.shape == (tokens,) and rows.get_device() == dev and
+         (tokens <= 1 or rows.stride(0) == 1)) and
+        _current_device() == dev and not ((qkv.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled()))
+
+
+def _check_append(qkv, k_pages, v_pages, table, positions, heads, rows, rotary, rope_base) -> None:
     what = "paged_append"
     _pages(what, k_pages, v_pages)
     _table(what, table)
-    pages, hkv, page, hd = k_pages.shape
-    rotary = hd if rotary_dim is None else rotary_dim
+    hkv, hd = k_pages.shape[1], k_pages.shape[3]
     if rotary < 0 or rotary % 2 or rotary > hd:
         raise ValueError(f"{what}: rotary_dim must be even and in [0, {hd}], got {rotary}")
     if heads <= 0 or qkv.dim() != 2 or qkv.shape[1] != (heads + 2 * hkv) * hd:
@@ -233,22 +295,6 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         raise ValueError(f"{what}: {tokens} tokens without `rows` for a table of {table.shape[0]} rows")
     _here(what, qkv, k_pages, v_pages, table, positions, rows)
     _no_grad(what, qkv, k_pages, v_pages)
-    if not qkv.is_cuda:
-        q, k = paged_append_reference(qkv, k_pages, v_pages, table, positions, heads, rows, rotary, rope_base)
-        return (q, k) if keys else q
-    if qkv.stride(1) != 1:
-        qkv = qkv.contiguous()
-    q = torch.empty(tokens, heads, hd, dtype=qkv.dtype, device=qkv.device)
-    k = torch.empty(tokens, hkv, hd, dtype=qkv.dtype, device=qkv.device) if keys else None
-    kp, kh, kt, _ = k_pages.stride()
-    vp, vh, vt, _ = v_pages.stride()
-    a = AppendArgs(qkv.data_ptr(), q.data_ptr(), N.ptr(k), k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(),
-                   positions.data_ptr(), N.ptr(rows), qkv.stride(0), kp, kh, kt, vp, vh, vt, table.stride(0),
-                   tokens, heads, hkv, hd, rotary, page, table.shape[1], pages, table.shape[0], qkv.dtype == torch.float32,
-                   rope_base)
-    N.check(_lib().dptb_paged_append(a, N.stream_ptr()), what)
-    torch.autograd.graph.increment_version((k_pages, v_pages))
-    return (q, k) if keys else q
 
 
 # ------------------------------------------------------------------------------------------------------------ pages
@@ -295,31 +341,52 @@ def fork_pages(table: torch.Tensor, lens: torch.Tensor, pages: int, page: int, p
     a part-filled last page that others list too is replaced by a copy of the row's own, except for the first row that grows into it.
     Returns ``(table, lens, src, dst)``: the new table and lengths, and for every row the page to copy and its copy (-1: none), which
     ``copy_pages`` takes before anything is appended.  The old table is left as it is."""
+    dev, each = table.get_device(), isinstance(grow, torch.Tensor)
+    if dev < 0 or _fork_is_off(table, lens, pages, page, parents, grow, each, dev):
+        _check_fork(table, lens, pages, page, parents, grow, each)
+        if dev < 0:
+            return fork_pages_reference(table, lens, pages, page, parents, grow)
+    rows_in, width = table.shape
+    rows = rows_in if parents is None else parents.shape[0]
+    new_table, new_lens = table.new_empty((rows, width)), table.new_empty((rows,))
+    src, dst = table.new_empty((rows,)), table.new_empty((rows,))
+    stream = _raw_stream(dev)
+    N.check(_lib().dptb_fork_pages(_FORK_ARGS.pack(
+        table.data_ptr(), lens.data_ptr(), 0 if parents is None else parents.data_ptr(), grow.data_ptr() if each else 0,
+        new_table.data_ptr(), new_lens.data_ptr(), src.data_ptr(), dst.data_ptr(), _scratch(dev, stream)[0].data_ptr(), table.stride(0),
+        rows_in, rows, width, pages, page, 0 if each else grow), stream), "fork_pages")
+    return new_table, new_lens, src, dst
+
+
+def _fork_is_off(table, lens, pages, page, parents, grow, each, dev) -> bool:
+    """Whether ``_check_fork`` has to look (see ``_attention_is_off``)."""
+    if table.dim() != 2 or parents is not None and parents.dim() != 1:
+        return True
+    rows_in = table.shape[0]
+    rows = rows_in if parents is None else parents.shape[0]
+    return not (
+        table.dtype is _I32 and lens.dtype is _I32 and lens.shape == (rows_in,) and rows_in <= MAX_ROWS and rows <= MAX_ROWS and
+        0 <= pages <= MAX_PAGES and 0 < page and (table.stride(1) == 1 or table.shape[1] <= 1) and (rows_in <= 1 or lens.stride(0) == 1) and
+        (parents is None or parents.dtype is _I32 and parents.get_device() == dev and (rows <= 1 or parents.stride(0) == 1)) and
+        (grow.dtype is _I32 and grow.shape == (rows,) and grow.get_device() == dev and (rows <= 1 or grow.stride(0) == 1) if each
+         else 0 <= grow < 1 << 31) and lens.get_device() == dev and _current_device() == dev)
+
+
+def _check_fork(table, lens, pages, page, parents, grow, each) -> None:
     what = "fork_pages"
     _table(what, table)
-    rows_in, width = table.shape
+    rows_in = table.shape[0]
     _ints(what, "lens", lens, rows_in)
     rows = rows_in if parents is None else parents.numel()
     if parents is not None:
         _ints(what, "parents", parents, rows)
-    each = isinstance(grow, torch.Tensor)
     if each:
         _ints(what, "grow", grow, rows)
-    elif grow < 0:
+    elif not 0 <= grow < 1 << 31:
         raise ValueError(f"{what}: rows grow by 0 or more tokens, got {grow}")
     if rows > MAX_ROWS or not 0 <= pages <= MAX_PAGES or page <= 0:
         raise ValueError(f"{what}: {rows} rows (at most {MAX_ROWS}), {pages} pages (at most {MAX_PAGES}) of {page} tokens")
     _here(what, table, lens, parents, grow if each else None)
-    if not table.is_cuda:
-        return fork_pages_reference(table, lens, pages, page, parents, grow)
-    new_table = torch.empty(rows, width, dtype=torch.int32, device=table.device)
-    new_lens, src, dst = torch.empty(3, rows, dtype=torch.int32, device=table.device).unbind(0)
-    free = torch.empty(max(pages, 1), dtype=torch.int32, device=table.device)
-    a = ForkArgs(table.data_ptr(), lens.data_ptr(), N.ptr(parents), grow.data_ptr() if each else None, new_table.data_ptr(),
-                 new_lens.data_ptr(), src.data_ptr(), dst.data_ptr(), free.data_ptr(), table.stride(0), rows_in, rows, width,
-                 pages, page, 0 if each else grow)
-    N.check(_lib().dptb_fork_pages(a, N.stream_ptr()), what)
-    return new_table, new_lens, src, dst
 
 
 def compact_pages_reference(table, pages):
@@ -338,49 +405,60 @@ def compact_pages(table: torch.Tensor, pages: int) -> Tuple[torch.Tensor, torch.
     """The ``n`` listed pages of a pool numbered 0 to ``n - 1``: those numbered ``n`` and above move, in order, to the unlisted
     numbers below.  Returns ``(table, src, dst, live)``: the table in the new numbers, the moves (``[pages // 2]``, -1 behind
     the last) for ``copy_pages``, and ``n`` as an int32 ``[1]``."""
-    what = "compact_pages"
-    _table(what, table)
-    if not 0 <= pages <= MAX_PAGES:
-        raise ValueError(f"{what}: a pool of {pages} pages (at most {MAX_PAGES})")
-    _here(what, table)
-    if not table.is_cuda:
-        return compact_pages_reference(table, pages)
-    new = torch.empty(table.shape, dtype=torch.int32, device=table.device)
-    src, dst = torch.empty(2, pages // 2, dtype=torch.int32, device=table.device).unbind(0)
-    live = torch.empty(1, dtype=torch.int32, device=table.device)
-    a = CompactArgs(table.data_ptr(), new.data_ptr(), src.data_ptr(), dst.data_ptr(), live.data_ptr(), table.stride(0),
-                    *table.shape, pages)
-    N.check(_lib().dptb_compact_pages(a, N.stream_ptr()), what)
+    dev = table.get_device()
+    if dev < 0 or not (table.dim() == 2 and table.dtype is _I32 and table.shape[0] <= MAX_ROWS and 0 <= pages <= MAX_PAGES and
+                       (table.stride(1) == 1 or table.shape[1] <= 1) and _current_device() == dev):
+        _table("compact_pages", table)
+        if not 0 <= pages <= MAX_PAGES:
+            raise ValueError(f"compact_pages: a pool of {pages} pages (at most {MAX_PAGES})")
+        _here("compact_pages", table)
+        if dev < 0:
+            return compact_pages_reference(table, pages)
+    rows, width = table.shape
+    new, live = table.new_empty((rows, width)), table.new_empty((1,))
+    src, dst = table.new_empty((pages // 2,)), table.new_empty((pages // 2,))
+    N.check(_lib().dptb_compact_pages(_COMPACT_ARGS.pack(
+        table.data_ptr(), new.data_ptr(), src.data_ptr(), dst.data_ptr(), live.data_ptr(), table.stride(0), rows, width, pages),
+        _raw_stream(dev)), "compact_pages")
     return new, src, dst, live
 
 
 def copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None:
     """In place: page ``dst[i]`` of ``pool [..., pages, kv_heads, page, head_dim]`` (contiguous; every layer's keys and values at
     once) becomes a copy of page ``src[i]``; pairs with a -1 are passed over.  A page that is copied to must be in no other pair."""
+    dev, shape = pool.get_device(), pool.shape
+    if dev < 0 or not (
+            len(shape) >= 4 and pool.is_contiguous() and (pool.dtype is _BF16 or pool.dtype is _F32) and src.dim() == 1 and
+            src.dtype is _I32 and dst.dtype is _I32 and src.shape == dst.shape and src.get_device() == dev and
+            dst.get_device() == dev and (src.shape[0] <= 1 or src.stride(0) == 1 and dst.stride(0) == 1) and
+            _current_device() == dev and not (pool.requires_grad and torch.is_grad_enabled())):
+        _check_copy(pool, src, dst)
+    pages = shape[-4]
+    outer = math.prod(shape[:-4])
+    if dev < 0:
+        real = (src >= 0) & (dst >= 0)
+        x, y = src[real].long(), dst[real].long()
+        if bool((x >= pages).any()) or bool((y >= pages).any()):
+            raise ValueError(f"copy_pages: a page outside the pool of {pages}")
+        flat = pool.view(outer, pages, -1)
+        flat[:, y] = flat[:, x]
+        return
+    if outer > 65535:
+        raise ValueError(f"copy_pages: at most 65535 pools at once, got {outer}")
+    N.check(_lib().dptb_copy_pages(pool.data_ptr(), src.data_ptr(), dst.data_ptr(), src.shape[0], outer, pages,
+                                   shape[-3] * shape[-2] * shape[-1] * pool.element_size(), _raw_stream(dev)), "copy_pages")
+    _increment_version((pool,))
+
+
+def _check_copy(pool, src, dst) -> None:
     what = "copy_pages"
     if pool.dim() < 4 or not pool.is_contiguous():
         raise ValueError(f"{what}: the pool must be a contiguous [..., pages, kv_heads, page, head_dim], got {list(pool.shape)}")
     if pool.dtype not in (torch.bfloat16, torch.float32):
         raise TypeError(f"{what}: pages must be float32 or bfloat16, got {pool.dtype}")
-    _ints(what, "src", src, *src.shape)
-    _ints(what, "dst", dst, *src.shape)
     if src.dim() != 1:
         raise ValueError(f"{what}: src and dst must be lists of pages")
+    _ints(what, "src", src, *src.shape)
+    _ints(what, "dst", dst, *src.shape)
     _here(what, pool, src, dst)
     _no_grad(what, pool)
-    pages = pool.shape[-4]
-    outer = math.prod(pool.shape[:-4])
-    if not pool.is_cuda:
-        real = (src >= 0) & (dst >= 0)
-        x, y = src[real].long(), dst[real].long()
-        if bool((x >= pages).any()) or bool((y >= pages).any()):
-            raise ValueError(f"{what}: a page outside the pool of {pages}")
-        flat = pool.view(outer, pages, -1)
-        flat[:, y] = flat[:, x]
-        return
-    if outer > 65535:
-        raise ValueError(f"{what}: at most 65535 pools at once, got {outer}")
-    size = math.prod(pool.shape[-3:]) * pool.element_size()
-    N.check(_lib().dptb_copy_pages(pool.data_ptr(), src.data_ptr(), dst.data_ptr(), src.numel(), outer, pages, size,
-                                   N.stream_ptr()), what)
-    torch.autograd.graph.increment_version(pool)
