@@ -9,17 +9,17 @@ from typing import Optional, Tuple
 import torch
 
 from .. import _native as N
-from .kernels import SPLITK_WS_BYTES as WS_BYTES
+from .kernels import SPLITK_COUNTERS, SPLITK_WS_BYTES
 from .paged import _BF16, _F32, _current_device, _here, _no_grad, _raw_stream, _scratch
 
-c_void_p, c_int, c_ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
+c_void_p, c_int = ctypes.c_void_p, ctypes.c_int
 
 MAX_BEAMS = 32
 MAX_ROWS = 1 << 20
 
 
 # The C struct's fields in order (see ops/paged.py).
-_BEAM_ARGS = struct.Struct("8P 2q 5i4x")
+_BEAM_ARGS = struct.Struct("9P 2q 10i")
 
 _declared = False
 
@@ -29,7 +29,6 @@ def _lib():
     lib = N.load()
     if not _declared:
         lib.dptb_beam_step.argtypes, lib.dptb_beam_step.restype = [ctypes.c_char_p, c_void_p], c_int
-        lib.dptb_beam_ws_bytes.argtypes, lib.dptb_beam_ws_bytes.restype = [c_int, c_int], c_ll
         _declared = True
     return lib
 
@@ -84,15 +83,11 @@ def beam_step(logits: torch.Tensor, scores: torch.Tensor, finished: Optional[tor
     out_tokens = torch.empty((items, beams), dtype=torch.long, device=logits.device)
     out_finished = torch.empty((items, beams), dtype=torch.bool, device=logits.device)
     lib, stream = _lib(), _raw_stream(dev)
-    ws = _scratch(dev, stream)[0]
-    room = WS_BYTES
-    if lib.dptb_beam_ws_bytes(items, beams) > room:
-        room = lib.dptb_beam_ws_bytes(items, beams)
-        ws = torch.empty(room, dtype=torch.uint8, device=logits.device)
+    ws, counters = _scratch(dev, stream)
     N.check(lib.dptb_beam_step(_BEAM_ARGS.pack(
         logits.data_ptr(), scores.data_ptr(), 0 if finished is None else finished.data_ptr(), out_scores.data_ptr(),
-        out_parents.data_ptr(), out_tokens.data_ptr(), out_finished.data_ptr(), ws.data_ptr(), logits.stride(0), room, items, beams,
-        vocab, last, logits.dtype is _F32), stream), "beam_step")
+        out_parents.data_ptr(), out_tokens.data_ptr(), out_finished.data_ptr(), ws.data_ptr(), counters.data_ptr(), logits.stride(0), SPLITK_WS_BYTES,
+        items, beams, vocab, last, logits.dtype is _F32, SPLITK_COUNTERS, 0, 0, 0, 0), stream), "beam_step")
     return out_scores, out_parents, out_tokens, out_finished
 
 
@@ -100,7 +95,7 @@ def _beam_is_off(logits, scores, finished, eos, dev) -> bool:
     """Whether ``_check_beam`` has to look: everything it asks for, at the price of a call on each step."""
     (items, beams), (rows, vocab) = scores.shape, logits.shape
     return not (
-        scores.dtype is _F32 and (logits.dtype is _BF16 or logits.dtype is _F32) and rows == items * beams and 0 < vocab < 1 << 31 and
+        scores.dtype is _F32 and (logits.dtype is _BF16 or logits.dtype is _F32) and rows == items * beams and 0 < vocab <= 1 << 30 and
         0 < beams <= MAX_BEAMS and rows <= MAX_ROWS and scores.is_contiguous() and logits.stride(1) == 1 and
         (eos is None or 0 <= eos < vocab) and scores.get_device() == dev and _current_device() == dev and
         (finished is None or eos is not None and finished.dtype is torch.bool and finished.shape == scores.shape and
@@ -117,8 +112,8 @@ def _check_beam(logits, scores, finished, eos) -> None:
         raise ValueError(f"{what}: logits {list(logits.shape)} are not [{items} * {beams}, vocab]")
     if logits.dtype not in (torch.bfloat16, torch.float32):
         raise TypeError(f"{what}: logits must be float32 or bfloat16, got {logits.dtype}")
-    if not 0 < beams <= MAX_BEAMS or items * beams > MAX_ROWS or logits.shape[1] >= 1 << 31:
-        raise ValueError(f"{what}: 1 to {MAX_BEAMS} beams, at most {MAX_ROWS} rows, got {items} x {beams}")
+    if not 0 < beams <= MAX_BEAMS or items * beams > MAX_ROWS or logits.shape[1] > 1 << 30:
+        raise ValueError(f"{what}: 1 to {MAX_BEAMS} beams, at most {MAX_ROWS} rows and {1 << 30} tokens, got {items} x {beams} x {logits.shape[1]}")
     if finished is not None and (finished.shape != scores.shape or finished.dtype != torch.bool):
         raise ValueError(f"{what}: finished must be bool {list(scores.shape)}")
     if eos is not None and not 0 <= eos < logits.shape[1]:
