@@ -3,16 +3,17 @@
 //   total[b, w, v] = score[b, w] + logit[b * W + w, v] - log sum_u exp(logit[b * W + w, u])
 //
 // Candidates are ranked by (total, then the lower w * V + v).  A finished beam has one continuation, `eos` at its old score; its others, those
-// of a beam whose score is -inf or NaN, and those of a row of logits without a distribution (a NaN, an infinity, nothing but
+// of a beam whose score is not finite, and those of a row of logits without a distribution (a NaN, an infinity, nothing but
 // -inf) are worth -inf.  Within a beam the order is that of the logits themselves, so that no rounding decides it; totals of different beams
 // meet in 64 bits.
 //
-// beam_kernel: a row is dealt to a few CTAs (chunks).  One pass over the logits keeps a running maximum and sum of exponentials in every
-// thread; that is all that is done for each logit.  The best W of a chunk lie with the threads of the W largest maxima, so those alone look at
-// their logits again and hand in what is not below the W-th of these maxima: W values and a few more, whatever the vocabulary.  The
-// last CTA of an item (a counter, no waiting) sums up its rows and chooses among their lists in the same way.
+// beam_kernel: a row is dealt to warps.  One pass over the logits keeps a running maximum and sum of exponentials in every lane; that is
+// all that is done for each logit (5.5 instructions in bf16).  The CTA of an item's last warp to finish (a counter, no waiting) sums up its rows,
+// and the lanes' maxima tell where to look: the best W continuations lie with the lanes of the W largest (each counted with its beam's score),
+// and only these lanes' logits are read once more, by the value of the W-th.  That is a few hundred logits, whatever the vocabulary.
 //
-// Bound by memory for many rows, by a chain of latencies for few.
+// Bound by memory for many rows, by a chain of latencies for few.  Choosing in every warp, or in CTAs barrier after barrier, cost more than the pass
+// itself: 45 and 61 us for 256 rows of 128256 logits.
 #include <cuda_bf16.h>
 
 #include "common/host.h"
@@ -21,9 +22,11 @@
 namespace dptb {
 
 constexpr int kMaxBeams = 32;
-constexpr int kBeamThreads = 512, kBeamWarps = kBeamThreads / 32;
-constexpr int kBeamPool = 1024;        // candidates that are ranked at once
-constexpr int kMaxChunks = 32;
+constexpr int kBeamThreads = 256, kBeamWarps = kBeamThreads / 32;
+constexpr int kWarpPool = 128;         // candidates of a warp that are ranked at once
+constexpr int kItemPool = 1024;        // and of an item
+constexpr int kHotLanes = 512;         // lanes whose logits are read again
+constexpr int kMaxLists = 64;          // parts of a row
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct BeamArgs {
@@ -34,11 +37,11 @@ struct BeamArgs {
   int* out_parents;              // row of the parent
   long long* out_tokens;
   unsigned char* out_finished;
-  void* ws;                      // per row and chunk: sum of exponentials, maximum, the best keys
+  void* ws;                      // BeamPart of every row and warp
   unsigned* counters;            // a zeroed word per item of a launch; zero again afterwards
   long long ld, ws_bytes;
   int items, beams, vocab, eos, f32, num_counters;
-  int chunk, chunks, vec, first_item;   // set by the launcher
+  int chunk, lists, vec, first_item;   // set by the launcher: logits of a warp, warps of a row
 };
 static_assert(sizeof(BeamArgs) == 128, "packed by the caller");
 
@@ -60,9 +63,9 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-// The k-th largest of the block's values, k <= 32: warps sort theirs, and lists are merged pairwise, the 32 largest of two at a time.
-__device__ __forceinline__ float kth_largest(float v, int k, float* lists) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// Descending over the lanes.
+__device__ __forceinline__ float sort_lanes(float v) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int n = 2; n <= 32; n <<= 1)
 #pragma unroll
@@ -70,6 +73,12 @@ __device__ __forceinline__ float kth_largest(float v, int k, float* lists) {
       const float o = __shfl_xor_sync(0xffffffffu, v, j);
       v = ((lane & j) == 0) == ((lane & n) == 0) ? fmaxf(v, o) : fminf(v, o);
     }
+  return v;
+}
+// The k-th largest of the block's values, k <= 32: warps sort theirs, and lists are merged pairwise, the 32 largest of two at a time.
+__device__ __forceinline__ float kth_largest(float v, int k, float* lists) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  v = sort_lanes(v);
   lists[warp * 32 + lane] = v;
   __syncthreads();
 #pragma unroll 1
@@ -88,230 +97,249 @@ __device__ __forceinline__ float kth_largest(float v, int k, float* lists) {
   return lists[k - 1];
 }
 
-// A thread's pieces of a row: 16 bytes each, kBeamThreads pieces apart.
+// 16 bytes of a row.
 template <typename T>
-struct Piece {
-  static constexpr int N = 16 / sizeof(T);
-  T e[N];
-  // Elements first .. first + N of a row of `end`; those beyond are -inf.
-  __device__ __forceinline__ void load(const T* row, int first, int end, bool vec) {
-    if (vec && first + N <= end) {
-      *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(row + first);
-    } else {
+struct Piece;
+template <>
+struct Piece<float> {
+  static constexpr int N = 4;
+  uint32_t u[4];
+  __device__ __forceinline__ float at(int i) const { return __uint_as_float(u[i]); }
+  __device__ __forceinline__ float top() const { return fmaxf(fmaxf(at(0), at(1)), fmaxf(at(2), at(3))); }
+};
+template <>
+struct Piece<__nv_bfloat16> {
+  static constexpr int N = 8;
+  uint32_t u[4];
+  __device__ __forceinline__ float at(int i) const { return __uint_as_float(i & 1 ? u[i >> 1] & 0xffff0000u : u[i >> 1] << 16); }
+  __device__ __forceinline__ float top() const {
+    __nv_bfloat162 h[4];
 #pragma unroll
-      for (int i = 0; i < N; ++i) e[i] = first + i < end ? row[first + i] : from_f32<T>(-INFINITY);
-    }
+    for (int i = 0; i < 4; ++i) h[i] = reinterpret_cast<const __nv_bfloat162*>(u)[i];
+    const float2 f = __bfloat1622float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+    return fmaxf(f.x, f.y);
   }
+};
+// Elements first .. first + N of a row of `end`; those beyond are -inf.
+__device__ __noinline__ uint4 edge_bits(const unsigned short* row, int first, int end) {      // bf16
+  uint32_t e[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) e[i] = first + i < end ? row[first + i] : 0xff80u;
+  return make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+}
+__device__ __noinline__ uint4 edge_bits(const uint32_t* row, int first, int end) {            // fp32
+  uint32_t e[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) e[i] = first + i < end ? row[first + i] : 0xff800000u;
+  return make_uint4(e[0], e[1], e[2], e[3]);
+}
+template <typename T>
+__device__ __forceinline__ Piece<T> load_edge(const T* row, int first, int end) {
+  uint4 u;
+  if constexpr (sizeof(T) == 2) u = edge_bits(reinterpret_cast<const unsigned short*>(row), first, end);
+  else u = edge_bits(reinterpret_cast<const uint32_t*>(row), first, end);
+  return Piece<T>{u.x, u.y, u.z, u.w};
+}
+template <typename T>
+__device__ __forceinline__ Piece<T> load_whole(const T* row, int first) {
+  const uint4 u = *reinterpret_cast<const uint4*>(row + first);
+  return Piece<T>{u.x, u.y, u.z, u.w};
+}
+template <typename T>
+__device__ __forceinline__ Piece<T> load_piece(const T* row, int first, int end, bool vec) {
+  return vec && first + Piece<T>::N <= end ? load_whole<T>(row, first) : load_edge<T>(row, first, end);
+}
+
+// What a warp leaves of its logits: the sum of exponentials, what it is relative to, every lane's maximum.
+struct BeamPart {
+  double sum, base;
+  float high[32];
 };
 
 struct BeamShared {
+  unsigned long long keys[kItemPool];      // each warp's kWarpPool; of an item: (beam, token)
+  double totals[kItemPool];
   float lists[kBeamThreads];
-  float red[33];
-  double sums[kBeamWarps];
-  unsigned long long keys[kBeamPool];      // of a chunk; of the item: (beam, token)
-  double totals[kBeamPool];
   double score[kMaxBeams], top[kMaxBeams], norm[kMaxBeams];
+  float from[kMaxBeams], offset[kMaxBeams], least[kMaxBeams];      // fp32 totals: x - from + offset; what x - from has to reach
   unsigned char kind[kMaxBeams];           // 0: by its logits, 1: finished, 2: nothing to offer
-  int count, scan[33], last;
+  int hot[kHotLanes];
+  int count, hots, counts[kBeamWarps], done[kBeamWarps];
 };
+static_assert(kBeamWarps * kWarpPool <= kItemPool, "the warps' pools");
 
-__device__ __forceinline__ int block_scan_total(int v, int* scratch, int& total) {      // exclusive sum
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int s = v;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(0xffffffffu, s, o);
-    if (lane >= o) s += u;
-  }
-  __syncthreads();
-  if (lane == 31) scratch[warp] = s;
-  __syncthreads();
-  int before = 0;
-  total = 0;
-  for (int w = 0; w < kBeamWarps; ++w) {
-    if (w < warp) before += scratch[w];
-    total += scratch[w];
-  }
-  return before + s - v;
-}
-
-// Of the logits [begin, end) the best `count` as keys in `out`, best first, 0 behind the last.  Threads hand in what is not below the threshold; where too many
-// logits equal it (a masked vocabulary), those above it, and the first of the equal ones in their order.
+// Of a warp's logits [begin, end), of which this lane's have the maximum `mine`, the best K as keys in `out`, best first, 0 behind the last.  Where too many
+// equal the threshold (a masked vocabulary), those above it, and the first of the equal ones in their order.
 template <typename T>
-__device__ __forceinline__ void best_of_chunk(const BeamArgs& a, const T* row, int begin, int end, float mine, unsigned long long* out, BeamShared& sh) {
+__device__ __forceinline__ void best_of_warp(const T* row, int begin, int end, bool vec, float mine, int K, unsigned long long* out, unsigned long long* keys, int* count) {
   constexpr int N = Piece<T>::N;
-  const int tid = threadIdx.x, K = a.beams;
-  const float limit = kth_largest(mine, K, sh.lists);
+  const int lane = threadIdx.x & 31;
+  const float limit = __shfl_sync(0xffffffffu, sort_lanes(mine), K - 1);
+  int n = 0;
 #pragma unroll 1
   for (int round = 0; round < 2; ++round) {
-    if (tid == 0) sh.count = 0;
-    __syncthreads();
+    __syncwarp();
+    if (lane == 0) *count = 0;
+    __syncwarp();
     if (round == 0 ? mine >= limit : mine > limit) {
 #pragma unroll 4
-      for (int i = begin + tid * N; i < end; i += kBeamThreads * N) {
-        Piece<T> p;
-        p.load(row, i, end, a.vec);
+      for (int i = begin + lane * N; i < end; i += 32 * N) {
+        const Piece<T> p = load_piece<T>(row, i, end, vec);
+        const float top = p.top();
+        if (round == 0 ? top >= limit : top > limit)
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const float x = to_f32(p.e[e]);
-          if (i + e < end && (round == 0 ? x >= limit : x > limit)) {
-            const int at = atomicAdd(&sh.count, 1);
-            if (at < kBeamPool) sh.keys[at] = rank_key(x, i + e);
+          for (int e = 0; e < N; ++e) {
+            const float x = p.at(e);
+            if (i + e < end && (round == 0 ? x >= limit : x > limit)) {
+              const int at = atomicAdd(count, 1);
+              if (at < kWarpPool) keys[at] = rank_key(x, i + e);
+            }
           }
-        }
       }
     }
-    __syncthreads();
-    const int above = sh.count;                   // (everybody's, before it changes)
-    __syncthreads();
-    if (above <= kBeamPool - (round ? K : 0)) {
-      if (round == 0) break;
-      int found = above;
-      for (int i0 = begin; i0 < end && found - above < K; i0 += kBeamThreads * N) {
-        const int i = i0 + tid * N;
-        Piece<T> p;
-        p.load(row, i, end, a.vec);
-        int equal = 0, total;
+    __syncwarp();
+    n = *(volatile int*)count;
+    if (n > kWarpPool - (round ? K : 0)) continue;
+    if (round == 1) {
+      const int above = n;
+#pragma unroll 1
+      for (int i0 = begin; i0 < end && n - above < K; i0 += 32 * N) {
+        const int i = i0 + lane * N;
+        const Piece<T> p = load_piece<T>(row, i, end, vec);
+        int equal = 0;
 #pragma unroll
-        for (int e = 0; e < N; ++e) equal += i + e < end && to_f32(p.e[e]) == limit;
-        int at = found + block_scan_total(equal, sh.scan, total);
+        for (int e = 0; e < N; ++e) equal += i + e < end && p.at(e) == limit;
+        int at = equal;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int u = __shfl_up_sync(0xffffffffu, at, o);
+          if (lane >= o) at += u;
+        }
+        const int total = __shfl_sync(0xffffffffu, at, 31);
+        at += n - equal;
 #pragma unroll
         for (int e = 0; e < N; ++e)
-          if (i + e < end && to_f32(p.e[e]) == limit) {
-            if (at - above < K) sh.keys[at] = rank_key(limit, i + e);
+          if (i + e < end && p.at(e) == limit) {
+            if (at - above < K) keys[at] = rank_key(limit, i + e);
             ++at;
           }
-        found += total;
+        n += total;
       }
-      __syncthreads();
-      if (tid == 0) sh.count = min(found, above + K);
-      __syncthreads();
-      break;
+      n = min(n, above + K);
+      __syncwarp();
     }
-    if (round == 1) {
-      // Too many above it as well: the best, one after the other.
-      unsigned long long last = ~0ull;
-      for (int k = 0; k < K; ++k) {
-        unsigned long long top = 0;
-        for (int i = begin + tid; i < end; i += kBeamThreads) {
-          const unsigned long long key = rank_key(to_f32(row[i]), i);
-          if (key < last && key > top) top = key;
-        }
-        for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if ((tid & 31) == 0) sh.keys[K + (tid >> 5)] = top;
-        __syncthreads();
-        for (int w = 0; w < kBeamWarps; ++w) top = max(top, sh.keys[K + w]);
-        if (tid == 0) sh.keys[k] = top;
-        last = top;
-        __syncthreads();
-      }
-      if (tid == 0) sh.count = min(K, end - begin);
-      __syncthreads();
-    }
+    break;
   }
-  const int n = sh.count;
-  for (int i = tid; i < n; i += kBeamThreads) {
-    const unsigned long long key = sh.keys[i];
+  if (n > kWarpPool) {         // too many above the threshold as well: the best, one after the other
+    unsigned long long last = ~0ull;
+#pragma unroll 1
+    for (int k = 0; k < K; ++k) {
+      unsigned long long top = 0;
+      for (int i = begin + lane; i < end; i += 32) {
+        const unsigned long long key = rank_key(to_f32(row[i]), i);
+        if (key < last && key > top) top = key;
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (lane == 0) out[k] = top;
+      last = top;
+    }
+    return;
+  }
+  for (int i = lane; i < n; i += 32) {
+    const unsigned long long key = keys[i];
     int rank = 0;
-    for (int j = 0; j < n; ++j) rank += sh.keys[j] > key;
+    for (int j = 0; j < n; ++j) rank += keys[j] > key;
     if (rank < K) out[rank] = key;
   }
-  for (int i = n + tid; i < K; i += kBeamThreads) out[i] = 0;
+  for (int i = n + lane; i < K; i += 32) out[i] = 0;
 }
 
-// Candidate c of an item: entry c % (chunks * beams) of beam c / (chunks * beams); false if there is none.
-__device__ __forceinline__ bool candidate(const BeamArgs& a, const BeamShared& sh, const unsigned char* parts, long long part, int c, int& beam, int& token, double& total) {
-  const int each = a.chunks * a.beams;
-  beam = c / each;
-  const int i = c - beam * each;
-  total = -INFINITY;
-  if (sh.kind[beam]) {
-    if (i >= min(a.beams, a.vocab)) return false;
-    token = i;
-    if (sh.kind[beam] == 1 && a.eos >= 0) {       // eos first, then the others
-      if (i == 0) {
-        token = a.eos;
-        total = sh.score[beam];
-      } else {
-        token = i - 1 + (i - 1 >= a.eos);
-      }
-    }
-    return true;
-  }
-  const int chunk = i / a.beams;
-  const unsigned long long key = __ldcg(reinterpret_cast<const unsigned long long*>(parts + (beam * (long long)a.chunks + chunk) * part + 16) + (i - chunk * a.beams));
-  if (key == 0) return false;
-  token = key_index(key);
-  total = sh.score[beam] + ((double)key_value(key) - sh.top[beam] - sh.norm[beam]);     // (a row masked by the lowest value loses nothing to its size)
-  if (total != total) total = -INFINITY;          // an infinite score on a token of no probability
-  return true;
+// A sum relative to the maximum `m`, or its shift, relative to `top` > m, or its.
+constexpr float kLarge = 1048576.0f;
+__device__ __noinline__ double rescaled_large(double s, float m, float shift, float top, float next) {
+  const double from = fabsf(m) < kLarge ? (double)shift / (double)kLog2e : (double)m, to = fabsf(top) < kLarge ? (double)next / (double)kLog2e : (double)top;
+  return s * exp(from - to);
+}
+__device__ __forceinline__ double rescaled(double s, float m, float shift, float top, float next) {
+  if (m == top || m == -INFINITY) return s;       // (nothing but -inf so far: a sum of 0, or NaN)
+  if (fabsf(m) < kLarge && fabsf(top) < kLarge) return next - shift > 1000.0f ? 0.0 * s : s * __longlong_as_double((long long)(1023 + (int)(shift - next)) << 52);
+  return rescaled_large(s, m, shift, top, next);
 }
 
+// A continuation by its beam's logits.
+__device__ __forceinline__ double total_of(const BeamShared& sh, int w, float x) {
+  return sh.score[w] + ((double)x - sh.top[w] - sh.norm[w]);      // (a row masked by the lowest value loses nothing to its size)
+}
+// Continuation i, best first, of a beam that does not go by its logits.
+__device__ __forceinline__ double special(const BeamArgs& a, const BeamShared& sh, int w, int i, int& token) {
+  token = i;
+  if (sh.kind[w] != 1 || a.eos < 0) return -INFINITY;
+  token = i == 0 ? a.eos : i - 1 + (i - 1 >= a.eos);      // eos, then the others
+  return i == 0 ? sh.score[w] : -INFINITY;
+}
+
+// Where too many are equal, or there are fewer than beams (a masked vocabulary): the best of every row, by a warp.
 template <typename T>
-__global__ void __launch_bounds__(kBeamThreads)
-beam_kernel(const BeamArgs a) {
-  constexpr int N = Piece<T>::N, U = 4;           // pieces in flight
-  __shared__ BeamShared sh;
+__device__ __noinline__ void best_of_rows(const BeamArgs& a, BeamShared& sh, const T* rows) {
+  constexpr int N = Piece<T>::N;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = a.beams;
-  const int local = blockIdx.y / K, item = a.first_item + local;
-  const int row_index = item * K + blockIdx.y % K, chunk = blockIdx.x;
-  const T* row = static_cast<const T*>(a.logits) + row_index * a.ld;
-  const int begin = chunk * a.chunk, end = min(a.vocab, begin + a.chunk);
-  const long long part = 16 + 8LL * K;
-  unsigned char* parts = static_cast<unsigned char*>(a.ws) + (long long)local * K * a.chunks * part;     // of the item
-  float m = -INFINITY, s = 0.0f;
-  for (int i = begin + tid * N; i < end; i += U * kBeamThreads * N) {
-    Piece<T> p[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) p[u].load(row, i + u * kBeamThreads * N, end, a.vec);
-    float top = m;
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int e = 0; e < N; ++e) top = fmaxf(top, to_f32(p[u].e[e]));
-    const float base = top == -INFINITY ? 0.0f : top;
-    if (top != m) s *= exp2_fast((m - base) * kLog2e);
-    m = top;
-    float t[2] = {0.0f, 0.0f};
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int e = 0; e < N; ++e) t[e & 1] += exp2_fast((to_f32(p[u].e[e]) - base) * kLog2e);
-    s += t[0] + t[1];
-  }
-  const float best = block_max(m, sh.red), base = best == -INFINITY ? 0.0f : best;
-  double sum = (double)(s * exp2_fast((m - base) * kLog2e));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) sh.sums[warp] = sum;
-  unsigned char* mine = parts + ((blockIdx.y % K) * (long long)a.chunks + chunk) * part;
-  best_of_chunk<T>(a, row, begin, end, m, reinterpret_cast<unsigned long long*>(mine + 16), sh);
-  if (tid == 0) {
-    double t = 0.0;
-    for (int w = 0; w < kBeamWarps; ++w) t += sh.sums[w];
-    *reinterpret_cast<double*>(mine) = t;          // NaN where the chunk holds a NaN or an infinity
-    *reinterpret_cast<double*>(mine + 8) = best;
-  }
-  __threadfence();
-  __syncthreads();
-  if (tid == 0) {
-    const bool last = atomicAdd(a.counters + local, 1u) == (unsigned)(K * a.chunks) - 1;
-    if (last) a.counters[local] = 0;
-    sh.last = last;
-    sh.count = 0;
-  }
-  __syncthreads();
-  if (!sh.last) return;
-  __threadfence();
+  auto* keys = reinterpret_cast<unsigned long long*>(sh.totals);
+#pragma unroll 1
   for (int w = warp; w < K; w += kBeamWarps) {
-    const unsigned char* p = parts + (w * (long long)a.chunks + lane) * part;
-    const bool in = lane < a.chunks;
-    const double m_part = in ? __ldcg(reinterpret_cast<const double*>(p + 8)) : -INFINITY;
-    const double s_part = in ? __ldcg(reinterpret_cast<const double*>(p)) : 0.0;
-    double top = m_part;
+    if (sh.kind[w]) continue;
+    const T* row = rows + w * a.ld;
+    float mine = -INFINITY;
+    for (int i = lane * N; i < a.vocab; i += 32 * N) mine = fmaxf(mine, load_piece<T>(row, i, a.vocab, a.vec).top());
+    best_of_warp<T>(row, 0, a.vocab, a.vec, mine, K, keys + w * K, sh.keys + warp * kWarpPool, sh.counts + warp);
+  }
+  __syncthreads();
+  for (int c = tid; c < K * K; c += kBeamThreads) {
+    const int w = c / K, i = c - w * K;
+    const unsigned long long key = keys[c];
+    int token = 0;
+    double total = -INFINITY;
+    bool valid;
+    if (sh.kind[w]) {
+      valid = i < min(K, a.vocab);
+      total = special(a, sh, w, i, token);
+    } else {
+      valid = key != 0;
+      token = key_index(key);
+      if (valid) total = total_of(sh, w, key_value(key));
+    }
+    sh.totals[c] = total;
+    sh.keys[c] = valid ? (unsigned long long)w << 32 | (unsigned)token : ~0ull;
+  }
+  if (tid == 0) sh.count = K * K;
+  __syncthreads();
+}
+
+// The choice for an item, by the whole CTA.
+template <typename T>
+__device__ __noinline__ void choose(const BeamArgs& a, BeamShared& sh, int local) {
+  constexpr int N = Piece<T>::N;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = a.beams, item = a.first_item + local;
+  const BeamPart* parts = static_cast<const BeamPart*>(a.ws) + (long long)local * K * a.lists;
+  const T* rows = static_cast<const T*>(a.logits) + (long long)item * K * a.ld;
+  if (tid == 0) sh.count = sh.hots = 0;
+#pragma unroll 1
+  for (int w = warp; w < K; w += kBeamWarps) {
+    const BeamPart* p = parts + w * a.lists;
+    double base[2], sum[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {          // (kMaxLists)
+      const int l = lane + 32 * x;
+      const bool in = l < a.lists;
+      base[x] = in ? __ldcg(&p[l].base) : -INFINITY;
+      sum[x] = in ? __ldcg(&p[l].sum) : 0.0;
+    }
+    double top = fmax(base[0], base[1]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
-    double t = in ? s_part * exp(m_part - (top == -INFINITY ? 0.0 : top)) : 0.0;
+    double t = 0.0;
+#pragma unroll 1
+    for (int x = 0; x < 2 && 32 * x < a.lists; ++x) t += sum[x] == 0.0 ? 0.0 : sum[x] * exp(base[x] - top);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
     if (lane == 0) {
@@ -321,82 +349,204 @@ beam_kernel(const BeamArgs a) {
       sh.score[w] = score;
       sh.top[w] = top;
       sh.norm[w] = norm;
-      sh.kind[w] = !(score > -INFINITY) ? 2 : fin ? 1 : fabs(top) < INFINITY && fabs(norm) < INFINITY ? 0 : 2;
+      sh.from[w] = (float)top;
+      sh.offset[w] = (float)(score - norm);
+      sh.kind[w] = !(fabsf(score) < INFINITY) ? 2 : fin ? 1 : fabs(top) < INFINITY && fabs(norm) < INFINITY ? 0 : 2;
     }
   }
   __syncthreads();
-  const int n = K * K * a.chunks;
-  int beam, token;
-  double total;
-  float high = -INFINITY;
-  for (int c = tid; c < n; c += kBeamThreads)
-    if (candidate(a, sh, parts, part, c, beam, token, total)) high = fmaxf(high, (float)total);
-  const float limit = kth_largest(high, K, sh.lists);          // (rounding to fp32 keeps the order)
-  for (int c = tid; c < n; c += kBeamThreads)
-    if (candidate(a, sh, parts, part, c, beam, token, total) && (float)total >= limit) {
-      const int at = atomicAdd(&sh.count, 1);
-      if (at < kBeamPool) {
-        sh.totals[at] = total;
-        sh.keys[at] = (unsigned long long)beam << 32 | (unsigned)token;
-      }
-    }
-  __syncthreads();
-  auto write = [&](int at, unsigned long long key, double t) {
-    const int w = (int)(key >> 32), tok = (int)(unsigned)key, out = item * K + at;
-    a.out_scores[out] = (float)t;
-    a.out_parents[out] = item * K + w;
-    a.out_tokens[out] = tok;
-    a.out_finished[out] = (a.finished && a.finished[item * K + w]) || tok == a.eos;
-  };
-  const int found = sh.count;
-  if (found <= kBeamPool) {
-    for (int i = tid; i < found; i += kBeamThreads) {
-      const double t = sh.totals[i];
-      const unsigned long long key = sh.keys[i];
-      int rank = 0;
-      for (int j = 0; j < found; ++j) rank += sh.totals[j] > t || (sh.totals[j] == t && sh.keys[j] < key);
-      if (rank < K) write(rank, key, t);
-    }
-    return;
-  }
-  // Too many equal ones: one after the other.
-  double last_total = INFINITY;
-  unsigned long long last_key = 0;
-  for (int k = 0; k < K; ++k) {
-    double t = -INFINITY;
-    unsigned long long key = ~0ull;
-    for (int c = tid; c < n; c += kBeamThreads)
-      if (candidate(a, sh, parts, part, c, beam, token, total)) {
-        const unsigned long long id = (unsigned long long)beam << 32 | (unsigned)token;
-        const bool after = k == 0 || total < last_total || (total == last_total && id > last_key);
-        if (after && (total > t || (total == t && id < key))) {
-          t = total;
-          key = id;
-        }
+  // The W-th largest of the lanes' maxima, and the lanes that reach it, both in fp32 and with room for its roundings: `from` and `offset`
+  // are off by 2^-24 of themselves, and so are the two sums.
+  const int quads = a.lists * 8, all = K * quads;
+  float limit = 0.0f, high = -INFINITY;
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+    constexpr int B = 4;                             // loads in flight
+#pragma unroll 1
+    for (int c0 = tid; c0 < all; c0 += B * kBeamThreads) {
+      float4 v[B];
+#pragma unroll
+      for (int x = 0; x < B; ++x) {
+        const int c = c0 + x * kBeamThreads;
+        v[x] = c < all ? __ldcg(reinterpret_cast<const float4*>(parts[c >> 3].high) + (c & 7)) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
       }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const double u = __shfl_xor_sync(0xffffffffu, t, o);
-      const unsigned long long x = __shfl_xor_sync(0xffffffffu, key, o);
-      if (u > t || (u == t && x < key)) {
-        t = u;
-        key = x;
+      for (int x = 0; x < B; ++x) {
+        const int c = min(c0 + x * kBeamThreads, all - 1), w = c / quads;
+        if (sh.kind[w]) continue;
+        const float e[4] = {v[x].x, v[x].y, v[x].z, v[x].w};
+        const float top = fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])) - sh.from[w];
+        if (pass == 0) {
+          high = fmaxf(high, top + sh.offset[w]);
+        } else if (top >= sh.least[w]) {
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+            if (e[y] - sh.from[w] >= sh.least[w]) {
+              const int at = atomicAdd(&sh.hots, 1);
+              if (at < kHotLanes) sh.hot[at] = 4 * c + y;
+            }
+        }
+      }
+    }
+    for (int c = tid; c < K * K; c += kBeamThreads) {
+      const int w = c / K, i = c - w * K;
+      if (!sh.kind[w] || i >= a.vocab) continue;
+      int token;
+      const double total = special(a, sh, w, i, token);
+      if (pass == 0) {
+        high = fmaxf(high, (float)total);
+      } else if (total >= limit) {
+        const int at = atomicAdd(&sh.count, 1);
+        if (at < kItemPool) {
+          sh.totals[at] = total;
+          sh.keys[at] = (unsigned long long)w << 32 | (unsigned)token;
+        }
+      }
+    }
+    if (pass == 0) {
+      limit = kth_largest(high, K, sh.lists);
+      if (limit == -INFINITY) break;
+      const bool mine = lane < K && sh.kind[lane] == 0;
+      const float size = warp_max(mine ? fabsf(sh.offset[lane]) + fminf(fabsf(sh.from[lane]), 2.0f * kLarge) : 0.0f);
+      limit -= (size + fabsf(limit)) * 0x1p-21f;
+      if (warp == 0 && mine) {
+        const float d = (float)((double)limit - sh.score[lane] + sh.norm[lane]);
+        sh.least[lane] = d - (size + fabsf(d)) * 0x1p-21f;
+      }
+      __syncthreads();
+    }
+  }
+  __syncthreads();
+  const int hots = sh.hots;
+  bool wide = limit == -INFINITY || hots > kHotLanes;
+  if (!wide) {
+    // A hot lane's pieces by as many lanes as there are pieces.
+    const int pieces = min(32, (min(a.chunk, a.vocab) + 32 * N - 1) / (32 * N)), width = pieces > 1 ? 1 << (32 - __clz(pieces - 1)) : 1;
+#pragma unroll 1
+    for (int h = tid / width; h < hots; h += kBeamThreads / width) {
+      const int j = sh.hot[h], part = j >> 5, w = part / a.lists, l = part - w * a.lists;
+      const T* row = rows + w * a.ld;
+      const int begin = l * a.chunk, end = min(a.vocab, begin + a.chunk);
+      const float from = sh.from[w], least = sh.least[w];
+#pragma unroll 1
+      for (int i = begin + ((j & 31) + 32 * (tid & (width - 1))) * N; i < end; i += width * 32 * N) {
+        const Piece<T> p = load_piece<T>(row, i, end, a.vec);
+        if (p.top() - from < least) continue;
+#pragma unroll 1
+        for (int e = 0; e < N && i + e < end; ++e) {
+          float x = p.at(0);
+#pragma unroll
+          for (int q = 1; q < N; ++q) x = e == q ? p.at(q) : x;
+          if (x - from >= least) {
+            const int at = atomicAdd(&sh.count, 1);
+            if (at < kItemPool) {
+              sh.totals[at] = total_of(sh, w, x);
+              sh.keys[at] = (unsigned long long)w << 32 | (unsigned)(i + e);
+            }
+          }
+        }
       }
     }
     __syncthreads();
+    wide = sh.count > kItemPool;
+  }
+  if (wide) {
+    __syncthreads();
+    best_of_rows<T>(a, sh, rows);
+  }
+  const int found = sh.count;
+  for (int i = tid; i < found; i += kBeamThreads) {
+    const double t = sh.totals[i];
+    const unsigned long long key = sh.keys[i];
+    int rank = 0;
+    for (int j = 0; j < found; ++j) rank += sh.totals[j] > t || (sh.totals[j] == t && sh.keys[j] < key);
+    if (rank < K && key != ~0ull) {
+      const int w = (int)(key >> 32), tok = (int)(unsigned)key, out = item * K + rank;
+      a.out_scores[out] = (float)t;
+      a.out_parents[out] = item * K + w;
+      a.out_tokens[out] = tok;
+      a.out_finished[out] = (a.finished && a.finished[item * K + w]) || tok == a.eos;
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kBeamThreads, 4)
+beam_kernel(const __grid_constant__ BeamArgs a, int rows) {
+  constexpr int N = Piece<T>::N, U = 4;           // pieces in flight
+  __shared__ BeamShared sh;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = a.beams;
+  const int unit = blockIdx.x * kBeamWarps + warp, local_row = unit / a.lists, list = unit - local_row * a.lists;
+  int done = -1;
+  if (local_row < rows) {
+    const T* row = static_cast<const T*>(a.logits) + ((long long)a.first_item * K + local_row) * a.ld;
+    const int begin = list * a.chunk, end = min(a.vocab, begin + a.chunk);
+    // Sums of 2^(x log2(e) - shift): `shift` is a whole number, so that sums are brought to another one exactly, and stands for shift / log2(e),
+    // divided out in 64 bits, so that the rounding of log2(e) moves no sum against another.  What is left is the error of an exponential, 2^-22, and of
+    // sums of 32.  Maxima that are too large for it (masks of the type's lowest value among them) go by differences, from themselves.
+    float m = -INFINITY, shift = 0.0f;
+    double s = 0.0;
+    for (int i = begin + lane * N; i < end; i += U * 32 * N) {
+      Piece<T> p[U];
+      if (a.vec && i + (U - 1) * 32 * N + N <= end) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) p[u] = load_whole<T>(row, i + u * 32 * N);
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u) p[u] = load_edge<T>(row, i + u * 32 * N, end);
+      }
+      const float top = fmaxf(fmaxf(p[0].top(), p[1].top()), fmaxf(p[2].top(), p[3].top()));
+      if (top > m) {
+        const float next = ceilf(top * kLog2e);
+        s = rescaled(s, m, shift, top, next);
+        shift = next;
+        m = top;
+      }
+      float t[2] = {0.0f, 0.0f};
+      if (fabsf(m) < kLarge) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int e = 0; e < N; ++e) t[e & 1] += exp2_fast(fmaf(p[u].at(e), kLog2e, -shift));
+      } else {
+        const float from = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int e = 0; e < N; ++e) t[0] += exp2_fast((p[u].at(e) - from) * kLog2e);
+      }
+      s += (double)(t[0] + t[1]);
+    }
+    const float best = warp_max(m), last = ceilf(best * kLog2e);
+    double sum = best == -INFINITY ? s : rescaled(s, m, shift, best, last);
+    const double base = fabsf(best) < kLarge ? (double)last / (double)kLog2e : (double)best;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    BeamPart* part = static_cast<BeamPart*>(a.ws) + unit;
+    part->high[lane] = m;
     if (lane == 0) {
-      sh.totals[warp] = t;
-      sh.keys[warp] = key;
+      part->sum = sum;           // NaN where there is one
+      part->base = base;
     }
-    __syncthreads();
-    for (int w = 0; w < kBeamWarps; ++w)
-      if (sh.totals[w] > t || (sh.totals[w] == t && sh.keys[w] < key)) {
-        t = sh.totals[w];
-        key = sh.keys[w];
+    __threadfence();
+    __syncwarp();
+    if (lane == 0) {
+      const int local = local_row / K;
+      if (atomicAdd(a.counters + local, 1u) == (unsigned)(K * a.lists) - 1) {
+        a.counters[local] = 0;
+        done = local;
       }
-    if (tid == 0) write(k, key, t);
-    last_total = t;
-    last_key = key;
+    }
+  }
+  if (lane == 0) sh.done[warp] = done;
+  __syncthreads();
+#pragma unroll 1
+  for (int w = 0; w < kBeamWarps; ++w) {
+    const int local = sh.done[w];
+    if (local < 0) continue;
+    __threadfence();
+    choose<T>(a, sh, local);
+    __syncthreads();
   }
 }
 
@@ -410,26 +560,28 @@ extern "C" int dptb_beam_step(const BeamArgs* args, void* stream) {
   if (a.items < 0 || a.beams <= 0 || a.beams > kMaxBeams || a.vocab <= 0 || a.vocab > 1 << 30 || a.ld < 0 || (long long)a.items * a.beams > 1 << 20 ||
       (reinterpret_cast<uintptr_t>(a.ws) & 7))
     return kErrBadShape;
-  // Chunks: as many CTAs as are resident at once (4 an SM), as far as each has a round of loads to do (4 pieces a thread).
-  const int rows = a.items * a.beams, unit = kBeamThreads * (a.f32 ? 4 : 8);
-  long long chunk = ((long long)a.vocab * rows + 4LL * sm_count() - 1) / (4LL * sm_count());
-  chunk = max(chunk, (long long)unit);
-  chunk = max(chunk, ((long long)a.vocab + kMaxChunks - 1) / kMaxChunks);
-  chunk = (chunk + unit - 1) / unit * unit;
-  a.chunk = (int)min(chunk, 0x7fffffffLL / unit * unit);
-  a.chunks = (a.vocab + a.chunk - 1) / a.chunk;
+  // Logits of a warp: a row's share when all that are resident (32 an SM) have one, a round of loads (4 pieces a lane) at least, and not so many
+  // parts of a row that the choice among them is what takes the time.
+  const int unit = 4 * 32 * (a.f32 ? 4 : 8), most_lists = kMaxLists;
+  const long long rows = (long long)a.items * a.beams, warps = 32LL * sm_count();
+  long long chunk = ((long long)a.vocab * rows + warps - 1) / warps;
+  chunk = max(chunk, ((long long)a.vocab + most_lists - 1) / most_lists);
+  chunk = max((chunk + unit - 1) / unit, 1LL) * unit;
+  a.chunk = (int)chunk;
+  a.lists = (int)((a.vocab + chunk - 1) / chunk);
   const int size = a.f32 ? 4 : 2;
   a.vec = (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0 && a.ld * size % 16 == 0;
   // Items that the workspace and the counters hold go together.
-  const long long part = (long long)a.beams * a.chunks * (16 + 8LL * a.beams);
-  const int most = (int)min(min((long long)a.num_counters, a.ws_bytes / part), 65535LL / a.beams);
+  const long long part = (long long)a.beams * a.lists * (long long)sizeof(BeamPart);
+  const int most = (int)min((long long)a.num_counters, a.ws_bytes / part);
   if (most < 1) return kErrTooLarge;
   auto st = static_cast<cudaStream_t>(stream);
   int launches = 0;
   for (a.first_item = 0; a.first_item < a.items; a.first_item += most, ++launches) {
-    const dim3 grid(a.chunks, min(most, a.items - a.first_item) * a.beams);
-    if (a.f32) beam_kernel<float><<<grid, kBeamThreads, 0, st>>>(a);
-    else       beam_kernel<__nv_bfloat16><<<grid, kBeamThreads, 0, st>>>(a);
+    const int r = min(most, a.items - a.first_item) * a.beams;
+    const unsigned grid = (unsigned)(((long long)r * a.lists + kBeamWarps - 1) / kBeamWarps);
+    if (a.f32) beam_kernel<float><<<grid, kBeamThreads, 0, st>>>(a, r);
+    else       beam_kernel<__nv_bfloat16><<<grid, kBeamThreads, 0, st>>>(a, r);
   }
   return counted(launches, (int)cudaGetLastError());
 }

@@ -41,7 +41,8 @@ def beam_step_reference(logits, scores, finished=None, eos=-1):
     lp = torch.log_softmax(x, -1)
     lp = torch.where(lp.isfinite().any(-1, keepdim=True) & ~lp.isnan().any(-1, keepdim=True), lp, -math.inf)
     start = scores.double()[..., None]
-    total = torch.where(start > -math.inf, start + lp, -math.inf)
+    start = torch.where(start.isfinite(), start, -math.inf)
+    total = start + lp
     if finished is not None:
         only = torch.where(torch.arange(vocab, device=x.device) == eos, start, -math.inf)
         total = torch.where(finished[..., None], only, total)
@@ -62,7 +63,7 @@ def beam_step(logits: torch.Tensor, scores: torch.Tensor, finished: Optional[tor
     best ``beams``, by ``scores [items, beams]`` (fp32) plus the log-probability that ``logits [items * beams, vocab]`` (bf16 or
     fp32) gives the token; equal ones in the order of beam and token.
 
-    A beam of ``finished [items, beams]`` (bool) goes on with ``eos`` alone, at its old score.  A beam of score -inf (or NaN) and a
+    A beam of ``finished [items, beams]`` (bool) goes on with ``eos`` alone, at its old score.  A beam whose score is not finite and a
     row of logits that is no distribution (a NaN, an infinity, nothing but -inf) have continuations worth -inf only, so a search starts
     with the scores ``0, -inf, -inf, ...``.
 

@@ -81,7 +81,7 @@ def beam(logits, scores, finished, eos):
             row = x[i, j]
             done = finished is not None and bool(finished[i, j])
             lone = np.full(vocab, -np.inf)
-            if start[i, j] > -np.inf:
+            if np.isfinite(start[i, j]):
                 if done:
                     lone[eos] = start[i, j]
                 elif not np.isnan(row).any() and np.max(row) < np.inf and np.max(row) > -np.inf:

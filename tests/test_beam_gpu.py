@@ -57,7 +57,7 @@ def test_masked_and_broken_rows(dtype, vocab):
     logits[6, vocab - 2] = -5.0
     agree(ops.beam_step(logits, scores), oracle.beam(logits, scores, None, -1))
     agree(ops.beam_step(logits, scores, finished, 3), oracle.beam(logits, scores, finished, 3))
-    scores[0, 5], scores[1, 2] = float("nan"), -INF
+    scores[0, 5], scores[1, 2], scores[0, 3] = float("nan"), -INF, INF
     finished[1, 2] = True
     agree(ops.beam_step(logits, scores, finished, 3), oracle.beam(logits, scores, finished, 3))
     scores[:] = -INF
