@@ -25,7 +25,7 @@ constexpr int kMaxBeams = 32;
 constexpr int kBeamThreads = 256, kBeamWarps = kBeamThreads / 32;
 constexpr int kWarpPool = 128;         // candidates of a warp that are ranked at once
 constexpr int kItemPool = 1024;        // and of an item
-constexpr int kHotLanes = 512;         // lanes whose logits are read again
+constexpr int kHotLanes = 256;         // lanes whose logits are read again
 constexpr int kMaxLists = 64;          // parts of a row
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -153,6 +153,7 @@ __device__ __forceinline__ Piece<T> load_piece(const T* row, int first, int end,
 // What a warp leaves of its logits: the sum of exponentials, what it is relative to, every lane's maximum.
 struct BeamPart {
   double sum, base;
+  float shift, pad[3];           // `base` in whole powers of two, NaN where it is none
   float high[32];
 };
 
@@ -161,10 +162,10 @@ struct BeamShared {
   double totals[kItemPool];
   float lists[kBeamThreads];
   double score[kMaxBeams], top[kMaxBeams], norm[kMaxBeams];
-  float from[kMaxBeams], offset[kMaxBeams], least[kMaxBeams];      // fp32 totals: x - from + offset; what x - from has to reach
+  float size[kMaxBeams];                   // of what fp32 totals are made of
   unsigned char kind[kMaxBeams];           // 0: by its logits, 1: finished, 2: nothing to offer
-  int hot[kHotLanes];
-  int count, hots, counts[kBeamWarps], done[kBeamWarps];
+  float from[kMaxBeams], least[kMaxBeams];  // what a logit less `from` has to reach
+  int hot[kHotLanes], count, hots, counts[kBeamWarps], done[kBeamWarps];
 };
 static_assert(kBeamWarps * kWarpPool <= kItemPool, "the warps' pools");
 
@@ -315,7 +316,40 @@ __device__ __noinline__ void best_of_rows(const BeamArgs& a, BeamShared& sh, con
   __syncthreads();
 }
 
-// The choice for an item, by the whole CTA.
+// The sum of a row's parts: what its logits are taken relative to, and the logarithm of the sum (not finite: no distribution).
+__device__ __forceinline__ void sum_row(const BeamPart* p, int lists, double& top, double& norm) {
+  const int lane = threadIdx.x & 31;
+  double base[2], sum[2], t = 0.0;
+  float shift[2];
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {          // (kMaxLists)
+    const bool in = lane + 32 * x < lists;
+    base[x] = in ? __ldcg(&p[lane + 32 * x].base) : -INFINITY;
+    sum[x] = in ? __ldcg(&p[lane + 32 * x].sum) : 0.0;
+    shift[x] = in ? __ldcg(&p[lane + 32 * x].shift) : -INFINITY;
+  }
+  if (__any_sync(0xffffffffu, shift[0] != shift[0] || shift[1] != shift[1])) {
+    top = fmax(base[0], base[1]);
+#pragma unroll 1
+    for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
+#pragma unroll 1
+    for (int x = 0; x < 2; ++x) t += sum[x] == 0.0 ? 0.0 : sum[x] * exp(base[x] - top);
+  } else {
+    const float most = warp_max(fmaxf(shift[0], shift[1]));
+    top = (double)most / (double)kLog2e;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const float down = fminf(most - shift[x], 1000.0f);
+      t += sum[x] * __longlong_as_double((long long)(1023 - (int)down) << 52);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  norm = log(t);
+}
+
+// The choice for an item, by the whole CTA.  A row belongs to a warp, or to as many as there are when beams are few.  Instructions, more than memory, are
+// what this costs: it runs once.
 template <typename T>
 __device__ __noinline__ void choose(const BeamArgs& a, BeamShared& sh, int local) {
   constexpr int N = Piece<T>::N;
@@ -323,132 +357,112 @@ __device__ __noinline__ void choose(const BeamArgs& a, BeamShared& sh, int local
   const BeamPart* parts = static_cast<const BeamPart*>(a.ws) + (long long)local * K * a.lists;
   const T* rows = static_cast<const T*>(a.logits) + (long long)item * K * a.ld;
   if (tid == 0) sh.count = sh.hots = 0;
+  const int mates = K <= 1 ? 8 : K <= 2 ? 4 : K <= 4 ? 2 : 1, w0 = warp / mates, dw = kBeamWarps / mates;      // warps of a row; rows of this warp
+  const int quads = a.lists * 8, q0 = (warp - w0 * mates) * 32 + lane, dq = mates * 32;                       // four lanes' maxima at a time
+  auto quad = [&](int w, int q) { return __ldcg(reinterpret_cast<const float4*>(parts[w * a.lists + (q >> 3)].high) + (q & 7)); };
+  // The W-th largest of the lanes' maxima, and the lanes that reach it, both in fp32, as x - from + offset, and with room for its roundings:
+  // `from` and `offset` are off by 2^-24 of themselves, and so are the two sums.
+  float high = -INFINITY;
 #pragma unroll 1
-  for (int w = warp; w < K; w += kBeamWarps) {
-    const BeamPart* p = parts + w * a.lists;
-    double base[2], sum[2];
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {          // (kMaxLists)
-      const int l = lane + 32 * x;
-      const bool in = l < a.lists;
-      base[x] = in ? __ldcg(&p[l].base) : -INFINITY;
-      sum[x] = in ? __ldcg(&p[l].sum) : 0.0;
-    }
-    double top = fmax(base[0], base[1]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
-    double t = 0.0;
-#pragma unroll 1
-    for (int x = 0; x < 2 && 32 * x < a.lists; ++x) t += sum[x] == 0.0 ? 0.0 : sum[x] * exp(base[x] - top);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  for (int w = w0; w < K; w += dw) {
+    double top, norm;
+    sum_row(parts + w * a.lists, a.lists, top, norm);
+    const float score = a.scores[item * K + w];
+    const bool fin = a.finished && a.finished[item * K + w];
+    const int kind = !(fabsf(score) < INFINITY) ? 2 : fin ? 1 : fabs(top) < INFINITY && fabs(norm) < INFINITY ? 0 : 2;
+    const float from = (float)top, offset = (float)(score - norm);
     if (lane == 0) {
-      const float score = a.scores[item * K + w];
-      const bool fin = a.finished && a.finished[item * K + w];
-      const double norm = log(t);
       sh.score[w] = score;
       sh.top[w] = top;
       sh.norm[w] = norm;
-      sh.from[w] = (float)top;
-      sh.offset[w] = (float)(score - norm);
-      sh.kind[w] = !(fabsf(score) < INFINITY) ? 2 : fin ? 1 : fabs(top) < INFINITY && fabs(norm) < INFINITY ? 0 : 2;
+      sh.kind[w] = kind;
+      sh.size[w] = kind ? 0.0f : fabsf(offset) + fminf(fabsf(from), 2.0f * kLarge);
+    }
+    if (kind == 0) {
+      float most = -INFINITY;
+#pragma unroll 4
+      for (int q = q0; q < quads; q += dq) {
+        const float4 v = quad(w, q);
+        most = fmaxf(most, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
+      }
+      high = fmaxf(high, most - from + offset);
+    } else if (q0 < min(K, a.vocab)) {
+      high = fmaxf(high, kind == 1 && a.eos >= 0 && q0 == 0 ? score : -INFINITY);
     }
   }
-  __syncthreads();
-  // The W-th largest of the lanes' maxima, and the lanes that reach it, both in fp32 and with room for its roundings: `from` and `offset`
-  // are off by 2^-24 of themselves, and so are the two sums.
-  const int quads = a.lists * 8, all = K * quads;
-  float limit = 0.0f, high = -INFINITY;
-#pragma unroll 1
-  for (int pass = 0; pass < 2; ++pass) {
-    constexpr int B = 4;                             // loads in flight
-#pragma unroll 1
-    for (int c0 = tid; c0 < all; c0 += B * kBeamThreads) {
-      float4 v[B];
-#pragma unroll
-      for (int x = 0; x < B; ++x) {
-        const int c = c0 + x * kBeamThreads;
-        v[x] = c < all ? __ldcg(reinterpret_cast<const float4*>(parts[c >> 3].high) + (c & 7)) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-      }
-#pragma unroll
-      for (int x = 0; x < B; ++x) {
-        const int c = min(c0 + x * kBeamThreads, all - 1), w = c / quads;
-        if (sh.kind[w]) continue;
-        const float e[4] = {v[x].x, v[x].y, v[x].z, v[x].w};
-        const float top = fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])) - sh.from[w];
-        if (pass == 0) {
-          high = fmaxf(high, top + sh.offset[w]);
-        } else if (top >= sh.least[w]) {
-#pragma unroll
-          for (int y = 0; y < 4; ++y)
-            if (e[y] - sh.from[w] >= sh.least[w]) {
-              const int at = atomicAdd(&sh.hots, 1);
-              if (at < kHotLanes) sh.hot[at] = 4 * c + y;
-            }
-        }
-      }
-    }
-    for (int c = tid; c < K * K; c += kBeamThreads) {
-      const int w = c / K, i = c - w * K;
-      if (!sh.kind[w] || i >= a.vocab) continue;
-      int token;
-      const double total = special(a, sh, w, i, token);
-      if (pass == 0) {
-        high = fmaxf(high, (float)total);
-      } else if (total >= limit) {
-        const int at = atomicAdd(&sh.count, 1);
-        if (at < kItemPool) {
-          sh.totals[at] = total;
-          sh.keys[at] = (unsigned long long)w << 32 | (unsigned)token;
-        }
-      }
-    }
-    if (pass == 0) {
-      limit = kth_largest(high, K, sh.lists);
-      if (limit == -INFINITY) break;
-      const bool mine = lane < K && sh.kind[lane] == 0;
-      const float size = warp_max(mine ? fabsf(sh.offset[lane]) + fminf(fabsf(sh.from[lane]), 2.0f * kLarge) : 0.0f);
-      limit -= (size + fabsf(limit)) * 0x1p-21f;
-      if (warp == 0 && mine) {
-        const float d = (float)((double)limit - sh.score[lane] + sh.norm[lane]);
-        sh.least[lane] = d - (size + fabsf(d)) * 0x1p-21f;
-      }
-      __syncthreads();
-    }
-  }
-  __syncthreads();
-  const int hots = sh.hots;
-  bool wide = limit == -INFINITY || hots > kHotLanes;
+  float limit = kth_largest(high, K, sh.lists);                // (its barriers cover sh)
+  bool wide = limit == -INFINITY;
   if (!wide) {
-    // A hot lane's pieces by as many lanes as there are pieces.
-    const int pieces = min(32, (min(a.chunk, a.vocab) + 32 * N - 1) / (32 * N)), width = pieces > 1 ? 1 << (32 - __clz(pieces - 1)) : 1;
+    const float size = warp_max(lane < K ? sh.size[lane] : 0.0f);
+    limit -= (size + fabsf(limit)) * 0x1p-21f;
 #pragma unroll 1
-    for (int h = tid / width; h < hots; h += kBeamThreads / width) {
-      const int j = sh.hot[h], part = j >> 5, w = part / a.lists, l = part - w * a.lists;
+    for (int w = w0; w < K; w += dw) {
+      if (sh.kind[w]) {
+        int token;
+        const double total = special(a, sh, w, q0, token);
+        if (q0 < min(K, a.vocab) && total >= limit) {
+          const int at = atomicAdd(&sh.count, 1);
+          if (at < kItemPool) {
+            sh.totals[at] = total;
+            sh.keys[at] = (unsigned long long)w << 32 | (unsigned)token;
+          }
+        }
+        continue;
+      }
       const T* row = rows + w * a.ld;
-      const int begin = l * a.chunk, end = min(a.vocab, begin + a.chunk);
-      const float from = sh.from[w], least = sh.least[w];
+      const float from = (float)sh.top[w], d = (float)((double)limit - sh.score[w] + sh.norm[w]), least = d - (size + fabsf(d)) * 0x1p-21f;
+      sh.from[w] = from;
+      sh.least[w] = least;
+      if (high < limit) continue;                               // none of this thread's, in any row
 #pragma unroll 1
-      for (int i = begin + ((j & 31) + 32 * (tid & (width - 1))) * N; i < end; i += width * 32 * N) {
-        const Piece<T> p = load_piece<T>(row, i, end, a.vec);
-        if (p.top() - from < least) continue;
-#pragma unroll 1
-        for (int e = 0; e < N && i + e < end; ++e) {
-          float x = p.at(0);
+      for (int q = q0; q < quads; q += 4 * dq) {
+        float4 v[4];
 #pragma unroll
-          for (int q = 1; q < N; ++q) x = e == q ? p.at(q) : x;
-          if (x - from >= least) {
-            const int at = atomicAdd(&sh.count, 1);
-            if (at < kItemPool) {
-              sh.totals[at] = total_of(sh, w, x);
-              sh.keys[at] = (unsigned long long)w << 32 | (unsigned)(i + e);
+        for (int x = 0; x < 4; ++x) v[x] = q + x * dq < quads ? quad(w, q + x * dq) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        unsigned mine = 0;
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          mine |= ((v[x].x - from >= least) | (v[x].y - from >= least) << 1 | (v[x].z - from >= least) << 2 | (v[x].w - from >= least) << 3) << 4 * x;
+#pragma unroll 1
+        for (; mine; mine &= mine - 1) {
+          const int at = atomicAdd(&sh.hots, 1), i = __ffs(mine) - 1;
+          if (at < kHotLanes) sh.hot[at] = (w * quads + q + (i >> 2) * dq) * 4 + (i & 3);
+        }
+      }
+    }
+    __syncthreads();
+    const int hots = sh.hots;
+    if (hots <= kHotLanes) {
+      // A hot lane's pieces by as many lanes as there are pieces.
+      const int pieces = min(32, (min(a.chunk, a.vocab) + 32 * N - 1) / (32 * N)), width = pieces > 1 ? 1 << (32 - __clz(pieces - 1)) : 1;
+#pragma unroll 1
+      for (int h = tid / width; h < hots; h += kBeamThreads / width) {
+        const int j = sh.hot[h], part = j >> 5, w = part / a.lists;
+        const T* row = rows + w * a.ld;
+        const int begin = (part - w * a.lists) * a.chunk, end = min(a.vocab, begin + a.chunk);
+        const float from = sh.from[w], least = sh.least[w];
+#pragma unroll 1
+        for (int i = begin + ((j & 31) + 32 * (tid & (width - 1))) * N; i < end; i += width * 32 * N) {
+          const Piece<T> p = load_piece<T>(row, i, end, a.vec);
+          if (p.top() - from < least) continue;
+#pragma unroll 1
+          for (int e = 0; e < N && i + e < end; ++e) {
+            float x = p.at(0);
+#pragma unroll
+            for (int n = 1; n < N; ++n) x = e == n ? p.at(n) : x;
+            if (x - from >= least) {
+              const int at = atomicAdd(&sh.count, 1);
+              if (at < kItemPool) {
+                sh.totals[at] = total_of(sh, w, x);
+                sh.keys[at] = (unsigned long long)w << 32 | (unsigned)(i + e);
+              }
             }
           }
         }
       }
     }
     __syncthreads();
-    wide = sh.count > kItemPool;
+    wide = sh.hots > kHotLanes || sh.count > kItemPool;
   }
   if (wide) {
     __syncthreads();
@@ -527,12 +541,14 @@ beam_kernel(const __grid_constant__ BeamArgs a, int rows) {
     if (lane == 0) {
       part->sum = sum;           // NaN where there is one
       part->base = base;
+      part->shift = fabsf(best) < kLarge ? last : NAN;
     }
-    __threadfence();
     __syncwarp();
     if (lane == 0) {
       const int local = local_row / K;
-      if (atomicAdd(a.counters + local, 1u) == (unsigned)(K * a.lists) - 1) {
+      unsigned before;      // releases what the warp has written, acquires what those before it have
+      asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(a.counters + local) : "memory");
+      if (before == (unsigned)(K * a.lists) - 1) {
         a.counters[local] = 0;
         done = local;
       }
@@ -544,7 +560,6 @@ beam_kernel(const __grid_constant__ BeamArgs a, int rows) {
   for (int w = 0; w < kBeamWarps; ++w) {
     const int local = sh.done[w];
     if (local < 0) continue;
-    __threadfence();
     choose<T>(a, sh, local);
     __syncthreads();
   }
