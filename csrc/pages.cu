@@ -6,6 +6,7 @@
 //
 // All of it runs on the device without the host's knowledge, so that a decoding loop needs no synchronisation and can be captured.
 #include <cuda_bf16.h>
+#include <math.h>
 
 #include "common/host.h"
 #include "common/ptx.cuh"
@@ -19,7 +20,8 @@ namespace dptb {
 // negative position has no place and passes unturned (padding).  The angle is formed and reduced to one turn in 64 bits: in 32 a position of
 // 100000 leaves it 0.004 rad off.
 //
-// Bound by memory, or by the launch for a step.  A CTA per token, its angles in shared memory, heads by in 16-byte groups.
+// Bound by memory, or by the launch for a step.  A CTA takes up to 8 tokens: their angles first, one a thread, into shared memory, then the
+// heads by in 16-byte groups.
 struct AppendArgs {
   const void* qkv;
   void* q;                // [tokens, heads, hd], contiguous
@@ -31,12 +33,30 @@ struct AppendArgs {
   const int* rows;        // null: token t belongs to row t
   long long ld, k_page, k_head, k_tok, v_page, v_head, v_tok, table_row;
   int tokens, heads, kv_heads, hd, rotary, page, width, pages, table_rows, f32;
-  double base;
+  double base;            // its logarithm to base 2 in the kernel
 };
 static_assert(sizeof(AppendArgs) == 176, "packed by the caller");
 
 constexpr int kAppendThreads = 256;
 constexpr int kAppendPairs = 128;    // of a head of 256 features
+constexpr int kAppendTokens = 8;
+
+// n / d = n * mul >> shift for 0 <= n < 2^31: mul = ceil(2^shift / d) with 2^(shift - 31) >= d, whose excess, less than one, adds less than the
+// last place of a quotient.
+struct Divisor {
+  unsigned mul, shift;
+  static Divisor of(int d) {
+    Divisor x{0, 31};
+    while (1LL << (x.shift - 31) < d) ++x.shift;
+    if (d > 0) x.mul = (unsigned)(((1ULL << x.shift) + d - 1) / d);
+    return x;
+  }
+  __device__ __forceinline__ int divide(int n) const { return (int)((unsigned long long)(unsigned)n * mul >> shift); }
+};
+struct AppendShape {
+  Divisor pairs, whole, tail, by_turned, by_kv;      // groups of a half, of a head, behind the turned features; heads
+  int tokens;                                        // of a CTA
+};
 
 template <typename T, int VEC>
 __device__ __forceinline__ void load_group(const T* p, float (&f)[VEC]) {
@@ -57,83 +77,103 @@ __device__ __forceinline__ void store_group(T* p, const float (&f)[VEC]) {
 
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kAppendThreads)
-paged_append_kernel(const AppendArgs a) {
-  __shared__ float2 turn[kAppendPairs];
-  const long long t = blockIdx.x;
+paged_append_kernel(const AppendArgs a, const AppendShape shape) {
+  __shared__ float2 turn[kAppendTokens * kAppendPairs];
+  __shared__ int page_of[kAppendTokens], off_of[kAppendTokens];
+  const int t0 = blockIdx.x * shape.tokens, nt = min(shape.tokens, a.tokens - t0);
   const int tid = threadIdx.x, half = a.rotary / 2;
-  const int pos = a.positions[t], row = a.rows ? a.rows[t] : (int)t;
-  int page = -1;
-  if (pos >= 0) {
-    if (row >= 0 && row < a.table_rows && pos / a.page < a.width) page = a.table[row * a.table_row + pos / a.page];
-    if (page < 0 || page >= a.pages) {      // no place for it: nothing is written
-      if (tid == 0) report_error(kBadPage);
-      page = -1;
+  if (tid < nt) {
+    const int pos = a.positions[t0 + tid], row = a.rows ? a.rows[t0 + tid] : t0 + tid;
+    int page = -1;
+    if (pos >= 0) {
+      const int slot = pos / a.page;
+      if (row >= 0 && row < a.table_rows && slot < a.width) page = a.table[row * a.table_row + slot];
+      if (page < 0 || page >= a.pages) {      // no place for it: nothing is written
+        report_error(kBadPage);
+        page = -1;
+      }
+      off_of[tid] = pos - slot * a.page;
     }
+    page_of[tid] = page;
   }
-  for (int d = tid; d < half; d += kAppendThreads) {
+  for (int i = tid; i < nt * half; i += kAppendThreads) {
+    const int t = i / half, d = i - t * half, pos = a.positions[t0 + t];
     float sn = 0.0f, cs = 1.0f;
     if (pos > 0) {
-      constexpr double kTurn = 6.283185307179586476925;
-      const double angle = pos * pow(a.base, -2.0 * d / a.rotary);
-      sincosf((float)(angle - kTurn * rint(angle / kTurn)), &sn, &cs);
+      constexpr double kTurn = 6.283185307179586476925, kTurns = 1.0 / kTurn;
+      const double turns = pos * exp2(-2.0 * d / a.rotary * a.base) * kTurns;
+      sincosf((float)((turns - rint(turns)) * kTurn), &sn, &cs);
     }
-    turn[d] = make_float2(cs, sn);
+    turn[i] = make_float2(cs, sn);
   }
   __syncthreads();
-  const T* x = static_cast<const T*>(a.qkv) + t * a.ld;
   const int turned = a.heads + a.kv_heads;
-  T* kp = static_cast<T*>(a.k) + page * a.k_page + (pos % a.page) * a.k_tok;
-  T* vp = static_cast<T*>(a.v) + page * a.v_page + (pos % a.page) * a.v_tok;
-  auto put = [&](int h, int d, const float (&f)[VEC]) {
+  auto put = [&](int t, int h, int d, const float (&f)[VEC]) {
+    const long long tok = t0 + t;
     if (h < a.heads) {
-      store_group<T, VEC>(static_cast<T*>(a.q) + (t * a.heads + h) * a.hd + d, f);
-    } else if (h < turned) {
-      const int g = h - a.heads;
-      if (a.keys) store_group<T, VEC>(static_cast<T*>(a.keys) + (t * a.kv_heads + g) * a.hd + d, f);
-      if (page >= 0) store_group<T, VEC>(kp + g * a.k_head + d, f);
+      store_group<T, VEC>(static_cast<T*>(a.q) + (tok * a.heads + h) * a.hd + d, f);
+      return;
+    }
+    const int page = page_of[t], g = h - a.heads;
+    if (h < turned) {
+      if (a.keys) store_group<T, VEC>(static_cast<T*>(a.keys) + (tok * a.kv_heads + g) * a.hd + d, f);
+      if (page >= 0) store_group<T, VEC>(static_cast<T*>(a.k) + page * a.k_page + off_of[t] * a.k_tok + g * a.k_head + d, f);
     } else if (page >= 0) {
-      store_group<T, VEC>(vp + (h - turned) * a.v_head + d, f);
+      store_group<T, VEC>(static_cast<T*>(a.v) + page * a.v_page + off_of[t] * a.v_tok + (h - turned) * a.v_head + d, f);
     }
   };
+  const T* x = static_cast<const T*>(a.qkv) + t0 * a.ld;
   const int pairs = half / VEC, whole = a.hd / VEC, tail = (a.hd - a.rotary) / VEC;
-  for (int i = tid; i < turned * pairs; i += kAppendThreads) {
-    const int h = i / pairs, d = i % pairs * VEC;
+#pragma unroll 2
+  for (int i = tid; i < nt * turned * pairs; i += kAppendThreads) {
+    const int n = shape.pairs.divide(i), d = (i - n * pairs) * VEC, t = shape.by_turned.divide(n), h = n - t * turned;
+    const T* src = x + t * a.ld + h * a.hd + d;
+    const float2* w = turn + t * half + d;
     float lo[VEC], hi[VEC];
-    load_group<T, VEC>(x + (long long)h * a.hd + d, lo);
-    load_group<T, VEC>(x + (long long)h * a.hd + half + d, hi);
+    load_group<T, VEC>(src, lo);
+    load_group<T, VEC>(src + half, hi);
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
-      const float2 c = turn[d + j];
+      const float2 c = w[j];
       const float p = lo[j] * c.x - hi[j] * c.y, q = hi[j] * c.x + lo[j] * c.y;
       lo[j] = p;
       hi[j] = q;
     }
-    put(h, d, lo);
-    put(h, half + d, hi);
+    put(t, h, d, lo);
+    put(t, h, half + d, hi);
   }
-  for (int i = tid; i < turned * tail; i += kAppendThreads) {     // features that are not turned
-    const int h = i / tail, d = a.rotary + i % tail * VEC;
+  if (tail > 0)
+    for (int i = tid; i < nt * turned * tail; i += kAppendThreads) {     // features that are not turned
+      const int n = shape.tail.divide(i), d = a.rotary + (i - n * tail) * VEC, t = shape.by_turned.divide(n), h = n - t * turned;
+      float f[VEC];
+      load_group<T, VEC>(x + t * a.ld + h * a.hd + d, f);
+      put(t, h, d, f);
+    }
+#pragma unroll 2
+  for (int i = tid; i < nt * a.kv_heads * whole; i += kAppendThreads) {
+    const int n = shape.whole.divide(i), d = (i - n * whole) * VEC, t = shape.by_kv.divide(n), h = turned + n - t * a.kv_heads;
     float f[VEC];
-    load_group<T, VEC>(x + (long long)h * a.hd + d, f);
-    put(h, d, f);
-  }
-  for (int i = tid; i < a.kv_heads * whole; i += kAppendThreads) {
-    const int h = turned + i / whole, d = i % whole * VEC;
-    float f[VEC];
-    load_group<T, VEC>(x + (long long)h * a.hd + d, f);
-    put(h, d, f);
+    load_group<T, VEC>(x + t * a.ld + h * a.hd + d, f);
+    put(t, h, d, f);
   }
 }
 
 template <typename T, int VEC>
-static int launch_append(const AppendArgs& a, cudaStream_t st) {
+static int launch_append(AppendArgs a, cudaStream_t st) {
   auto whole = [](const void* p, long long s0, long long s1, long long s2) {
     return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && s0 % VEC == 0 && s1 % VEC == 0 && s2 % VEC == 0;
   };
   const bool vec = a.hd % VEC == 0 && a.rotary / 2 % VEC == 0 && whole(a.qkv, a.ld, 0, 0) && whole(a.q, 0, 0, 0) &&
                    whole(a.keys, 0, 0, 0) && whole(a.k, a.k_page, a.k_head, a.k_tok) && whole(a.v, a.v_page, a.v_head, a.v_tok);
-  if (vec) paged_append_kernel<T, VEC><<<a.tokens, kAppendThreads, 0, st>>>(a);
-  else     paged_append_kernel<T, 1><<<a.tokens, kAppendThreads, 0, st>>>(a);
+  const int v = vec ? VEC : 1, half = a.rotary / 2;
+  a.base = log2(a.base);
+  // At least four CTAs an SM before one takes several tokens.
+  const int per = a.tokens / (4 * sm_count());
+  const AppendShape shape{Divisor::of(half / v), Divisor::of(a.hd / v), Divisor::of((a.hd - a.rotary) / v), Divisor::of(a.heads + a.kv_heads),
+                          Divisor::of(a.kv_heads), per < 1 ? 1 : per > kAppendTokens ? kAppendTokens : per};
+  const int grid = (a.tokens + shape.tokens - 1) / shape.tokens;
+  if (vec) paged_append_kernel<T, VEC><<<grid, kAppendThreads, 0, st>>>(a, shape);
+  else     paged_append_kernel<T, 1><<<grid, kAppendThreads, 0, st>>>(a, shape);
   return counted(1, (int)cudaGetLastError());
 }
 
