@@ -179,8 +179,9 @@ static int launch_append(AppendArgs a, cudaStream_t st) {
 
 // ------------------------------------------------------------------------------------------------------------ who holds what
 constexpr int kPageThreads = 1024;
-constexpr int kMaxForkRows = 4096;
-constexpr int kMaxPages = 1 << 19;
+constexpr int kMaxForkRows = 4096, kRowBits = 12;
+constexpr int kMaxPages = 1 << 19;       // with a row in 31 bits
+constexpr int kPageCluster = 8;
 constexpr int kPageSmem = 224 << 10;    // both bit maps of the largest pool, and the rows
 
 // Exclusive sum over the block; `total` is everybody's sum.  `scratch`: 33 ints.
@@ -216,12 +217,29 @@ __device__ __forceinline__ void mark(unsigned* bits, int page) {
   if (!(reinterpret_cast<volatile unsigned*>(bits)[page >> 5] & b)) atomicOr(bits + (page >> 5), b);
 }
 
+// CTAs of a cluster mark pages in maps of their own; this one's word i joined with the others'.
+__device__ __forceinline__ unsigned joined(const unsigned* bits, int i, unsigned ctas) {
+  unsigned v = 0;
+  for (unsigned c = 0; c < ctas; ++c) {
+    unsigned u;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(u) : "r"(map_to_cta(bits + i, c)) : "memory");
+    v |= u;
+  }
+  return v;
+}
+__device__ __forceinline__ unsigned cluster_ctas() {
+  unsigned n;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n));
+  return n;
+}
+
 // New row r is row parents[r] of the old table (-1: empty), longer by `grow` tokens.  Pages for these come from the free ones, lowest numbers
 // first, in the order of the rows.  The last page of a row that grows into it must be the row's own: it is when no other row lists it but
 // such as grow into it too, and the first of these keeps it; the others take a copy, which (src, dst) name for the kernel that copies.
 //
-// One CTA: bit maps of the pages in shared memory (listed at all; listed by somebody who does not grow into it), a hash table from a page to the first
-// row that grows into it, and sums over rows and pages for the order.
+// One cluster: the CTAs share the rows, a warp a row, and mark pages in bit maps in shared memory (listed at all; listed by somebody who does not grow
+// into it).  The first CTA joins the maps and does what needs all rows: a hash table from a page to the first row that grows into it, and sums over rows and pages
+// for the order.  Bound by a chain of a dozen latencies.  One CTA for all rows took 36 us for 256 rows of up to 100 pages.
 struct ForkArgs {
   const int* table;
   const int* lens;
@@ -231,7 +249,7 @@ struct ForkArgs {
   int* new_lens;
   int* src;               // [rows]
   int* dst;
-  int* free_list;         // [pages] of scratch
+  int* free_list;         // [pages] of scratch: the pages to be given
   long long table_row;
   int rows_in, rows, width, pages, page, grow_all;
 };
@@ -261,48 +279,74 @@ fork_pages_kernel(const ForkArgs a, int words, int slots) {
   extern __shared__ unsigned smem[];
   unsigned* used = smem;                                     // [words]
   unsigned* others = used + words;                           // [words]
-  int* key = reinterpret_cast<int*>(others + words);         // [slots]: pages that rows grow into
-  int* first = key + slots;                                  // [slots]: the lowest such row
-  int* rank = first + slots;                                 // [rows]: pages given to the rows before
+  // Of the first CTA:
+  unsigned* hash = others + words;                           // [slots]: page and first row that grows into it
+  int* tail = reinterpret_cast<int*>(hash + slots);          // [rows]: page that a row grows into, -1 if none
+  int* held = tail + a.rows;                                 // [rows]
+  int* rank = held + a.rows;                                 // [rows]: pages that a row wants; pages given to the rows before
   __shared__ int scratch[33];
+  constexpr unsigned kEmpty = 0xffffffffu;
+  const unsigned cta = cluster_cta_rank(), ctas = cluster_ctas();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = kPageThreads / 32;
   for (int i = tid; i < 2 * words; i += kPageThreads) used[i] = 0;
-  for (int i = tid; i < slots; i += kPageThreads) {
-    key[i] = -1;
-    first[i] = 0x7fffffff;
-  }
-  __syncthreads();
-  auto find = [&](int page) {
-    int i = (int)((unsigned)page * 2654435761u % (unsigned)slots);
-    for (int n = 0; n < slots; ++n) {                        // (more slots than rows: it ends)
-      const int had = atomicCAS(key + i, -1, page);
-      if (had == -1 || had == page) return i;
-      i = i + 1 == slots ? 0 : i + 1;
-    }
-    return 0;
-  };
-  for (int r = warp; r < a.rows; r += nw) {
+  if (cta == 0)
+    for (int i = tid; i < slots; i += kPageThreads) hash[i] = kEmpty;
+  cluster_sync_all();                                        // (every CTA has started: its memory can be written)
+  for (int r = cta * nw + warp; r < a.rows; r += ctas * nw) {
     const ForkRow f = fork_row(a, r);
     if (lane == 0) {
       const bool bad = a.parents && a.parents[r] >= a.rows_in;
       const long long more = a.grow ? max(a.grow[r], 0) : f.parent >= 0 ? a.grow_all : 0;
       if (bad || f.parent >= 0 && a.lens[f.parent] > f.old_len || f.new_len < f.old_len + more) report_error(kBadPage);
+      a.new_lens[r] = f.new_len;
+      st_cluster_u32(map_to_cta(held + r, 0), f.held);
+      st_cluster_u32(map_to_cta(rank + r, 0), f.want - f.held);
+      if (!f.grows) st_cluster_u32(map_to_cta(tail + r, 0), kEmpty);
     }
     const int* row = a.table + (f.parent < 0 ? 0 : f.parent) * a.table_row;
-    for (int s = lane; s < a.width; s += 32) {
-      int page = -1;
-      if (s < f.held) {
-        page = row[s];
-        if (page < 0 || page >= a.pages) {
-          report_error(kBadPage);
-          page = -1;
-        } else {
-          mark(used, page);
-          if (f.grows && s == f.held - 1) atomicMin(first + find(page), r);
-          else mark(others, page);
+    int* out = a.new_table + (long long)r * a.width;
+    for (int s0 = lane; s0 < a.width; s0 += 4 * 32) {
+      int page[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) page[x] = s0 + 32 * x < f.held ? row[s0 + 32 * x] : -1;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int s = s0 + 32 * x;
+        if (s >= a.width) break;
+        if (s < f.held) {
+          if ((unsigned)page[x] >= (unsigned)a.pages) {
+            report_error(kBadPage);
+            page[x] = -1;
+          } else {
+            mark(used, page[x]);
+          }
+          if (f.grows && s == f.held - 1) st_cluster_u32(map_to_cta(tail + r, 0), page[x]);
+          else if (page[x] >= 0) mark(others, page[x]);
         }
+        out[s] = page[x];
       }
-      a.new_table[(long long)r * a.width + s] = page;
+    }
+  }
+  cluster_sync_all();
+  if (cta == 0 && ctas > 1)
+    for (int i = tid; i < 2 * words; i += kPageThreads) used[i] = joined(used, i, ctas);
+  if (ctas > 1) cluster_sync_all();                          // the first CTA has read the others' maps
+  if (cta != 0) return;
+  __syncthreads();
+  auto place = [&](int page) { return (int)((unsigned)page * 2654435761u % (unsigned)slots); };
+  for (int r = tid; r < a.rows; r += kPageThreads) {
+    const int page = tail[r];
+    if (page < 0) continue;
+    const unsigned mine = (unsigned)page << kRowBits | (unsigned)r;
+    int i = place(page);
+    for (int n = 0; n < slots; ++n) {                        // (more slots than rows: it ends)
+      const unsigned had = atomicCAS(hash + i, kEmpty, mine);
+      if (had == kEmpty) break;
+      if (had >> kRowBits == (unsigned)page) {
+        atomicMin(hash + i, mine);
+        break;
+      }
+      i = i + 1 == slots ? 0 : i + 1;
     }
   }
   __syncthreads();
@@ -312,12 +356,14 @@ fork_pages_kernel(const ForkArgs a, int words, int slots) {
     int need = 0;
     bool copies = false;
     if (r < a.rows) {
-      const ForkRow f = fork_row(a, r);
-      if (f.grows) {
-        const int page = a.new_table[(long long)r * a.width + f.held - 1];
-        copies = page >= 0 && ((others[page >> 5] >> (page & 31) & 1) || first[find(page)] != r);
+      const int page = tail[r];
+      if (page >= 0) {
+        int i = place(page);
+        while (hash[i] >> kRowBits != (unsigned)page) i = i + 1 == slots ? 0 : i + 1;      // (it is there)
+        copies = (others[page >> 5] >> (page & 31) & 1) || (hash[i] & ((1u << kRowBits) - 1)) != (unsigned)r;
       }
-      need = f.want - f.held + copies;
+      need = rank[r] + copies;
+      a.src[r] = a.dst[r] = -1;
     }
     int total;
     const int before = block_scan(need, scratch, total);
@@ -339,27 +385,19 @@ fork_pages_kernel(const ForkArgs a, int words, int slots) {
   }
   __syncthreads();
   if (found < need_all && tid == 0) report_error(kPoolFull);
-  for (int r = warp; r < a.rows; r += nw) {
-    const ForkRow f = fork_row(a, r);
-    const bool copies = rank[r] & 1;
-    const int at = rank[r] >> 1;
-    int* row = a.new_table + (long long)r * a.width;
-    for (int s = f.held + lane; s < f.want; s += 32) {
-      const int i = at + copies + s - f.held;
-      row[s] = i < found ? a.free_list[i] : -1;
+  for (int k = tid; k < need_all; k += kPageThreads) {       // the k-th page to be given, and whose it is
+    int r = 0, hi = a.rows - 1;
+    while (r < hi) {
+      const int mid = (r + hi + 1) / 2;
+      if (rank[mid] >> 1 <= k) r = mid;
+      else hi = mid - 1;
     }
-    if (lane == 0) {
-      int from = -1, to = -1;
-      if (copies) {
-        if (at < found) {
-          from = row[f.held - 1];
-          to = a.free_list[at];
-        }
-        row[f.held - 1] = to;
-      }
-      a.src[r] = from;
-      a.dst[r] = to;
-      a.new_lens[r] = f.new_len;
+    const bool copies = rank[r] & 1;
+    const int i = k - (rank[r] >> 1), page = k < found ? a.free_list[k] : -1;
+    a.new_table[(long long)r * a.width + held[r] + i - copies] = page;
+    if (copies && i == 0 && page >= 0) {
+      a.src[r] = tail[r];
+      a.dst[r] = page;
     }
   }
 }
@@ -376,50 +414,89 @@ struct CompactArgs {
 };
 static_assert(sizeof(CompactArgs) == 64, "packed by the caller");
 
+// One cluster: the CTAs share the rows, each has the joined map, and they share the pages.
 __global__ void __launch_bounds__(kPageThreads)
 compact_pages_kernel(const CompactArgs a, int words) {
   extern __shared__ unsigned smem[];
-  unsigned* used = smem;                                     // [words]
+  unsigned* mine = smem;                                     // [words]: pages that this CTA's rows list
+  unsigned* used = mine + words;                             // [words]: that any lists
   int* before = reinterpret_cast<int*>(used + words);        // [words]: listed pages ahead of a word
   __shared__ int scratch[33];
-  const int tid = threadIdx.x;
-  for (int i = tid; i < words; i += kPageThreads) used[i] = 0;
+  const unsigned cta = cluster_cta_rank(), ctas = cluster_ctas();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = kPageThreads / 32;
+  for (int i = tid; i < words; i += kPageThreads) mine[i] = 0;
   __syncthreads();
-  const long long entries = (long long)a.rows * a.width;
-  for (long long i = tid; i < entries; i += kPageThreads) {
-    const int page = a.table[i / a.width * a.table_row + i % a.width];
-    if (page >= a.pages) report_error(kBadPage);
-    else if (page >= 0) mark(used, page);
-  }
-  __syncthreads();
+  for (int r = cta * nw + warp; r < a.rows; r += ctas * nw)
+    for (int s0 = lane; s0 < a.width; s0 += 4 * 32) {
+      int page[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) page[x] = s0 + 32 * x < a.width ? a.table[r * a.table_row + s0 + 32 * x] : -1;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        if (page[x] >= a.pages) report_error(kBadPage);
+        else if (page[x] >= 0) mark(mine, page[x]);
+      }
+    }
+  cluster_sync_all();
   int live = 0;
   for (int w0 = 0; w0 < words; w0 += kPageThreads) {
     const int w = w0 + tid;
+    const unsigned bits = w < words ? joined(mine, w, ctas) : 0;
     int total;
-    const int at = live + block_scan(w < words ? __popc(used[w]) : 0, scratch, total);
-    if (w < words) before[w] = at;
+    const int at = live + block_scan(__popc(bits), scratch, total);
+    if (w < words) {
+      used[w] = bits;
+      before[w] = at;
+    }
     live += total;
   }
   __syncthreads();
   auto rank = [&](int page) { return before[page >> 5] + __popc(used[page >> 5] & ((1u << (page & 31)) - 1)); };
   const int kept = live < a.pages ? rank(live) : live;       // live pages that stay: those below `live`
-  const int moves = live - kept;
-  for (int i = tid; i < a.pages / 2; i += kPageThreads) {
+  const int moves = live - kept, first = cta * kPageThreads + tid, step = ctas * kPageThreads;
+  for (int i = first; i < a.pages / 2; i += step) {
     if (i >= moves) a.src[i] = a.dst[i] = -1;
   }
-  for (int p = tid; p < a.pages; p += kPageThreads) {
+  for (int p = first; p < a.pages; p += step) {
     const bool on = used[p >> 5] >> (p & 31) & 1;
     if (p < live && !on) a.dst[p - rank(p)] = p;
     if (p >= live && on) a.src[rank(p) - kept] = p;
   }
-  __syncthreads();
-  for (long long i = tid; i < entries; i += kPageThreads) {
-    int page = a.table[i / a.width * a.table_row + i % a.width];
-    if (page < 0 || page >= a.pages) page = -1;
-    else if (page >= live) page = a.dst[rank(page) - kept];
-    a.new_table[i] = page;
-  }
-  if (tid == 0) *a.live = live;
+  if (first == 0) *a.live = live;
+  cluster_sync_all();                                        // dst is there, and nobody reads another's map any more
+  for (int r = cta * nw + warp; r < a.rows; r += ctas * nw)
+    for (int s0 = lane; s0 < a.width; s0 += 4 * 32) {
+      int page[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) page[x] = s0 + 32 * x < a.width ? a.table[r * a.table_row + s0 + 32 * x] : -1;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        if (page[x] < 0 || page[x] >= a.pages) page[x] = -1;
+        else if (page[x] >= live) page[x] = __ldcg(a.dst + rank(page[x]) - kept);
+      }
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        if (s0 + 32 * x < a.width) a.new_table[(long long)r * a.width + s0 + 32 * x] = page[x];
+    }
+}
+
+// Up to 32 rows a CTA has a warp for each; more are shared by a cluster.
+template <typename... KArgs>
+static int launch_page_kernel(void (*kernel)(KArgs...), SmemLimit& limit, int rows, size_t smem, cudaStream_t st, KArgs... args) {
+  if (smem > kPageSmem) return kErrTooLarge;
+  DPTB_CUDA_OK(limit.raise((const void*)kernel, kPageSmem));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(rows <= 32 ? 1 : kPageCluster);
+  cfg.blockDim = dim3(kPageThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = cfg.gridDim.x;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return counted(1, (int)cudaLaunchKernelEx(&cfg, kernel, args...));
 }
 
 // pool[o, dst[i]] = pool[o, src[i]] for every o < outer and every i with a src, `bytes` a page.  Nobody's dst is somebody's src.
@@ -437,7 +514,16 @@ copy_pages_kernel(unsigned char* pool, const int* __restrict__ src, const int* _
     }
     const V* x = reinterpret_cast<const V*>(base + from * bytes);
     V* y = reinterpret_cast<V*>(base + to * bytes);
-    for (long long j = threadIdx.x; j < bytes / (long long)sizeof(V); j += kCopyThreads) y[j] = x[j];
+    const int count = (int)(bytes / (long long)sizeof(V));
+    for (int j = threadIdx.x; j < count; j += 4 * kCopyThreads) {
+      V v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (j + u * kCopyThreads < count) v[u] = x[j + u * kCopyThreads];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (j + u * kCopyThreads < count) y[j + u * kCopyThreads] = v[u];
+    }
   }
 }
 
@@ -462,30 +548,23 @@ extern "C" int dptb_fork_pages(const ForkArgs* args, void* stream) {
       a.grow_all < 0)
     return kErrBadShape;
   const int words = (a.pages + 31) / 32, slots = 2 * a.rows;
-  const size_t smem = (2 * (size_t)words + 2 * (size_t)slots + a.rows) * 4;
   static SmemLimit limit;
-  if (smem > kPageSmem) return kErrTooLarge;
-  DPTB_CUDA_OK(limit.raise((const void*)fork_pages_kernel, kPageSmem));
-  fork_pages_kernel<<<1, kPageThreads, smem, static_cast<cudaStream_t>(stream)>>>(a, words, slots);
-  return counted(1, (int)cudaGetLastError());
+  return launch_page_kernel(fork_pages_kernel, limit, a.rows, (2 * (size_t)words + (size_t)slots + 3 * (size_t)a.rows) * 4,
+                            static_cast<cudaStream_t>(stream), a, words, slots);
 }
 
 extern "C" int dptb_compact_pages(const CompactArgs* args, void* stream) {
   const CompactArgs& a = *args;
   if (a.rows < 0 || a.width < 0 || a.pages < 0 || a.pages > kMaxPages) return kErrBadShape;
   const int words = (a.pages + 31) / 32;
-  const size_t smem = 2 * (size_t)words * 4;
   static SmemLimit limit;
-  if (smem > kPageSmem) return kErrTooLarge;
-  DPTB_CUDA_OK(limit.raise((const void*)compact_pages_kernel, kPageSmem));
-  compact_pages_kernel<<<1, kPageThreads, smem, static_cast<cudaStream_t>(stream)>>>(a, words);
-  return counted(1, (int)cudaGetLastError());
+  return launch_page_kernel(compact_pages_kernel, limit, a.rows, 3 * (size_t)words * 4, static_cast<cudaStream_t>(stream), a, words);
 }
 
 extern "C" int dptb_copy_pages(void* pool, const int* src, const int* dst, int n, long long outer, int pages, long long bytes,
                                void* stream) {
   if (n == 0 || outer == 0 || bytes == 0) return 0;
-  if (n < 0 || outer < 0 || outer > 65535 || pages < 0 || bytes < 0) return kErrBadShape;
+  if (n < 0 || outer < 0 || outer > 65535 || pages < 0 || bytes < 0 || bytes > 0x7fffffff) return kErrBadShape;
   const dim3 grid(n < 8 * 148 ? n : 8 * 148, (unsigned)outer);
   auto st = static_cast<cudaStream_t>(stream);
   auto* p = static_cast<unsigned char*>(pool);
