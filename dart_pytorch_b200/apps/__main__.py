@@ -203,7 +203,9 @@ def cmd_hf_runner(args):
             h.close()
         return
     req = {"maxNewTokens": args.max_new_tokens, "temperature": args.temperature, "topK": args.top_k, "seed": args.seed,
-           "useCache": not args.no_cache}
+           "useCache": not args.no_cache, "beams": args.beams, "lengthPenalty": args.length_penalty}
+    if args.eos is not None:
+        req["eos"] = args.eos
     if args.tokens:
         req["tokens"] = [int(t) for t in args.tokens.split(",")]
     else:
@@ -397,6 +399,9 @@ def main(argv=None):
         p.add_argument("--top-k", type=int, default=0)
         p.add_argument("--seed", type=int, default=None)
         p.add_argument("--no-cache", action="store_true")
+        p.add_argument("--beams", type=int, default=1, help="beam search of this width instead of sampling")
+        p.add_argument("--eos", type=int, default=None, help="token that ends a beam")
+        p.add_argument("--length-penalty", type=float, default=0.0)
         p.add_argument("--serve", action="store_true")
         p.add_argument("--host", default="127.0.0.1")
         p.add_argument("--port", type=int, default=8080)

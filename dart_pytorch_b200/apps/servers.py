@@ -3,7 +3,8 @@ bin/_gptj_hf_api_common.dart, bin/rag_chat_server.dart:1-700, bin/llama_chat.dar
 
 ``GenerationService`` wraps a loaded causal LM + optional tokenizer: ``run({...})`` answers the JSON contract of
 ``POST /generate`` (``text | tokens, maxNewTokens, temperature, topK, seed, useCache`` ->
-``tokens, newTokens, text, elapsedMs``); ``serve()`` exposes ``GET /health``, ``GET /info``, ``POST /generate``.
+``tokens, newTokens, text, elapsedMs``; with ``beams`` > 1, ``eos`` and ``lengthPenalty``: beam search, and the ``beams`` with
+their scores); ``serve()`` exposes ``GET /health``, ``GET /info``, ``POST /generate``.
 
 ``RagChatService`` is the chunked-RAG chat pipeline: uploaded documents are token-chunked (200 tokens, stride 100),
 each chunk embedded with the LM's last-token hidden state, centred on the corpus mean and L2-normalised into an
@@ -158,8 +159,21 @@ class GenerationService:
         top_k = int(req.get("topK", 0)) or None
         seed = req.get("seed")
         rng = random.Random(int(seed)) if seed is not None else random.Random()
+        beams = int(req.get("beams", 1))
+        if beams > 1 and not hasattr(self.model, "generate_beams"):
+            return 400, {"error": f"{self.model_name} has no beam search"}
+        if not 1 <= beams <= 32:
+            return 400, {"error": '"beams" must be between 1 and 32'}
         t0 = time.perf_counter()
         with self._lock:
+            if beams > 1:
+                eos = req.get("eos")
+                best = self.model.generate_beams([tokens], max_new, beams, None if eos is None else int(eos),
+                                                 float(req.get("lengthPenalty", 0.0)))[0]
+                ids = best[0][0]
+                return 200, {"tokens": ids, "newTokens": ids[len(tokens):], "text": self.tok.decode(ids) if self.tok else None,
+                             "beams": [{"newTokens": seq[len(tokens):], "score": score} for seq, score in best],
+                             "elapsedMs": int((time.perf_counter() - t0) * 1000)}
             out = self.model.generate(tokens, max_new, temperature=temperature, top_k=top_k, rng=rng,
                                       use_cache=bool(req.get("useCache", True)))
         ids = [int(t) for t in out]

@@ -19,7 +19,9 @@ from ..ops.stack import plain
 from ..nn.attention import EncoderCache
 from ..nn.layers import Dropout, Embedding, LearnedPositionalEmbedding, Linear
 from ..nn.module import Module
+from ..nn.paged import PagedCache
 from ..nn.transformer import Activation, TransformerEncoder
+from .beam import beam_search
 
 
 @dataclass
@@ -130,6 +132,14 @@ class GPT(Module):
         h = self.hidden(tokens, start_pos, cache)
         return F.linear(h, self.head_weight)
 
+    paged_head_dim = property(lambda self: self.config.embed_dim // self.config.num_heads)
+
+    def paged_hidden(self, tokens, cache: PagedCache):
+        """Final hidden states of ``tokens [B, N]`` that ``cache`` was last extended by (``prompts``, ``fork``)."""
+        h = F.embedding(self.token_emb.weight, tokens)
+        at = F.embedding(self.pos_emb.table.weight, cache.positions.clamp(min=0).long().view(tokens.shape))
+        return self.encoder(self.embed_drop(F.add(h, at)), cache=cache, causal=tokens.shape[1] > 1)
+
     def loss(self, tokens, targets):
         """Mean next-token cross-entropy; equals ``self(tokens).crossEntropy(targets).mean()`` of the reference recipe
         (bin/gpt_train.dart:111-131) without a logits tensor surviving to the backward."""
@@ -162,6 +172,12 @@ class GPT(Module):
         finally:
             if was_training:
                 self.train()
+
+    def generate_beams(self, prompts, max_new_tokens: int, beams: int = 4, eos: Optional[int] = None,
+                       length_penalty: float = 0.0):
+        """Beam search from ``prompts``, token sequences of any lengths; for each the best ``beams`` as ``(tokens, score)``
+        (see ``models/beam.py``)."""
+        return beam_search(self, prompts, max_new_tokens, beams, eos, length_penalty)
 
     def _sample(self, logits_row: torch.Tensor, temperature, top_k, rng) -> int:
         v = self.config.vocab_size

@@ -19,6 +19,8 @@ from ..ops.stack import plain
 from ..nn.attention import EncoderCache, MHACache, MultiHeadAttention, RopeCache, stock_attention, stock_cache
 from ..nn.layers import Embedding, Linear, RMSNorm, SwiGluFfn
 from ..nn.module import Module
+from ..nn.paged import PagedCache
+from .beam import beam_search
 from .gpt import _as_token_tensor
 
 
@@ -159,6 +161,12 @@ class Llama(Module):
         tokens = _as_token_tensor(tokens, self.device)
         return F.linear(self.hidden(tokens, start_pos, cache), self.head_weight)
 
+    paged_head_dim = property(lambda self: self.config.head_dim)
+
+    def paged_hidden(self, tokens, cache: PagedCache):
+        """Final hidden states of ``tokens [B, N]`` that ``cache`` was last extended by (``prompts``, ``fork``)."""
+        return self.hidden_from_embeddings(F.embedding(self.embed_in.weight, tokens), 0, cache)
+
     def loss(self, tokens, targets):
         tokens = _as_token_tensor(tokens, self.device)
         targets = _as_token_tensor(targets, self.device)
@@ -237,3 +245,9 @@ class Llama(Module):
         finally:
             if was_training:
                 self.train()
+
+    def generate_beams(self, prompts, max_new_tokens: int, beams: int = 4, eos: Optional[int] = None,
+                       length_penalty: float = 0.0):
+        """Beam search from ``prompts``, token sequences of any lengths; for each the best ``beams`` as ``(tokens, score)``
+        (see ``models/beam.py``)."""
+        return beam_search(self, prompts, max_new_tokens, beams, eos, length_penalty)

@@ -3,6 +3,7 @@ from .module import Module, make_param
 from .layers import (Linear, LayerNorm, RMSNorm, Embedding, Dropout, SinusoidalPositionalEncoding,
                      LearnedPositionalEmbedding, SwiGluFfn, VisionProjector, causal_mask, activation_name)
 from .attention import RopeCache, MHACache, EncoderCache, MultiHeadAttention, MultiHeadCrossAttention
+from .paged import PagedCache, PagedLayer
 from .transformer import (Activation, TransformerBlock, TransformerEncoder, TransformerDecoderBlock,
                           TransformerDecoder)
 

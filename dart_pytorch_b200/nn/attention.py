@@ -16,6 +16,7 @@ from .. import ops as F
 from ..ops.stack import plain
 from .layers import Dropout, Linear
 from .module import Module, make_param, uniform_, normal_
+from .paged import PagedLayer
 
 
 class RopeCache:
@@ -268,6 +269,11 @@ class MultiHeadAttention(Module):
         dq, dkv = H * hd, Hkv * hd
         x2 = x.reshape(B * S, self.embed_dim)
         qkv = F.linear(x2, self.w_qkv, self.b_qkv)  # [B*S, dq + 2 dkv]
+        if isinstance(cache, PagedLayer):
+            if mask is not None:
+                raise ValueError("MultiHeadAttention: a paged cache takes no mask")
+            out = self.wo(cache.attend(qkv, B, S, H, self.rope), residual=None if residual is None else residual.reshape(B * S, -1))
+            return (out if self.attn_dropout is None else self.attn_dropout(out)).reshape(*x.shape[:-1], self.embed_dim)
         if self.rope is not None:
             self.rope.check_window(start_pos, S)
         # rotation and append in one kernel; another class of cache (or a replaced append) gets its rows by `append`
