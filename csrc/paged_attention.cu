@@ -255,8 +255,13 @@ struct Bf16Round {
 };
 
 // ------------------------------------------------------------------------------------------------------------ fp32
-// GP: query heads at a time.  Lane s of the 8 lanes of a key holds pieces s + 8 i of it; four keys go by at once, two steps a round.  The
+// GP: query heads at a time.  Lane t of the 8 lanes of a key holds pieces t + 8 i of it; four keys go by at once, two steps a round.  The
 // queries are read from shared memory where they are needed (features beyond the head's are zeros there).
+//
+// A step's products leave 2 GP sums of 8 lanes each (head, step).  They are added in halves: with every exchange a lane keeps half of its sums, so that
+// in the end it has one (of head head_of(t)), for which it alone keeps maximum and sum and takes the exponential; the weights go
+// back to the lanes by shuffle.  Multiply-adds are packed in pairs.  With every sum in every lane, and single multiply-adds, 13 sequences of up to
+// 1531 keys (10 heads of 80 on 5) took 22 us.
 template <int HD, int GP>
 struct F32Round {
   using T = float;
@@ -264,124 +269,148 @@ struct F32Round {
   static constexpr int P = HD / 32;                      // pieces of a key per lane
   static constexpr int kSegs = P, kSeg = kKeys * 128, kBytes = 2 * kSegs * kSeg;         // a tile for every 32 features
   static constexpr int kQueryBytes = GP * HD * 4;
+  static constexpr int kSums = 2 * GP, kOwn = kSums > 8 ? kSums / 8 : 1, kSpread = kSums >= 8 ? 1 : 8 / kSums;     // sums; of a lane; lanes of a sum
 
-  float m[GP], l[GP];
-  float4 o[GP][P];
+  float m, l;
+  f32x2 o[GP][P][2];
+
+  // The lane (of 8) that keeps sum (head, step).
+  static __device__ __forceinline__ constexpr int lane_of(int h, int j) { return kOwn == 2 ? h : (2 * h + j) * kSpread; }
 
   __device__ __forceinline__ void start(const PagedAttnArgs&, const unsigned char*, int, int) {
+    m = -INFINITY;
+    l = 0.0f;
 #pragma unroll
-    for (int h = 0; h < GP; ++h) {
-      m[h] = -INFINITY;
-      l[h] = 0.0f;
+    for (int h = 0; h < GP; ++h)
 #pragma unroll
-      for (int i = 0; i < P; ++i) o[h][i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    }
+      for (int i = 0; i < P; ++i) o[h][i][0] = o[h][i][1] = 0ull;
   }
 
   __device__ __forceinline__ void compute(uint32_t ring, unsigned keys, float scale2, const unsigned char* queries, int lane) {
     const int g = lane >> 3, t = lane & 7;
-    const unsigned live = keys >> g & 1 | (keys >> (g + 4) & 1) << 1;
-    auto piece = [&](int seg, int j) {                   // of key g + 4 j
+    auto piece = [&](int seg, int j, f32x2 (&v)[2]) {    // of key g + 4 j
       const int key = g + 4 * j;
-      return read_piece(ring + seg * kSeg + key * 128 + ((t ^ key) << 4));
+      const uint4 u = read_piece(ring + seg * kSeg + key * 128 + ((t ^ key) << 4));
+      v[0] = f2_pack(__uint_as_float(u.x), __uint_as_float(u.y));
+      v[1] = f2_pack(__uint_as_float(u.z), __uint_as_float(u.w));
     };
-    const float4* q4 = reinterpret_cast<const float4*>(queries) + (lane & 7);
-    float p[GP][2];
+    const ulonglong2* q = reinterpret_cast<const ulonglong2*>(queries) + t;
+    float v[kSums];
+    {
+      f32x2 k[2][P][2];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      float4 k[P];
+      for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int i = 0; i < P; ++i) {
-        const uint4 u = piece(i, j);
-        k[i] = make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w));
-      }
+        for (int i = 0; i < P; ++i) piece(i, j, k[j][i]);
 #pragma unroll
       for (int h = 0; h < GP; ++h) {
-        float s = 0.0f, s1 = 0.0f;
+        f32x2 s[2] = {0ull, 0ull};
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-          const float4 w = q4[h * (HD / 4) + 8 * i];
-          s = fmaf(k[i].x, w.x, s);
-          s1 = fmaf(k[i].y, w.y, s1);
-          s = fmaf(k[i].z, w.z, s);
-          s1 = fmaf(k[i].w, w.w, s1);
+          const ulonglong2 w = q[h * (HD / 4) + 8 * i];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) s[j] = f2_fma(k[j][i][1], w.y, f2_fma(k[j][i][0], w.x, s[j]));
         }
-        p[h][j] = s + s1;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float lo, hi;
+          f2_unpack(s[j], lo, hi);
+          v[2 * h + j] = lo + hi;
+        }
       }
     }
-    bool moved = false;
-    float corr[GP];
+    int n = kSums;
 #pragma unroll
-    for (int h = 0; h < GP; ++h) {
+    for (int off = 4; off > 0; off >>= 1) {
+      const bool upper = t & off;
+      if (n > 1) {
+        n >>= 1;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float s = p[h][j];
-#pragma unroll
-        for (int off = 1; off < 8; off <<= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-        p[h][j] = live >> j & 1 ? s * scale2 : -INFINITY;
+        for (int i = 0; i < n; ++i) {
+          const float keep = upper ? v[i + n] : v[i], give = upper ? v[i] : v[i + n];
+          v[i] = keep + __shfl_xor_sync(0xffffffffu, give, off);
+        }
+      } else {
+        v[0] += __shfl_xor_sync(0xffffffffu, v[0], off);
       }
-      float mx = fmaxf(p[h][0], p[h][1]);
-#pragma unroll
-      for (int off = 8; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-      const float nm = fmaxf(m[h], mx), sub = nm == -INFINITY ? 0.0f : nm;
-      moved |= nm != m[h];
-      corr[h] = exp2_fast(m[h] - sub);
-#pragma unroll
-      for (int j = 0; j < 2; ++j) p[h][j] = live >> j & 1 ? exp2_fast(p[h][j] - sub) : 0.0f;
-      l[h] = l[h] * corr[h] + (p[h][0] + p[h][1]);
-      m[h] = nm;
     }
+    float p[kOwn], mx = -INFINITY;
+    bool live[kOwn];
+#pragma unroll
+    for (int r = 0; r < kOwn; ++r) {
+      const int j = kOwn == 2 ? r : t / kSpread & 1;
+      live[r] = keys >> (g + 4 * j) & 1;
+      p[r] = live[r] ? v[r] * scale2 : -INFINITY;
+      mx = fmaxf(mx, p[r]);
+    }
+    if (kOwn == 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, kSpread));        // the other step
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+    const float nm = fmaxf(m, mx), sub = nm == -INFINITY ? 0.0f : nm, corr = exp2_fast(m - sub);
+    const bool moved = nm != m;
+    l *= corr;
+#pragma unroll
+    for (int r = 0; r < kOwn; ++r) {
+      p[r] = live[r] ? exp2_fast(p[r] - sub) : 0.0f;
+      l += p[r];
+    }
+    m = nm;
     if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-      for (int h = 0; h < GP; ++h)
+      for (int h = 0; h < GP; ++h) {
+        const f32x2 c = f2_splat(__shfl_sync(0xffffffffu, corr, lane & 24 | lane_of(h, 0)));
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-          o[h][i].x *= corr[h];
-          o[h][i].y *= corr[h];
-          o[h][i].z *= corr[h];
-          o[h][i].w *= corr[h];
-        }
-    }
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int i = 0; i < P; ++i) {
-        const uint4 u = piece(kSegs + i, j);
-#pragma unroll
-        for (int h = 0; h < GP; ++h) {
-          o[h][i].x = fmaf(p[h][j], __uint_as_float(u.x), o[h][i].x);
-          o[h][i].y = fmaf(p[h][j], __uint_as_float(u.y), o[h][i].y);
-          o[h][i].z = fmaf(p[h][j], __uint_as_float(u.z), o[h][i].z);
-          o[h][i].w = fmaf(p[h][j], __uint_as_float(u.w), o[h][i].w);
+          o[h][i][0] = f2_mul(o[h][i][0], c);
+          o[h][i][1] = f2_mul(o[h][i][1], c);
         }
       }
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      f32x2 w[GP];
+#pragma unroll
+      for (int h = 0; h < GP; ++h) w[h] = f2_splat(__shfl_sync(0xffffffffu, p[kOwn == 2 ? j : 0], lane & 24 | lane_of(h, j)));
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        f32x2 x[2];
+        piece(kSegs + i, j, x);
+#pragma unroll
+        for (int h = 0; h < GP; ++h) {
+          o[h][i][0] = f2_fma(w[h], x[0], o[h][i][0]);
+          o[h][i][1] = f2_fma(w[h], x[1], o[h][i][1]);
+        }
+      }
+    }
   }
 
   __device__ __forceinline__ void finish(int) {
+    if (kOwn == 1) l += __shfl_xor_sync(0xffffffffu, l, kSpread);
 #pragma unroll
-    for (int h = 0; h < GP; ++h)
+    for (int off = 8; off < 32; off <<= 1) {
+      l += __shfl_xor_sync(0xffffffffu, l, off);
 #pragma unroll
-      for (int off = 8; off < 32; off <<= 1) {
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], off);
+      for (int h = 0; h < GP; ++h)
 #pragma unroll
-        for (int i = 0; i < P; ++i) {
-          o[h][i].x += __shfl_xor_sync(0xffffffffu, o[h][i].x, off);
-          o[h][i].y += __shfl_xor_sync(0xffffffffu, o[h][i].y, off);
-          o[h][i].z += __shfl_xor_sync(0xffffffffu, o[h][i].z, off);
-          o[h][i].w += __shfl_xor_sync(0xffffffffu, o[h][i].w, off);
-        }
-      }
+        for (int i = 0; i < P; ++i)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) o[h][i][e] = f2_add(o[h][i][e], __shfl_xor_sync(0xffffffffu, o[h][i][e], off));
+    }
   }
   template <typename F>
   __device__ __forceinline__ void each(int lane, F put) const {
-    if (lane >= 8) return;
 #pragma unroll
-    for (int h = 0; h < GP; ++h)
+    for (int h = 0; h < GP; ++h) {
+      const float mh = __shfl_sync(0xffffffffu, m, lane_of(h, 0)), lh = __shfl_sync(0xffffffffu, l, lane_of(h, 0));
+      if (lane < 8)
 #pragma unroll
-      for (int i = 0; i < P; ++i) {
-        const float f[4] = {o[h][i].x, o[h][i].y, o[h][i].z, o[h][i].w};
-        put(h, 4 * (lane + 8 * i), f, m[h], l[h]);
-      }
+        for (int i = 0; i < P; ++i) {
+          float f[4];
+          f2_unpack(o[h][i][0], f[0], f[1]);
+          f2_unpack(o[h][i][1], f[2], f[3]);
+          put(h, 4 * (lane + 8 * i), f, mh, lh);
+        }
+    }
   }
 };
 
@@ -920,13 +949,15 @@ extern "C" int dptb_paged_attention(const PagedAttnArgs* args, void* stream) {
       if (a.hd <= 128) { if (group <= 8) DPTB_PAGED(B128, 8, 2); DPTB_PAGED(C128, 6, 2); }
       DPTB_PAGED(B256, 4, 2);
     }
-    using F1_64 = F32Round<64, 1>; using F4_64 = F32Round<64, 4>; using F8_64 = F32Round<64, 8>;
-    using F1_128 = F32Round<128, 1>; using F4_128 = F32Round<128, 4>; using F8_128 = F32Round<128, 8>;
-    using F1_256 = F32Round<256, 1>; using F4_256 = F32Round<256, 4>;
-    if (a.hd <= 64) { if (group == 1) DPTB_PAGED(F1_64, 8, 4); if (group <= 4) DPTB_PAGED(F4_64, 8, 4); DPTB_PAGED(F8_64, 8, 4); }
-    if (a.hd <= 128) { if (group == 1) DPTB_PAGED(F1_128, 8, 2); if (group <= 4) DPTB_PAGED(F4_128, 8, 2); DPTB_PAGED(F8_128, 7, 2); }
-    if (group == 1) DPTB_PAGED(F1_256, 4, 2);
-    DPTB_PAGED(F4_256, 4, 2);
+#define DPTB_PAGED_F32(HD, W, S) \
+    if (group == 1) { using R1 = F32Round<HD, 1>; DPTB_PAGED(R1, W, S); } \
+    if (group == 2) { using R2 = F32Round<HD, 2>; DPTB_PAGED(R2, W, S); } \
+    if (group <= 4 || HD == 256) { using R4 = F32Round<HD, 4>; DPTB_PAGED(R4, W, S); }
+    if (a.hd <= 64) { DPTB_PAGED_F32(64, 8, 4) using R8 = F32Round<64, 8>; DPTB_PAGED(R8, 8, 4); }
+    if (a.hd <= 96) { DPTB_PAGED_F32(96, 8, 2) using R8 = F32Round<96, 8>; DPTB_PAGED(R8, 8, 2); }
+    if (a.hd <= 128) { DPTB_PAGED_F32(128, 8, 2) using R8 = F32Round<128, 8>; DPTB_PAGED(R8, 7, 2); }
+    DPTB_PAGED_F32(256, 4, 2)
+#undef DPTB_PAGED_F32
 #undef DPTB_PAGED
   }
   const dim3 grid(a.heads, a.rows);

@@ -79,10 +79,8 @@ def beam_step(logits: torch.Tensor, scores: torch.Tensor, finished: Optional[tor
         scores = scores.contiguous()
         finished = None if finished is None else finished.contiguous()
     (items, beams), vocab = scores.shape, logits.shape[1]
-    out_scores = scores.new_empty((items, beams))
-    out_parents = torch.empty((items, beams), dtype=torch.int32, device=logits.device)
-    out_tokens = torch.empty((items, beams), dtype=torch.long, device=logits.device)
-    out_finished = torch.empty((items, beams), dtype=torch.bool, device=logits.device)
+    out_scores, out_parents = torch.empty_like(scores), torch.empty_like(scores, dtype=torch.int32)
+    out_tokens, out_finished = torch.empty_like(scores, dtype=torch.long), torch.empty_like(scores, dtype=torch.bool)
     lib, stream = _lib(), _raw_stream(dev)
     ws, counters = _scratch(dev, stream)
     N.check(lib.dptb_beam_step(_BEAM_ARGS.pack(

@@ -149,7 +149,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
             q = q.contiguous()
             q_row, q_head, _ = q.stride()
     if out is None:
-        out = q.new_empty((rows, heads, hd))
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((rows, heads, hd))
         o_row, o_head = heads * hd, hd
     else:
         o_row, o_head, _ = out.stride()
@@ -348,8 +348,9 @@ def fork_pages(table: torch.Tensor, lens: torch.Tensor, pages: int, page: int, p
             return fork_pages_reference(table, lens, pages, page, parents, grow)
     rows_in, width = table.shape
     rows = rows_in if parents is None else parents.shape[0]
-    new_table, new_lens = table.new_empty((rows, width)), table.new_empty((rows,))
-    src, dst = table.new_empty((rows,)), table.new_empty((rows,))
+    new_table = torch.empty_like(table) if rows == rows_in and table.is_contiguous() else table.new_empty((rows, width))
+    like = lens if parents is None else parents
+    new_lens, src, dst = torch.empty_like(like), torch.empty_like(like), torch.empty_like(like)
     stream = _raw_stream(dev)
     N.check(_lib().dptb_fork_pages(_FORK_ARGS.pack(
         table.data_ptr(), lens.data_ptr(), 0 if parents is None else parents.data_ptr(), grow.data_ptr() if each else 0,
@@ -415,8 +416,10 @@ def compact_pages(table: torch.Tensor, pages: int) -> Tuple[torch.Tensor, torch.
         if dev < 0:
             return compact_pages_reference(table, pages)
     rows, width = table.shape
-    new, live = table.new_empty((rows, width)), table.new_empty((1,))
-    src, dst = table.new_empty((pages // 2,)), table.new_empty((pages // 2,))
+    new = torch.empty_like(table) if table.is_contiguous() else table.new_empty((rows, width))
+    live = table.new_empty((1,))
+    src = table.new_empty((pages // 2,))
+    dst = torch.empty_like(src)
     N.check(_lib().dptb_compact_pages(_COMPACT_ARGS.pack(
         table.data_ptr(), new.data_ptr(), src.data_ptr(), dst.data_ptr(), live.data_ptr(), table.stride(0), rows, width, pages),
         _raw_stream(dev)), "compact_pages")
