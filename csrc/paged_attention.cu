@@ -109,11 +109,12 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kTiny = 1.2e-38f;
 
 // ------------------------------------------------------------------------------------------------------------ bf16
-// HD: features of a head, padded with zeros; NT: tiles of 8 query heads.
-template <int HD, int NT>
+// HD: features of a head, padded with zeros; NT: tiles of 8 query heads; M: times 16 keys a round (two where rows are short: a request and a
+// maximum for each 16 keys of 64 features kept 16 sequences of 4096 keys at 39 us).
+template <int HD, int NT, int M>
 struct Bf16Round {
   using T = __nv_bfloat16;
-  static constexpr int kKeys = 16, kKeyShift = 4, kHeads = 8 * NT, kHD = HD;
+  static constexpr int kKeys = 16 * M, kKeyShift = M == 2 ? 5 : 4, kHeads = 8 * NT, kHD = HD;
   static constexpr int kSegs = HD / 64, kSeg = kKeys * 128, kBytes = 2 * kSegs * kSeg;   // keys, then values: a tile for every 64 features
   static constexpr int kQueryBytes = kHeads * HD * 2;
 
@@ -153,48 +154,57 @@ struct Bf16Round {
     const int t = lane & 3, mine = order(lane >> 2);
     const uint32_t swz = (mine ^ t) << 4;              // piece t of row `mine`, and piece `mine` of row t
     const uint32_t kr = ring + mine * 128, vr = ring + kSegs * kSeg + t * 128;
-    const unsigned live = keys >> mine & 1 | (keys >> (mine + 8) & 1) << 1;
-    float sc[NT][2][4] = {};
+    float sc[NT][M][2][4] = {};
 #pragma unroll
-    for (int i = 0; i < HD / 32; ++i) {
-      const uint32_t at = kr + (i >> 1) * kSeg + (swz ^ (i & 1) << 6);
-      const uint4 k0 = read_piece(at), k1 = read_piece(at + 1024);
-      const uint32_t fa[4] = {k0.x, k1.x, k0.y, k1.y}, fb[4] = {k0.z, k1.z, k0.w, k1.w};
+    for (int i = 0; i < HD / 32; ++i)
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        mma_bf16_16816(sc[n][0], fa, q[n][i].x, q[n][i].y);
-        mma_bf16_16816(sc[n][1], fb, q[n][i].z, q[n][i].w);
+      for (int b = 0; b < M; ++b) {
+        const uint32_t at = kr + (i >> 1) * kSeg + b * 2048 + (swz ^ (i & 1) << 6);
+        const uint4 k0 = read_piece(at), k1 = read_piece(at + 1024);
+        const uint32_t fa[4] = {k0.x, k1.x, k0.y, k1.y}, fb[4] = {k0.z, k1.z, k0.w, k1.w};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          mma_bf16_16816(sc[n][b][0], fa, q[n][i].x, q[n][i].y);
+          mma_bf16_16816(sc[n][b][1], fb, q[n][i].z, q[n][i].w);
+        }
       }
-    }
-    uint32_t pp[NT][2][2];      // [part][keys, keys + 8]: pairs of keys of head lane / 4
+    const unsigned there = keys >> mine;               // bits 0, 8, ...: this lane's keys
+    uint32_t pp[NT][M][2][2];   // [16 keys][part][keys, keys + 8]: pairs of keys of head lane / 4
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      float p[2][2], corr[2];   // [key, key + 8][head]
+      float p[2 * M][2], corr[2];   // [key, key + 8, ...][head]
       bool moved = false;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float s[2];
+        float s[2 * M], mx = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < 2; ++r) s[r] = live >> r & 1 ? (sc[n][0][2 * r + e] + sc[n][1][2 * r + e]) * scale2 : -INFINITY;
-        float mx = fmaxf(s[0], s[1]);
+        for (int r = 0; r < 2 * M; ++r) {
+          const float x = (sc[n][r >> 1][0][2 * (r & 1) + e] + sc[n][r >> 1][1][2 * (r & 1) + e]) * scale2;
+          s[r] = there >> (8 * r) & 1 ? x : -INFINITY;
+          mx = fmaxf(mx, s[r]);
+        }
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
         const float nm = fmaxf(m[n][e], mx), sub = nm == -INFINITY ? 0.0f : nm;
         moved |= nm != m[n][e];
         corr[e] = exp2_fast(m[n][e] - sub);
+        float sum = 0.0f;
 #pragma unroll
-        for (int r = 0; r < 2; ++r) p[r][e] = live >> r & 1 ? exp2_fast(s[r] - sub) : 0.0f;
-        l[n][e] = l[n][e] * corr[e] + (p[0][e] + p[1][e]);
+        for (int r = 0; r < 2 * M; ++r) {
+          p[r][e] = there >> (8 * r) & 1 ? exp2_fast(s[r] - sub) : 0.0f;
+          sum += p[r][e];
+        }
+        l[n][e] = l[n][e] * corr[e] + sum;
         m[n][e] = nm;
       }
       // Leading 8 bits and the rest.  Parts of a positive weight stay positive: its product with an infinite value is infinite in each.
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
+      for (int r = 0; r < 2 * M; ++r) {
         const uint32_t u0 = __float_as_uint(p[r][0]), u1 = __float_as_uint(p[r][1]);
-        pp[n][0][r] = movmatrix_trans((u0 >> 16) | (u1 & 0xffff0000u));
+        pp[n][r >> 1][0][r & 1] = movmatrix_trans((u0 >> 16) | (u1 & 0xffff0000u));
         const float r0 = p[r][0] > 0.0f ? fmaxf(p[r][0] - __uint_as_float(u0 & 0xffff0000u), kTiny) : 0.0f;
         const float r1 = p[r][1] > 0.0f ? fmaxf(p[r][1] - __uint_as_float(u1 & 0xffff0000u), kTiny) : 0.0f;
-        pp[n][1][r] = movmatrix_trans(pack_bf16x2(r0, r1));
+        pp[n][r >> 1][1][r & 1] = movmatrix_trans(pack_bf16x2(r0, r1));
       }
       if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
@@ -206,24 +216,26 @@ struct Bf16Round {
       }
     }
 #pragma unroll
-    for (int b = 0; b < HD / 64; ++b) {
-      uint32_t v[4][4];
+    for (int b = 0; b < HD / 64; ++b)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint4 u = read_piece(vr + b * kSeg + j * 512 + (swz ^ (j & 1) << 6));       // keys t, t + 4, t + 8, t + 12
-        v[j][0] = u.x; v[j][1] = u.y; v[j][2] = u.z; v[j][3] = u.w;
-      }
+      for (int c = 0; c < M; ++c) {
+        uint32_t v[4][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t f[4] = {__byte_perm(v[0][i], v[1][i], 0x5410), __byte_perm(v[0][i], v[1][i], 0x7632),
-                               __byte_perm(v[2][i], v[3][i], 0x5410), __byte_perm(v[2][i], v[3][i], 0x7632)};
+        for (int j = 0; j < 4; ++j) {
+          const uint4 u = read_piece(vr + b * kSeg + c * 2048 + j * 512 + (swz ^ (j & 1) << 6));       // keys t, t + 4, t + 8, t + 12
+          v[j][0] = u.x; v[j][1] = u.y; v[j][2] = u.z; v[j][3] = u.w;
+        }
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          mma_bf16_16816(o[n][b][i], f, pp[n][0][0], pp[n][0][1]);
-          mma_bf16_16816(o[n][b][i], f, pp[n][1][0], pp[n][1][1]);
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t f[4] = {__byte_perm(v[0][i], v[1][i], 0x5410), __byte_perm(v[0][i], v[1][i], 0x7632),
+                                 __byte_perm(v[2][i], v[3][i], 0x5410), __byte_perm(v[2][i], v[3][i], 0x7632)};
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            mma_bf16_16816(o[n][b][i], f, pp[n][c][0][0], pp[n][c][0][1]);
+            mma_bf16_16816(o[n][b][i], f, pp[n][c][1][0], pp[n][c][1][1]);
+          }
         }
       }
-    }
   }
 
   __device__ __forceinline__ void finish(int lane) {
@@ -255,27 +267,27 @@ struct Bf16Round {
 };
 
 // ------------------------------------------------------------------------------------------------------------ fp32
-// GP: query heads at a time.  Lane t of the 8 lanes of a key holds pieces t + 8 i of it; four keys go by at once, two steps a round.  The
+// GP: query heads at a time.  Lane t of the 8 lanes of a key holds pieces t + 8 i of it; four keys go by at once, NJ steps a round.  The
 // queries are read from shared memory where they are needed (features beyond the head's are zeros there).
 //
-// A step's products leave 2 GP sums of 8 lanes each (head, step).  They are added in halves: with every exchange a lane keeps half of its sums, so that
-// in the end it has one (of head head_of(t)), for which it alone keeps maximum and sum and takes the exponential; the weights go
+// A round's products leave NJ GP sums of 8 lanes each (head, step).  They are added in halves: with every exchange a lane keeps half of its sums, so that
+// in the end it has one or a few of one head, for which it alone keeps maximum and sum and takes the exponentials; the weights go
 // back to the lanes by shuffle.  Multiply-adds are packed in pairs.  With every sum in every lane, and single multiply-adds, 13 sequences of up to
 // 1531 keys (10 heads of 80 on 5) took 22 us.
-template <int HD, int GP>
+template <int HD, int GP, int NJ>
 struct F32Round {
   using T = float;
-  static constexpr int kKeys = 8, kKeyShift = 3, kHeads = GP, kHD = HD;
+  static constexpr int kKeys = 4 * NJ, kKeyShift = NJ == 4 ? 4 : 3, kHeads = GP, kHD = HD;
   static constexpr int P = HD / 32;                      // pieces of a key per lane
   static constexpr int kSegs = P, kSeg = kKeys * 128, kBytes = 2 * kSegs * kSeg;         // a tile for every 32 features
   static constexpr int kQueryBytes = GP * HD * 4;
-  static constexpr int kSums = 2 * GP, kOwn = kSums > 8 ? kSums / 8 : 1, kSpread = kSums >= 8 ? 1 : 8 / kSums;     // sums; of a lane; lanes of a sum
+  static constexpr int kSums = NJ * GP, kOwn = kSums > 8 ? kSums / 8 : 1, kSpread = kSums >= 8 ? 1 : 8 / kSums;     // sums; of a lane; lanes of a sum
 
   float m, l;
   f32x2 o[GP][P][2];
 
   // The lane (of 8) that keeps sum (head, step).
-  static __device__ __forceinline__ constexpr int lane_of(int h, int j) { return kOwn == 2 ? h : (2 * h + j) * kSpread; }
+  static __device__ __forceinline__ constexpr int lane_of(int h, int j) { return (NJ * h + j) / kOwn * kSpread; }
 
   __device__ __forceinline__ void start(const PagedAttnArgs&, const unsigned char*, int, int) {
     m = -INFINITY;
@@ -290,32 +302,32 @@ struct F32Round {
     const int g = lane >> 3, t = lane & 7;
     auto piece = [&](int seg, int j, f32x2 (&v)[2]) {    // of key g + 4 j
       const int key = g + 4 * j;
-      const uint4 u = read_piece(ring + seg * kSeg + key * 128 + ((t ^ key) << 4));
+      const uint4 u = read_piece(ring + seg * kSeg + key * 128 + ((t ^ key & 7) << 4));
       v[0] = f2_pack(__uint_as_float(u.x), __uint_as_float(u.y));
       v[1] = f2_pack(__uint_as_float(u.z), __uint_as_float(u.w));
     };
     const ulonglong2* q = reinterpret_cast<const ulonglong2*>(queries) + t;
     float v[kSums];
     {
-      f32x2 k[2][P][2];
+      f32x2 k[NJ][P][2];
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < NJ; ++j)
 #pragma unroll
         for (int i = 0; i < P; ++i) piece(i, j, k[j][i]);
 #pragma unroll
       for (int h = 0; h < GP; ++h) {
-        f32x2 s[2] = {0ull, 0ull};
+        f32x2 s[NJ] = {};
 #pragma unroll
         for (int i = 0; i < P; ++i) {
           const ulonglong2 w = q[h * (HD / 4) + 8 * i];
 #pragma unroll
-          for (int j = 0; j < 2; ++j) s[j] = f2_fma(k[j][i][1], w.y, f2_fma(k[j][i][0], w.x, s[j]));
+          for (int j = 0; j < NJ; ++j) s[j] = f2_fma(k[j][i][1], w.y, f2_fma(k[j][i][0], w.x, s[j]));
         }
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < NJ; ++j) {
           float lo, hi;
           f2_unpack(s[j], lo, hi);
-          v[2 * h + j] = lo + hi;
+          v[NJ * h + j] = lo + hi;
         }
       }
     }
@@ -338,12 +350,13 @@ struct F32Round {
     bool live[kOwn];
 #pragma unroll
     for (int r = 0; r < kOwn; ++r) {
-      const int j = kOwn == 2 ? r : t / kSpread & 1;
+      const int j = (t / kSpread * kOwn + r) % NJ;
       live[r] = keys >> (g + 4 * j) & 1;
       p[r] = live[r] ? v[r] * scale2 : -INFINITY;
       mx = fmaxf(mx, p[r]);
     }
-    if (kOwn == 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, kSpread));        // the other step
+#pragma unroll
+    for (int off = kSpread; off < 8 / GP; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));      // the head's other steps
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
     const float nm = fmaxf(m, mx), sub = nm == -INFINITY ? 0.0f : nm, corr = exp2_fast(m - sub);
@@ -367,10 +380,10 @@ struct F32Round {
       }
     }
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < NJ; ++j) {
       f32x2 w[GP];
 #pragma unroll
-      for (int h = 0; h < GP; ++h) w[h] = f2_splat(__shfl_sync(0xffffffffu, p[kOwn == 2 ? j : 0], lane & 24 | lane_of(h, j)));
+      for (int h = 0; h < GP; ++h) w[h] = f2_splat(__shfl_sync(0xffffffffu, p[(NJ * h + j) % kOwn], lane & 24 | lane_of(h, j)));
 #pragma unroll
       for (int i = 0; i < P; ++i) {
         f32x2 x[2];
@@ -385,7 +398,8 @@ struct F32Round {
   }
 
   __device__ __forceinline__ void finish(int) {
-    if (kOwn == 1) l += __shfl_xor_sync(0xffffffffu, l, kSpread);
+#pragma unroll
+    for (int off = kSpread; off < 8 / GP; off <<= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
 #pragma unroll
     for (int off = 8; off < 32; off <<= 1) {
       l += __shfl_xor_sync(0xffffffffu, l, off);
@@ -425,7 +439,11 @@ struct PageMaps {
   CUtensorMap k, v;      // (feature, token of the page, head, page)
 };
 
-// A round that is not full, or spans pages: in boxes of as many tokens as fit a page.  Out of line: the kernel's code is fetched anew at every
+// All keys of a round, a bit each.
+template <typename R>
+__device__ __forceinline__ unsigned all_keys() { return R::kKeys == 32 ? 0xffffffffu : (1u << (R::kKeys & 31)) - 1; }
+
+// A round that is not full, or of very small pages: in boxes of as many tokens as fit a page.  Out of line: the kernel's code is fetched anew at every
 // launch, and most rounds do not come here.
 template <typename R>
 __device__ __noinline__ unsigned issue_boxes(const PagedAttnArgs& a, const PageMaps& maps, int entry, int first_slot, int kv, int p0, int len, int box_shift,
@@ -437,7 +455,7 @@ __device__ __noinline__ unsigned issue_boxes(const PagedAttnArgs& a, const PageM
   const unsigned mine = page_of(slot_of(a, pos));
   const bool bad = pos < end && mine >= (unsigned)a.pages;
   if (bad) report_error(kBadPage);
-  const unsigned keys = __ballot_sync(0xffffffffu, pos < end && !bad) & ((1u << R::kKeys) - 1);      // (orders the lanes before the copies too)
+  const unsigned keys = __ballot_sync(0xffffffffu, pos < end && !bad) & all_keys<R>();      // (orders the lanes before the copies too)
   const int per_shift = R::kKeyShift - box_shift, boxes = 2 * R::kSegs << per_shift;
 #pragma unroll 1
   for (int b0 = 0; b0 < boxes; b0 += 32) {
@@ -458,19 +476,19 @@ __device__ __noinline__ unsigned issue_boxes(const PagedAttnArgs& a, const PageM
 template <typename R>
 __device__ __forceinline__ unsigned issue_round(const PagedAttnArgs& a, const PageMaps& maps, PageWindow& win, const Cursor& c, int len, int box_shift,
                                                 unsigned char* ring, uint64_t* bar, int lane) {
-  const int p0 = c.k * R::kKeys, slot0 = slot_of(a, p0);
+  const int p0 = c.k * R::kKeys, slot0 = slot_of(a, p0), per_shift = R::kKeyShift - box_shift, boxes = 2 * R::kSegs << per_shift;
   win.cover(a, c.row, slot0, slot_of(a, min(p0 + R::kKeys, len) - 1), len, lane);
-  const int page = win.at(slot0);
-  if (1 << box_shift != R::kKeys || p0 + R::kKeys > len || (unsigned)page >= (unsigned)a.pages)
+  const int first = (lane & ((1 << per_shift) - 1)) << box_shift, tile = lane >> per_shift, slot = slot_of(a, p0 + first), page = win.at(slot);
+  if (boxes > 32 || p0 + R::kKeys > len || __any_sync(0xffffffffu, lane < boxes && (unsigned)page >= (unsigned)a.pages))
     return issue_boxes<R>(a, maps, win.entry, win.first, c.kv, p0, len, box_shift, ring, bar, lane);
   if (lane == 0) mbar_arrive_expect_tx(bar, R::kBytes);
   __syncwarp();
-  if (lane < 2 * R::kSegs) {                       // a full round of one page: a box for each tile
-    const bool is_v = lane >= R::kSegs;
-    tma_load_4d(ring + lane * R::kSeg, is_v ? &maps.v : &maps.k, bar, (is_v ? lane - R::kSegs : lane) * (128 / (int)sizeof(typename R::T)),
-                p0 - slot0 * a.page, c.kv, page);
+  if (lane < boxes) {                              // a full round: a box a lane
+    const bool is_v = tile >= R::kSegs;
+    tma_load_4d(ring + tile * R::kSeg + first * 128, is_v ? &maps.v : &maps.k, bar, (is_v ? tile - R::kSegs : tile) * (128 / (int)sizeof(typename R::T)),
+                p0 + first - slot * a.page, c.kv, page);
   }
-  return (1u << R::kKeys) - 1;
+  return all_keys<R>();
 }
 
 template <typename T, int N>
@@ -699,7 +717,8 @@ paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_con
       if (x.row < a.rows) x.n = before[x.row + 1] - before[x.row] - 1;
     };
     PageWindow win;
-    unsigned long long there = 0;                              // 16 bits for each round of the ring: its keys
+    static_assert(S * R::kKeys <= 64, "a bit for each key of the ring");
+    unsigned long long there = 0;
     int put = 0, take = 0, len = 0, len_row = -1, put_job = 0, take_job = 0;
     bool new_job = true;
     auto length_of = [&](int r) { return (before[r + 1] - before[r] - 2) * R::kKeys + tails[r]; };
@@ -728,7 +747,7 @@ paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_con
         put_job = put_job + 1 == S ? 0 : put_job + 1;
       }
       const unsigned keys = issue_round<R>(a, maps, win, ahead, len, box_shift, ring + put * R::kBytes, bar, lane);
-      there = (there & ~(0xffffull << (16 * put))) | (unsigned long long)keys << (16 * put);
+      there = (there & ~((unsigned long long)all_keys<R>() << (R::kKeys * put))) | (unsigned long long)keys << (R::kKeys * put);
       put = put + 1 == S ? 0 : put + 1;
       const int was = ahead.row;
       if (new_job && win.next_row <= was) {                    // the row after this one
@@ -763,8 +782,8 @@ paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_con
         x.start(a, my_queries + take_job * R::kQueryBytes, count, lane);
         fresh = false;
       }
-      const unsigned keys = (unsigned)(there >> (16 * take)) & 0xffffu;
-      if (keys != (1u << R::kKeys) - 1) {
+      const unsigned keys = (unsigned)(there >> (R::kKeys * take)) & all_keys<R>();
+      if (keys != all_keys<R>()) {
         // What lies where no key is may be NaN: a weight of zero times a value of zero instead.
         unsigned char* values = ring + take * R::kBytes + R::kSegs * R::kSeg;
         for (int i = lane; i < R::kSegs * R::kKeys * 8; i += 32)
@@ -931,32 +950,34 @@ extern "C" int dptb_paged_attention(const PagedAttnArgs* args, void* stream) {
   auto whole = [&](const void* p, long long s0, long long s1, long long s2) {
     return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && s0 % per == 0 && s1 % per == 0 && s2 % per == 0;
   };
+  // Keys of a round: 8 KB of them where rows are short.
+  const int keys = a.f32 ? (a.hd <= 64 ? 16 : 8) : a.hd <= 64 ? 32 : 16;
   PageMaps maps;
   int box = 1;
-  while (2 * box <= (a.f32 ? 8 : 16) && a.page % (2 * box) == 0) box *= 2;
+  while (2 * box <= keys && a.page % (2 * box) == 0) box *= 2;
   if (a.hd % per == 0 && whole(a.k, a.k_page, a.k_head, a.k_tok) && whole(a.v, a.v_page, a.v_head, a.v_tok) &&
       map_pages(&maps.k, a, a.k, a.k_page, a.k_head, a.k_tok, box) == 0 && map_pages(&maps.v, a, a.v, a.v_page, a.v_head, a.v_tok, box) == 0) {
     const bool qv = whole(a.q, a.q_row, a.q_head, 0), ov = whole(a.o, a.o_row, a.o_head, 0);
     const int group = a.heads / a.kv_heads;
     // rounds, and all else that is counted, in 32 bits
-    if ((double)a.rows * ((double)a.width * a.page / (a.f32 ? 8 : 16) + 1) * a.heads >= 2147483000.0) return kErrTooLarge;
+    if ((double)a.rows * ((double)a.width * a.page / keys + 2) * a.heads >= 2147483000.0) return kErrTooLarge;
 #define DPTB_PAGED(R, W, S) return launch_paged<R, W, S>(a, maps, (group + R::kHeads - 1) / R::kHeads, R::kHeads, qv, ov, st)
     if (!a.f32) {
-      using B64 = Bf16Round<64, 1>; using C64 = Bf16Round<64, 2>;
-      using B128 = Bf16Round<128, 1>; using C128 = Bf16Round<128, 2>;
-      using B256 = Bf16Round<256, 1>;
-      if (a.hd <= 64) { if (group <= 8) DPTB_PAGED(B64, 8, 4); DPTB_PAGED(C64, 8, 3); }
+      using B64 = Bf16Round<64, 1, 2>; using C64 = Bf16Round<64, 2, 2>;
+      using B128 = Bf16Round<128, 1, 1>; using C128 = Bf16Round<128, 2, 1>;
+      using B256 = Bf16Round<256, 1, 1>;
+      if (a.hd <= 64) { if (group <= 8) DPTB_PAGED(B64, 8, 2); DPTB_PAGED(C64, 8, 2); }
       if (a.hd <= 128) { if (group <= 8) DPTB_PAGED(B128, 8, 2); DPTB_PAGED(C128, 6, 2); }
       DPTB_PAGED(B256, 4, 2);
     }
-#define DPTB_PAGED_F32(HD, W, S) \
-    if (group == 1) { using R1 = F32Round<HD, 1>; DPTB_PAGED(R1, W, S); } \
-    if (group == 2) { using R2 = F32Round<HD, 2>; DPTB_PAGED(R2, W, S); } \
-    if (group <= 4 || HD == 256) { using R4 = F32Round<HD, 4>; DPTB_PAGED(R4, W, S); }
-    if (a.hd <= 64) { DPTB_PAGED_F32(64, 8, 4) using R8 = F32Round<64, 8>; DPTB_PAGED(R8, 8, 4); }
-    if (a.hd <= 96) { DPTB_PAGED_F32(96, 8, 2) using R8 = F32Round<96, 8>; DPTB_PAGED(R8, 8, 2); }
-    if (a.hd <= 128) { DPTB_PAGED_F32(128, 8, 2) using R8 = F32Round<128, 8>; DPTB_PAGED(R8, 7, 2); }
-    DPTB_PAGED_F32(256, 4, 2)
+#define DPTB_PAGED_F32(HD, NJ, W, S) \
+    if (group == 1) { using R1 = F32Round<HD, 1, NJ>; DPTB_PAGED(R1, W, S); } \
+    if (group == 2) { using R2 = F32Round<HD, 2, NJ>; DPTB_PAGED(R2, W, S); } \
+    if (group <= 4 || HD == 256) { using R4 = F32Round<HD, 4, NJ>; DPTB_PAGED(R4, W, S); }
+    if (a.hd <= 64) { DPTB_PAGED_F32(64, 4, 8, 2) using R8 = F32Round<64, 8, 4>; DPTB_PAGED(R8, 8, 2); }
+    if (a.hd <= 96) { DPTB_PAGED_F32(96, 2, 8, 2) using R8 = F32Round<96, 8, 2>; DPTB_PAGED(R8, 8, 2); }
+    if (a.hd <= 128) { DPTB_PAGED_F32(128, 2, 8, 2) using R8 = F32Round<128, 8, 2>; DPTB_PAGED(R8, 7, 2); }
+    DPTB_PAGED_F32(256, 2, 4, 2)
 #undef DPTB_PAGED_F32
 #undef DPTB_PAGED
   }
