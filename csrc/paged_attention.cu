@@ -532,20 +532,19 @@ __device__ __noinline__ void join_parts(const PagedAttnArgs& a, Parts<W>& sh, co
     } else {
       __syncthreads();
       if (sh.shared[0] < 0 && sh.shared[1] < 0) return;
-      __threadfence();
-      __syncthreads();
       if (tid < 2) {
         const int i = sh.shared[tid];
         int last = 0;
         if (i >= 0) {
           const int first = sh.begin[i] / share, n = (sh.begin[i] + sh.rounds[i] - 1) / share - first;
-          last = atomicAdd(a.counters + first, 1u) == (unsigned)n;
+          unsigned before;      // releases what this CTA has written (the barrier above), acquires what those before it have (the one below)
+          asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(a.counters + first) : "memory");
+          last = before == (unsigned)n;
           if (last) a.counters[first] = 0;
         }
         sh.merges[tid] = last;
       }
       __syncthreads();
-      __threadfence();
       jobs = (sh.merges[0] ? 1u << sh.shared[0] : 0) | (sh.merges[1] ? 1u << sh.shared[1] : 0);
     }
     int unit = 0;
@@ -569,14 +568,34 @@ __device__ __noinline__ void join_parts(const PagedAttnArgs& a, Parts<W>& sh, co
           } else if (j < n) {
             part = a.ws + ((first + j) * 2LL + (j == 0 && jb > first * share)) * kPart;
           }
-          const float mine = part ? *(const volatile float*)(part + kMax + h) : -INFINITY;
+          // The values of the first parts are on their way while the weights are worked out.
+          const float mine = part ? *(const volatile float*)(part + kMax + h) : -INFINITY, of = part ? *(const volatile float*)(part + kSum + h) : 0.0f;
+          unsigned parts = __ballot_sync(0xffffffffu, part != nullptr);
+          constexpr int kEarly = 3;
+          float early[kEarly][kPer];
+          int who[kEarly];
+#pragma unroll
+          for (int y = 0; y < kEarly; ++y) {
+            who[y] = parts ? __ffs(parts) - 1 : 0;
+            const volatile float* src = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(part), who[y])) + h * R::kHD + lane;
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) early[y][e] = parts ? src[32 * e] : 0.0f;
+            if (!parts) who[y] = -1;
+            parts &= parts - 1;
+          }
           const float nm = fmaxf(m, warp_max(mine)), sub = nm == -INFINITY ? 0.0f : nm, corr = exp2_fast(m - sub);
           const float w = part ? exp2_fast(mine - sub) : 0.0f;
-          l = l * corr + warp_sum(part ? w * *(const volatile float*)(part + kSum + h) : 0.0f);
+          l = l * corr + warp_sum(w * of);
           m = nm;
 #pragma unroll
           for (int e = 0; e < kPer; ++e) f[e] *= corr;
-          unsigned parts = __ballot_sync(0xffffffffu, part != nullptr);
+#pragma unroll
+          for (int y = 0; y < kEarly; ++y) {
+            const float wy = __shfl_sync(0xffffffffu, w, max(who[y], 0));
+            if (who[y] >= 0)
+#pragma unroll
+              for (int e = 0; e < kPer; ++e) f[e] += wy * early[y][e];
+          }
 #pragma unroll 4
           for (; parts; parts &= parts - 1) {
             const int x = __ffs(parts) - 1;
