@@ -644,7 +644,7 @@ paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_con
   __shared__ int aborted;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int tiles = a.kv_heads * head_tiles;                                // jobs of a row
-  const int room = (int)min((long long)a.width * a.page, 0x7fffffffLL);
+  const int room = (int)min((long long)a.width * a.page, 0x7fffff00LL);      // (the end of its last round is a position, too)
   const int group = a.heads / a.kv_heads;
 
   // Units ahead of every row: a job is its rounds and, before them, one unit for what it costs to begin and end it (2100 cycles where a round took

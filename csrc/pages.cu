@@ -244,7 +244,7 @@ struct ForkArgs {
   const int* table;
   const int* lens;
   const int* parents;     // null: every row itself
-  const int* grow;        // null: grow_all for every row that has a parent
+  const int* grow;        // null: grow_all for every row that holds tokens
   int* new_table;         // [rows, width]
   int* new_lens;
   int* src;               // [rows]
@@ -266,7 +266,7 @@ __device__ __forceinline__ ForkRow fork_row(const ForkArgs& a, int r) {
   if (f.parent >= a.rows_in) f.parent = -1;
   const long long room = min((long long)a.width * a.page, 0x7fffffffLL);
   f.old_len = f.parent >= 0 ? (int)min((long long)max(a.lens[f.parent], 0), room) : 0;
-  const long long more = a.grow ? max(a.grow[r], 0) : f.parent >= 0 ? a.grow_all : 0;
+  const long long more = a.grow ? max(a.grow[r], 0) : f.old_len > 0 ? a.grow_all : 0;
   f.new_len = (int)min(f.old_len + more, room);
   f.held = (f.old_len + a.page - 1) / a.page;
   f.want = (int)(((long long)f.new_len + a.page - 1) / a.page);
@@ -296,7 +296,7 @@ fork_pages_kernel(const ForkArgs a, int words, int slots) {
     const ForkRow f = fork_row(a, r);
     if (lane == 0) {
       const bool bad = a.parents && a.parents[r] >= a.rows_in;
-      const long long more = a.grow ? max(a.grow[r], 0) : f.parent >= 0 ? a.grow_all : 0;
+      const long long more = a.grow ? max(a.grow[r], 0) : f.old_len > 0 ? a.grow_all : 0;
       if (bad || f.parent >= 0 && a.lens[f.parent] > f.old_len || f.new_len < f.old_len + more) report_error(kBadPage);
       a.new_lens[r] = f.new_len;
       st_cluster_u32(map_to_cta(held + r, 0), f.held);

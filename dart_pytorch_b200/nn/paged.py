@@ -62,12 +62,14 @@ class PagedCache:
         self.pool = torch.zeros(num_layers, 2, self.num_pages, num_kv_heads, page_size, head_dim, dtype=dtype, device=device)
         self.table = torch.full((rows, width), -1, dtype=torch.int32, device=device)
         self.lens = torch.zeros(rows, dtype=torch.int32, device=device)
-        self.longest = 0                                   # no row is longer
+        self.longest = 0                                   # no row is longer (one that has ended may have been as long)
         self.positions: Optional[torch.Tensor] = None      # of the tokens that the cache was last extended by
         self.rows: Optional[torch.Tensor] = None           # and their rows; None: one token of every row
         self.layers: List[PagedLayer] = [PagedLayer(self, i) for i in range(num_layers)]
 
     def _fork(self, parents, grow, longest: int) -> None:
+        if longest > self.max_len and isinstance(grow, int):     # rows that have ended may have been the longest: look
+            longest = int(self.lens.max()) + grow
         if longest > self.max_len:
             raise ValueError(f"PagedCache: a row of {longest} tokens in a cache of {self.max_len}")
         self.table, self.lens, src, dst = F.fork_pages(self.table, self.lens, self.num_pages, self.page_size, parents, grow)
@@ -87,13 +89,15 @@ class PagedCache:
         for r, m in zip(rows, lengths):
             parents[r], grow[r] = -1, m
         ints = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
-        self._fork(ints(parents), ints(grow), max(self.longest, n))
+        if n > self.max_len:
+            raise ValueError(f"PagedCache: a prompt of {n} tokens in a cache of {self.max_len}")
+        self._fork(ints(parents), ints(grow), max(min(self.longest, self.max_len), n))
         self.rows = ints([r for r in rows for _ in range(n)])
         self.positions = ints([t if t < m else -1 for m in lengths for t in range(n)])
 
     def fork(self, parents: Optional[torch.Tensor] = None) -> None:
         """Every row becomes a copy of row ``parents[r]`` (int32; itself without ``parents``; -1: empty) with room for a token,
-        which the model's step brings."""
+        which the model's step brings; rows that hold nothing stay empty."""
         self._fork(parents, 1, self.longest + 1)
         self.rows, self.positions = None, self.lens - 1
 

@@ -301,7 +301,7 @@ def _check_append(qkv, k_pages, v_pages, table, positions, heads, rows, rotary, 
 def fork_pages_reference(table, lens, pages, page, parents, grow):
     t_in, l_in, width = table.tolist(), lens.tolist(), table.shape[1]
     who = list(range(len(t_in))) if parents is None else parents.tolist()
-    more = grow.tolist() if isinstance(grow, torch.Tensor) else [grow if p >= 0 else 0 for p in who]
+    more = grow.tolist() if isinstance(grow, torch.Tensor) else [grow if 0 <= p < len(l_in) and l_in[p] > 0 else 0 for p in who]
     held, old, new = [], [], []
     for p, g in zip(who, more):
         if p >= len(t_in):
@@ -336,7 +336,7 @@ def fork_pages_reference(table, lens, pages, page, parents, grow):
 def fork_pages(table: torch.Tensor, lens: torch.Tensor, pages: int, page: int, parents: Optional[torch.Tensor] = None,
                grow: Union[int, torch.Tensor] = 0) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """The rows of a cache anew: row ``r`` becomes row ``parents[r]`` (itself without ``parents``; -1: empty, which frees its
-    pages), longer by ``grow`` tokens: an int for every row that has a parent, or int32 ``[rows]``, which starts empty rows as well.
+    pages), longer by ``grow`` tokens: an int for every row that holds tokens, or int32 ``[rows]``, which starts empty rows as well.
     Pages of a ``pages``-page pool (``page`` tokens each) are taken for them, free ones of the lowest numbers first, row by row;
     a part-filled last page that others list too is replaced by a copy of the row's own, except for the first row that grows into it.
     Returns ``(table, lens, src, dst)``: the new table and lengths, and for every row the page to copy and its copy (-1: none), which

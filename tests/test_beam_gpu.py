@@ -111,3 +111,34 @@ def test_scores_beyond_float_and_far_apart():
     agree(ops.beam_step(logits, scores), oracle.beam(logits, scores, None, -1))
     scores[0] = torch.tensor([-1e6, -1e6 + 1, -1e6 - 2])
     agree(ops.beam_step(logits * 30, scores), oracle.beam(logits * 30, scores, None, -1))
+
+
+def test_more_items_than_there_are_counters():
+    logits, scores, finished = data(5000, 2, 37, torch.float32, 11)
+    got = ops.beam_step(logits, scores, finished, 4)
+    agree(got, oracle.beam(logits, scores, finished, 4))
+    part = ops.beam_step(logits[:20], scores[:10].contiguous(), finished[:10].contiguous(), 4)
+    assert all(torch.equal(a[:10], b) for a, b in zip(got, part))
+
+
+@pytest.mark.parametrize("beams,vocab", [(8, 50000), (32, 30000)])
+def test_few_valid_tokens_and_few_live_beams(beams, vocab):
+    """Constrained decoding: all but a few tokens masked, by -inf or by the lowest value, in the first step too."""
+    logits, scores, finished = data(2, beams, vocab, torch.float32, 3)
+    for low in (-INF, torch.finfo(torch.float32).min):
+        masked = torch.full_like(logits, low)
+        masked[:, 17::9973] = logits[:, 17::9973]
+        agree(ops.beam_step(masked, scores), oracle.beam(masked, scores, None, -1))
+        agree(ops.beam_step(masked, scores, finished, 17), oracle.beam(masked, scores, finished, 17))
+        first = torch.full_like(scores, -INF)
+        first[:, 0] = 0
+        agree(ops.beam_step(masked, first), oracle.beam(masked, first, None, -1))
+
+
+def test_many_close_totals():
+    """Thousands of logits within a few steps of one another, more than are ranked at once, in no order."""
+    g = torch.Generator().manual_seed(2)
+    for dtype, spread in ((torch.bfloat16, 4), (torch.float32, 300)):
+        logits = torch.randint(0, spread, (8, 20000), generator=g).float().mul_(1 / 64).to(dtype).cuda()
+        scores = torch.zeros(1, 8, device="cuda")
+        agree(ops.beam_step(logits, scores), oracle.beam(logits, scores, None, -1))

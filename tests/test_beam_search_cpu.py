@@ -118,6 +118,22 @@ def test_cache_rows_come_and_go():
     assert torch.allclose(got[0], alone(b + [13]), atol=1e-5) and torch.allclose(got[1], alone(a1 + [14]), atol=1e-5)
 
 
+def test_a_cache_outlives_many_rows():
+    """What has ended does not count: rows that come and go for longer than any of them may be."""
+    model = llama()
+    cache = PagedCache(2, 2, 8, 2, 8, 4)
+    for i in range(5):
+        cache.prompts([3], [i % 2])
+        with torch.no_grad():
+            model.paged_hidden(torch.tensor([[1, 2, 3]]), cache)
+        for _ in range(4):
+            cache.fork()
+            with torch.no_grad():
+                model.paged_hidden(torch.zeros(2, 1, dtype=torch.long), cache)
+        assert cache.lens.tolist() == ([7, 0] if i % 2 == 0 else [0, 7])
+        cache.free([i % 2])
+
+
 def test_service_answers_with_beams():
     svc = GenerationService(llama(), None, "tiny")
     code, out = svc.run({"tokens": [3, 1, 4], "maxNewTokens": 5, "beams": 3, "eos": 7})

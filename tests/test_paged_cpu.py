@@ -75,7 +75,7 @@ class Story:
         ops.copy_pages(self.pool, src, dst)
         who = list(range(len(old_lens))) if parents is None else parents
         self.text = [list(self.text[p]) if p >= 0 else [] for p in who]
-        more = grow if isinstance(grow, list) else [grow if p >= 0 else 0 for p in who]
+        more = grow if isinstance(grow, list) else [grow if p >= 0 and old_lens[p] > 0 else 0 for p in who]
         for r, n in enumerate(more):
             for _ in range(n):
                 at = len(self.text[r])

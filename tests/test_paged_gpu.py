@@ -395,3 +395,58 @@ def test_tensors_of_another_device_are_refused():
         ops.fork_pages(table, lens.cpu(), 4, 4)
     with pytest.raises(ValueError, match="device"):
         ops.copy_pages(k, lens.cpu(), lens.cpu())
+
+
+# ------------------------------------------------------------------------------------------------------------ far ends
+@pytest.mark.parametrize("dtype,heads,hkv,hd", [(torch.bfloat16, 4, 1, 128), (torch.bfloat16, 16, 1, 128), (torch.float32, 8, 1, 128),
+                                                (torch.float32, 1, 1, 8)])
+def test_attention_of_as_many_rows_as_there_may_be(dtype, heads, hkv, hd):
+    rng = random.Random(heads)
+    lens = [rng.choice((0, 1, 2, 7, 33)) for _ in range(4096)]
+    check(*make(lens, heads, hkv, hd, 8, dtype))
+
+
+def test_pools_beyond_32_bits():
+    """Pages of a pool whose elements and bytes do not fit 32 bits: 2.4e9 bf16 values."""
+    pages, page, hd = 300_000, 64, 128
+    pool = torch.empty(2, pages, 1, page, hd, dtype=torch.bfloat16, device="cuda")
+    k, v = pool
+    lens = torch.tensor([130, 64], dtype=torch.int32, device="cuda")
+    table = torch.tensor([[pages - 1, 5, pages - 3], [pages - 2, -1, -1]], dtype=torch.int32, device="cuda")
+    used = table[table >= 0].long()
+    pool[:, used] = torch.randn(2, len(used), 1, page, hd, device="cuda").bfloat16()
+    q = torch.randn(2, 4, hd, device="cuda").bfloat16()
+    small = torch.tensor([[0, 1, 2], [3, -1, -1]], dtype=torch.int32, device="cuda")
+    got = ops.paged_attention(q, k, v, table, lens)
+    assert torch.equal(got, ops.paged_attention(q, *(t[used] for t in (k, v)), small, lens))
+    ops.copy_pages(pool, table[0, :1].contiguous(), torch.tensor([pages - 7], dtype=torch.int32, device="cuda"))
+    assert torch.equal(pool[:, pages - 7], pool[:, pages - 1])
+    qkv = torch.randn(2, 6 * hd, device="cuda").bfloat16()
+    ops.paged_append(qkv, k, v, table, torch.tensor([191, 0], dtype=torch.int32, device="cuda"), 4, rotary_dim=0)
+    assert torch.equal(k[pages - 3, 0, 63], qkv[0, 4 * hd:5 * hd]) and torch.equal(v[pages - 2, 0, 0], qkv[1, 5 * hd:])
+    odd = k.view(-1)[1:1 + (pages - 1) * page * hd].view(pages - 1, 1, page, hd)          # off 16 bytes: the other kernel
+    odd[pages - 2] = torch.randn(1, page, hd, device="cuda").bfloat16()
+    last, n = torch.full((2, 1), pages - 2, dtype=torch.int32, device="cuda"), torch.tensor([64, 9], dtype=torch.int32, device="cuda")
+    got = ops.paged_attention(q, odd, odd, last, n).float()
+    twin = odd[pages - 2:].clone()
+    assert torch.allclose(got, ops.paged_attention(q, twin, twin, last * 0, n).float(), rtol=2.0 ** -7, atol=2.0 ** -9)
+
+
+def test_results_over_the_queries_and_inference_mode():
+    q, k, v, table, lens = make(LENS + [3000], 8, 2, 64, 16, torch.bfloat16)
+    want = ops.paged_attention(q, k, v, table, lens)
+    with torch.inference_mode():
+        twin = q.clone()
+        assert ops.paged_attention(twin, k, v, table, lens, out=twin) is twin and torch.equal(twin, want)
+        kk, vv = torch.zeros_like(k), torch.zeros_like(v)
+        ops.paged_append(torch.randn(len(lens), 12 * 64, device="cuda").bfloat16(), kk, vv, table, (lens - 1).int(), 8)
+        ops.copy_pages(kk, table[2, :1].contiguous(), table[3, :1].contiguous())
+        assert torch.equal(kk[table[2, 0]], kk[table[3, 0]])
+
+
+def test_one_page_in_many_places():
+    """A table may list a page any number of times, in one row and in others."""
+    q, k, v, _, _ = make([64, 64, 64], 4, 2, 64, 16, torch.float32)
+    table = torch.tensor([[1, 1, 1, 1], [1, 0, 1, 0], [0, 0, 1, 1]], dtype=torch.int32, device="cuda")
+    k.normal_(), v.normal_()
+    check(q, k, v, table, torch.tensor([64, 60, 33], dtype=torch.int32, device="cuda"))
