@@ -147,7 +147,10 @@ __device__ __forceinline__ Piece<T> load_whole(const T* row, int first) {
 }
 template <typename T>
 __device__ __forceinline__ Piece<T> load_piece(const T* row, int first, int end, bool vec) {
-  return vec && first + Piece<T>::N <= end ? load_whole<T>(row, first) : load_edge<T>(row, first, end);
+  if (vec && first + Piece<T>::N <= end) return load_whole<T>(row, first);
+  if (first < end) return load_edge<T>(row, first, end);
+  constexpr uint32_t kNone = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
+  return Piece<T>{kNone, kNone, kNone, kNone};
 }
 
 // What a warp leaves of its logits: the sum of exponentials, what it is relative to, every lane's maximum.
@@ -168,93 +171,6 @@ struct BeamShared {
   int hot[kHotLanes], count, hots, counts[kBeamWarps], done[kBeamWarps];
 };
 static_assert(kBeamWarps * kWarpPool <= kItemPool, "the warps' pools");
-
-// Of a warp's logits [begin, end), of which this lane's have the maximum `mine`, the best K as keys in `out`, best first, 0 behind the last.  Where too many
-// equal the threshold (a masked vocabulary), those above it, and the first of the equal ones in their order.
-template <typename T>
-__device__ __forceinline__ void best_of_warp(const T* row, int begin, int end, bool vec, float mine, int K, unsigned long long* out, unsigned long long* keys, int* count) {
-  constexpr int N = Piece<T>::N;
-  const int lane = threadIdx.x & 31;
-  const float limit = __shfl_sync(0xffffffffu, sort_lanes(mine), K - 1);
-  int n = 0;
-#pragma unroll 1
-  for (int round = 0; round < 2; ++round) {
-    __syncwarp();
-    if (lane == 0) *count = 0;
-    __syncwarp();
-    if (round == 0 ? mine >= limit : mine > limit) {
-#pragma unroll 4
-      for (int i = begin + lane * N; i < end; i += 32 * N) {
-        const Piece<T> p = load_piece<T>(row, i, end, vec);
-        const float top = p.top();
-        if (round == 0 ? top >= limit : top > limit)
-#pragma unroll
-          for (int e = 0; e < N; ++e) {
-            const float x = p.at(e);
-            if (i + e < end && (round == 0 ? x >= limit : x > limit)) {
-              const int at = atomicAdd(count, 1);
-              if (at < kWarpPool) keys[at] = rank_key(x, i + e);
-            }
-          }
-      }
-    }
-    __syncwarp();
-    n = *(volatile int*)count;
-    if (n > kWarpPool - (round ? K : 0)) continue;
-    if (round == 1) {
-      const int above = n;
-#pragma unroll 1
-      for (int i0 = begin; i0 < end && n - above < K; i0 += 32 * N) {
-        const int i = i0 + lane * N;
-        const Piece<T> p = load_piece<T>(row, i, end, vec);
-        int equal = 0;
-#pragma unroll
-        for (int e = 0; e < N; ++e) equal += i + e < end && p.at(e) == limit;
-        int at = equal;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int u = __shfl_up_sync(0xffffffffu, at, o);
-          if (lane >= o) at += u;
-        }
-        const int total = __shfl_sync(0xffffffffu, at, 31);
-        at += n - equal;
-#pragma unroll
-        for (int e = 0; e < N; ++e)
-          if (i + e < end && p.at(e) == limit) {
-            if (at - above < K) keys[at] = rank_key(limit, i + e);
-            ++at;
-          }
-        n += total;
-      }
-      n = min(n, above + K);
-      __syncwarp();
-    }
-    break;
-  }
-  if (n > kWarpPool) {         // too many above the threshold as well: the best, one after the other
-    unsigned long long last = ~0ull;
-#pragma unroll 1
-    for (int k = 0; k < K; ++k) {
-      unsigned long long top = 0;
-      for (int i = begin + lane; i < end; i += 32) {
-        const unsigned long long key = rank_key(to_f32(row[i]), i);
-        if (key < last && key > top) top = key;
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      if (lane == 0) out[k] = top;
-      last = top;
-    }
-    return;
-  }
-  for (int i = lane; i < n; i += 32) {
-    const unsigned long long key = keys[i];
-    int rank = 0;
-    for (int j = 0; j < n; ++j) rank += keys[j] > key;
-    if (rank < K) out[rank] = key;
-  }
-  for (int i = n + lane; i < K; i += 32) out[i] = 0;
-}
 
 // A sum relative to the maximum `m`, or its shift, relative to `top` > m, or its.
 constexpr float kLarge = 1048576.0f;
@@ -280,19 +196,114 @@ __device__ __forceinline__ double special(const BeamArgs& a, const BeamShared& s
   return i == 0 ? sh.score[w] : -INFINITY;
 }
 
-// Where too many are equal, or there are fewer than beams (a masked vocabulary): the best of every row, by a warp.
+// Of a row of logits the best K as keys in `out`, best first, 0 behind the last; by a warp.  The threshold is the K-th largest of the lanes' maxima: what is above
+// it lies with fewer than K lanes; of what equals it the first are wanted, in lists where a lane reaches it, and each such list has one or
+// is among the fewer than K that have more.  So a masked or flat row is not read again from end to end.
 template <typename T>
-__device__ __noinline__ void best_of_rows(const BeamArgs& a, BeamShared& sh, const T* rows) {
+__device__ __noinline__ void best_of_row(const BeamArgs& a, const T* row, const BeamPart* p, unsigned long long* out, unsigned long long* keys, int* count) {
   constexpr int N = Piece<T>::N;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = a.beams;
+  const int lane = threadIdx.x & 31, K = a.beams;
+  float best = -INFINITY, limit = -INFINITY;      // the 32 largest, descending; the K-th
+#pragma unroll 1
+  for (int l = 0; l < a.lists; ++l) {
+    float v = __ldcg(&p[l].high[lane]);
+    if (!__any_sync(0xffffffffu, v > limit)) continue;
+    best = fmaxf(best, __shfl_sync(0xffffffffu, sort_lanes(v), 31 - lane));
+#pragma unroll
+    for (int j = 16; j > 0; j >>= 1) {
+      const float o = __shfl_xor_sync(0xffffffffu, best, j);
+      best = (lane & j) == 0 ? fmaxf(best, o) : fminf(best, o);
+    }
+    limit = __shfl_sync(0xffffffffu, best, K - 1);
+  }
+  if (lane == 0) *count = 0;
+  __syncwarp();
+#pragma unroll 1
+  for (int l = 0; l < a.lists; ++l) {
+    const int begin = l * a.chunk, end = min(a.vocab, begin + a.chunk);
+#pragma unroll 1
+    for (unsigned some = __ballot_sync(0xffffffffu, __ldcg(&p[l].high[lane]) > limit); some; some &= some - 1) {
+      const int j = __ffs(some) - 1;
+#pragma unroll 1
+      for (int i = begin + (j + 32 * lane) * N; i < end; i += 32 * 32 * N) {
+        const Piece<T> x = load_piece<T>(row, i, end, a.vec);
+        if (!(x.top() > limit)) continue;
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (i + e < end && x.at(e) > limit) {
+            const int at = atomicAdd(count, 1);
+            if (at < kWarpPool) keys[at] = rank_key(x.at(e), i + e);
+          }
+      }
+    }
+  }
+  __syncwarp();
+  const int above = *(volatile int*)count;
+  if (above > kWarpPool - K) {       // very many with few lanes: the best, one after the other
+    unsigned long long last = ~0ull;
+#pragma unroll 1
+    for (int k = 0; k < K; ++k) {
+      unsigned long long top = 0;
+      for (int i = lane; i < a.vocab; i += 32) {
+        const unsigned long long key = rank_key(to_f32(row[i]), i);
+        if (key < last && key > top) top = key;
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (lane == 0) out[k] = top;
+      last = top;
+    }
+    return;
+  }
+  int n = above;
+#pragma unroll 1
+  for (int l = 0; l < a.lists && n - above < K; ++l) {
+    if (!__any_sync(0xffffffffu, __ldcg(&p[l].high[lane]) >= limit)) continue;
+    const int begin = l * a.chunk, end = min(a.vocab, begin + a.chunk);
+#pragma unroll 1
+    for (int i0 = begin; i0 < end && n - above < K; i0 += 32 * N) {
+      const int i = i0 + lane * N;
+      const Piece<T> x = load_piece<T>(row, i, end, a.vec);
+      int equal = 0;
+#pragma unroll
+      for (int e = 0; e < N; ++e) equal += i + e < end && x.at(e) == limit;
+      int at = equal;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, at, o);
+        if (lane >= o) at += u;
+      }
+      const int total = __shfl_sync(0xffffffffu, at, 31);
+      at += n - equal;
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (i + e < end && x.at(e) == limit) {
+          if (at - above < K) keys[at] = rank_key(limit, i + e);
+          ++at;
+        }
+      n += total;
+    }
+  }
+  n = min(n, above + K);
+  __syncwarp();
+  for (int i = lane; i < n; i += 32) {
+    const unsigned long long key = keys[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += keys[j] > key;
+    if (rank < K) out[rank] = key;
+  }
+  for (int i = n + lane; i < K; i += 32) out[i] = 0;
+}
+
+// Where too many are equal, or fewer lanes than beams have anything to offer (a masked vocabulary): the best of every row first.
+template <typename T>
+__device__ __noinline__ void best_of_rows(const BeamArgs& a, BeamShared& sh, const T* rows, const BeamPart* parts) {
+  const int tid = threadIdx.x, warp = tid >> 5, K = a.beams;
   auto* keys = reinterpret_cast<unsigned long long*>(sh.totals);
 #pragma unroll 1
   for (int w = warp; w < K; w += kBeamWarps) {
-    if (sh.kind[w]) continue;
-    const T* row = rows + w * a.ld;
-    float mine = -INFINITY;
-    for (int i = lane * N; i < a.vocab; i += 32 * N) mine = fmaxf(mine, load_piece<T>(row, i, a.vocab, a.vec).top());
-    best_of_warp<T>(row, 0, a.vocab, a.vec, mine, K, keys + w * K, sh.keys + warp * kWarpPool, sh.counts + warp);
+    __syncwarp();
+    if (sh.kind[w] == 0) best_of_row<T>(a, rows + w * a.ld, parts + w * a.lists, keys + w * K, sh.keys + warp * kWarpPool, sh.counts + warp);
   }
   __syncthreads();
   for (int c = tid; c < K * K; c += kBeamThreads) {
@@ -466,7 +477,7 @@ __device__ __noinline__ void choose(const BeamArgs& a, BeamShared& sh, int local
   }
   if (wide) {
     __syncthreads();
-    best_of_rows<T>(a, sh, rows);
+    best_of_rows<T>(a, sh, rows, parts);
   }
   const int found = sh.count;
   for (int i = tid; i < found; i += kBeamThreads) {
@@ -507,7 +518,7 @@ beam_kernel(const __grid_constant__ BeamArgs a, int rows) {
         for (int u = 0; u < U; ++u) p[u] = load_whole<T>(row, i + u * 32 * N);
       } else {
 #pragma unroll
-        for (int u = 0; u < U; ++u) p[u] = load_edge<T>(row, i + u * 32 * N, end);
+        for (int u = 0; u < U; ++u) p[u] = load_piece<T>(row, i + u * 32 * N, end, a.vec);
       }
       const float top = fmaxf(fmaxf(p[0].top(), p[1].top()), fmaxf(p[2].top(), p[3].top()));
       if (top > m) {
@@ -575,13 +586,15 @@ extern "C" int dptb_beam_step(const BeamArgs* args, void* stream) {
   if (a.items < 0 || a.beams <= 0 || a.beams > kMaxBeams || a.vocab <= 0 || a.vocab > 1 << 30 || a.ld < 0 || (long long)a.items * a.beams > 1 << 20 ||
       (reinterpret_cast<uintptr_t>(a.ws) & 7))
     return kErrBadShape;
-  // Logits of a warp: a row's share when all that are resident (32 an SM) have one, a round of loads (4 pieces a lane) at least, and not so many
-  // parts of a row that the choice among them is what takes the time.
-  const int unit = 4 * 32 * (a.f32 ? 4 : 8), most_lists = kMaxLists;
+  // Logits of a warp: a row's share when all that are resident (32 an SM) have one, and not so many parts of a row that the choice among them is
+  // what takes the time; four parts at least, so that one live beam has as many lanes to choose from as a search may have beams; a piece a lane.
+  const int unit = 32 * (a.f32 ? 4 : 8), most_lists = kMaxLists;
   const long long rows = (long long)a.items * a.beams, warps = 32LL * sm_count();
-  long long chunk = ((long long)a.vocab * rows + warps - 1) / warps;
-  chunk = max(chunk, ((long long)a.vocab + most_lists - 1) / most_lists);
-  chunk = max((chunk + unit - 1) / unit, 1LL) * unit;
+  auto up = [](long long n, long long d) { return (n + d - 1) / d; };
+  long long chunk = max(up((long long)a.vocab * rows, warps), 4LL * unit);
+  chunk = min(chunk, up(a.vocab, 4));
+  chunk = max(chunk, up(a.vocab, most_lists));
+  chunk = up(chunk, chunk >= 4 * unit ? 4 * unit : unit) * (chunk >= 4 * unit ? 4 * unit : unit);
   a.chunk = (int)chunk;
   a.lists = (int)((a.vocab + chunk - 1) / chunk);
   const int size = a.f32 ? 4 : 2;
