@@ -7,23 +7,26 @@
 // outside the pool hides its keys and records kBadPage in the status word, which the host turns into an exception.
 //
 // paged_attention_kernel reads every key and value once for all heads of its group.  The keys of all (row, kv head) pairs, "jobs", are one
-// sequence of rounds (16 keys in bf16, 8 in fp32) that is dealt out evenly: a CTA an SM takes a contiguous range, each of its warps a contiguous
-// part of that, so lengths from one token to the longest mix without an idle SM and without the host knowing them.  A warp keeps the running
-// maximum, sum and weighted values of its job in registers.  Parts of a job that fell to several warps are joined in shared memory, and
-// of several CTAs through a workspace by the last of them to finish (a counter, no waiting; parts are added in order, so results
-// repeat to the bit).
+// sequence of rounds, 8 KB of keys and values or a little more, that is dealt out evenly: a CTA an SM takes a contiguous range, each of its
+// warps a contiguous part of that, so lengths from one token to the longest mix without an idle SM and without the host knowing them.
+// A warp keeps the running maximum, sum and weighted values of its job in registers.  Parts of a job that fell to several warps are joined in
+// shared memory, and of several CTAs through a workspace by the last of them to finish (a counter, no waiting; parts are added in order, so
+// results repeat to the bit).
 //
 // Loads: TMA tiles of 128-byte rows, 128-byte swizzled, a ring of rounds for every warp that runs on across jobs; a few instructions a round
 // for any strides and page sizes (a page that a round does not fit into is fetched in several boxes).  The features of a fragment are dealt to
 // the lanes in another order than the matrix instruction's, and the keys of a round too, in all its operands alike, which a sum does not
-// notice: so a lane reads 16 bytes at a time, and the eight lanes of a read fall on different banks.
+// notice: so a lane reads 16 bytes at a time, and the eight lanes of a read fall on different banks.  Head sizes, strides and addresses off 16 bytes
+// have the same rounds filled element by element, by the warp that works on them.
 //
 // bf16: S^T = K Q^T and O^T = V^T P^T by mma.sync, the group's heads as the 8 columns (two tiles of them for 9 to 16 heads); the bound is
 // the cache stream, and a tcgen05 tile of 128 rows would be padding for the most part.  The weights enter as two bf16 parts (16 bits).
-// fp32: multiply-adds, 8 lanes a key.
+// fp32: multiply-adds, 8 lanes a key; they bound groups of four heads and more.
 //
-// paged_attention_simple_kernel takes what 16-byte pieces do not fit (head sizes, strides or addresses off them): a CTA per (row, query
-// head), a thread a key for the scores and a thread a feature for the weighted sum.
+// Device time on B200, pages of 16 tokens in random order: bf16, 32 heads of 128 on 8: four sequences of 65000 to 131072 keys 242 us (6.6 TB/s, the
+// rate of a plain copy), 32 sequences of 1 to 4096 53.5 us (5.0 TB/s; its floor is 41), 32 of 2048 52 us, one of 2048 15 us.  One sequence
+// of 65 keys, 12 heads of 64: 6.5 us.  fp32, 13 sequences of up to 1531 keys, 10 heads of 80 on 5: 18.2 us; 32 of 2048, 32 heads of 128 on 8:
+// 105 us.  Filled element by element the 32 sequences of 2048 keys take 180 us in bf16 and 186 us in fp32, the one of 65 keys 9 us.
 #include <cuda_bf16.h>
 
 #include "common/host.h"
@@ -107,10 +110,11 @@ struct Cursor {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kTiny = 1.2e-38f;
+constexpr int kMaxHeadDim = 256;
 
 // ------------------------------------------------------------------------------------------------------------ bf16
-// HD: features of a head, padded with zeros; NT: tiles of 8 query heads; M: times 16 keys a round (two where rows are short: a request and a
-// maximum for each 16 keys of 64 features kept 16 sequences of 4096 keys at 39 us).
+// HD: features of a head, padded with zeros; NT: tiles of 8 query heads; M: times 16 keys a round (two for heads of up to 64 features: a
+// request and a maximum for each 16 keys kept 16 sequences of 4096 at 39 us, each 32 take 32 us).
 template <int HD, int NT, int M>
 struct Bf16Round {
   using T = __nv_bfloat16;
@@ -273,7 +277,8 @@ struct Bf16Round {
 // A round's products leave NJ GP sums of 8 lanes each (head, step).  They are added in halves: with every exchange a lane keeps half of its sums, so that
 // in the end it has one or a few of one head, for which it alone keeps maximum and sum and takes the exponentials; the weights go
 // back to the lanes by shuffle.  Multiply-adds are packed in pairs.  With every sum in every lane, and single multiply-adds, 13 sequences of up to
-// 1531 keys (10 heads of 80 on 5) took 22 us.
+// 1531 keys (10 heads of 80 on 5) took 22 us, now 18.  Rounds of 16 keys for heads of up to 64 features (16 sequences of 4096 keys: 65 us with 8, 51 with
+// 16), of 8 above.
 template <int HD, int GP, int NJ>
 struct F32Round {
   using T = float;
@@ -491,6 +496,66 @@ __device__ __forceinline__ unsigned issue_round(const PagedAttnArgs& a, const Pa
   return all_keys<R>();
 }
 
+// The same for pages that TMA cannot fetch, element by element: by the warp itself, so that nothing is in flight afterwards.
+template <typename R>
+__device__ __forceinline__ unsigned fill_round(const PagedAttnArgs& a, PageWindow& win, const Cursor& c, int len, unsigned char* ring, int lane) {
+  using T = typename R::T;
+  const int p0 = c.k * R::kKeys, end = min(p0 + R::kKeys, len), slot0 = slot_of(a, p0);
+  win.cover(a, c.row, slot0, slot_of(a, end - 1), len, lane);
+  const int pos = p0 + (lane & (R::kKeys - 1)), slot = slot_of(a, pos), page = win.at(slot), tok = pos - slot * a.page;
+  const bool bad = pos < end && (unsigned)page >= (unsigned)a.pages;
+  if (bad) report_error(kBadPage);
+  const unsigned keys = __ballot_sync(0xffffffffu, pos < end && !bad) & all_keys<R>();
+  constexpr int kEach = R::kHD / 32, kAtOnce = 32 / kEach;      // elements of a lane; keys at a time
+#pragma unroll 1
+  for (int is_v = 0; is_v < 2; ++is_v) {
+    const T* base = static_cast<const T*>(is_v ? a.v : a.k) + c.kv * (is_v ? a.v_head : a.k_head);
+    const long long at = (long long)page * (is_v ? a.v_page : a.k_page) + (long long)tok * (is_v ? a.v_tok : a.k_tok);
+    unsigned char* tile = ring + is_v * R::kSegs * R::kSeg;
+#pragma unroll 1
+    for (int j0 = 0; j0 < R::kKeys; j0 += kAtOnce) {
+      T e[kAtOnce][kEach];
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {        // (a load that depends on nothing: what there is not reads a query)
+        const long long to = __shfl_sync(0xffffffffu, at, j0 + j);
+        const T* src = keys >> (j0 + j) & 1 ? base + to : static_cast<const T*>(a.q);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) e[j][i] = src[min(lane + 32 * i, a.hd - 1)];
+      }
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j)
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+          const int byte = (lane + 32 * i) * (int)sizeof(T), row = j0 + j;      // 128-byte swizzle, as a tile arrives
+          *reinterpret_cast<T*>(tile + (byte >> 7) * R::kSeg + row * 128 + ((byte & 127) ^ (row & 7) << 4)) =
+              (keys >> row & 1) && lane + 32 * i < a.hd ? e[j][i] : from_f32<T>(0.0f);
+        }
+    }
+  }
+  __syncwarp();
+  return keys;
+}
+
+// And the queries of a job.
+template <typename R>
+__device__ __noinline__ void fill_queries(const typename R::T* src, typename R::T* dst, int heads, int hd, long long q_head, int lane) {
+  constexpr int U = 8;
+#pragma unroll 1
+  for (int i0 = lane; i0 < heads * R::kHD; i0 += 32 * U) {
+    typename R::T e[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + 32 * u, h = i / R::kHD, f = i - h * R::kHD;
+      if (h < heads && f < hd) e[u] = src[h * q_head + f];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + 32 * u, h = i / R::kHD, f = i - h * R::kHD;
+      if (h < heads && f < hd) dst[i] = e[u];
+    }
+  }
+}
+
 template <typename T, int N>
 __device__ __forceinline__ void store_out(T* dst, const float (&f)[N], float by, int valid, bool vec) {
   T e[N];
@@ -626,7 +691,7 @@ __device__ __noinline__ void join_parts(const PagedAttnArgs& a, Parts<W>& sh, co
 }
 
 // W warps, S rounds of a warp in flight or in use.
-template <typename R, int W, int S>
+template <typename R, int W, int S, bool TMA>
 __global__ void __launch_bounds__(W * 32, 1)
 paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_constant__ PageMaps maps, int box_shift, int head_tiles, int tile_heads, int q_vec, int o_vec) {
   using T = typename R::T;
@@ -695,7 +760,8 @@ paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_con
   }
   const int total = before[a.rows] * tiles;                    // (below 2^31: the launcher sees to it)
   // A CTA takes a unit for each of its warps at least: parts of one CTA are joined sooner than those of several.  Whole jobs, where all
-  // are as long and short enough that each CTA still has its own at once.
+  // are as long and short enough that each CTA still has its own at once (one sequence of 250 keys, 32 heads of 128 on 8: 9.1 us, dealt out 11.4;
+  // of 65 keys, 12 heads of 64: 6.6 and 7.2).
   int share = max(W, (int)((unsigned)(total + gridDim.x - 1) / gridDim.x));
   if (equal && rounds0 > 0 && rounds0 <= 2 * W && a.rows * tiles <= gridDim.x) share = rounds0 + 1;
   const int begin = (int)min((long long)total, (long long)share * blockIdx.x), end = min(total, begin + share);
@@ -752,20 +818,22 @@ paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_con
         // The job's queries come with its first round: loaded when the job starts, they cost each job the latency of the memory.  A place is free
         // again when the job S before is done: a fetch is at most S - 1 rounds ahead.
         const int tile = ahead.vh - ahead.kv * head_tiles, heads = min(tile_heads, group - tile * tile_heads);
-        const T* src = static_cast<const T*>(a.q) + ahead.row * a.q_row + (long long)(ahead.kv * group + tile * tile_heads + lane) * a.q_head;
-        unsigned char* dst = my_queries + put_job * R::kQueryBytes + lane * (R::kHD * (int)sizeof(T));
+        const T* src = static_cast<const T*>(a.q) + ahead.row * a.q_row + (long long)(ahead.kv * group + tile * tile_heads) * a.q_head;
+        T* dst = reinterpret_cast<T*>(my_queries + put_job * R::kQueryBytes);
         const int bytes = a.hd * (int)sizeof(T);
-        if (q_vec) {
+        if (TMA && q_vec) {
           if (lane == 0) mbar_expect_tx(bar, heads * bytes);
           __syncwarp();
-          if (lane < heads) bulk_load(dst, src, bytes, bar);
-        } else if (lane < heads) {
-          for (int f = 0; f < a.hd; ++f) reinterpret_cast<T*>(dst)[f] = src[f];
+          if (lane < heads) bulk_load(dst + lane * R::kHD, src + lane * a.q_head, bytes, bar);
+        } else {
+          fill_queries<R>(src, dst, heads, a.hd, a.q_head, lane);
         }
         __syncwarp();
         put_job = put_job + 1 == S ? 0 : put_job + 1;
       }
-      const unsigned keys = issue_round<R>(a, maps, win, ahead, len, box_shift, ring + put * R::kBytes, bar, lane);
+      unsigned keys;
+      if constexpr (TMA) keys = issue_round<R>(a, maps, win, ahead, len, box_shift, ring + put * R::kBytes, bar, lane);
+      else               keys = fill_round<R>(a, win, ahead, len, ring + put * R::kBytes, lane);
       there = (there & ~((unsigned long long)all_keys<R>() << (R::kKeys * put))) | (unsigned long long)keys << (R::kKeys * put);
       put = put + 1 == S ? 0 : put + 1;
       const int was = ahead.row;
@@ -796,7 +864,7 @@ paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_con
         count = min(tile_heads, group - tile * tile_heads);
         from = c.k;
       }
-      mbar_wait(bars + take, phase, &aborted, kWaitFullTimeout);
+      if constexpr (TMA) mbar_wait(bars + take, phase, &aborted, kWaitFullTimeout);
       if (fresh) {
         x.start(a, my_queries + take_job * R::kQueryBytes, count, lane);
         fresh = false;
@@ -870,85 +938,18 @@ static int map_pages(CUtensorMap* map, const PagedAttnArgs& a, const void* base,
   return encode_tmap_nd(map, a.f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, 4, dims, strides, boxes);
 }
 
-template <typename R, int W, int S>
-static int launch_paged(const PagedAttnArgs& a, const PageMaps& maps, int head_tiles, int tile_heads, bool q_vec, bool o_vec, cudaStream_t st) {
+template <typename R, int W, int S, bool TMA = true>
+static int launch_paged(const PagedAttnArgs& a, const PageMaps& maps, bool q_vec, bool o_vec, cudaStream_t st) {
   const size_t smem = 1024 + (size_t)W * S * (R::kBytes + R::kQueryBytes) + W * Part<R>::kFloats * 4 + (a.rows + 1) * 4 + a.rows;
   constexpr int kLimit = 226 << 10;
   static SmemLimit limit;
   const int grid = sm_count();
   if (smem > kLimit || a.ws_floats < grid * 2LL * Part<R>::kFloats || a.num_counters < grid) return kErrTooLarge;
-  DPTB_CUDA_OK(limit.raise((const void*)paged_attention_kernel<R, W, S>, kLimit));
+  DPTB_CUDA_OK(limit.raise((const void*)paged_attention_kernel<R, W, S, TMA>, kLimit));
   int box_shift = 0;
   while (2 << box_shift <= R::kKeys && a.page % (2 << box_shift) == 0) ++box_shift;
-  paged_attention_kernel<R, W, S><<<grid, W * 32, smem, st>>>(a, maps, box_shift, head_tiles, tile_heads, q_vec, o_vec);
+  paged_attention_kernel<R, W, S, TMA><<<grid, W * 32, smem, st>>>(a, maps, box_shift, (a.heads / a.kv_heads + R::kHeads - 1) / R::kHeads, R::kHeads, q_vec, o_vec);
   return counted(1, (int)cudaGetLastError());
-}
-
-// ------------------------------------------------------------------------------------------------------------ any layout
-constexpr int kSimpleTile = 128;
-constexpr int kMaxHeadDim = 256;
-
-template <typename T>
-__global__ void __launch_bounds__(kSimpleTile)
-paged_attention_simple_kernel(const PagedAttnArgs a) {
-  __shared__ float s_q[kMaxHeadDim], s_p[kSimpleTile], s_red[33];
-  __shared__ int s_page[kSimpleTile];
-  const int h = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
-  const int g = h / (a.heads / a.kv_heads);
-  const int room = (int)min((long long)a.width * a.page, 0x7fffffffLL);
-  int n = a.lens[r];
-  if (n > room) {
-    if (tid == 0) report_error(kBadPage);
-    n = room;
-  }
-  const T* q = static_cast<const T*>(a.q) + r * a.q_row + h * a.q_head;
-  for (int d = tid; d < a.hd; d += kSimpleTile) s_q[d] = to_f32(q[d]) * a.scale;
-  const T* kb = static_cast<const T*>(a.k) + g * a.k_head;
-  const T* vb = static_cast<const T*>(a.v) + g * a.v_head;
-  float m = -INFINITY, l = 0.0f, acc[kMaxHeadDim / kSimpleTile] = {};
-  for (int j0 = 0; j0 < n; j0 += kSimpleTile) {
-    const int j = j0 + tid, nt = min(kSimpleTile, n - j0);
-    int page = -1;
-    if (j < n) {
-      page = a.table[r * a.table_row + j / a.page];
-      if (page < 0 || page >= a.pages) {
-        report_error(kBadPage);
-        page = -1;
-      }
-    }
-    __syncthreads();
-    s_page[tid] = page;
-    __syncthreads();
-    float s = -INFINITY;
-    if (page >= 0) {
-      const T* k = kb + page * a.k_page + (j % a.page) * a.k_tok;
-      s = 0.0f;
-      for (int d = 0; d < a.hd; ++d) s += s_q[d] * to_f32(k[d]);
-    }
-    const float nm = fmaxf(m, block_max(s, s_red)), sub = nm == -INFINITY ? 0.0f : nm;
-    const float corr = __expf(m - sub), p = page >= 0 ? __expf(s - sub) : 0.0f;
-    l = l * corr + block_sum(p, s_red);
-    m = nm;
-    s_p[tid] = p;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kMaxHeadDim / kSimpleTile; ++i) {
-      const int d = i * kSimpleTile + tid;
-      if (d >= a.hd) break;
-      float t = acc[i] * corr;
-      for (int x = 0; x < nt; ++x) {
-        const int pg = s_page[x];
-        if (pg >= 0) t += s_p[x] * to_f32(vb[pg * a.v_page + ((j0 + x) % a.page) * a.v_tok + d]);
-      }
-      acc[i] = t;
-    }
-  }
-  T* o = static_cast<T*>(a.o) + r * a.o_row + h * a.o_head;
-#pragma unroll
-  for (int i = 0; i < kMaxHeadDim / kSimpleTile; ++i) {
-    const int d = i * kSimpleTile + tid;
-    if (d < a.hd) o[d] = from_f32<T>(n > 0 ? acc[i] / l : 0.0f);
-  }
 }
 
 }  // namespace dptb
@@ -969,39 +970,43 @@ extern "C" int dptb_paged_attention(const PagedAttnArgs* args, void* stream) {
   auto whole = [&](const void* p, long long s0, long long s1, long long s2) {
     return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && s0 % per == 0 && s1 % per == 0 && s2 % per == 0;
   };
-  // Keys of a round: 8 KB of them where rows are short.
   const int keys = a.f32 ? (a.hd <= 64 ? 16 : 8) : a.hd <= 64 ? 32 : 16;
-  PageMaps maps;
+  // rounds, and all else that is counted, in 32 bits
+  if ((double)a.rows * ((double)a.width * a.page / keys + 2) * a.heads >= 2147483000.0) return kErrTooLarge;
+  const bool qv = whole(a.q, a.q_row, a.q_head, 0), ov = whole(a.o, a.o_row, a.o_head, 0);
+  const int group = a.heads / a.kv_heads;
+  PageMaps maps = {};
   int box = 1;
   while (2 * box <= keys && a.page % (2 * box) == 0) box *= 2;
-  if (a.hd % per == 0 && whole(a.k, a.k_page, a.k_head, a.k_tok) && whole(a.v, a.v_page, a.v_head, a.v_tok) &&
-      map_pages(&maps.k, a, a.k, a.k_page, a.k_head, a.k_tok, box) == 0 && map_pages(&maps.v, a, a.v, a.v_page, a.v_head, a.v_tok, box) == 0) {
-    const bool qv = whole(a.q, a.q_row, a.q_head, 0), ov = whole(a.o, a.o_row, a.o_head, 0);
-    const int group = a.heads / a.kv_heads;
-    // rounds, and all else that is counted, in 32 bits
-    if ((double)a.rows * ((double)a.width * a.page / keys + 2) * a.heads >= 2147483000.0) return kErrTooLarge;
-#define DPTB_PAGED(R, W, S) return launch_paged<R, W, S>(a, maps, (group + R::kHeads - 1) / R::kHeads, R::kHeads, qv, ov, st)
-    if (!a.f32) {
-      using B64 = Bf16Round<64, 1, 2>; using C64 = Bf16Round<64, 2, 2>;
-      using B128 = Bf16Round<128, 1, 1>; using C128 = Bf16Round<128, 2, 1>;
-      using B256 = Bf16Round<256, 1, 1>;
-      if (a.hd <= 64) { if (group <= 8) DPTB_PAGED(B64, 8, 2); DPTB_PAGED(C64, 8, 2); }
-      if (a.hd <= 128) { if (group <= 8) DPTB_PAGED(B128, 8, 2); DPTB_PAGED(C128, 6, 2); }
-      DPTB_PAGED(B256, 4, 2);
-    }
-#define DPTB_PAGED_F32(HD, NJ, W, S) \
-    if (group == 1) { using R1 = F32Round<HD, 1, NJ>; DPTB_PAGED(R1, W, S); } \
-    if (group == 2) { using R2 = F32Round<HD, 2, NJ>; DPTB_PAGED(R2, W, S); } \
-    if (group <= 4 || HD == 256) { using R4 = F32Round<HD, 4, NJ>; DPTB_PAGED(R4, W, S); }
-    if (a.hd <= 64) { DPTB_PAGED_F32(64, 4, 8, 2) using R8 = F32Round<64, 8, 4>; DPTB_PAGED(R8, 8, 2); }
-    if (a.hd <= 96) { DPTB_PAGED_F32(96, 2, 8, 2) using R8 = F32Round<96, 8, 2>; DPTB_PAGED(R8, 8, 2); }
-    if (a.hd <= 128) { DPTB_PAGED_F32(128, 2, 8, 2) using R8 = F32Round<128, 8, 2>; DPTB_PAGED(R8, 7, 2); }
-    DPTB_PAGED_F32(256, 2, 4, 2)
-#undef DPTB_PAGED_F32
-#undef DPTB_PAGED
+  const bool tma = a.hd % per == 0 && whole(a.k, a.k_page, a.k_head, a.k_tok) && whole(a.v, a.v_page, a.v_head, a.v_tok) &&
+                   map_pages(&maps.k, a, a.k, a.k_page, a.k_head, a.k_tok, box) == 0 && map_pages(&maps.v, a, a.v, a.v_page, a.v_head, a.v_tok, box) == 0;
+#define DPTB_PAGED(...) return launch_paged<__VA_ARGS__>(a, maps, qv, ov, st)
+  if (!tma && a.f32) {
+    if (a.hd <= 64) DPTB_PAGED(F32Round<64, 4, 4>, 8, 2, false);
+    if (a.hd <= 128) DPTB_PAGED(F32Round<128, 4, 2>, 8, 2, false);
+    DPTB_PAGED(F32Round<256, 4, 2>, 4, 2, false);
   }
-  const dim3 grid(a.heads, a.rows);
-  if (a.f32) paged_attention_simple_kernel<float><<<grid, kSimpleTile, 0, st>>>(a);
-  else       paged_attention_simple_kernel<__nv_bfloat16><<<grid, kSimpleTile, 0, st>>>(a);
-  return counted(1, (int)cudaGetLastError());
+  if (!tma) {
+    if (a.hd <= 64) DPTB_PAGED(Bf16Round<64, 1, 2>, 8, 2, false);
+    if (a.hd <= 128) DPTB_PAGED(Bf16Round<128, 1, 1>, 8, 2, false);
+    DPTB_PAGED(Bf16Round<256, 1, 1>, 4, 2, false);
+  }
+  if (!a.f32) {
+    if (a.hd <= 64 && group <= 8) DPTB_PAGED(Bf16Round<64, 1, 2>, 8, 2);
+    if (a.hd <= 64) DPTB_PAGED(Bf16Round<64, 2, 2>, 8, 2);
+    if (a.hd <= 128 && group <= 8) DPTB_PAGED(Bf16Round<128, 1, 1>, 8, 2);
+    if (a.hd <= 128) DPTB_PAGED(Bf16Round<128, 2, 1>, 6, 2);
+    DPTB_PAGED(Bf16Round<256, 1, 1>, 4, 2);
+  }
+#define DPTB_PAGED_GROUP(HD, NJ, W) \
+  if (group == 1) DPTB_PAGED(F32Round<HD, 1, NJ>, W, 2); \
+  if (group == 2) DPTB_PAGED(F32Round<HD, 2, NJ>, W, 2); \
+  if (group <= 4) DPTB_PAGED(F32Round<HD, 4, NJ>, W, 2)
+  if (a.hd <= 64) { DPTB_PAGED_GROUP(64, 4, 8); DPTB_PAGED(F32Round<64, 8, 4>, 8, 2); }
+  if (a.hd <= 96) { DPTB_PAGED_GROUP(96, 2, 8); DPTB_PAGED(F32Round<96, 8, 2>, 8, 2); }
+  if (a.hd <= 128) { DPTB_PAGED_GROUP(128, 2, 8); DPTB_PAGED(F32Round<128, 8, 2>, 7, 2); }
+  DPTB_PAGED_GROUP(256, 2, 4);
+  DPTB_PAGED(F32Round<256, 4, 2>, 4, 2);
+#undef DPTB_PAGED_GROUP
+#undef DPTB_PAGED
 }

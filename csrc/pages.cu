@@ -249,7 +249,7 @@ __device__ __forceinline__ unsigned cluster_ctas() {
 //
 // One cluster: the CTAs share the rows, a warp a row, and mark pages in bit maps in shared memory (listed at all; listed by somebody who does not grow
 // into it).  The first CTA joins the maps and does what needs all rows: a hash table from a page to the first row that grows into it, and sums over rows and pages
-// for the order.  Bound by a chain of a dozen latencies.  One CTA for all rows took 36 us for 256 rows of up to 100 pages.
+// for the order.  Bound by a chain of a dozen latencies: 4.9 us for four rows of 13 pages, 10 us for 256 rows of 94.
 struct ForkArgs {
   const int* table;
   const int* lens;
@@ -490,7 +490,8 @@ compact_pages_kernel(const CompactArgs a, int words) {
     }
 }
 
-// Up to 32 rows a CTA has a warp for each; more are shared by a cluster.
+// Up to 32 rows a CTA has a warp for each; more are shared by a cluster (a fork of 4 rows takes 4.9 to 5.7 us in one CTA and 6.1 in eight, of 32 rows of
+// 94 pages 7.3 and 7.9, of 64 9.8 and 8.4, of 256 23 and 10).
 template <typename... KArgs>
 static int launch_page_kernel(void (*kernel)(KArgs...), SmemLimit& limit, int rows, size_t smem, cudaStream_t st, KArgs... args) {
   if (smem > kPageSmem) return kErrTooLarge;

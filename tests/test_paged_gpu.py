@@ -76,6 +76,12 @@ def test_attention_layouts(dtype, layout, hd):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,hkv,hd,page", [(1, 1, 33, 16), (8, 1, 100, 5), (12, 1, 64, 32), (40, 2, 128, 16), (9, 3, 255, 24), (6, 1, 256, 1)])
+def test_attention_heads_off_16_bytes(dtype, heads, hkv, hd, page):
+    check(*make(LENS + [3000], heads, hkv, hd, page, dtype, layout="off"))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("lens", [[4097], [2500, 1, 0, 0, 3001], [0, 0], [1] * 50, [16 * i for i in range(40)],
                                   [random.Random(3).randint(0, 90) for _ in range(300)]])
 def test_attention_lengths(dtype, lens):
