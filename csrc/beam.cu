@@ -12,8 +12,9 @@
 // and the lanes' maxima tell where to look: the best W continuations lie with the lanes of the W largest (each counted with its beam's score),
 // and only these lanes' logits are read once more, by the value of the W-th.  That is a few hundred logits, whatever the vocabulary.
 //
-// Bound by memory for many rows, by a chain of latencies for few.  Choosing in every warp, or in CTAs barrier after barrier, cost more than the pass
-// itself: 45 and 61 us for 256 rows of 128256 logits.
+// Bound by memory for many rows, by a chain of latencies for few.  256 rows of 128256 logits in bf16, 8 beams an item, take 25 us, of which the pass is half
+// (66 MB in 11.5 us) and the choice in each item's last CTA the other; four rows of 50257 in fp32 12 us.  Choosing in every warp, or in CTAs barrier
+// after barrier, cost more than the pass itself: 45 and 61 us for the 256 rows.
 #include <cuda_bf16.h>
 
 #include "common/host.h"

@@ -138,12 +138,20 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     """Attention of one new token per row, ``q [rows, heads, head_dim]``, over the ``lens[r]`` tokens of its pages (the new one
     among them).  Query heads share key heads in groups of ``heads // kv_heads``; a row of no tokens gives zeros.  bf16 or fp32, one type for all; sums in
     fp32.  ``scale`` is ``head_dim ** -0.5`` unless given.  Returns ``[rows, heads, head_dim]``."""
-    dev = q.get_device()
-    if not (dev >= 0 and q.dim() == 3 and k_pages.dim() == 4 and table.dim() == 2):
+    dev, q_shape, k_shape, t_shape, dtype = q.get_device(), q.shape, k_pages.shape, table.shape, q.dtype
+    if dev < 0 or len(q_shape) != 3 or len(k_shape) != 4 or len(t_shape) != 2 or v_pages.shape != k_shape:
         return _attention_on_cpu(q, k_pages, v_pages, table, lens, scale, out)
-    (rows, heads, hd), (pages, hkv, page, _), (_, width) = q.shape, k_pages.shape, table.shape
-    (q_row, q_head, q_one), (kp, kh, kt, k_one), (vp, vh, vt, v_one) = q.stride(), k_pages.stride(), v_pages.stride()
-    if q_one != 1 or out is not None or _attention_is_off(q, k_pages, v_pages, table, lens, dev, q.dtype, k_one, v_one):
+    (rows, heads, hd), (pages, hkv, page, k_hd), (t_rows, width) = q_shape, k_shape, t_shape
+    (q_row, q_head, q_one), (kp, kh, kt, k_one), (vp, vh, vt, v_one), (t_row, t_one) = (
+        q.stride(), k_pages.stride(), v_pages.stride(), table.stride())
+    if not (                 # all that the checks ask for, in less time
+            out is None and (dtype is _BF16 or dtype is _F32) and k_pages.dtype is dtype and v_pages.dtype is dtype and
+            table.dtype is _I32 and lens.dtype is _I32 and k_hd == hd and t_rows == rows and lens.shape == (rows,) and
+            0 < hd <= MAX_HEAD_DIM and 0 < hkv and heads % hkv == 0 and 0 < page and pages <= MAX_PAGES and rows <= MAX_ROWS and
+            q_one == 1 and k_one == 1 and v_one == 1 and (t_one == 1 or width <= 1) and (rows <= 1 or lens.stride(0) == 1) and
+            k_pages.get_device() == dev and v_pages.get_device() == dev and table.get_device() == dev and
+            lens.get_device() == dev and _current_device() == dev and
+            not (torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad))):
         _check_attention(q, k_pages, v_pages, table, lens, out)
         if q_one != 1 and hd > 1:
             q = q.contiguous()
@@ -157,26 +165,13 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     ws, counters = _scratch(dev, stream)
     rc = _lib().dptb_paged_attention(_ATTN_ARGS.pack(
         q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), table.data_ptr(), lens.data_ptr(),
-        q_row, q_head, o_row, o_head, kp, kh, kt, vp, vh, vt, table.stride(0),
-        rows, heads, hkv, hd, page, width, pages, q.dtype is _F32, hd ** -0.5 if scale is None else scale,
+        q_row, q_head, o_row, o_head, kp, kh, kt, vp, vh, vt, t_row,
+        rows, heads, hkv, hd, page, width, pages, dtype is _F32, hd ** -0.5 if scale is None else scale,
         ws.data_ptr(), kernels.SPLITK_WS_BYTES // 4, counters.data_ptr(), kernels.SPLITK_COUNTERS, 0, 0), stream)
     if rc == TOO_LARGE:
         raise ValueError(f"paged_attention: {rows} rows of up to {width * page} tokens and {heads} heads in one call are too many")
     N.check(rc, "paged_attention")
     return out
-
-
-def _attention_is_off(q, k, v, table, lens, dev, dtype, k_one, v_one) -> bool:
-    """Whether ``_check_attention`` has to look: everything it asks for, at the price of a call on each step."""
-    rows, heads, hd = q.shape
-    pages, hkv, page, k_hd = k.shape
-    return not (
-        (dtype is _BF16 or dtype is _F32) and k.dtype is dtype and v.dtype is dtype and table.dtype is _I32 and lens.dtype is _I32 and
-        v.shape == k.shape and k_hd == hd and table.shape[0] == rows and lens.shape == (rows,) and 0 < hd <= MAX_HEAD_DIM and
-        0 < hkv and heads % hkv == 0 and 0 < page and pages <= MAX_PAGES and rows <= MAX_ROWS and k_one == 1 and v_one == 1 and
-        (table.stride(1) == 1 or table.shape[1] <= 1) and (rows <= 1 or lens.stride(0) == 1) and
-        k.get_device() == dev and v.get_device() == dev and table.get_device() == dev and lens.get_device() == dev and
-        _current_device() == dev and not ((q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled()))
 
 
 def _check_attention(q, k_pages, v_pages, table, lens, out) -> None:
@@ -235,43 +230,38 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     and writes nothing.  Queries and keys are turned by the half-split rotary embedding over ``rotary_dim`` features (all of
     them unless given; 0: not at all).  Returns the turned queries ``[tokens, heads, head_dim]``, and with ``keys`` the turned keys
     too; ``qkv`` stays as it is.  No two tokens may have one place."""
-    rotary = k_pages.shape[-1] if rotary_dim is None else rotary_dim
-    dev = qkv.get_device()
-    if dev < 0 or _append_is_off(qkv, k_pages, v_pages, table, positions, heads, rows, rotary, rope_base, dev, qkv.dtype):
+    dev, x_shape, k_shape, t_shape, dtype = qkv.get_device(), qkv.shape, k_pages.shape, table.shape, qkv.dtype
+    rotary = k_shape[-1] if rotary_dim is None else rotary_dim
+    if dev < 0 or len(x_shape) != 2 or len(k_shape) != 4 or len(t_shape) != 2 or v_pages.shape != k_shape:
         _check_append(qkv, k_pages, v_pages, table, positions, heads, rows, rotary, rope_base)
-        if dev < 0:
-            q, k = paged_append_reference(qkv, k_pages, v_pages, table, positions, heads, rows, rotary, rope_base)
-            return (q, k) if keys else q
-        if qkv.stride(1) != 1:
+        q, k = paged_append_reference(qkv, k_pages, v_pages, table, positions, heads, rows, rotary, rope_base)
+        return (q, k) if keys else q
+    (tokens, features), (pages, hkv, page, hd), (table_rows, width) = x_shape, k_shape, t_shape
+    (x_row, x_one), (kp, kh, kt, k_one), (vp, vh, vt, v_one), (t_row, t_one) = (
+        qkv.stride(), k_pages.stride(), v_pages.stride(), table.stride())
+    if not (                 # all that the checks ask for, in less time
+            (dtype is _BF16 or dtype is _F32) and k_pages.dtype is dtype and v_pages.dtype is dtype and table.dtype is _I32 and
+            positions.dtype is _I32 and positions.shape == (tokens,) and (tokens <= 1 or positions.stride(0) == 1) and
+            0 < hd <= MAX_HEAD_DIM and 0 < hkv and 0 < page and pages <= MAX_PAGES and table_rows <= MAX_ROWS and
+            heads > 0 and features == (heads + 2 * hkv) * hd and 0 <= rotary <= hd and rotary % 2 == 0 and rope_base > 0 and
+            x_one == 1 and k_one == 1 and v_one == 1 and (t_one == 1 or width <= 1) and
+            k_pages.get_device() == dev and v_pages.get_device() == dev and table.get_device() == dev and
+            positions.get_device() == dev and _current_device() == dev and
+            (table_rows == tokens if rows is None else rows.dtype is _I32 and rows.shape == (tokens,) and
+             rows.get_device() == dev and (tokens <= 1 or rows.stride(0) == 1)) and
+            not (torch.is_grad_enabled() and (qkv.requires_grad or k_pages.requires_grad or v_pages.requires_grad))):
+        _check_append(qkv, k_pages, v_pages, table, positions, heads, rows, rotary, rope_base)
+        if x_one != 1:
             qkv = qkv.contiguous()
-    tokens, (pages, hkv, page, hd) = qkv.shape[0], k_pages.shape
+            x_row = features
     q = qkv.new_empty((tokens, heads, hd))
     k = qkv.new_empty((tokens, hkv, hd)) if keys else None
-    (kp, kh, kt, _), (vp, vh, vt, _) = k_pages.stride(), v_pages.stride()
-    table_rows, width = table.shape
     N.check(_lib().dptb_paged_append(_APPEND_ARGS.pack(
         qkv.data_ptr(), q.data_ptr(), k.data_ptr() if keys else 0, k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(),
-        positions.data_ptr(), 0 if rows is None else rows.data_ptr(), qkv.stride(0), kp, kh, kt, vp, vh, vt, table.stride(0),
-        tokens, heads, hkv, hd, rotary, page, width, pages, table_rows, qkv.dtype is _F32, rope_base), _raw_stream(dev)), "paged_append")
+        positions.data_ptr(), 0 if rows is None else rows.data_ptr(), x_row, kp, kh, kt, vp, vh, vt, t_row,
+        tokens, heads, hkv, hd, rotary, page, width, pages, table_rows, dtype is _F32, rope_base), _raw_stream(dev)), "paged_append")
     _increment_version((k_pages, v_pages))
     return (q, k) if keys else q
-
-
-def _append_is_off(qkv, k, v, table, positions, heads, rows, rotary, rope_base, dev, dtype) -> bool:
-    """Whether ``_check_append`` has to look (see ``_attention_is_off``)."""
-    if qkv.dim() != 2 or k.dim() != 4 or v.dim() != 4 or table.dim() != 2:
-        return True
-    tokens, pages, hkv, page, hd = qkv.shape[0], *k.shape
-    return not (
-        (dtype is _BF16 or dtype is _F32) and k.dtype is dtype and v.dtype is dtype and v.shape == k.shape and table.dtype is _I32 and
-        positions.dtype is _I32 and positions.shape == (tokens,) and (tokens <= 1 or positions.stride(0) == 1) and
-        0 < hd <= MAX_HEAD_DIM and 0 < hkv and 0 < page and pages <= MAX_PAGES and table.shape[0] <= MAX_ROWS and
-        heads > 0 and qkv.shape[1] == (heads + 2 * hkv) * hd and 0 <= rotary <= hd and rotary % 2 == 0 and rope_base > 0 and
-        qkv.stride(1) == 1 and k.stride(3) == 1 and v.stride(3) == 1 and (table.stride(1) == 1 or table.shape[1] <= 1) and
-        k.get_device() == dev and v.get_device() == dev and table.get_device() == dev and positions.get_device() == dev and
-        (table.shape[0] == tokens if rows is None else rows.dtype is _I32 and rows.shape == (tokens,) and rows.get_device() == dev and
-         (tokens <= 1 or rows.stride(0) == 1)) and
-        _current_device() == dev and not ((qkv.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled()))
 
 
 def _check_append(qkv, k_pages, v_pages, table, positions, heads, rows, rotary, rope_base) -> None:
@@ -360,7 +350,7 @@ def fork_pages(table: torch.Tensor, lens: torch.Tensor, pages: int, page: int, p
 
 
 def _fork_is_off(table, lens, pages, page, parents, grow, each, dev) -> bool:
-    """Whether ``_check_fork`` has to look (see ``_attention_is_off``)."""
+    """Whether ``_check_fork`` has to look : everything it asks for, in less time."""
     if table.dim() != 2 or parents is not None and parents.dim() != 1:
         return True
     rows_in = table.shape[0]
