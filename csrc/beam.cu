@@ -8,12 +8,12 @@
 // meet in 64 bits.
 //
 // beam_kernel: a row is dealt to warps.  One pass over the logits keeps a running maximum and sum of exponentials in every lane; that is
-// all that is done for each logit (5.5 instructions in bf16).  The CTA of an item's last warp to finish (a counter, no waiting) sums up its rows,
+// all that is done for each logit (5.5 instructions in bf16).  The last of an item's CTAs to finish (a counter, no waiting) sums up its rows,
 // and the lanes' maxima tell where to look: the best W continuations lie with the lanes of the W largest (each counted with its beam's score),
 // and only these lanes' logits are read once more, by the value of the W-th.  That is a few hundred logits, whatever the vocabulary.
 //
-// Bound by memory for many rows, by a chain of latencies for few.  256 rows of 128256 logits in bf16, 8 beams an item, take 25 us, of which the pass is half
-// (66 MB in 11.5 us) and the choice in each item's last CTA the other; four rows of 50257 in fp32 12 us.  Choosing in every warp, or in CTAs barrier
+// Bound by memory for many rows, by a chain of latencies for few.  256 rows of 128256 logits in bf16, 8 beams an item, take 22.5 us, of which the pass is half
+// (66 MB in 11.5 us) and the choice in each item's last CTA the other; four rows of 50257 in fp32 9.4 us, 35 of 321 6.9.  Choosing in every warp, or in CTAs barrier
 // after barrier, cost more than the pass itself: 45 and 61 us for the 256 rows.
 #include <cuda_bf16.h>
 
@@ -153,6 +153,30 @@ __device__ __forceinline__ Piece<T> load_piece(const T* row, int first, int end,
   constexpr uint32_t kNone = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
   return Piece<T>{kNone, kNone, kNone, kNone};
 }
+// What lane `lane` has of the 32 N logits from `first` on: neighbours if rows are on 16-byte boundaries, every 32nd if not, so that a warp's
+// loads are whole lines in either case.
+template <typename T>
+__device__ __forceinline__ int place_in(int first, int lane, int e, bool vec) { return vec ? first + lane * Piece<T>::N + e : first + e * 32 + lane; }
+template <typename T, bool VEC>
+__device__ __forceinline__ Piece<T> load_group(const T* row, int first, int lane, int end) {
+  constexpr int N = Piece<T>::N;
+  if constexpr (VEC) return load_piece<T>(row, first + lane * N, end, true);
+  const int i = first + lane;
+  Piece<T> p;
+  if constexpr (sizeof(T) == 2) {
+    const auto* bits = reinterpret_cast<const unsigned short*>(row);
+#pragma unroll
+    for (int e = 0; e < N; e += 2) {
+      const uint32_t lo = i + e * 32 < end ? bits[i + e * 32] : 0xff80u, hi = i + e * 32 + 32 < end ? bits[i + e * 32 + 32] : 0xff80u;
+      p.u[e / 2] = lo | hi << 16;
+    }
+  } else {
+    const auto* bits = reinterpret_cast<const uint32_t*>(row);
+#pragma unroll
+    for (int e = 0; e < N; ++e) p.u[e] = i + e * 32 < end ? bits[i + e * 32] : 0xff800000u;
+  }
+  return p;
+}
 
 // What a warp leaves of its logits: the sum of exponentials, what it is relative to, every lane's maximum.
 struct BeamPart {
@@ -167,16 +191,17 @@ struct BeamShared {
   float lists[kBeamThreads];
   double score[kMaxBeams], top[kMaxBeams], norm[kMaxBeams];
   float size[kMaxBeams];                   // of what fp32 totals are made of
-  unsigned char kind[kMaxBeams];           // 0: by its logits, 1: finished, 2: nothing to offer
+  unsigned char kind[kMaxBeams], fin[kMaxBeams];     // 0: by its logits, 1: finished, 2: nothing to offer; whether finished
   float from[kMaxBeams], least[kMaxBeams];  // what a logit less `from` has to reach
-  int hot[kHotLanes], count, hots, counts[kBeamWarps], done[kBeamWarps];
+  int hot[kHotLanes], count, hots, counts[kBeamWarps], last;
 };
 static_assert(kBeamWarps * kWarpPool <= kItemPool, "the warps' pools");
 
 // A sum relative to the maximum `m`, or its shift, relative to `top` > m, or its.
 constexpr float kLarge = 1048576.0f;
+constexpr double kLn2 = 1.0 / (double)kLog2e;      // of the rounded kLog2e
 __device__ __noinline__ double rescaled_large(double s, float m, float shift, float top, float next) {
-  const double from = fabsf(m) < kLarge ? (double)shift / (double)kLog2e : (double)m, to = fabsf(top) < kLarge ? (double)next / (double)kLog2e : (double)top;
+  const double from = fabsf(m) < kLarge ? (double)shift * kLn2 : (double)m, to = fabsf(top) < kLarge ? (double)next * kLn2 : (double)top;
   return s * exp(from - to);
 }
 __device__ __forceinline__ double rescaled(double s, float m, float shift, float top, float next) {
@@ -226,14 +251,14 @@ __device__ __noinline__ void best_of_row(const BeamArgs& a, const T* row, const 
     for (unsigned some = __ballot_sync(0xffffffffu, __ldcg(&p[l].high[lane]) > limit); some; some &= some - 1) {
       const int j = __ffs(some) - 1;
 #pragma unroll 1
-      for (int i = begin + (j + 32 * lane) * N; i < end; i += 32 * 32 * N) {
-        const Piece<T> x = load_piece<T>(row, i, end, a.vec);
+      for (int i = begin + 32 * lane * N; i < end; i += 32 * 32 * N) {
+        const Piece<T> x = a.vec ? load_group<T, true>(row, i, j, end) : load_group<T, false>(row, i, j, end);
         if (!(x.top() > limit)) continue;
 #pragma unroll
         for (int e = 0; e < N; ++e)
-          if (i + e < end && x.at(e) > limit) {
+          if (x.at(e) > limit) {
             const int at = atomicAdd(count, 1);
-            if (at < kWarpPool) keys[at] = rank_key(x.at(e), i + e);
+            if (at < kWarpPool) keys[at] = rank_key(x.at(e), place_in<T>(i, j, e, a.vec));
           }
       }
     }
@@ -348,7 +373,7 @@ __device__ __forceinline__ void sum_row(const BeamPart* p, int lists, double& to
     for (int x = 0; x < 2; ++x) t += sum[x] == 0.0 ? 0.0 : sum[x] * exp(base[x] - top);
   } else {
     const float most = warp_max(fmaxf(shift[0], shift[1]));
-    top = (double)most / (double)kLog2e;
+    top = (double)most * kLn2;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       const float down = fminf(most - shift[x], 1000.0f);
@@ -371,16 +396,24 @@ __device__ __noinline__ void choose(const BeamArgs& a, BeamShared& sh, int local
   if (tid == 0) sh.count = sh.hots = 0;
   const int mates = K <= 1 ? 8 : K <= 2 ? 4 : K <= 4 ? 2 : 1, w0 = warp / mates, dw = kBeamWarps / mates;      // warps of a row; rows of this warp
   const int quads = a.lists * 8, q0 = (warp - w0 * mates) * 32 + lane, dq = mates * 32;                       // four lanes' maxima at a time
-  auto quad = [&](int w, int q) { return __ldcg(reinterpret_cast<const float4*>(parts[w * a.lists + (q >> 3)].high) + (q & 7)); };
+  auto quad = [&](int w, int q) {
+    return q < quads ? __ldcg(reinterpret_cast<const float4*>(parts[w * a.lists + (q >> 3)].high) + (q & 7))
+                     : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+  };
+  auto most_of = [](const float4& v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); };
+  constexpr int H = 4;                  // of them at once
   // The W-th largest of the lanes' maxima, and the lanes that reach it, both in fp32, as x - from + offset, and with room for its roundings:
   // `from` and `offset` are off by 2^-24 of themselves, and so are the two sums.
   float high = -INFINITY;
 #pragma unroll 1
   for (int w = w0; w < K; w += dw) {
-    double top, norm;
-    sum_row(parts + w * a.lists, a.lists, top, norm);
     const float score = a.scores[item * K + w];
     const bool fin = a.finished && a.finished[item * K + w];
+    float4 v[H];                        // on their way while the row is summed up
+#pragma unroll
+    for (int x = 0; x < H; ++x) v[x] = quad(w, q0 + x * dq);
+    double top, norm;
+    sum_row(parts + w * a.lists, a.lists, top, norm);
     const int kind = !(fabsf(score) < INFINITY) ? 2 : fin ? 1 : fabs(top) < INFINITY && fabs(norm) < INFINITY ? 0 : 2;
     const float from = (float)top, offset = (float)(score - norm);
     if (lane == 0) {
@@ -388,15 +421,13 @@ __device__ __noinline__ void choose(const BeamArgs& a, BeamShared& sh, int local
       sh.top[w] = top;
       sh.norm[w] = norm;
       sh.kind[w] = kind;
+      sh.fin[w] = fin;
       sh.size[w] = kind ? 0.0f : fabsf(offset) + fminf(fabsf(from), 2.0f * kLarge);
     }
     if (kind == 0) {
-      float most = -INFINITY;
+      float most = fmaxf(fmaxf(most_of(v[0]), most_of(v[1])), fmaxf(most_of(v[2]), most_of(v[3])));
 #pragma unroll 4
-      for (int q = q0; q < quads; q += dq) {
-        const float4 v = quad(w, q);
-        most = fmaxf(most, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
-      }
+      for (int q = q0 + H * dq; q < quads; q += dq) most = fmaxf(most, most_of(quad(w, q)));
       high = fmaxf(high, most - from + offset);
     } else if (q0 < min(K, a.vocab)) {
       high = fmaxf(high, kind == 1 && a.eos >= 0 && q0 == 0 ? score : -INFINITY);
@@ -421,7 +452,6 @@ __device__ __noinline__ void choose(const BeamArgs& a, BeamShared& sh, int local
         }
         continue;
       }
-      const T* row = rows + w * a.ld;
       const float from = (float)sh.top[w], d = (float)((double)limit - sh.score[w] + sh.norm[w]), least = d - (size + fabsf(d)) * 0x1p-21f;
       sh.from[w] = from;
       sh.least[w] = least;
@@ -430,7 +460,7 @@ __device__ __noinline__ void choose(const BeamArgs& a, BeamShared& sh, int local
       for (int q = q0; q < quads; q += 4 * dq) {
         float4 v[4];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) v[x] = q + x * dq < quads ? quad(w, q + x * dq) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        for (int x = 0; x < 4; ++x) v[x] = quad(w, q + x * dq);
         unsigned mine = 0;
 #pragma unroll
         for (int x = 0; x < 4; ++x)
@@ -454,20 +484,21 @@ __device__ __noinline__ void choose(const BeamArgs& a, BeamShared& sh, int local
         const int begin = (part - w * a.lists) * a.chunk, end = min(a.vocab, begin + a.chunk);
         const float from = sh.from[w], least = sh.least[w];
 #pragma unroll 1
-        for (int i = begin + ((j & 31) + 32 * (tid & (width - 1))) * N; i < end; i += width * 32 * N) {
-          const Piece<T> p = load_piece<T>(row, i, end, a.vec);
-          if (p.top() - from < least) continue;
+        for (int i = begin + 32 * (tid & (width - 1)) * N; i < end; i += width * 32 * N) {
+          const Piece<T> p = a.vec ? load_group<T, true>(row, i, j & 31, end) : load_group<T, false>(row, i, j & 31, end);
+          unsigned mine = 0;
+#pragma unroll
+          for (int e = 0; e < N; ++e) mine |= (unsigned)(p.at(e) - from >= least) << e;
 #pragma unroll 1
-          for (int e = 0; e < N && i + e < end; ++e) {
+          for (; mine; mine &= mine - 1) {
+            const int e = __ffs(mine) - 1;
             float x = p.at(0);
 #pragma unroll
             for (int n = 1; n < N; ++n) x = e == n ? p.at(n) : x;
-            if (x - from >= least) {
-              const int at = atomicAdd(&sh.count, 1);
-              if (at < kItemPool) {
-                sh.totals[at] = total_of(sh, w, x);
-                sh.keys[at] = (unsigned long long)w << 32 | (unsigned)(i + e);
-              }
+            const int at = atomicAdd(&sh.count, 1);
+            if (at < kItemPool) {
+              sh.totals[at] = total_of(sh, w, x);
+              sh.keys[at] = (unsigned long long)w << 32 | (unsigned)place_in<T>(i, j & 31, e, a.vec);
             }
           }
         }
@@ -491,35 +522,36 @@ __device__ __noinline__ void choose(const BeamArgs& a, BeamShared& sh, int local
       a.out_scores[out] = (float)t;
       a.out_parents[out] = item * K + w;
       a.out_tokens[out] = tok;
-      a.out_finished[out] = (a.finished && a.finished[item * K + w]) || tok == a.eos;
+      a.out_finished[out] = sh.fin[w] || tok == a.eos;
     }
   }
 }
 
-template <typename T>
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(kBeamThreads, 4)
-beam_kernel(const __grid_constant__ BeamArgs a, int rows) {
+beam_kernel(const __grid_constant__ BeamArgs a) {
   constexpr int N = Piece<T>::N, U = 4;           // pieces in flight
   __shared__ BeamShared sh;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = a.beams;
-  const int unit = blockIdx.x * kBeamWarps + warp, local_row = unit / a.lists, list = unit - local_row * a.lists;
-  int done = -1;
-  if (local_row < rows) {
-    const T* row = static_cast<const T*>(a.logits) + ((long long)a.first_item * K + local_row) * a.ld;
+  // An item has whole CTAs to itself.
+  const int units = K * a.lists, ctas = (units + kBeamWarps - 1) / kBeamWarps, local = blockIdx.x / ctas;
+  const int unit = (blockIdx.x - local * ctas) * kBeamWarps + warp, w = unit / a.lists, list = unit - w * a.lists;
+  if (unit < units) {
+    const T* row = static_cast<const T*>(a.logits) + ((long long)(a.first_item + local) * K + w) * a.ld;
     const int begin = list * a.chunk, end = min(a.vocab, begin + a.chunk);
     // Sums of 2^(x log2(e) - shift): `shift` is a whole number, so that sums are brought to another one exactly, and stands for shift / log2(e),
     // divided out in 64 bits, so that the rounding of log2(e) moves no sum against another.  What is left is the error of an exponential, 2^-22, and of
     // sums of 32.  Maxima that are too large for it (masks of the type's lowest value among them) go by differences, from themselves.
     float m = -INFINITY, shift = 0.0f;
     double s = 0.0;
-    for (int i = begin + lane * N; i < end; i += U * 32 * N) {
+    for (int i = begin; i < end; i += U * 32 * N) {
       Piece<T> p[U];
-      if (a.vec && i + (U - 1) * 32 * N + N <= end) {
+      if (VEC && i + U * 32 * N <= end) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) p[u] = load_whole<T>(row, i + u * 32 * N);
+        for (int u = 0; u < U; ++u) p[u] = load_whole<T>(row, i + (u * 32 + lane) * N);
       } else {
 #pragma unroll
-        for (int u = 0; u < U; ++u) p[u] = load_piece<T>(row, i + u * 32 * N, end, a.vec);
+        for (int u = 0; u < U; ++u) p[u] = load_group<T, VEC>(row, i + u * 32 * N, lane, end);
       }
       const float top = fmaxf(fmaxf(p[0].top(), p[1].top()), fmaxf(p[2].top(), p[3].top()));
       if (top > m) {
@@ -545,36 +577,26 @@ beam_kernel(const __grid_constant__ BeamArgs a, int rows) {
     }
     const float best = warp_max(m), last = ceilf(best * kLog2e);
     double sum = best == -INFINITY ? s : rescaled(s, m, shift, best, last);
-    const double base = fabsf(best) < kLarge ? (double)last / (double)kLog2e : (double)best;
+    const double base = fabsf(best) < kLarge ? (double)last * kLn2 : (double)best;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    BeamPart* part = static_cast<BeamPart*>(a.ws) + unit;
+    BeamPart* part = static_cast<BeamPart*>(a.ws) + (long long)local * units + unit;
     part->high[lane] = m;
     if (lane == 0) {
       part->sum = sum;           // NaN where there is one
       part->base = base;
-      part->shift = fabsf(best) < kLarge ? last : NAN;
-    }
-    __syncwarp();
-    if (lane == 0) {
-      const int local = local_row / K;
-      unsigned before;      // releases what the warp has written, acquires what those before it have
-      asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(a.counters + local) : "memory");
-      if (before == (unsigned)(K * a.lists) - 1) {
-        a.counters[local] = 0;
-        done = local;
-      }
+      part->shift = fabsf(best) < kLarge ? last : sum == 0.0 ? -INFINITY : NAN;
     }
   }
-  if (lane == 0) sh.done[warp] = done;
   __syncthreads();
-#pragma unroll 1
-  for (int w = 0; w < kBeamWarps; ++w) {
-    const int local = sh.done[w];
-    if (local < 0) continue;
-    choose<T>(a, sh, local);
-    __syncthreads();
+  if (tid == 0) {
+    unsigned before;      // releases what the CTA has written (the barrier above), acquires what those before it have (the one below)
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(a.counters + local) : "memory");
+    sh.last = before == (unsigned)ctas - 1;
+    if (sh.last) a.counters[local] = 0;
   }
+  __syncthreads();
+  if (sh.last) choose<T>(a, sh, local);
 }
 
 }  // namespace dptb
@@ -607,10 +629,10 @@ extern "C" int dptb_beam_step(const BeamArgs* args, void* stream) {
   auto st = static_cast<cudaStream_t>(stream);
   int launches = 0;
   for (a.first_item = 0; a.first_item < a.items; a.first_item += most, ++launches) {
-    const int r = min(most, a.items - a.first_item) * a.beams;
-    const unsigned grid = (unsigned)(((long long)r * a.lists + kBeamWarps - 1) / kBeamWarps);
-    if (a.f32) beam_kernel<float><<<grid, kBeamThreads, 0, st>>>(a, r);
-    else       beam_kernel<__nv_bfloat16><<<grid, kBeamThreads, 0, st>>>(a, r);
+    const unsigned grid = (unsigned)(min(most, a.items - a.first_item) * up((long long)a.beams * a.lists, kBeamWarps));
+    auto kernel = a.f32 ? a.vec ? beam_kernel<float, true> : beam_kernel<float, false>
+                        : a.vec ? beam_kernel<__nv_bfloat16, true> : beam_kernel<__nv_bfloat16, false>;
+    kernel<<<grid, kBeamThreads, 0, st>>>(a);
   }
   return counted(launches, (int)cudaGetLastError());
 }
