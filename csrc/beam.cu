@@ -12,8 +12,8 @@
 // and the lanes' maxima tell where to look: the best W continuations lie with the lanes of the W largest (each counted with its beam's score),
 // and only these lanes' logits are read once more, by the value of the W-th.  That is a few hundred logits, whatever the vocabulary.
 //
-// Bound by memory for many rows, by a chain of latencies for few.  256 rows of 128256 logits in bf16, 8 beams an item, take 22.5 us, of which the pass is half
-// (66 MB in 11.5 us) and the choice in each item's last CTA the other; four rows of 50257 in fp32 9.4 us, 35 of 321 6.9.  Choosing in every warp, or in CTAs barrier
+// Bound by memory for many rows, by a chain of latencies for few.  256 rows of 128256 logits in bf16, 8 beams an item, take 21.4 us, of which the pass is half
+// (66 MB in 9 to 11 us) and the choice in each item's last CTA the other; four rows of 50257 in fp32 8.9 us, 35 of 321 7.0.  Choosing in every warp, or in CTAs barrier
 // after barrier, cost more than the pass itself: 45 and 61 us for the 256 rows.
 #include <cuda_bf16.h>
 
@@ -28,6 +28,8 @@ constexpr int kWarpPool = 128;         // candidates of a warp that are ranked a
 constexpr int kItemPool = 1024;        // and of an item
 constexpr int kHotLanes = 256;         // lanes whose logits are read again
 constexpr int kMaxLists = 64;          // parts of a row
+constexpr int kHeld = 5;               // times four lanes' maxima that a thread holds where the choice is made
+__host__ __device__ constexpr int mates_of(int beams) { return beams <= 1 ? 8 : beams <= 2 ? 4 : beams <= 4 ? 2 : 1; }      // warps of a row there
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct BeamArgs {
@@ -394,24 +396,23 @@ __device__ __noinline__ void choose(const BeamArgs& a, BeamShared& sh, int local
   const BeamPart* parts = static_cast<const BeamPart*>(a.ws) + (long long)local * K * a.lists;
   const T* rows = static_cast<const T*>(a.logits) + (long long)item * K * a.ld;
   if (tid == 0) sh.count = sh.hots = 0;
-  const int mates = K <= 1 ? 8 : K <= 2 ? 4 : K <= 4 ? 2 : 1, w0 = warp / mates, dw = kBeamWarps / mates;      // warps of a row; rows of this warp
+  const int mates = mates_of(K), w0 = warp / mates, dw = kBeamWarps / mates;      // rows of this warp
   const int quads = a.lists * 8, q0 = (warp - w0 * mates) * 32 + lane, dq = mates * 32;                       // four lanes' maxima at a time
   auto quad = [&](int w, int q) {
     return q < quads ? __ldcg(reinterpret_cast<const float4*>(parts[w * a.lists + (q >> 3)].high) + (q & 7))
                      : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
   };
   auto most_of = [](const float4& v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); };
-  constexpr int H = 4;                  // of them at once
   // The W-th largest of the lanes' maxima, and the lanes that reach it, both in fp32, as x - from + offset, and with room for its roundings:
   // `from` and `offset` are off by 2^-24 of themselves, and so are the two sums.
   float high = -INFINITY;
+  float4 v[kHeld];
 #pragma unroll 1
   for (int w = w0; w < K; w += dw) {
     const float score = a.scores[item * K + w];
     const bool fin = a.finished && a.finished[item * K + w];
-    float4 v[H];                        // on their way while the row is summed up
-#pragma unroll
-    for (int x = 0; x < H; ++x) v[x] = quad(w, q0 + x * dq);
+#pragma unroll                          // on their way while the row is summed up
+    for (int x = 0; x < kHeld; ++x) v[x] = quad(w, q0 + x * dq);
     double top, norm;
     sum_row(parts + w * a.lists, a.lists, top, norm);
     const int kind = !(fabsf(score) < INFINITY) ? 2 : fin ? 1 : fabs(top) < INFINITY && fabs(norm) < INFINITY ? 0 : 2;
@@ -425,9 +426,11 @@ __device__ __noinline__ void choose(const BeamArgs& a, BeamShared& sh, int local
       sh.size[w] = kind ? 0.0f : fabsf(offset) + fminf(fabsf(from), 2.0f * kLarge);
     }
     if (kind == 0) {
-      float most = fmaxf(fmaxf(most_of(v[0]), most_of(v[1])), fmaxf(most_of(v[2]), most_of(v[3])));
+      float most = most_of(v[0]);
+#pragma unroll
+      for (int x = 1; x < kHeld; ++x) most = fmaxf(most, most_of(v[x]));
 #pragma unroll 4
-      for (int q = q0 + H * dq; q < quads; q += dq) most = fmaxf(most, most_of(quad(w, q)));
+      for (int q = q0 + kHeld * dq; q < quads; q += dq) most = fmaxf(most, most_of(quad(w, q)));
       high = fmaxf(high, most - from + offset);
     } else if (q0 < min(K, a.vocab)) {
       high = fmaxf(high, kind == 1 && a.eos >= 0 && q0 == 0 ? score : -INFINITY);
@@ -457,13 +460,14 @@ __device__ __noinline__ void choose(const BeamArgs& a, BeamShared& sh, int local
       sh.least[w] = least;
       if (high < limit) continue;                               // none of this thread's, in any row
 #pragma unroll 1
-      for (int q = q0; q < quads; q += 4 * dq) {
-        float4 v[4];
+      for (int q = q0; q < quads; q += kHeld * dq) {
+        if (K > dw || quads > kHeld * dq) {                           // (else this thread still has them)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) v[x] = quad(w, q + x * dq);
+          for (int x = 0; x < kHeld; ++x) v[x] = quad(w, q + x * dq);
+        }
         unsigned mine = 0;
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
+        for (int x = 0; x < kHeld; ++x)
           mine |= ((v[x].x - from >= least) | (v[x].y - from >= least) << 1 | (v[x].z - from >= least) << 2 | (v[x].w - from >= least) << 3) << 4 * x;
 #pragma unroll 1
         for (; mine; mine &= mine - 1) {
@@ -476,7 +480,7 @@ __device__ __noinline__ void choose(const BeamArgs& a, BeamShared& sh, int local
     const int hots = sh.hots;
     if (hots <= kHotLanes) {
       // A hot lane's pieces by as many lanes as there are pieces.
-      const int pieces = min(32, (min(a.chunk, a.vocab) + 32 * N - 1) / (32 * N)), width = pieces > 1 ? 1 << (32 - __clz(pieces - 1)) : 1;
+      const int pieces = min(32, (min(a.chunk, a.vocab) + 32 * N - 1) / (32 * N)), width = pieces > 2 ? 1 << (31 - __clz(pieces - 1)) : 1;
 #pragma unroll 1
       for (int h = tid / width; h < hots; h += kBeamThreads / width) {
         const int j = sh.hot[h], part = j >> 5, w = part / a.lists;
@@ -484,21 +488,23 @@ __device__ __noinline__ void choose(const BeamArgs& a, BeamShared& sh, int local
         const int begin = (part - w * a.lists) * a.chunk, end = min(a.vocab, begin + a.chunk);
         const float from = sh.from[w], least = sh.least[w];
 #pragma unroll 1
-        for (int i = begin + 32 * (tid & (width - 1)) * N; i < end; i += width * 32 * N) {
-          const Piece<T> p = a.vec ? load_group<T, true>(row, i, j & 31, end) : load_group<T, false>(row, i, j & 31, end);
+        for (int i0 = begin + 32 * (tid & (width - 1)) * N; i0 < end; i0 += 2 * width * 32 * N) {
+          const int i1 = i0 + width * 32 * N;
+          const Piece<T> p[2] = {a.vec ? load_group<T, true>(row, i0, j & 31, end) : load_group<T, false>(row, i0, j & 31, end),
+                                 a.vec ? load_group<T, true>(row, i1, j & 31, end) : load_group<T, false>(row, i1, j & 31, end)};
           unsigned mine = 0;
 #pragma unroll
-          for (int e = 0; e < N; ++e) mine |= (unsigned)(p.at(e) - from >= least) << e;
+          for (int e = 0; e < 2 * N; ++e) mine |= (unsigned)(p[e / N].at(e % N) - from >= least) << e;
 #pragma unroll 1
           for (; mine; mine &= mine - 1) {
             const int e = __ffs(mine) - 1;
-            float x = p.at(0);
+            float x = p[0].at(0);
 #pragma unroll
-            for (int n = 1; n < N; ++n) x = e == n ? p.at(n) : x;
+            for (int n = 1; n < 2 * N; ++n) x = e == n ? p[n / N].at(n % N) : x;
             const int at = atomicAdd(&sh.count, 1);
             if (at < kItemPool) {
               sh.totals[at] = total_of(sh, w, x);
-              sh.keys[at] = (unsigned long long)w << 32 | (unsigned)place_in<T>(i, j & 31, e, a.vec);
+              sh.keys[at] = (unsigned long long)w << 32 | (unsigned)place_in<T>(e < N ? i0 : i1, j & 31, e & (N - 1), a.vec);
             }
           }
         }
@@ -617,6 +623,10 @@ extern "C" int dptb_beam_step(const BeamArgs* args, void* stream) {
   long long chunk = max(up((long long)a.vocab * rows, warps), 4LL * unit);
   chunk = min(chunk, up(a.vocab, 4));
   chunk = max(chunk, up(a.vocab, most_lists));
+  // A little more if a row's maxima then fit the choice's registers (four rows of 50257 in fp32 9.6 us in 50 parts, 8.9 in 33); not at the price of many
+  // more rounds in a row.
+  const long long held = up(a.vocab, 4 * kHeld * mates_of(a.beams));
+  if (a.beams <= kBeamWarps && held <= 12 * unit) chunk = max(chunk, held);
   chunk = up(chunk, chunk >= 4 * unit ? 4 * unit : unit) * (chunk >= 4 * unit ? 4 * unit : unit);
   a.chunk = (int)chunk;
   a.lists = (int)((a.vocab + chunk - 1) / chunk);
