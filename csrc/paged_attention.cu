@@ -25,7 +25,7 @@
 //
 // Device time on B200, pages of 16 tokens in random order: bf16, 32 heads of 128 on 8: four sequences of 65000 to 131072 keys 242 us (6.6 TB/s, the
 // rate of a plain copy), 32 sequences of 1 to 4096 53.5 us (5.0 TB/s; its floor is 41), 32 of 2048 52 us, one of 2048 15 us.  One sequence
-// of 65 keys, 12 heads of 64: 6.5 us.  fp32, 13 sequences of up to 1531 keys, 10 heads of 80 on 5: 18.2 us; 32 of 2048, 32 heads of 128 on 8:
+// of 65 keys, 12 heads of 64: 6.5 us.  fp32, 13 sequences of up to 1531 keys, 10 heads of 80 on 5: 16.6 us; 32 of 2048, 32 heads of 128 on 8:
 // 105 us.  Filled element by element the 32 sequences of 2048 keys take 180 us in bf16 and 186 us in fp32, the one of 65 keys 9 us.
 #include <cuda_bf16.h>
 
@@ -277,7 +277,7 @@ struct Bf16Round {
 // A round's products leave NJ GP sums of 8 lanes each (head, step).  They are added in halves: with every exchange a lane keeps half of its sums, so that
 // in the end it has one or a few of one head, for which it alone keeps maximum and sum and takes the exponentials; the weights go
 // back to the lanes by shuffle.  Multiply-adds are packed in pairs.  With every sum in every lane, and single multiply-adds, 13 sequences of up to
-// 1531 keys (10 heads of 80 on 5) took 22 us, now 18.  Rounds of 16 keys for heads of up to 64 features (16 sequences of 4096 keys: 65 us with 8, 51 with
+// 1531 keys (10 heads of 80 on 5) took 22 us, 18 so.  Rounds of 16 keys for heads of up to 64 features (16 sequences of 4096 keys: 65 us with 8, 51 with
 // 16), of 8 above.
 template <int HD, int GP, int NJ>
 struct F32Round {
@@ -998,14 +998,17 @@ extern "C" int dptb_paged_attention(const PagedAttnArgs* args, void* stream) {
     if (a.hd <= 128) DPTB_PAGED(Bf16Round<128, 2, 1>, 6, 2);
     DPTB_PAGED(Bf16Round<256, 1, 1>, 4, 2);
   }
-#define DPTB_PAGED_GROUP(HD, NJ, W) \
+  // Eight warps, fewer where registers or shared memory hold no more; twelve and ten where a round is short, 6 KB (16 sequences of 2048 keys, 8 kv heads
+  // of 80: 44 us with eight, 37 with twelve; group of four 53 and 50 with ten).  Of 8 KB rounds eight warps have enough in flight: heads of 128,
+  // 64 sequences of 500 keys, 71 us, 73 with eleven.
+#define DPTB_PAGED_GROUP(HD, NJ, W, W4) \
   if (group == 1) DPTB_PAGED(F32Round<HD, 1, NJ>, W, 2); \
   if (group == 2) DPTB_PAGED(F32Round<HD, 2, NJ>, W, 2); \
-  if (group <= 4) DPTB_PAGED(F32Round<HD, 4, NJ>, W, 2)
-  if (a.hd <= 64) { DPTB_PAGED_GROUP(64, 4, 8); DPTB_PAGED(F32Round<64, 8, 4>, 8, 2); }
-  if (a.hd <= 96) { DPTB_PAGED_GROUP(96, 2, 8); DPTB_PAGED(F32Round<96, 8, 2>, 8, 2); }
-  if (a.hd <= 128) { DPTB_PAGED_GROUP(128, 2, 8); DPTB_PAGED(F32Round<128, 8, 2>, 7, 2); }
-  DPTB_PAGED_GROUP(256, 2, 4);
+  if (group <= 4) DPTB_PAGED(F32Round<HD, 4, NJ>, W4, 2)
+  if (a.hd <= 64) { DPTB_PAGED_GROUP(64, 4, 8, 8); DPTB_PAGED(F32Round<64, 8, 4>, 8, 2); }
+  if (a.hd <= 96) { DPTB_PAGED_GROUP(96, 2, 12, 10); DPTB_PAGED(F32Round<96, 8, 2>, 8, 2); }
+  if (a.hd <= 128) { DPTB_PAGED_GROUP(128, 2, 8, 8); DPTB_PAGED(F32Round<128, 8, 2>, 7, 2); }
+  DPTB_PAGED_GROUP(256, 2, 4, 4);
   DPTB_PAGED(F32Round<256, 4, 2>, 4, 2);
 #undef DPTB_PAGED_GROUP
 #undef DPTB_PAGED
