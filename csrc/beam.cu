@@ -467,8 +467,9 @@ __device__ __noinline__ void choose(const BeamArgs& a, BeamShared& sh, int local
         }
         unsigned mine = 0;
 #pragma unroll
-        for (int x = 0; x < kHeld; ++x)
-          mine |= ((v[x].x - from >= least) | (v[x].y - from >= least) << 1 | (v[x].z - from >= least) << 2 | (v[x].w - from >= least) << 3) << 4 * x;
+        for (int x = 0; x < kHeld; ++x)            // (`least` may be -inf, which the places behind a row's maxima reach)
+          if (q + x * dq < quads)
+            mine |= ((v[x].x - from >= least) | (v[x].y - from >= least) << 1 | (v[x].z - from >= least) << 2 | (v[x].w - from >= least) << 3) << 4 * x;
 #pragma unroll 1
         for (; mine; mine &= mine - 1) {
           const int at = atomicAdd(&sh.hots, 1), i = __ffs(mine) - 1;
@@ -494,7 +495,8 @@ __device__ __noinline__ void choose(const BeamArgs& a, BeamShared& sh, int local
                                  a.vec ? load_group<T, true>(row, i1, j & 31, end) : load_group<T, false>(row, i1, j & 31, end)};
           unsigned mine = 0;
 #pragma unroll
-          for (int e = 0; e < 2 * N; ++e) mine |= (unsigned)(p[e / N].at(e % N) - from >= least) << e;
+          for (int e = 0; e < 2 * N; ++e)
+            mine |= (unsigned)(p[e / N].at(e % N) - from >= least && place_in<T>(e < N ? i0 : i1, j & 31, e % N, a.vec) < end) << e;
 #pragma unroll 1
           for (; mine; mine &= mine - 1) {
             const int e = __ffs(mine) - 1;

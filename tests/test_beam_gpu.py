@@ -46,6 +46,20 @@ def test_ties_go_to_the_first(dtype, vocab):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab,pad", [(127, 3), (128, 0), (9000, 0), (9001, 2)])
+@pytest.mark.parametrize("beams", [3, 8, 9])
+def test_fewer_tokens_than_beams_above_the_lowest_value(dtype, vocab, pad, beams):
+    """What has to be reached lies below the lowest fp32 value then."""
+    logits = torch.full((2 * beams, vocab + pad), torch.finfo(dtype).min, dtype=dtype, device="cuda")[:, :vocab]
+    logits[:, vocab // 3], logits[:, vocab - 2] = 17.0, 12.0
+    scores = torch.full((2, beams), -INF, device="cuda")
+    scores[:, 0] = torch.tensor([0.0, -1.0e30], device="cuda")
+    finished = torch.arange(2 * beams, device="cuda").view(2, beams) % 3 == 2
+    agree(ops.beam_step(logits, scores), oracle.beam(logits, scores, None, -1))
+    agree(ops.beam_step(logits, scores, finished, 5), oracle.beam(logits, scores, finished, 5))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("vocab", [12, 9000])
 def test_masked_and_broken_rows(dtype, vocab):
     logits, scores, finished = data(2, 6, vocab, dtype, 1)
