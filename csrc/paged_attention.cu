@@ -111,6 +111,7 @@ struct Cursor {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kTiny = 1.2e-38f;
 constexpr int kMaxHeadDim = 256;
+constexpr int kAlone = 2;          // rounds of a warp that a join across CTAs costs
 
 // ------------------------------------------------------------------------------------------------------------ bf16
 // HD: features of a head, padded with zeros; NT: tiles of 8 query heads; M: times 16 keys a round (two for heads of up to 64 features: a
@@ -703,7 +704,7 @@ paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_con
   unsigned char* queries = reinterpret_cast<unsigned char*>(leads + W * kPart);   // [W][S] jobs' queries
   int* before = reinterpret_cast<int*>(queries + W * S * R::kQueryBytes);   // [rows + 1]: units of a kv head ahead of a row
   unsigned char* tails = reinterpret_cast<unsigned char*>(before + a.rows + 1);   // [rows]: tokens of a row's last round
-  __shared__ int scan[W + 1];
+  __shared__ int scan[W], most[W];
   __shared__ Parts<W> sh;
   __shared__ uint64_t landed[W * S];
   __shared__ int aborted;
@@ -715,17 +716,15 @@ paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_con
   // Units ahead of every row: a job is its rounds and, before them, one unit for what it costs to begin and end it (2100 cycles where a round took
   // 2500; without it the warps of the shortest rows came last by a quarter).
   auto length = [&](int r) { return max(0, min(a.lens[r], room)); };
-  bool equal = true;
-  int rounds0;
+  bool alone;                  // a job a CTA
   {
     const int each = (a.rows + W * 32 - 1) / (W * 32), r0 = min(a.rows, tid * each), r1 = min(a.rows, r0 + each);
-    int mine = 0;
-    rounds0 = (length(0) + R::kKeys - 1) / R::kKeys;
+    int mine = 0, longest = 0;
     for (int r = r0; r < r1; ++r) {
       const int n = a.lens[r], k = (max(0, min(n, room)) + R::kKeys - 1) / R::kKeys;
       if (n > room && blockIdx.x == 0) report_error(kBadPage);
       mine += k + (k > 0);
-      equal = equal && k == rounds0;
+      longest = max(longest, k);
     }
     int s = mine;
 #pragma unroll
@@ -734,7 +733,18 @@ paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_con
       if (lane >= o) s += u;
     }
     if (lane == 31) scan[warp] = s;
+    const bool few = a.rows * tiles <= gridDim.x;
+    if (few) {
+      longest = __reduce_max_sync(0xffffffffu, longest);
+      if (lane == 0) most[warp] = longest;
+    }
     __syncthreads();
+    int sum = 0, top = 0;
+    for (int w = 0; w < W; ++w) {
+      sum += scan[w];
+      if (few) top = max(top, most[w]);
+    }
+    alone = few && (top + W - 1) / W <= (int)(((unsigned)(sum * tiles) + W * gridDim.x - 1) / (W * gridDim.x)) + kAlone;
     int at = s - mine;
     for (int w = 0; w < warp; ++w) at += scan[w];
     for (int r = r0; r < r1; ++r) {
@@ -743,11 +753,7 @@ paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_con
       tails[r] = n - (n - 1) / R::kKeys * R::kKeys;
       at += (n + R::kKeys - 1) / R::kKeys + (n > 0);
     }
-    if (tid == 0) {
-      int t = 0;
-      for (int w = 0; w < W; ++w) t += scan[w];
-      before[a.rows] = t;
-    }
+    if (tid == 0) before[a.rows] = sum;
     if (tid < 2 * W) sh.job[tid] = -1;
     if (tid < 2) sh.shared[tid] = -1;
     if (a.hd < R::kHD)
@@ -756,15 +762,19 @@ paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_con
     if (tid < W * S) mbar_init(landed + tid, 1);
     if (tid == 0) aborted = 0;
     mbar_fence_init();
-    equal = __syncthreads_and(equal);
+    __syncthreads();
   }
   const int total = before[a.rows] * tiles;                    // (below 2^31: the launcher sees to it)
-  // A CTA takes a unit for each of its warps at least: parts of one CTA are joined sooner than those of several.  Whole jobs, where all
-  // are as long and short enough that each CTA still has its own at once (one sequence of 250 keys, 32 heads of 128 on 8: 9.1 us, dealt out 11.4;
-  // of 65 keys, 12 heads of 64: 6.6 and 7.2).
-  int share = max(W, (int)((unsigned)(total + gridDim.x - 1) / gridDim.x));
-  if (equal && rounds0 > 0 && rounds0 <= 2 * W && a.rows * tiles <= gridDim.x) share = rounds0 + 1;
-  const int begin = (int)min((long long)total, (long long)share * blockIdx.x), end = min(total, begin + share);
+  // A CTA takes a unit for each of its warps at least: parts of one CTA are joined sooner than those of several.  So a CTA takes a job, if there are no more of
+  // them than CTAs and the longest keeps its warps for at most two rounds more than a share would (32 heads of 128 on 8, 16 sequences of 250 keys:
+  // 10.8 us, shared 14.3; of 2000 keys 29.8 and 32.9; with five rounds more, 4 sequences of 800 keys take 16.3 instead of 14).
+  const int share = max(W, (int)((unsigned)(total + gridDim.x - 1) / gridDim.x));
+  int begin = (int)min((long long)total, (long long)share * blockIdx.x), end = min(total, begin + share);
+  if (alone) {
+    const int row = min((int)blockIdx.x / tiles, a.rows), units = row < a.rows ? before[row + 1] - before[row] : 0;
+    begin = before[row] * tiles + ((int)blockIdx.x - row * tiles) * units;
+    end = begin + units;
+  }
   for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {       // rows of no tokens
     if (before[r + 1] > before[r]) continue;
     for (int x = tid; x < a.heads * a.hd; x += W * 32) static_cast<T*>(a.o)[r * a.o_row + x / a.hd * a.o_head + x % a.hd] = from_f32<T>(0.0f);
