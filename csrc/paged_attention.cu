@@ -25,7 +25,7 @@
 //
 // Device time on B200, pages of 16 tokens in random order: bf16, 32 heads of 128 on 8: four sequences of 65000 to 131072 keys 242 us (6.6 TB/s, the
 // rate of a plain copy), 32 sequences of 1 to 4096 53.5 us (5.0 TB/s; its floor is 41), 32 of 2048 52 us, one of 2048 15 us.  One sequence
-// of 65 keys, 12 heads of 64: 6.5 us.  fp32, 13 sequences of up to 1531 keys, 10 heads of 80 on 5: 16.6 us; 32 of 2048, 32 heads of 128 on 8:
+// of 65 keys, 12 heads of 64: 6.5 us.  fp32, 13 sequences of up to 1531 keys, 10 heads of 80 on 5: 17.2 us; 32 of 2048, 32 heads of 128 on 8:
 // 105 us.  Filled element by element the 32 sequences of 2048 keys take 180 us in bf16 and 186 us in fp32, the one of 65 keys 9 us.
 #include <cuda_bf16.h>
 
@@ -111,7 +111,7 @@ struct Cursor {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kTiny = 1.2e-38f;
 constexpr int kMaxHeadDim = 256;
-constexpr int kAlone = 2;          // rounds of a warp that a join across CTAs costs
+constexpr int kAlone = 2, kSnap = 3;      // rounds of a warp that may be had for no joins across CTAs
 
 // ------------------------------------------------------------------------------------------------------------ bf16
 // HD: features of a head, padded with zeros; NT: tiles of 8 query heads; M: times 16 keys a round (two for heads of up to 64 features: a
@@ -716,7 +716,7 @@ paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_con
   // Units ahead of every row: a job is its rounds and, before them, one unit for what it costs to begin and end it (2100 cycles where a round took
   // 2500; without it the warps of the shortest rows came last by a quarter).
   auto length = [&](int r) { return max(0, min(a.lens[r], room)); };
-  bool alone;                  // a job a CTA
+  bool alone, snap, single;    // a job a CTA; CTAs of whole jobs; jobs of a round each
   {
     const int each = (a.rows + W * 32 - 1) / (W * 32), r0 = min(a.rows, tid * each), r1 = min(a.rows, r0 + each);
     int mine = 0, longest = 0;
@@ -733,17 +733,17 @@ paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_con
       if (lane >= o) s += u;
     }
     if (lane == 31) scan[warp] = s;
-    const bool few = a.rows * tiles <= gridDim.x;
-    if (few) {
-      longest = __reduce_max_sync(0xffffffffu, longest);
-      if (lane == 0) most[warp] = longest;
-    }
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    if (lane == 0) most[warp] = longest;
     __syncthreads();
     int sum = 0, top = 0;
     for (int w = 0; w < W; ++w) {
       sum += scan[w];
-      if (few) top = max(top, most[w]);
+      top = max(top, most[w]);
     }
+    const bool few = a.rows * tiles <= gridDim.x;
+    snap = !few && top <= kSnap * W;
+    single = top <= 1;
     alone = few && (top + W - 1) / W <= (int)(((unsigned)(sum * tiles) + W * gridDim.x - 1) / (W * gridDim.x)) + kAlone;
     int at = s - mine;
     for (int w = 0; w < warp; ++w) at += scan[w];
@@ -765,15 +765,35 @@ paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_con
     __syncthreads();
   }
   const int total = before[a.rows] * tiles;                    // (below 2^31: the launcher sees to it)
+  auto row_of = [&](int unit) {        // the last row with no more units ahead, which has some itself; a warp looks at 32 at a time
+    int row = 0;
+    for (int n = a.rows; n > 1;) {
+      const int step = (n + 31) / 32, at = lane * step;
+      const int skip = (__popc(__ballot_sync(0xffffffffu, at < n && before[min(row + at, a.rows)] * tiles <= unit)) - 1) * step;
+      row += skip;
+      n = min(step, n - skip);
+    }
+    return row;
+  };
   // A CTA takes a unit for each of its warps at least: parts of one CTA are joined sooner than those of several.  So a CTA takes a job, if there are no more of
   // them than CTAs and the longest keeps its warps for at most two rounds more than a share would (32 heads of 128 on 8, 16 sequences of 250 keys:
-  // 10.8 us, shared 14.3; of 2000 keys 29.8 and 32.9; with five rounds more, 4 sequences of 800 keys take 16.3 instead of 14).
-  const int share = max(W, (int)((unsigned)(total + gridDim.x - 1) / gridDim.x));
+  // 10.8 us, shared 14.3; of 2000 keys 29.8 and 32.9; with five rounds more, 4 sequences of 800 keys take 16.3 instead of 14).  If there are more jobs and
+  // all are short, a CTA takes those that begin in its share (32 sequences of up to 250 keys: 14.3 and 17.1; 1024 of 250, 8 heads on 2: 55 and 61).
+  int share = max(W, (int)((unsigned)(total + gridDim.x - 1) / gridDim.x));
+  if (single) share += share & 1;                              // two units each: no job is cut
   int begin = (int)min((long long)total, (long long)share * blockIdx.x), end = min(total, begin + share);
   if (alone) {
     const int row = min((int)blockIdx.x / tiles, a.rows), units = row < a.rows ? before[row + 1] - before[row] : 0;
     begin = before[row] * tiles + ((int)blockIdx.x - row * tiles) * units;
     end = begin + units;
+  } else if (snap && !single) {
+    auto start_of_job = [&](int unit) {                        // at `unit` or after it
+      if (unit >= total) return total;
+      const int row = row_of(unit), units = before[row + 1] - before[row], first = before[row] * tiles;
+      return first + (unit - first + units - 1) / units * units;
+    };
+    begin = start_of_job(begin);
+    end = start_of_job(end);
   }
   for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {       // rows of no tokens
     if (before[r + 1] > before[r]) continue;
@@ -786,15 +806,7 @@ paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_con
     unsigned char* ring = rings + warp * S * R::kBytes;
     uint64_t* bars = landed + warp * S;
     unsigned char* my_queries = queries + warp * S * R::kQueryBytes;
-    int row = 0;
-    {
-      int hi = a.rows - 1;                                     // the last row with no more units ahead than w0, which has some itself
-      while (row < hi) {
-        const int mid = (row + hi + 1) / 2;
-        if (before[mid] * tiles <= w0) row = mid;
-        else hi = mid - 1;
-      }
-    }
+    const int row = row_of(w0);
     const int n0 = before[row + 1] - before[row] - 1, rem = w0 - before[row] * tiles, vh0 = rem / (n0 + 1), u0 = rem - vh0 * (n0 + 1);
     Cursor c{row, vh0, max(u0 - 1, 0), n0, head_tiles == 1 ? vh0 : vh0 / head_tiles, w0 + (u0 == 0)}, ahead = c;
     auto advance = [&](Cursor& x) {
