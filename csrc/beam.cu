@@ -12,8 +12,8 @@
 // and the lanes' maxima tell where to look: the best W continuations lie with the lanes of the W largest (each counted with its beam's score),
 // and only these lanes' logits are read once more, by the value of the W-th.  That is a few hundred logits, whatever the vocabulary.
 //
-// Bound by memory for many rows, by a chain of latencies for few.  256 rows of 128256 logits in bf16, 8 beams an item, take 21.4 us, of which the pass is half
-// (66 MB in 9 to 11 us) and the choice in each item's last CTA the other; four rows of 50257 in fp32 8.9 us, 35 of 321 7.0.  Choosing in every warp, or in CTAs barrier
+// Bound by memory for many rows, by a chain of latencies for few.  256 rows of 128256 logits in bf16, 8 beams an item, take 22 us, of which the pass is half
+// (66 MB in 9 to 11 us) and the choice in each item's last CTA the other; four rows of 50257 in fp32 9.2 us, 35 of 321 7.2.  Choosing in every warp, or in CTAs barrier
 // after barrier, cost more than the pass itself: 45 and 61 us for the 256 rows.
 #include <cuda_bf16.h>
 
@@ -183,7 +183,7 @@ __device__ __forceinline__ Piece<T> load_group(const T* row, int first, int lane
 // What a warp leaves of its logits: the sum of exponentials, what it is relative to, every lane's maximum.
 struct BeamPart {
   double sum, base;
-  float shift, pad[3];           // `base` in whole powers of two, NaN where it is none
+  float shift, best, pad[2];     // `base` in whole powers of two, NaN where it is none; the largest logit
   float high[32];
 };
 
@@ -381,27 +381,26 @@ __device__ __noinline__ void best_of_rows(const BeamArgs& a, BeamShared& sh, con
   __syncthreads();
 }
 
-// The sum of a row's parts: what its logits are taken relative to, and the logarithm of the sum (not finite: no distribution).
+// The sum of a row's parts: what its logits are taken relative to, and the logarithm of the sum (not finite: no distribution).  The largest logit's own
+// term is taken out as it was put in and stands for 1, so that a row of one token is worth nothing but its score and no row more.
 __device__ __forceinline__ void sum_row(const BeamPart* p, int lists, double& top, double& norm) {
   const int lane = threadIdx.x & 31;
   double base[2], sum[2], t = 0.0;
-  float shift[2];
+  float shift[2], best[2];
 #pragma unroll
   for (int x = 0; x < 2; ++x) {          // (kMaxLists)
     const bool in = lane + 32 * x < lists;
     base[x] = in ? __ldcg(&p[lane + 32 * x].base) : -INFINITY;
     sum[x] = in ? __ldcg(&p[lane + 32 * x].sum) : 0.0;
     shift[x] = in ? __ldcg(&p[lane + 32 * x].shift) : -INFINITY;
+    best[x] = in ? __ldcg(&p[lane + 32 * x].best) : -INFINITY;
   }
+  const float m = warp_max(fmaxf(best[0], best[1])), most = ceilf(m * kLog2e);      // (`most` is the largest shift)
   if (__any_sync(0xffffffffu, shift[0] != shift[0] || shift[1] != shift[1])) {
-    top = fmax(base[0], base[1]);
+    const double to = fabsf(m) < kLarge ? (double)most * kLn2 : (double)m;
 #pragma unroll 1
-    for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
-#pragma unroll 1
-    for (int x = 0; x < 2; ++x) t += sum[x] == 0.0 ? 0.0 : sum[x] * exp(base[x] - top);
+    for (int x = 0; x < 2; ++x) t += sum[x] == 0.0 ? 0.0 : sum[x] * exp(base[x] - to);
   } else {
-    const float most = warp_max(fmaxf(shift[0], shift[1]));
-    top = (double)most * kLn2;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       const float down = fminf(most - shift[x], 1000.0f);
@@ -410,6 +409,8 @@ __device__ __forceinline__ void sum_row(const BeamPart* p, int lists, double& to
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  if (fabsf(m) < kLarge) t = (t - (double)exp2_fast(fmaf(m, kLog2e, -most))) * exp((double)most * kLn2 - (double)m) + 1.0;
+  top = m;
   norm = log(t);
 }
 
@@ -643,6 +644,7 @@ beam_kernel(const __grid_constant__ BeamArgs a) {
     part->high[lane] = m;
     if (lane == 0) {
       part->sum = sum;           // NaN where there is one
+      part->best = best;
       part->base = base;
       part->shift = fabsf(best) < kLarge ? last : sum == 0.0 ? -INFINITY : NAN;
     }

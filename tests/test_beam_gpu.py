@@ -60,6 +60,23 @@ def test_fewer_tokens_than_beams_above_the_lowest_value(dtype, vocab, pad, beams
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("mask", ["-inf", "lowest"])
+@pytest.mark.parametrize("vocab", [9, 321, 50257, 128256])
+def test_a_token_without_choice_costs_nothing(dtype, mask, vocab):
+    """Rows of one token keep their scores to the bit, and beams of equal scores their order; no score grows."""
+    beams = 6
+    logits = torch.full((beams, vocab), -INF if mask == "-inf" else torch.finfo(dtype).min, device="cuda", dtype=dtype)
+    only = torch.tensor([vocab - 1, 0, 7, vocab // 2, 3, vocab // 3], device="cuda")
+    logits[torch.arange(beams, device="cuda"), only] = torch.tensor([0.3, -7.7, 17.3, 1e-3, -41.0, 1e4], device="cuda").to(dtype)
+    for scores in (torch.full((1, beams), -0.7, device="cuda"), -torch.arange(beams, device="cuda").view(1, beams).float() / 3):
+        got, parents, tokens, _ = ops.beam_step(logits, scores)
+        assert torch.equal(got, scores) and parents[0].tolist() == list(range(beams)) and tokens[0].tolist() == only.tolist()
+    g = torch.Generator().manual_seed(vocab)
+    peaked = (torch.randn(beams, vocab, generator=g) * 30).to(dtype).cuda()
+    assert bool((ops.beam_step(peaked, torch.zeros(1, beams, device="cuda"))[0] <= 0).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("vocab", [12, 9000])
 def test_masked_and_broken_rows(dtype, vocab):
     logits, scores, finished = data(2, 6, vocab, dtype, 1)
