@@ -511,6 +511,15 @@ static int launch_page_kernel(void (*kernel)(KArgs...), SmemLimit& limit, int ro
 }
 
 // pool[o, dst[i]] = pool[o, src[i]] for every o < outer and every i with a src, `bytes` a page.  Nobody's dst is somebody's src.
+struct CopyArgs {
+  void* pool;
+  const int* src;
+  const int* dst;
+  long long outer, bytes;
+  int n, pages;
+};
+static_assert(sizeof(CopyArgs) == 48, "packed by the caller");
+
 constexpr int kCopyThreads = 256;
 template <typename V>
 __global__ void __launch_bounds__(kCopyThreads)
@@ -572,16 +581,16 @@ extern "C" int dptb_compact_pages(const CompactArgs* args, void* stream) {
   return launch_page_kernel(compact_pages_kernel, limit, a.rows, 3 * (size_t)words * 4, static_cast<cudaStream_t>(stream), a, words);
 }
 
-extern "C" int dptb_copy_pages(void* pool, const int* src, const int* dst, int n, long long outer, int pages, long long bytes,
-                               void* stream) {
-  if (n == 0 || outer == 0 || bytes == 0) return 0;
-  if (n < 0 || outer < 0 || outer > 65535 || pages < 0 || bytes < 0 || bytes > 0x7fffffff) return kErrBadShape;
-  const dim3 grid(n < 8 * 148 ? n : 8 * 148, (unsigned)outer);
+extern "C" int dptb_copy_pages(const CopyArgs* args, void* stream) {
+  const CopyArgs& a = *args;
+  if (a.n == 0 || a.outer == 0 || a.bytes == 0) return 0;
+  if (a.n < 0 || a.outer < 0 || a.outer > 65535 || a.pages < 0 || a.bytes < 0 || a.bytes > 0x7fffffff) return kErrBadShape;
+  const dim3 grid(a.n < 8 * 148 ? a.n : 8 * 148, (unsigned)a.outer);
   auto st = static_cast<cudaStream_t>(stream);
-  auto* p = static_cast<unsigned char*>(pool);
-  if (((reinterpret_cast<uintptr_t>(pool) | (uintptr_t)bytes) & 15) == 0)
-    copy_pages_kernel<uint4><<<grid, kCopyThreads, 0, st>>>(p, src, dst, n, pages, bytes);
+  auto* p = static_cast<unsigned char*>(a.pool);
+  if (((reinterpret_cast<uintptr_t>(p) | (uintptr_t)a.bytes) & 15) == 0)
+    copy_pages_kernel<uint4><<<grid, kCopyThreads, 0, st>>>(p, a.src, a.dst, a.n, a.pages, a.bytes);
   else
-    copy_pages_kernel<unsigned short><<<grid, kCopyThreads, 0, st>>>(p, src, dst, n, pages, bytes);
+    copy_pages_kernel<unsigned short><<<grid, kCopyThreads, 0, st>>>(p, a.src, a.dst, a.n, a.pages, a.bytes);
   return counted(1, (int)cudaGetLastError());
 }

@@ -23,7 +23,7 @@ import torch
 from .. import _native as N
 from . import kernels
 
-c_void_p, c_int, c_ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
+c_void_p, c_int = ctypes.c_void_p, ctypes.c_int
 _current_device, _raw_stream, _increment_version = None, None, torch._C._increment_version
 if torch.cuda.is_available():
     _current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
@@ -41,6 +41,7 @@ _ATTN_ARGS = struct.Struct("6P 11q 8i f4x Pq P iII4x")
 _APPEND_ARGS = struct.Struct("8P 8q 10i d")
 _FORK_ARGS = struct.Struct("9P q 6i")
 _COMPACT_ARGS = struct.Struct("5P q 3i4x")
+_COPY_ARGS = struct.Struct("3P 2q 2i")
 
 _declared = False
 
@@ -49,11 +50,9 @@ def _lib():
     global _declared
     lib = N.load()
     if not _declared:
-        for name in ("dptb_paged_attention", "dptb_paged_append", "dptb_fork_pages", "dptb_compact_pages"):
+        for name in ("dptb_paged_attention", "dptb_paged_append", "dptb_fork_pages", "dptb_compact_pages", "dptb_copy_pages"):
             fn = getattr(lib, name)
             fn.argtypes, fn.restype = [ctypes.c_char_p, c_void_p], c_int
-        lib.dptb_copy_pages.argtypes = [c_void_p, c_void_p, c_void_p, c_int, c_ll, c_int, c_ll, c_void_p]
-        lib.dptb_copy_pages.restype = c_int
         _declared = True
     return lib
 
@@ -438,8 +437,9 @@ def copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None
         return
     if outer > 65535:
         raise ValueError(f"copy_pages: at most 65535 pools at once, got {outer}")
-    N.check(_lib().dptb_copy_pages(pool.data_ptr(), src.data_ptr(), dst.data_ptr(), src.shape[0], outer, pages,
-                                   shape[-3] * shape[-2] * shape[-1] * pool.element_size(), _raw_stream(dev)), "copy_pages")
+    N.check(_lib().dptb_copy_pages(_COPY_ARGS.pack(
+        pool.data_ptr(), src.data_ptr(), dst.data_ptr(), outer, shape[-3] * shape[-2] * shape[-1] * pool.element_size(),
+        src.shape[0], pages), _raw_stream(dev)), "copy_pages")
     _increment_version((pool,))
 
 

@@ -430,7 +430,7 @@ def test_pools_beyond_32_bits():
     qkv = torch.randn(2, 6 * hd, device="cuda").bfloat16()
     ops.paged_append(qkv, k, v, table, torch.tensor([191, 0], dtype=torch.int32, device="cuda"), 4, rotary_dim=0)
     assert torch.equal(k[pages - 3, 0, 63], qkv[0, 4 * hd:5 * hd]) and torch.equal(v[pages - 2, 0, 0], qkv[1, 5 * hd:])
-    odd = k.view(-1)[1:1 + (pages - 1) * page * hd].view(pages - 1, 1, page, hd)          # off 16 bytes: the other kernel
+    odd = k.view(-1)[1:1 + (pages - 1) * page * hd].view(pages - 1, 1, page, hd)          # off 16 bytes: filled element by element
     odd[pages - 2] = torch.randn(1, page, hd, device="cuda").bfloat16()
     last, n = torch.full((2, 1), pages - 2, dtype=torch.int32, device="cuda"), torch.tensor([64, 9], dtype=torch.int32, device="cuda")
     got = ops.paged_attention(q, odd, odd, last, n).float()
