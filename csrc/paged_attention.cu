@@ -6,7 +6,8 @@
 // length zero gives zeros.  Positions from lens[r] on are never read as numbers: what lies there may be anything.  A page number
 // outside the pool hides its keys and records kBadPage in the status word, which the host turns into an exception.
 //
-// paged_attention_kernel reads every key and value once for all heads of its group.  The keys of all (row, kv head) pairs, "jobs", are one
+// paged_attention_kernel reads every key and value once for all heads of its group (once for 16 in bf16, 8 above 128 features; 8 in fp32, 4 above
+// 128).  The keys of all (row, kv head) pairs, "jobs", are one
 // sequence of rounds, 8 KB of keys and values or a little more, that is dealt out evenly: a CTA an SM takes a contiguous range, each of its
 // warps a contiguous part of that, so lengths from one token to the longest mix without an idle SM and without the host knowing them.
 // A warp keeps the running maximum, sum and weighted values of its job in registers.  Parts of a job that fell to several warps are joined in
@@ -694,7 +695,8 @@ __device__ __noinline__ void join_parts(const PagedAttnArgs& a, Parts<W>& sh, co
 // W warps, S rounds of a warp in flight or in use.
 template <typename R, int W, int S, bool TMA>
 __global__ void __launch_bounds__(W * 32, 1)
-paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_constant__ PageMaps maps, int box_shift, int head_tiles, int tile_heads, int q_vec, int o_vec) {
+paged_attention_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_constant__ PageMaps maps, int box_shift, int head_tiles, int tile_heads,
+                       int q_vec, int o_vec) {
   using T = typename R::T;
   constexpr int kPart = Part<R>::kFloats;
   static_assert(S * R::kBytes >= kPart * 4, "a warp's ring holds its last part");
