@@ -21,7 +21,8 @@
 // have the same rounds filled element by element, by the warp that works on them.
 //
 // bf16: S^T = K Q^T and O^T = V^T P^T by mma.sync, the group's heads as the 8 columns (two tiles of them for 9 to 16 heads); the bound is
-// the cache stream, and a tcgen05 tile of 128 rows would be padding for the most part.  The weights enter as two bf16 parts (16 bits).
+// the cache stream, and a tcgen05 tile of 128 rows would be padding for the most part.  The weights enter as three bf16 parts, all 24 bits of them:
+// with two, 16 bits, one output in 450 of 32 sequences of 1 to 4096 keys was a step off its rounding, so one in 1100 (53.8 us and 53.9).
 // fp32: multiply-adds, 8 lanes a key; they bound groups of four heads and more.
 //
 // Device time on B200, pages of 16 tokens in random order: bf16, 32 heads of 128 on 8: four sequences of 65000 to 131072 keys 242 us (6.6 TB/s, the
@@ -175,7 +176,7 @@ struct Bf16Round {
         }
       }
     const unsigned there = keys >> mine;               // bits 0, 8, ...: this lane's keys
-    uint32_t pp[NT][M][2][2];   // [16 keys][part][keys, keys + 8]: pairs of keys of head lane / 4
+    uint32_t pp[NT][M][3][2];   // [16 keys][part][keys, keys + 8]: pairs of keys of head lane / 4
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       float p[2 * M][2], corr[2];   // [key, key + 8, ...][head]
@@ -203,14 +204,18 @@ struct Bf16Round {
         l[n][e] = l[n][e] * corr[e] + sum;
         m[n][e] = nm;
       }
-      // Leading 8 bits and the rest.  Parts of a positive weight stay positive: its product with an infinite value is infinite in each.
+      // All 24 bits of a weight: its leading 8, the next, the rest.  Parts of a positive weight stay positive: its product with an infinite value is
+      // infinite in each.
 #pragma unroll
       for (int r = 0; r < 2 * M; ++r) {
-        const uint32_t u0 = __float_as_uint(p[r][0]), u1 = __float_as_uint(p[r][1]);
-        pp[n][r >> 1][0][r & 1] = movmatrix_trans((u0 >> 16) | (u1 & 0xffff0000u));
-        const float r0 = p[r][0] > 0.0f ? fmaxf(p[r][0] - __uint_as_float(u0 & 0xffff0000u), kTiny) : 0.0f;
-        const float r1 = p[r][1] > 0.0f ? fmaxf(p[r][1] - __uint_as_float(u1 & 0xffff0000u), kTiny) : 0.0f;
-        pp[n][r >> 1][1][r & 1] = movmatrix_trans(pack_bf16x2(r0, r1));
+        float rest[2] = {p[r][0], p[r][1]};
+#pragma unroll
+        for (int part = 0; part < 3; ++part) {
+          const uint32_t u0 = __float_as_uint(rest[0]), u1 = __float_as_uint(rest[1]);
+          pp[n][r >> 1][part][r & 1] = movmatrix_trans((u0 >> 16) | (u1 & 0xffff0000u));
+          rest[0] = p[r][0] > 0.0f ? fmaxf(rest[0] - __uint_as_float(u0 & 0xffff0000u), kTiny) : 0.0f;
+          rest[1] = p[r][1] > 0.0f ? fmaxf(rest[1] - __uint_as_float(u1 & 0xffff0000u), kTiny) : 0.0f;
+        }
       }
       if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
@@ -236,10 +241,9 @@ struct Bf16Round {
           const uint32_t f[4] = {__byte_perm(v[0][i], v[1][i], 0x5410), __byte_perm(v[0][i], v[1][i], 0x7632),
                                  __byte_perm(v[2][i], v[3][i], 0x5410), __byte_perm(v[2][i], v[3][i], 0x7632)};
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            mma_bf16_16816(o[n][b][i], f, pp[n][c][0][0], pp[n][c][0][1]);
-            mma_bf16_16816(o[n][b][i], f, pp[n][c][1][0], pp[n][c][1][1]);
-          }
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int part = 0; part < 3; ++part) mma_bf16_16816(o[n][b][i], f, pp[n][c][part][0], pp[n][c][part][1]);
         }
       }
   }
