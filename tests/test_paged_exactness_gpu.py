@@ -9,11 +9,11 @@ pytestmark = pytest.mark.gpu
 
 @pytest.mark.parametrize("hd,heads,page", [(64, 1, 16), (128, 4, 16), (64, 16, 8), (128, 12, 1), (256, 2, 32), (33, 1, 4)])
 def test_weights_have_all_their_bits(hd, heads, page):
-    """Two keys of weights 1 and exp(-x) with values 1 and -1 leave tanh(x / 2), a few 2^-16 of either.
+    """Two keys of weights 1 and exp(-x) with values 1 and -1 leave tanh(x / 2), a few 2^-18 of either.
 
     exp2 is off by 2^-22 of its result at most, a sum of 32 bits that truncates by 2^-23 for each of the three parts of a weight, and the
     quotient by less; half of that reaches the output, which is rounded to 8 bits.  Weights of 16 bits would be off by up to 2^-18."""
-    x = torch.arange(1, 65, device="cuda", dtype=torch.float32) * 2.0 ** -16           # (exact in bf16, as is all that follows)
+    x = torch.arange(1, 128, 2, device="cuda", dtype=torch.float32) * 2.0 ** -18       # (exact in bf16; 16 bits would end at 2^-17)
     rows = len(x)
     pages = -(-2 // page)
     k, v = (torch.zeros(rows * pages, 1, page, hd, dtype=torch.bfloat16, device="cuda") for _ in range(2))
