@@ -22,7 +22,9 @@
 //
 // bf16: S^T = K Q^T and O^T = V^T P^T by mma.sync, the group's heads as the 8 columns (two tiles of them for 9 to 16 heads); the bound is
 // the cache stream, and a tcgen05 tile of 128 rows would be padding for the most part.  The weights enter as three bf16 parts, all 24 bits of them:
-// with two, 16 bits, one output in 450 of 32 sequences of 1 to 4096 keys was a step off its rounding, so one in 1100 (53.8 us and 53.9).
+// with two, 16 bits, one output in 450 of 32 sequences of 1 to 4096 keys was a step off its rounding, so one in 1100
+// (53.8 us and 53.9).  What they add up to runs on in fp32, rounded to nearest: of those outputs one in 3400 is off then, and of four sequences of 65000 to
+// 131072 keys one in 3300 instead of one in 200 (heads of 256, 16 sequences of 2048 keys: 33.4 us instead of 32.1; the others within 2 %).
 // fp32: multiply-adds, 8 lanes a key; they bound groups of four heads and more.
 //
 // Device time on B200, pages of 16 tokens in random order: bf16, 32 heads of 128 on 8: four sequences of 65000 to 131072 keys 242 us (6.6 TB/s, the
@@ -176,11 +178,11 @@ struct Bf16Round {
         }
       }
     const unsigned there = keys >> mine;               // bits 0, 8, ...: this lane's keys
+    float corr[NT][2];
     uint32_t pp[NT][M][3][2];   // [16 keys][part][keys, keys + 8]: pairs of keys of head lane / 4
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      float p[2 * M][2], corr[2];   // [key, key + 8, ...][head]
-      bool moved = false;
+      float p[2 * M][2];   // [key, key + 8, ...][head]
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         float s[2 * M], mx = -INFINITY;
@@ -193,15 +195,14 @@ struct Bf16Round {
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
         const float nm = fmaxf(m[n][e], mx), sub = nm == -INFINITY ? 0.0f : nm;
-        moved |= nm != m[n][e];
-        corr[e] = exp2_fast(m[n][e] - sub);
+        corr[n][e] = exp2_fast(m[n][e] - sub);
         float sum = 0.0f;
 #pragma unroll
         for (int r = 0; r < 2 * M; ++r) {
           p[r][e] = there >> (8 * r) & 1 ? exp2_fast(s[r] - sub) : 0.0f;
           sum += p[r][e];
         }
-        l[n][e] = l[n][e] * corr[e] + sum;
+        l[n][e] = l[n][e] * corr[n][e] + sum;
         m[n][e] = nm;
       }
       // All 24 bits of a weight: its leading 8, the next, the rest.  Parts of a positive weight stay positive: its product with an infinite value is
@@ -217,35 +218,37 @@ struct Bf16Round {
           rest[1] = p[r][1] > 0.0f ? fmaxf(rest[1] - __uint_as_float(u1 & 0xffff0000u), kTiny) : 0.0f;
         }
       }
-      if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-        for (int b = 0; b < HD / 64; ++b)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[n][b][i][e] *= corr[e & 1];
-      }
     }
+    // A round's products are summed on their own, the smallest parts first, and added to the running values by multiply-adds: the matrix instructions cut
+    // off what does not fit their sums, so values that ran on in them would shrink by up to 2^-24 a step (8e-6 of them after 512 rounds).
 #pragma unroll
-    for (int b = 0; b < HD / 64; ++b)
+    for (int b = 0; b < HD / 64; ++b) {
+      uint32_t v[M][4][4];
 #pragma unroll
-      for (int c = 0; c < M; ++c) {
-        uint32_t v[4][4];
+      for (int c = 0; c < M; ++c)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint4 u = read_piece(vr + b * kSeg + c * 2048 + j * 512 + (swz ^ (j & 1) << 6));       // keys t, t + 4, t + 8, t + 12
-          v[j][0] = u.x; v[j][1] = u.y; v[j][2] = u.z; v[j][3] = u.w;
+          v[c][j][0] = u.x; v[c][j][1] = u.y; v[c][j][2] = u.z; v[c][j][3] = u.w;
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t f[4] = {__byte_perm(v[0][i], v[1][i], 0x5410), __byte_perm(v[0][i], v[1][i], 0x7632),
-                                 __byte_perm(v[2][i], v[3][i], 0x5410), __byte_perm(v[2][i], v[3][i], 0x7632)};
+      for (int i = 0; i < 4; ++i) {
+        float sum[NT][4] = {};
+#pragma unroll
+        for (int c = 0; c < M; ++c) {
+          const uint32_t f[4] = {__byte_perm(v[c][0][i], v[c][1][i], 0x5410), __byte_perm(v[c][0][i], v[c][1][i], 0x7632),
+                                 __byte_perm(v[c][2][i], v[c][3][i], 0x5410), __byte_perm(v[c][2][i], v[c][3][i], 0x7632)};
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int part = 0; part < 3; ++part) mma_bf16_16816(o[n][b][i], f, pp[n][c][part][0], pp[n][c][part][1]);
+            for (int part = 2; part >= 0; --part) mma_bf16_16816(sum[n], f, pp[n][c][part][0], pp[n][c][part][1]);
         }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[n][b][i][e] = fmaf(o[n][b][i][e], corr[n][e & 1], sum[n][e]);
       }
+    }
   }
 
   __device__ __forceinline__ void finish(int lane) {

@@ -27,3 +27,21 @@ def test_weights_have_all_their_bits(hd, heads, page):
     got = ops.paged_attention(q, k, v, table, torch.full((rows,), 2, dtype=torch.int32, device="cuda"), scale=1.0).double()
     want = torch.tanh(x.double() / 2)[:, None, None]
     assert bool(((got - want).abs() <= want * 2.0 ** -8 + 5 * 2.0 ** -24).all())
+
+
+@pytest.mark.parametrize("hd,heads", [(64, 1), (128, 4), (128, 16), (64, 9), (256, 2)])
+def test_long_sums_do_not_drift(hd, heads):
+    """Half of the keys again, with values of the other sign: what is summed up first goes down to zero, one row a warp.
+
+    A running sum of at most 1.5 takes 512 roundings or fewer each way, 2^-24 of it: at worst an output is off by 1024 * 1.5 * 2^-24, and
+    rounded to nearest there is no sign to it, so the mean of n of them stays below 7 / sqrt(n) of that.  Values of a sum that truncates shrink in both
+    halves, all to one side: by 8e-6."""
+    g = torch.Generator(device="cuda").manual_seed(hd + heads)
+    n, page, rows = 4096, 16, 1184
+    k = torch.randn(n // page, 1, page, hd, generator=g, device="cuda").bfloat16()
+    v = (torch.rand(n // page, 1, page, hd, generator=g, device="cuda") + 0.5).bfloat16()
+    table = torch.arange(2 * n // page, device="cuda", dtype=torch.int32).expand(rows, -1).contiguous()
+    q = torch.randn(rows, heads, hd, generator=g, device="cuda").bfloat16()
+    o = ops.paged_attention(q, torch.cat([k, k]), torch.cat([v, -v]), table, torch.full((rows,), 2 * n, device="cuda", dtype=torch.int32)).double()
+    worst = 1024 * 1.5 * 2.0 ** -24
+    assert float(o.abs().max()) <= worst and abs(float(o.mean())) <= 7 * worst / o.numel() ** 0.5
