@@ -17,8 +17,8 @@ namespace dptb {
 // ------------------------------------------------------------------------------------------------------------ append
 // Row t of `qkv` is [Hq | Hkv | Hkv] heads of a token at positions[t] of sequence rows[t].  Queries and keys are turned in half-split
 // form, pair (d, d + rotary / 2) by position * base^(-2 d / rotary); keys and values go to their place in the pages.  A token of
-// negative position has no place and passes unturned (padding).  The angle is formed and reduced to one turn in 64 bits: in 32 a position of
-// 100000 leaves it 0.004 rad off.
+// negative position has no place and passes unturned (padding).  The angle, its sine and its cosine are formed in 64 bits and rounded once: in 32
+// a position of 100000 leaves the angle 0.004 rad off, and one that is reduced to a turn before it is rounded is off by up to 2^-23.
 //
 // Bound by memory, or by the launch for a step.  A CTA takes up to four tokens: their angles first, one a thread, into shared memory, then the
 // heads in 16-byte groups.  3.6 us for 32 tokens of 32 + 2 x 8 heads of 128 in bf16; 14.5 us where 72 MB move (5.0 TB/s; eight tokens a CTA: 14.7).
@@ -102,9 +102,11 @@ paged_append_kernel(const AppendArgs a, const AppendShape shape) {
     const int t = i / half, d = i - t * half, pos = a.positions[t0 + t];
     float sn = 0.0f, cs = 1.0f;
     if (pos > 0) {
-      constexpr double kTurn = 6.283185307179586476925, kTurns = 1.0 / kTurn;
-      const double turns = pos * exp2(-2.0 * d / a.rotary * a.base) * kTurns;
-      sincosf((float)((turns - rint(turns)) * kTurn), &sn, &cs);
+      constexpr double kHalfTurns = 1.0 / 3.141592653589793238463;
+      double s64, c64;
+      sincospi(pos * exp2(-2.0 * d / a.rotary * a.base) * kHalfTurns, &s64, &c64);
+      sn = (float)s64;
+      cs = (float)c64;
     }
     turn[i] = make_float2(cs, sn);
   }

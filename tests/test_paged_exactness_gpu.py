@@ -45,3 +45,25 @@ def test_long_sums_do_not_drift(hd, heads):
     o = ops.paged_attention(q, torch.cat([k, k]), torch.cat([v, -v]), table, torch.full((rows,), 2 * n, device="cuda", dtype=torch.int32)).double()
     worst = 1024 * 1.5 * 2.0 ** -24
     assert float(o.abs().max()) <= worst and abs(float(o.mean())) <= 7 * worst / o.numel() ** 0.5
+
+
+@pytest.mark.parametrize("rotary,hd", [(64, 64), (128, 128), (32, 80)])
+@pytest.mark.parametrize("base", [10000.0, 500000.0])
+def test_sine_and_cosine_are_rounded_once(rotary, hd, base):
+    """Pairs (1, 0) and (0, 1) become the cosine and the sine themselves: half a step from the angle's in 64 bits, which a position p has to
+    2^-50 p (three roundings of it, and exp2)."""
+    positions = [1, 2, 3, 7, 100, 777, 4095, 30011, 131071, 10 ** 6, 2 ** 31 - 1]
+    tokens, half = len(positions), rotary // 2
+    p = torch.tensor(positions, dtype=torch.float64)[:, None]
+    angle = p * base ** (-2.0 * torch.arange(half, dtype=torch.float64) / rotary)
+    cos, sin = torch.cos(angle), torch.sin(angle)
+    k, v = (torch.empty(1, 1, 2 ** 20, hd, device="cuda") for _ in range(2))            # one page in all places
+    table = torch.zeros(1, 2 ** 11, dtype=torch.int32, device="cuda")
+    qkv = torch.zeros(tokens, 4, hd, device="cuda")
+    qkv[:, 0, :half] = 1.0
+    qkv[:, 1, half:rotary] = 1.0
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    q = ops.paged_append(qkv.view(tokens, -1), k, v, table, ints(positions), 2, rows=ints([0] * tokens), rotary_dim=rotary,
+                         rope_base=base).double().cpu()
+    for got, want in ((q[:, 0, :half], cos), (q[:, 0, half:rotary], sin), (q[:, 1, :half], -sin), (q[:, 1, half:rotary], cos)):
+        assert bool(((got - want).abs() <= want.abs() * 2.0 ** -24 + p * 2.0 ** -50).all())
