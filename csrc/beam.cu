@@ -2,7 +2,7 @@
 //
 //   total[b, w, v] = score[b, w] + logit[b * W + w, v] - log sum_u exp(logit[b * W + w, u])
 //
-// Candidates are ranked by (total, then the lower w * V + v).  A finished beam has one continuation, `eos` at its old score; its others, those
+// Candidates are ranked by (total, then the lower beam, then the larger logit, then the lower token).  A finished beam has one continuation, `eos` at its old score; its others, those
 // of a beam whose score is not finite, and those of a row of logits without a distribution (a NaN, an infinity, nothing but
 // -inf) are worth -inf.  Within a beam the order is that of the logits themselves, so that no rounding decides it; totals of different beams
 // meet in 64 bits.
@@ -190,6 +190,7 @@ struct BeamPart {
 struct BeamShared {
   unsigned long long keys[kItemPool];      // each warp's kWarpPool; of an item: (beam, token)
   double totals[kItemPool];
+  unsigned orders[kItemPool];              // a continuation's logit, larger for a larger one; 0 where its beam does not go by logits
   float lists[kBeamThreads];
   double score[kMaxBeams], top[kMaxBeams], norm[kMaxBeams];
   float size[kMaxBeams];                   // of what fp32 totals are made of
@@ -478,6 +479,7 @@ __device__ __noinline__ void choose(const BeamArgs& a, BeamShared& sh, int local
           if (at < kItemPool) {
             sh.totals[at] = total;
             sh.keys[at] = (unsigned long long)w << 32 | (unsigned)token;
+            sh.orders[at] = 0;
           }
         }
         continue;
@@ -533,6 +535,7 @@ __device__ __noinline__ void choose(const BeamArgs& a, BeamShared& sh, int local
             const int at = atomicAdd(&sh.count, 1);
             if (at < kItemPool) {
               sh.totals[at] = total_of(sh, w, x);
+              sh.orders[at] = (unsigned)(rank_key(x, 0) >> 32);
               sh.keys[at] = (unsigned long long)w << 32 | (unsigned)place_in<T>(e < N ? i0 : i1, j & 31, e & (N - 1), a.vec);
             }
           }
@@ -581,8 +584,21 @@ __device__ __noinline__ void choose(const BeamArgs& a, BeamShared& sh, int local
   for (int i = tid; i < found; i += kBeamThreads) {
     const double t = sh.totals[i];
     const unsigned long long key = sh.keys[i];
-    int rank = 0;
-    for (int j = 0; j < found; ++j) rank += sh.totals[j] > t || (sh.totals[j] == t && sh.keys[j] < key);
+    int rank = 0, equal = 0;
+    for (int j = 0; j < found; ++j) {
+      rank += sh.totals[j] > t;
+      equal += sh.totals[j] == t;
+    }
+    // Of equal totals the lower beam's; of one beam the larger logit's, which its total may be too coarse to tell; then the lower token's.
+    if (equal > 1 && rank < K) {
+      const unsigned order = sh.orders[i];
+#pragma unroll 1
+      for (int j = 0; j < found; ++j) {
+        const unsigned long long other = sh.keys[j];
+        const bool by_key = (other ^ key) >> 32 || sh.orders[j] == order;
+        rank += sh.totals[j] == t && (by_key ? other < key : sh.orders[j] > order);
+      }
+    }
     if (rank < K) put(rank, t, key);
   }
 }

@@ -34,22 +34,23 @@ def _lib():
 
 
 def beam_step_reference(logits, scores, finished=None, eos=-1):
-    """64-bit formulas over all continuations, sorted by value and then by place."""
+    """64-bit formulas over all continuations, sorted by value, then by beam, and within a beam by logit and token."""
     items, beams = scores.shape
     x = logits.double().view(items, beams, -1)
     vocab = x.shape[-1]
+    ids = torch.arange(vocab, device=x.device)
     lp = torch.log_softmax(x, -1)
-    lp = torch.where(lp.isfinite().any(-1, keepdim=True) & ~lp.isnan().any(-1, keepdim=True), lp, -math.inf)
     start = scores.double()[..., None]
-    start = torch.where(start.isfinite(), start, -math.inf)
-    total = start + lp
+    fine = lp.isfinite().any(-1, keepdim=True) & ~lp.isnan().any(-1, keepdim=True) & start.isfinite()
+    total = torch.where(fine, start + lp, -math.inf)
     if finished is not None:
-        only = torch.where(torch.arange(vocab, device=x.device) == eos, start, -math.inf)
+        only = torch.where((ids == eos) & start.isfinite(), start, -math.inf)
         total = torch.where(finished[..., None], only, total)
-    total = torch.where(total.isnan(), -math.inf, total).view(items, -1)
-    total, order = torch.sort(total, dim=-1, descending=True, stable=True)
+        fine = fine & ~finished[..., None]
+    within = torch.where(fine, torch.sort(x, dim=-1, descending=True, stable=True).indices, ids)
+    total, order = torch.sort(total.gather(2, within).view(items, -1), dim=-1, descending=True, stable=True)
     total, order = total[:, :beams], order[:, :beams]
-    beam, token = order // vocab, order % vocab
+    beam, token = order // vocab, within.view(items, -1).gather(1, order)
     done = token == eos
     if finished is not None:
         done = done | finished.gather(1, beam)
@@ -61,7 +62,7 @@ def beam_step(logits: torch.Tensor, scores: torch.Tensor, finished: Optional[tor
               eos: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """One step of beam search for ``items`` searches of ``beams`` beams: of all ``beams * vocab`` continuations of an item the
     best ``beams``, by ``scores [items, beams]`` (fp32) plus the log-probability that ``logits [items * beams, vocab]`` (bf16 or
-    fp32) gives the token; equal ones in the order of beam and token.
+    fp32) gives the token; equal ones in the order of the beams, and within a beam of the logits, then of the tokens.
 
     A beam of ``finished [items, beams]`` (bool) goes on with ``eos`` alone, at its old score.  A beam whose score is not finite and a
     row of logits that is no distribution (a NaN, an infinity, nothing but -inf) have continuations worth -inf only, so a search starts
