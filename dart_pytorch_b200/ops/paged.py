@@ -24,9 +24,9 @@ from .. import _native as N
 from . import kernels
 
 c_void_p, c_int = ctypes.c_void_p, ctypes.c_int
-_current_device, _raw_stream, _increment_version = None, None, torch._C._increment_version
-if torch.cuda.is_available():
-    _current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+# (called for CUDA tensors only; looking for devices here would fix which are visible as soon as the package is imported)
+_current_device, _raw_stream = getattr(torch._C, "_cuda_getDevice", None), getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_increment_version = torch._C._increment_version
 _F32, _BF16, _I32 = torch.float32, torch.bfloat16, torch.int32
 
 MAX_HEAD_DIM = 256
