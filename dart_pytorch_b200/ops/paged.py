@@ -155,7 +155,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         if q_one != 1 and hd > 1:
             q = q.contiguous()
             q_row, q_head, _ = q.stride()
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((rows, heads, hd))
         o_row, o_head = heads * hd, hd
     else:
@@ -170,6 +171,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if rc == TOO_LARGE:
         raise ValueError(f"paged_attention: {rows} rows of up to {width * page} tokens and {heads} heads in one call are too many")
     N.check(rc, "paged_attention")
+    if given:
+        _increment_version((out,))
     return out
 
 
@@ -185,7 +188,7 @@ def _check_attention(q, k_pages, v_pages, table, lens, out) -> None:
     rows, heads, hd = q.shape
     _ints(what, "lens", lens, rows)
     _here(what, q, k_pages, v_pages, table, lens, out)
-    _no_grad(what, q, k_pages, v_pages)
+    _no_grad(what, q, k_pages, v_pages, out)
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 and hd > 1):
         raise ValueError(f"{what}: out must be {list(q.shape)} {q.dtype} with contiguous features")
 
