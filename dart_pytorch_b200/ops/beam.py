@@ -9,6 +9,7 @@ from typing import Optional, Tuple
 import torch
 
 from .. import _native as N
+from . import flash
 from .kernels import SPLITK_COUNTERS, SPLITK_WS_BYTES
 from .paged import _BF16, _F32, _current_device, _here, _no_grad, _raw_stream, _scratch
 
@@ -99,7 +100,7 @@ def _beam_is_off(logits, scores, finished, eos, dev) -> bool:
         0 < beams <= MAX_BEAMS and rows <= MAX_ROWS and scores.is_contiguous() and logits.stride(1) == 1 and
         (eos is None or 0 <= eos < vocab) and scores.get_device() == dev and _current_device() == dev and
         (finished is None or eos is not None and finished.dtype is torch.bool and finished.shape == scores.shape and
-         finished.get_device() == dev and finished.is_contiguous()) and
+         finished.get_device() == dev and finished.is_contiguous()) and flash._raw_call() and
         not ((logits.requires_grad or scores.requires_grad) and torch.is_grad_enabled()))
 
 

@@ -9,7 +9,7 @@ The operations on pages run on the device and return new tables; nothing is read
 number outside the pool or a pool without a free page, is recorded in the status word: the kernels skip such a page, and
 ``_native.raise_on_device_error`` raises.  CPU tensors run reference formulas with the same contracts, which raise at once.
 
-None of this has gradients: tensors that want them are refused.
+None of this has gradients: tensors that want them, or carry a tangent, are refused, and so are torch.func transforms.
 """
 from __future__ import annotations
 
@@ -21,7 +21,7 @@ from typing import Optional, Tuple, Union
 import torch
 
 from .. import _native as N
-from . import kernels
+from . import flash, kernels
 
 c_void_p, c_int = ctypes.c_void_p, ctypes.c_int
 # (called for CUDA tensors only; looking for devices here would fix which are visible as soon as the package is imported)
@@ -80,6 +80,11 @@ def _here(what: str, first: torch.Tensor, *others) -> None:
 def _no_grad(what: str, *tensors) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise ValueError(f"{what} has no gradients; call it under torch.no_grad()")
+    if torch._C._are_functorch_transforms_active():
+        raise ValueError(f"{what} has no derivatives and is not for torch.func transforms")
+    if torch.autograd.forward_ad._current_level >= 0 and any(
+            t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError(f"{what} has no derivatives; a tensor carries a tangent")
 
 
 def _ints(what: str, name: str, t: torch.Tensor, *shape) -> None:
@@ -149,7 +154,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
             0 < hd <= MAX_HEAD_DIM and 0 < hkv and heads % hkv == 0 and 0 < page and pages <= MAX_PAGES and rows <= MAX_ROWS and
             q_one == 1 and k_one == 1 and v_one == 1 and (t_one == 1 or width <= 1) and (rows <= 1 or lens.stride(0) == 1) and
             k_pages.get_device() == dev and v_pages.get_device() == dev and table.get_device() == dev and
-            lens.get_device() == dev and _current_device() == dev and
+            lens.get_device() == dev and _current_device() == dev and flash._raw_call() and
             not (torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad))):
         _check_attention(q, k_pages, v_pages, table, lens, out)
         if q_one != 1 and hd > 1:
@@ -250,7 +255,7 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
             k_pages.get_device() == dev and v_pages.get_device() == dev and table.get_device() == dev and
             positions.get_device() == dev and _current_device() == dev and
             (table_rows == tokens if rows is None else rows.dtype is _I32 and rows.shape == (tokens,) and
-             rows.get_device() == dev and (tokens <= 1 or rows.stride(0) == 1)) and
+             rows.get_device() == dev and (tokens <= 1 or rows.stride(0) == 1)) and flash._raw_call() and
             not (torch.is_grad_enabled() and (qkv.requires_grad or k_pages.requires_grad or v_pages.requires_grad))):
         _check_append(qkv, k_pages, v_pages, table, positions, heads, rows, rotary, rope_base)
         if x_one != 1:
@@ -426,7 +431,7 @@ def copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None
             len(shape) >= 4 and pool.is_contiguous() and (pool.dtype is _BF16 or pool.dtype is _F32) and src.dim() == 1 and
             src.dtype is _I32 and dst.dtype is _I32 and src.shape == dst.shape and src.get_device() == dev and
             dst.get_device() == dev and (src.shape[0] <= 1 or src.stride(0) == 1 and dst.stride(0) == 1) and
-            _current_device() == dev and not (pool.requires_grad and torch.is_grad_enabled())):
+            _current_device() == dev and flash._raw_call() and not (pool.requires_grad and torch.is_grad_enabled())):
         _check_copy(pool, src, dst)
     pages = shape[-4]
     outer = math.prod(shape[:-4])

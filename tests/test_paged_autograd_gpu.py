@@ -8,3 +8,7 @@ pytestmark = pytest.mark.gpu
 
 def test_out_is_known_to_autograd():
     on.out_is_known_to_autograd("cuda")
+
+
+def test_forward_mode_is_refused():
+    on.forward_mode_is_refused("cuda")
