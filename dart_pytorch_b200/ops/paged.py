@@ -87,6 +87,23 @@ def _no_grad(what: str, *tensors) -> None:
         raise ValueError(f"{what} has no derivatives; a tensor carries a tangent")
 
 
+def _overlaps_itself(t: torch.Tensor) -> bool:
+    """Whether elements may share a place: an axis that does not step over all that the smaller steps reach."""
+    reach = 1
+    for step, n in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1):
+        if step < reach:
+            return t.numel() > 0
+        reach += (n - 1) * step
+    return False
+
+
+def _meets(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the stretches of memory from first to last element meet."""
+    def end(t):
+        return t.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
+    return a.numel() > 0 and b.numel() > 0 and a.data_ptr() < end(b) and b.data_ptr() < end(a)
+
+
 def _ints(what: str, name: str, t: torch.Tensor, *shape) -> None:
     if t.dtype != torch.int32:
         raise TypeError(f"{what}: {name} must be int32, got {t.dtype}")
@@ -141,7 +158,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
                     scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of one new token per row, ``q [rows, heads, head_dim]``, over the ``lens[r]`` tokens of its pages (the new one
     among them).  Query heads share key heads in groups of ``heads // kv_heads``; a row of no tokens gives zeros.  bf16 or fp32, one type for all; sums in
-    fp32.  ``scale`` is ``head_dim ** -0.5`` unless given.  Returns ``[rows, heads, head_dim]``."""
+    fp32.  ``scale`` is ``head_dim ** -0.5`` unless given.  Returns ``[rows, heads, head_dim]``: ``out``, if given, which may lie over the
+    queries or any other argument."""
     dev, q_shape, k_shape, t_shape, dtype = q.get_device(), q.shape, k_pages.shape, table.shape, q.dtype
     if dev < 0 or len(q_shape) != 3 or len(k_shape) != 4 or len(t_shape) != 2 or v_pages.shape != k_shape:
         return _attention_on_cpu(q, k_pages, v_pages, table, lens, scale, out)
@@ -160,8 +178,11 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         if q_one != 1 and hd > 1:
             q = q.contiguous()
             q_row, q_head, _ = q.stride()
-    given = out is not None
-    if not given:
+    given = out
+    if given is not None and (any(_meets(out, t) for t in (k_pages, v_pages, table, lens)) or _meets(out, q) and not (
+            out.data_ptr() == q.data_ptr() and out.stride() == q.stride())):     # (a query itself is read before its result is written)
+        out = None
+    if out is None:
         out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((rows, heads, hd))
         o_row, o_head = heads * hd, hd
     else:
@@ -176,7 +197,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if rc == TOO_LARGE:
         raise ValueError(f"paged_attention: {rows} rows of up to {width * page} tokens and {heads} heads in one call are too many")
     N.check(rc, "paged_attention")
-    if given:
+    if given is not None:
+        if given is not out:
+            return given.copy_(out)
         _increment_version((out,))
     return out
 
@@ -196,6 +219,8 @@ def _check_attention(q, k_pages, v_pages, table, lens, out) -> None:
     _no_grad(what, q, k_pages, v_pages, out)
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 and hd > 1):
         raise ValueError(f"{what}: out must be {list(q.shape)} {q.dtype} with contiguous features")
+    if out is not None and _overlaps_itself(out):
+        raise ValueError(f"{what}: places of out {list(out.shape)} with strides {list(out.stride())} overlap")
 
 
 def _attention_on_cpu(q, k_pages, v_pages, table, lens, scale, out):
