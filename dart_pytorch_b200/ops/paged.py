@@ -261,7 +261,7 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     ``t`` is token ``positions[t]`` of row ``rows[t]`` (of row ``t`` without ``rows``); int32.  A negative position is padding
     and writes nothing.  Queries and keys are turned by the half-split rotary embedding over ``rotary_dim`` features (all of
     them unless given; 0: not at all).  Returns the turned queries ``[tokens, heads, head_dim]``, and with ``keys`` the turned keys
-    too; ``qkv`` stays as it is.  No two tokens may have one place."""
+    too; ``qkv``, which shares no memory with the pages, stays as it is.  No two tokens may have one place."""
     dev, x_shape, k_shape, t_shape, dtype = qkv.get_device(), qkv.shape, k_pages.shape, table.shape, qkv.dtype
     rotary = k_shape[-1] if rotary_dim is None else rotary_dim
     if dev < 0 or len(x_shape) != 2 or len(k_shape) != 4 or len(t_shape) != 2 or v_pages.shape != k_shape:
@@ -275,6 +275,10 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
             (dtype is _BF16 or dtype is _F32) and k_pages.dtype is dtype and v_pages.dtype is dtype and table.dtype is _I32 and
             positions.dtype is _I32 and positions.shape == (tokens,) and (tokens <= 1 or positions.stride(0) == 1) and
             0 < hd <= MAX_HEAD_DIM and 0 < hkv and 0 < page and pages <= MAX_PAGES and table_rows <= MAX_ROWS and
+            (kt >= hd and kh >= (page - 1) * kt + hd or kh >= hd and kt >= (hkv - 1) * kh + hd) and
+            (vt >= hd and vh >= (page - 1) * vt + hd or vh >= hd and vt >= (hkv - 1) * vh + hd) and
+            kp >= (hkv - 1) * kh + (page - 1) * kt + hd and vp >= (hkv - 1) * vh + (page - 1) * vt + hd and
+            k_pages.data_ptr() != v_pages.data_ptr() and
             heads > 0 and features == (heads + 2 * hkv) * hd and 0 <= rotary <= hd and rotary % 2 == 0 and rope_base > 0 and
             x_one == 1 and k_one == 1 and v_one == 1 and (t_one == 1 or width <= 1) and
             k_pages.get_device() == dev and v_pages.get_device() == dev and table.get_device() == dev and
@@ -317,6 +321,9 @@ def _check_append(qkv, k_pages, v_pages, table, positions, heads, rows, rotary, 
         raise ValueError(f"{what}: {tokens} tokens without `rows` for a table of {table.shape[0]} rows")
     _here(what, qkv, k_pages, v_pages, table, positions, rows)
     _no_grad(what, qkv, k_pages, v_pages)
+    if _overlaps_itself(k_pages) or _overlaps_itself(v_pages) or k_pages.numel() > 0 and k_pages.data_ptr() == v_pages.data_ptr():
+        raise ValueError(f"{what}: places of the pages overlap: {list(k_pages.shape)} with strides {list(k_pages.stride())} and "
+                         f"{list(v_pages.stride())}")
 
 
 # ------------------------------------------------------------------------------------------------------------ pages

@@ -45,3 +45,30 @@ def test_out_lies_anywhere():
 
 def test_out_over_itself_is_refused():
     out_over_itself_is_refused("cpu")
+
+
+def append_to_pages_over_themselves_is_refused(device):
+    table, at = torch.tensor([[0, 2], [1, -1]], dtype=torch.int32, device=device), torch.tensor([5, 0], dtype=torch.int32, device=device)
+    qkv = torch.randn(2, 8 * 8, device=device)
+    zeros = lambda *shape: torch.zeros(*shape, device=device)  # noqa: E731
+    k = zeros(3, 2, 4, 8)
+    for bad in (zeros(3, 1, 4, 8).expand(3, 2, 4, 8), zeros(3, 2, 1, 8).expand(3, 2, 4, 8), zeros(1, 2, 4, 8).expand(3, 2, 4, 8),
+                zeros(300).as_strided((3, 2, 4, 8), (64, 32, 7, 1)), zeros(300).as_strided((3, 2, 4, 8), (63, 32, 8, 1))):
+        for pages in ((bad, k), (k, bad)):
+            with pytest.raises(ValueError, match="overlap"):
+                ops.paged_append(qkv, *pages, table, at, 4)
+    with pytest.raises(ValueError, match="overlap"):
+        ops.paged_append(qkv, k, k, table, at, 4)
+    assert not k.any()
+    want = torch.zeros(2, 3, 2, 4, 8, device=device)
+    ops.paged_append(qkv, *want, table, at, 4)
+    # one head at any stride, pages of a pool of keys and values, tokens and heads the other way round
+    for shape, axes in (((2, 3, 2, 4, 8), (0, 1, 2, 3, 4)), ((3, 2, 2, 4, 8), (1, 0, 2, 3, 4)), ((2, 3, 4, 2, 8), (0, 1, 3, 2, 4)),
+                        ((4, 3, 2, 2, 8), (3, 1, 2, 0, 4)), ((2, 2, 4, 3, 8), (0, 3, 1, 2, 4))):
+        pool = torch.zeros(*shape, device=device).permute(*axes)
+        ops.paged_append(qkv, *pool, table, at, 4)
+        assert torch.equal(pool, want)
+
+
+def test_append_to_pages_over_themselves_is_refused():
+    append_to_pages_over_themselves_is_refused("cpu")

@@ -12,3 +12,7 @@ def test_out_lies_anywhere():
 
 def test_out_over_itself_is_refused():
     on.out_over_itself_is_refused("cuda")
+
+
+def test_append_to_pages_over_themselves_is_refused():
+    on.append_to_pages_over_themselves_is_refused("cuda")
