@@ -68,9 +68,7 @@ class _Search:
         self.graph, self.out = graph, out
 
     def replay(self):
-        if self.cache.longest + 1 > self.cache.max_len:
-            raise ValueError(f"PagedCache: a row of {self.cache.longest + 1} tokens in a cache of {self.cache.max_len}")
-        self.cache.longest += 1
+        self.cache.longest = self.cache.longer_by(1)
         self.graph.replay()
         return self.out
 

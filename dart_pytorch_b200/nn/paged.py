@@ -67,11 +67,21 @@ class PagedCache:
         self.rows: Optional[torch.Tensor] = None           # and their rows; None: one token of every row
         self.layers: List[PagedLayer] = [PagedLayer(self, i) for i in range(num_layers)]
 
-    def _fork(self, parents, grow, longest: int) -> None:
-        if longest > self.max_len and isinstance(grow, int):     # rows that have ended may have been the longest: look
-            longest = int(self.lens.max()) + grow
+    def longer_by(self, grow: int, parents=None) -> int:
+        """``longest`` of the rows after ``fork(parents)`` by ``grow`` tokens.  Rows that have ended, or that no row goes on from, may have
+        been the longest: where the bound kept here does not fit, the lengths themselves are looked at."""
+        longest = self.longest + grow
+        if longest > self.max_len:
+            lens = self.lens
+            if parents is not None:
+                lens = torch.where(parents >= 0, lens[parents.long().clamp(0, lens.shape[0] - 1)], 0)
+            longest = int(lens.max())
+            longest += grow if longest > 0 else 0
         if longest > self.max_len:
             raise ValueError(f"PagedCache: a row of {longest} tokens in a cache of {self.max_len}")
+        return longest
+
+    def _fork(self, parents, grow, longest: int) -> None:
         self.table, self.lens, src, dst = F.fork_pages(self.table, self.lens, self.num_pages, self.page_size, parents, grow)
         F.copy_pages(self.pool, src, dst)
         self.longest = longest
@@ -98,7 +108,7 @@ class PagedCache:
     def fork(self, parents: Optional[torch.Tensor] = None) -> None:
         """Every row becomes a copy of row ``parents[r]`` (int32; itself without ``parents``; -1: empty) with room for a token,
         which the model's step brings; rows that hold nothing stay empty."""
-        self._fork(parents, 1, self.longest + 1)
+        self._fork(parents, 1, self.longer_by(1, parents))
         self.rows, self.positions = None, self.lens - 1
 
     def free(self, rows: Sequence[int]) -> None:
