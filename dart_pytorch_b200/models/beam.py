@@ -97,9 +97,10 @@ def beam_search(model, prompts: Sequence[Sequence[float]], max_new_tokens: int, 
     model.eval()
     try:
         with torch.no_grad():
+            # (the last token is chosen and not appended, so no row is longer than the context)
             # pages: what the prompts fill, and each beam's own behind that (with the part-filled one that it copies)
             pages = sum(-(-len(p) // page_size) for p in prompts) + items * beams * (-(-new // page_size) + 1)
-            cache = PagedCache(c.num_layers, heads, model.paged_head_dim, items * beams, longest + new, page_size, pages,
+            cache = PagedCache(c.num_layers, heads, model.paged_head_dim, items * beams, longest + new - 1, page_size, pages,
                                dtype=model.head_weight.dtype, device=dev)
             cache.prompts([len(p) for p in prompts], [i * beams for i in range(items)])
             tokens = torch.tensor([p + [0] * (longest - len(p)) for p in prompts], dtype=torch.long, device=dev)

@@ -136,6 +136,7 @@ class GPT(Module):
 
     def paged_hidden(self, tokens, cache: PagedCache):
         """Final hidden states of ``tokens [B, N]`` that ``cache`` was last extended by (``prompts``, ``fork``)."""
+        cache.check_window("GPT", self.config.max_ctx)
         h = F.embedding(self.token_emb.weight, tokens)
         at = F.embedding(self.pos_emb.table.weight, cache.positions.clamp(min=0).long().view(tokens.shape))
         return self.encoder(self.embed_drop(F.add(h, at)), cache=cache, causal=tokens.shape[1] > 1)

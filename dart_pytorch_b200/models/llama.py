@@ -165,6 +165,7 @@ class Llama(Module):
 
     def paged_hidden(self, tokens, cache: PagedCache):
         """Final hidden states of ``tokens [B, N]`` that ``cache`` was last extended by (``prompts``, ``fork``)."""
+        cache.check_window("Llama", self.config.max_ctx)
         return self.hidden_from_embeddings(F.embedding(self.embed_in.weight, tokens), 0, cache)
 
     def loss(self, tokens, targets):

@@ -272,6 +272,8 @@ class MultiHeadAttention(Module):
         if isinstance(cache, PagedLayer):
             if mask is not None:
                 raise ValueError("MultiHeadAttention: a paged cache takes no mask")
+            if self.rope is not None:
+                cache.cache.check_window("RopeCache", self.rope.max_ctx)
             out = self.wo(cache.attend(qkv, B, S, H, self.rope), residual=None if residual is None else residual.reshape(B * S, -1))
             return (out if self.attn_dropout is None else self.attn_dropout(out)).reshape(*x.shape[:-1], self.embed_dim)
         if self.rope is not None:

@@ -81,6 +81,13 @@ class PagedCache:
             raise ValueError(f"PagedCache: a row of {longest} tokens in a cache of {self.max_len}")
         return longest
 
+    def check_window(self, what: str, max_ctx: int) -> None:
+        """Raises if a row is longer than ``max_ctx``."""
+        if self.longest > max_ctx:
+            self.longest = int(self.lens.max())
+        if self.longest > max_ctx:
+            raise ValueError(f"{what}: sequence of {self.longest} tokens exceeds maxCtx {max_ctx}")
+
     def _fork(self, parents, grow, longest: int) -> None:
         self.table, self.lens, src, dst = F.fork_pages(self.table, self.lens, self.num_pages, self.page_size, parents, grow)
         F.copy_pages(self.pool, src, dst)

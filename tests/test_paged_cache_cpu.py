@@ -2,8 +2,9 @@
 import pytest
 import torch
 
+from dart_pytorch_b200.models import GPT, GPTConfig, Llama, LlamaConfig
 from dart_pytorch_b200.models.beam import _Search
-from dart_pytorch_b200.nn import PagedCache
+from dart_pytorch_b200.nn import MultiHeadAttention, PagedCache, RopeCache
 
 
 def ints(*x):
@@ -47,3 +48,44 @@ def test_a_recorded_step_looks_at_the_lengths_too():
     with pytest.raises(ValueError, match="9 tokens"):
         search.replay()
     assert c.lens.tolist() == [0, 8]
+
+
+def family(name):
+    if name == "gpt":
+        return GPT(GPTConfig(vocab_size=37, max_ctx=8, embed_dim=32, num_layers=2, num_heads=4, seed=5, init_std=0.4))
+    return Llama(LlamaConfig(37, 8, 32, 2, 4, 4, 48, seed=3, init_std=0.4))
+
+
+@pytest.mark.parametrize("name", ["gpt", "llama"])
+def test_a_cache_may_be_longer_than_the_context_but_not_its_rows(name):
+    model = family(name)
+    c = PagedCache(2, 4, 8, 2, 64, 4)
+    step = lambda *rows: model.paged_hidden(torch.tensor(rows), c)  # noqa: E731
+    with torch.no_grad():
+        c.prompts([6, 2], [0, 1])
+        step([1, 2, 3, 4, 5, 6], [7, 8, 0, 0, 0, 0])
+        for _ in range(2):
+            c.fork()
+            step([1], [2])
+        assert c.lens.tolist() == [8, 4]
+        c.fork(ints(-1, 1))                            # the row that has as many as there may be ends
+        for _ in range(4):
+            h = step([1], [2])
+            c.fork()
+        assert torch.allclose(h[1, 0], model.hidden(torch.tensor([7, 8, 2, 2, 2, 2, 2, 2]))[-1], atol=1e-5)
+        with pytest.raises(ValueError, match="sequence of 9 tokens exceeds maxCtx 8"):
+            step([1], [2])
+        c.prompts([9], [0])
+        with pytest.raises(ValueError, match="exceeds maxCtx 8"):
+            step([1] * 9)
+
+
+def test_rotary_attention_over_pages_keeps_to_its_window():
+    m = MultiHeadAttention(32, 4, rope=RopeCache(8, 8), seed=1)
+    c = PagedCache(1, 4, 8, 1, 64, 4)
+    with torch.no_grad():
+        c.prompts([8], [0])
+        m(torch.randn(1, 8, 32), cache=c.layers[0], causal=True)
+        c.fork()
+        with pytest.raises(ValueError, match="RopeCache: sequence of 9 tokens"):
+            m(torch.randn(1, 1, 32), cache=c.layers[0])
