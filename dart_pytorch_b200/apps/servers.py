@@ -168,8 +168,11 @@ class GenerationService:
         with self._lock:
             if beams > 1:
                 eos = req.get("eos")
-                best = self.model.generate_beams([tokens], max_new, beams, None if eos is None else int(eos),
-                                                 float(req.get("lengthPenalty", 0.0)))[0]
+                try:
+                    best = self.model.generate_beams([tokens], max_new, beams, None if eos is None else int(eos),
+                                                     float(req.get("lengthPenalty", 0.0)))[0]
+                except ArithmeticError as e:       # the model has no continuation
+                    return 500, {"error": str(e)}
                 ids = best[0][0]
                 return 200, {"tokens": ids, "newTokens": ids[len(tokens):], "text": self.tok.decode(ids) if self.tok else None,
                              "beams": [{"newTokens": seq[len(tokens):], "score": score} for seq, score in best],

@@ -77,7 +77,8 @@ def beam_search(model, prompts: Sequence[Sequence[float]], max_new_tokens: int, 
                 length_penalty: float = 0.0, page_size: int = 16) -> List[List[Tuple[List[int], float]]]:
     """The ``beams`` most probable continuations found for every prompt, best first, as ``(tokens, score)``: prompt and new
     tokens, up to and with ``eos``, and the sum of the new tokens' log-probabilities.  They are ordered by ``score / (new
-    tokens) ** length_penalty``.  Prompts may differ in length."""
+    tokens) ** length_penalty``.  Prompts may differ in length.  Where the model's logits are no distribution, so that a prompt has no
+    continuation at all, that is an ``ArithmeticError``."""
     what = f"{type(model).__name__}.generate_beams"
     prompts = [[int(round(float(t))) for t in p] for p in prompts]
     if not prompts or any(not p for p in prompts):
@@ -143,6 +144,8 @@ def beam_search(model, prompts: Sequence[Sequence[float]], max_new_tokens: int, 
             if eos is not None and eos in path:
                 path = path[:path.index(eos) + 1]
             mine.append((p + path, scores[i][w], scores[i][w] / len(path) ** length_penalty))
+        if not mine:
+            raise ArithmeticError(f"{what}: no continuation of prompt {i} has a probability (the model's logits are not finite)")
         mine.sort(key=lambda x: -x[2])
         found.append([(seq, score) for seq, score, _ in mine])
     return found

@@ -1,0 +1,22 @@
+"""What a search answers when there is nothing to answer with, or when it is asked for what cannot be."""
+import pytest
+import torch
+
+from dart_pytorch_b200.apps.servers import GenerationService
+from test_beam_search_cpu import gpt, llama
+
+
+def broken(make, token):
+    model = make()
+    with torch.no_grad():
+        (model.embed_in if make is llama else model.token_emb).weight[token] = float("nan")
+    return model
+
+
+@pytest.mark.parametrize("make", [llama, gpt])
+def test_no_continuation_at_all_is_an_error_with_a_name(make):
+    model = broken(make, 5)
+    with pytest.raises(ArithmeticError, match="generate_beams: no continuation of prompt 0"):
+        model.generate_beams([[3, 5], [1, 2]], 4, 2)
+    code, out = GenerationService(model, None, "tiny").run({"tokens": [3, 5], "maxNewTokens": 4, "beams": 2})
+    assert code == 500 and "no continuation" in out["error"]
