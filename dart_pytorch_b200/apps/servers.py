@@ -164,13 +164,14 @@ class GenerationService:
             return 400, {"error": f"{self.model_name} has no beam search"}
         if not 1 <= beams <= 32:
             return 400, {"error": '"beams" must be between 1 and 32'}
+        eos = int(req["eos"]) if beams > 1 and req.get("eos") is not None else None
+        if eos is not None and not 0 <= eos < self.model.config.vocab_size:
+            return 400, {"error": f'"eos" must be a token, 0 to {self.model.config.vocab_size - 1}'}
         t0 = time.perf_counter()
         with self._lock:
             if beams > 1:
-                eos = req.get("eos")
                 try:
-                    best = self.model.generate_beams([tokens], max_new, beams, None if eos is None else int(eos),
-                                                     float(req.get("lengthPenalty", 0.0)))[0]
+                    best = self.model.generate_beams([tokens], max_new, beams, eos, float(req.get("lengthPenalty", 0.0)))[0]
                 except ArithmeticError as e:       # the model has no continuation
                     return 500, {"error": str(e)}
                 ids = best[0][0]

@@ -20,3 +20,14 @@ def test_no_continuation_at_all_is_an_error_with_a_name(make):
         model.generate_beams([[3, 5], [1, 2]], 4, 2)
     code, out = GenerationService(model, None, "tiny").run({"tokens": [3, 5], "maxNewTokens": 4, "beams": 2})
     assert code == 500 and "no continuation" in out["error"]
+
+
+def test_an_end_that_is_no_token_is_a_bad_request():
+    svc = GenerationService(llama(), None, "tiny")
+    for eos in (-1, 37, 10 ** 9):
+        code, out = svc.run({"tokens": [3], "maxNewTokens": 2, "beams": 2, "eos": eos})
+        assert code == 400 and '"eos"' in out["error"]
+    for eos in (0, 36, None):
+        assert svc.run({"tokens": [3], "maxNewTokens": 2, "beams": 2, "eos": eos})[0] == 200
+    for eos in (99, "none"):                             # sampling has no use for it
+        assert svc.run({"tokens": [3], "maxNewTokens": 2, "eos": eos})[0] == 200
