@@ -14,6 +14,7 @@ import torch
 from .. import _native as N
 from .. import ops as F
 from ..nn.paged import PagedCache
+from ..ops.paged import MAX_PAGES, MAX_ROWS
 
 
 class _Search:
@@ -94,13 +95,16 @@ def beam_search(model, prompts: Sequence[Sequence[float]], max_new_tokens: int, 
     if new <= 0:
         return [[(list(p), 0.0)] for p in prompts]
     items, dev, heads = len(prompts), model.device, getattr(c, "num_kv_heads", c.num_heads)
+    # pages: what the prompts fill, and each beam's own behind that (with the part-filled one that it copies)
+    pages = sum(-(-len(p) // page_size) for p in prompts) + items * beams * (-(-new // page_size) + 1)
+    if items * beams > MAX_ROWS or pages > MAX_PAGES:
+        raise ValueError(f"{what}: {items} prompts of {beams} beams and {new} new tokens are {items * beams} rows of {pages} pages; one call "
+                         f"takes {MAX_ROWS} rows and {MAX_PAGES} pages")
     was_training = model.training
     model.eval()
     try:
         with torch.no_grad():
             # (the last token is chosen and not appended, so no row is longer than the context)
-            # pages: what the prompts fill, and each beam's own behind that (with the part-filled one that it copies)
-            pages = sum(-(-len(p) // page_size) for p in prompts) + items * beams * (-(-new // page_size) + 1)
             cache = PagedCache(c.num_layers, heads, model.paged_head_dim, items * beams, longest + new - 1, page_size, pages,
                                dtype=model.head_weight.dtype, device=dev)
             cache.prompts([len(p) for p in prompts], [i * beams for i in range(items)])

@@ -31,3 +31,13 @@ def test_an_end_that_is_no_token_is_a_bad_request():
         assert svc.run({"tokens": [3], "maxNewTokens": 2, "beams": 2, "eos": eos})[0] == 200
     for eos in (99, "none"):                             # sampling has no use for it
         assert svc.run({"tokens": [3], "maxNewTokens": 2, "eos": eos})[0] == 200
+
+
+def test_more_than_one_call_takes_is_refused_before_it_starts(monkeypatch):
+    model = llama()
+    monkeypatch.setattr(type(model), "paged_hidden", lambda *a: pytest.fail("the model ran"))
+    with pytest.raises(ValueError, match="generate_beams: 129 prompts of 32 beams .* 4128 rows .* 4096 rows"):
+        model.generate_beams([[1]] * 129, 4, 32)
+    model.config.max_ctx = 1 << 16                      # (128 rows of 2^12 pages, and those of the prompts)
+    with pytest.raises(ValueError, match="524288 pages"):
+        model.generate_beams([[1]] * 4, 1 << 16, 32)
