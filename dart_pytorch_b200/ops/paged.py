@@ -278,13 +278,13 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
             (kt >= hd and kh >= (page - 1) * kt + hd or kh >= hd and kt >= (hkv - 1) * kh + hd) and
             (vt >= hd and vh >= (page - 1) * vt + hd or vh >= hd and vt >= (hkv - 1) * vh + hd) and
             kp >= (hkv - 1) * kh + (page - 1) * kt + hd and vp >= (hkv - 1) * vh + (page - 1) * vt + hd and
-            k_pages.data_ptr() != v_pages.data_ptr() and
             heads > 0 and features == (heads + 2 * hkv) * hd and 0 <= rotary <= hd and rotary % 2 == 0 and rope_base > 0 and
             x_one == 1 and k_one == 1 and v_one == 1 and (t_one == 1 or width <= 1) and
             k_pages.get_device() == dev and v_pages.get_device() == dev and table.get_device() == dev and
             positions.get_device() == dev and _current_device() == dev and
             (table_rows == tokens if rows is None else rows.dtype is _I32 and rows.shape == (tokens,) and
              rows.get_device() == dev and (tokens <= 1 or rows.stride(0) == 1)) and flash._raw_call() and
+            k_pages.data_ptr() != v_pages.data_ptr() and            # (that transforms' wrappers do not have)
             not (torch.is_grad_enabled() and (qkv.requires_grad or k_pages.requires_grad or v_pages.requires_grad))):
         _check_append(qkv, k_pages, v_pages, table, positions, heads, rows, rotary, rope_base)
         if x_one != 1:
