@@ -160,24 +160,17 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     among them).  Query heads share key heads in groups of ``heads // kv_heads``; a row of no tokens gives zeros.  bf16 or fp32, one type for all; sums in
     fp32.  ``scale`` is ``head_dim ** -0.5`` unless given.  Returns ``[rows, heads, head_dim]``: ``out``, if given, which may lie over the
     queries or any other argument."""
-    dev, q_shape, k_shape, t_shape, dtype = q.get_device(), q.shape, k_pages.shape, table.shape, q.dtype
-    if dev < 0 or len(q_shape) != 3 or len(k_shape) != 4 or len(t_shape) != 2 or v_pages.shape != k_shape:
-        return _attention_on_cpu(q, k_pages, v_pages, table, lens, scale, out)
-    (rows, heads, hd), (pages, hkv, page, k_hd), (t_rows, width) = q_shape, k_shape, t_shape
-    (q_row, q_head, q_one), (kp, kh, kt, k_one), (vp, vh, vt, v_one), (t_row, t_one) = (
-        q.stride(), k_pages.stride(), v_pages.stride(), table.stride())
-    if not (                 # all that the checks ask for, in less time
-            out is None and (dtype is _BF16 or dtype is _F32) and k_pages.dtype is dtype and v_pages.dtype is dtype and
-            table.dtype is _I32 and lens.dtype is _I32 and k_hd == hd and t_rows == rows and lens.shape == (rows,) and
-            0 < hd <= MAX_HEAD_DIM and 0 < hkv and heads % hkv == 0 and 0 < page and pages <= MAX_PAGES and rows <= MAX_ROWS and
-            q_one == 1 and k_one == 1 and v_one == 1 and (t_one == 1 or width <= 1) and (rows <= 1 or lens.stride(0) == 1) and
-            k_pages.get_device() == dev and v_pages.get_device() == dev and table.get_device() == dev and
-            lens.get_device() == dev and _current_device() == dev and flash._raw_call() and
-            not (torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad))):
+    dev = q.get_device()
+    sizes = None if dev < 0 or out is not None else _attention_sizes(q, k_pages, v_pages, table, lens, dev)
+    if sizes is None:
         _check_attention(q, k_pages, v_pages, table, lens, out)
-        if q_one != 1 and hd > 1:
+        if dev < 0:
+            o = paged_attention_reference(q, k_pages, v_pages, table, lens, scale)
+            return o if out is None else out.copy_(o)
+        if q.stride(2) != 1 and q.shape[2] > 1:
             q = q.contiguous()
-            q_row, q_head, _ = q.stride()
+        sizes = q.shape, k_pages.shape, table.shape[1], q.stride(), k_pages.stride(), v_pages.stride(), table.stride(0), q.dtype
+    (rows, heads, hd), (pages, hkv, page, _), width, (q_row, q_head, _), (kp, kh, kt, _), (vp, vh, vt, _), t_row, dtype = sizes
     given = out
     if given is not None and (any(_meets(out, t) for t in (k_pages, v_pages, table, lens)) or _meets(out, q) and not (
             out.data_ptr() == q.data_ptr() and out.stride() == q.stride())):     # (a query itself is read before its result is written)
@@ -204,6 +197,24 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     return out
 
 
+def _attention_sizes(q, k_pages, v_pages, table, lens, dev):
+    """Shapes and strides of a call without ``out`` that has all that ``_check_attention`` asks for, which takes longer; else None."""
+    q_shape, k_shape, t_shape, dtype = q.shape, k_pages.shape, table.shape, q.dtype
+    if len(q_shape) != 3 or len(k_shape) != 4 or len(t_shape) != 2 or v_pages.shape != k_shape:
+        return None
+    (rows, heads, hd), (pages, hkv, page, k_hd), (t_rows, width) = q_shape, k_shape, t_shape
+    q_by, k_by, v_by, (t_row, t_one) = q.stride(), k_pages.stride(), v_pages.stride(), table.stride()
+    if ((dtype is _BF16 or dtype is _F32) and k_pages.dtype is dtype and v_pages.dtype is dtype and
+            table.dtype is _I32 and lens.dtype is _I32 and k_hd == hd and t_rows == rows and lens.shape == (rows,) and
+            0 < hd <= MAX_HEAD_DIM and 0 < hkv and heads % hkv == 0 and 0 < page and pages <= MAX_PAGES and rows <= MAX_ROWS and
+            q_by[2] == 1 and k_by[3] == 1 and v_by[3] == 1 and (t_one == 1 or width <= 1) and (rows <= 1 or lens.stride(0) == 1) and
+            k_pages.get_device() == dev and v_pages.get_device() == dev and table.get_device() == dev and
+            lens.get_device() == dev and _current_device() == dev and flash._raw_call() and
+            not (torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad))):
+        return q_shape, k_shape, width, q_by, k_by, v_by, t_row, dtype
+    return None
+
+
 def _check_attention(q, k_pages, v_pages, table, lens, out) -> None:
     what = "paged_attention"
     _pages(what, k_pages, v_pages)
@@ -221,12 +232,6 @@ def _check_attention(q, k_pages, v_pages, table, lens, out) -> None:
         raise ValueError(f"{what}: out must be {list(q.shape)} {q.dtype} with contiguous features")
     if out is not None and _overlaps_itself(out):
         raise ValueError(f"{what}: places of out {list(out.shape)} with strides {list(out.stride())} overlap")
-
-
-def _attention_on_cpu(q, k_pages, v_pages, table, lens, scale, out):
-    _check_attention(q, k_pages, v_pages, table, lens, out)
-    o = paged_attention_reference(q, k_pages, v_pages, table, lens, scale)
-    return o if out is None else out.copy_(o)
 
 
 # ------------------------------------------------------------------------------------------------------------ append
@@ -262,34 +267,17 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     and writes nothing.  Queries and keys are turned by the half-split rotary embedding over ``rotary_dim`` features (all of
     them unless given; 0: not at all).  Returns the turned queries ``[tokens, heads, head_dim]``, and with ``keys`` the turned keys
     too; ``qkv``, which shares no memory with the pages, stays as it is.  No two tokens may have one place."""
-    dev, x_shape, k_shape, t_shape, dtype = qkv.get_device(), qkv.shape, k_pages.shape, table.shape, qkv.dtype
-    rotary = k_shape[-1] if rotary_dim is None else rotary_dim
-    if dev < 0 or len(x_shape) != 2 or len(k_shape) != 4 or len(t_shape) != 2 or v_pages.shape != k_shape:
+    dev, rotary = qkv.get_device(), k_pages.shape[-1] if rotary_dim is None else rotary_dim
+    sizes = None if dev < 0 else _append_sizes(qkv, k_pages, v_pages, table, positions, heads, rows, rotary, rope_base, dev)
+    if sizes is None:
         _check_append(qkv, k_pages, v_pages, table, positions, heads, rows, rotary, rope_base)
-        q, k = paged_append_reference(qkv, k_pages, v_pages, table, positions, heads, rows, rotary, rope_base)
-        return (q, k) if keys else q
-    (tokens, features), (pages, hkv, page, hd), (table_rows, width) = x_shape, k_shape, t_shape
-    (x_row, x_one), (kp, kh, kt, k_one), (vp, vh, vt, v_one), (t_row, t_one) = (
-        qkv.stride(), k_pages.stride(), v_pages.stride(), table.stride())
-    if not (                 # all that the checks ask for, in less time
-            (dtype is _BF16 or dtype is _F32) and k_pages.dtype is dtype and v_pages.dtype is dtype and table.dtype is _I32 and
-            positions.dtype is _I32 and positions.shape == (tokens,) and (tokens <= 1 or positions.stride(0) == 1) and
-            0 < hd <= MAX_HEAD_DIM and 0 < hkv and 0 < page and pages <= MAX_PAGES and table_rows <= MAX_ROWS and
-            (kt >= hd and kh >= (page - 1) * kt + hd or kh >= hd and kt >= (hkv - 1) * kh + hd) and
-            (vt >= hd and vh >= (page - 1) * vt + hd or vh >= hd and vt >= (hkv - 1) * vh + hd) and
-            kp >= (hkv - 1) * kh + (page - 1) * kt + hd and vp >= (hkv - 1) * vh + (page - 1) * vt + hd and
-            heads > 0 and features == (heads + 2 * hkv) * hd and 0 <= rotary <= hd and rotary % 2 == 0 and rope_base > 0 and
-            x_one == 1 and k_one == 1 and v_one == 1 and (t_one == 1 or width <= 1) and
-            k_pages.get_device() == dev and v_pages.get_device() == dev and table.get_device() == dev and
-            positions.get_device() == dev and _current_device() == dev and
-            (table_rows == tokens if rows is None else rows.dtype is _I32 and rows.shape == (tokens,) and
-             rows.get_device() == dev and (tokens <= 1 or rows.stride(0) == 1)) and flash._raw_call() and
-            k_pages.data_ptr() != v_pages.data_ptr() and            # (that transforms' wrappers do not have)
-            not (torch.is_grad_enabled() and (qkv.requires_grad or k_pages.requires_grad or v_pages.requires_grad))):
-        _check_append(qkv, k_pages, v_pages, table, positions, heads, rows, rotary, rope_base)
-        if x_one != 1:
+        if dev < 0:
+            q, k = paged_append_reference(qkv, k_pages, v_pages, table, positions, heads, rows, rotary, rope_base)
+            return (q, k) if keys else q
+        if qkv.stride(1) != 1:
             qkv = qkv.contiguous()
-            x_row = features
+        sizes = qkv.shape[0], k_pages.shape, table.shape, qkv.stride(0), k_pages.stride(), v_pages.stride(), table.stride(0), qkv.dtype
+    tokens, (pages, hkv, page, hd), (table_rows, width), x_row, (kp, kh, kt, _), (vp, vh, vt, _), t_row, dtype = sizes
     q = qkv.new_empty((tokens, heads, hd))
     k = qkv.new_empty((tokens, hkv, hd)) if keys else None
     N.check(_lib().dptb_paged_append(_APPEND_ARGS.pack(
@@ -298,6 +286,32 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         tokens, heads, hkv, hd, rotary, page, width, pages, table_rows, dtype is _F32, rope_base), _raw_stream(dev)), "paged_append")
     _increment_version((k_pages, v_pages))
     return (q, k) if keys else q
+
+
+def _append_sizes(qkv, k_pages, v_pages, table, positions, heads, rows, rotary, rope_base, dev):
+    """Shapes and strides of a call that has all that ``_check_append`` asks for, which takes longer, and pages in one of the usual orders;
+    else None."""
+    x_shape, k_shape, t_shape, dtype = qkv.shape, k_pages.shape, table.shape, qkv.dtype
+    if len(x_shape) != 2 or len(k_shape) != 4 or len(t_shape) != 2 or v_pages.shape != k_shape:
+        return None
+    (tokens, features), (pages, hkv, page, hd), (table_rows, width) = x_shape, k_shape, t_shape
+    (x_row, x_one), k_by, v_by, (t_row, t_one) = qkv.stride(), k_pages.stride(), v_pages.stride(), table.stride()
+    kp, kh, kt, k_one = k_by
+    if ((dtype is _BF16 or dtype is _F32) and k_pages.dtype is dtype and v_pages.dtype is dtype and table.dtype is _I32 and
+            positions.dtype is _I32 and positions.shape == (tokens,) and (tokens <= 1 or positions.stride(0) == 1) and
+            0 < hd <= MAX_HEAD_DIM and 0 < hkv and 0 < page and pages <= MAX_PAGES and table_rows <= MAX_ROWS and
+            (kt >= hd and kh >= (page - 1) * kt + hd or kh >= hd and kt >= (hkv - 1) * kh + hd) and
+            kp >= (hkv - 1) * kh + (page - 1) * kt + hd and v_by == k_by and
+            heads > 0 and features == (heads + 2 * hkv) * hd and 0 <= rotary <= hd and rotary % 2 == 0 and rope_base > 0 and
+            x_one == 1 and k_one == 1 and (t_one == 1 or width <= 1) and
+            k_pages.get_device() == dev and v_pages.get_device() == dev and table.get_device() == dev and
+            positions.get_device() == dev and _current_device() == dev and
+            (table_rows == tokens if rows is None else rows.dtype is _I32 and rows.shape == (tokens,) and
+             rows.get_device() == dev and (tokens <= 1 or rows.stride(0) == 1)) and flash._raw_call() and
+            k_pages.data_ptr() != v_pages.data_ptr() and            # (that transforms' wrappers do not have)
+            not (torch.is_grad_enabled() and (qkv.requires_grad or k_pages.requires_grad or v_pages.requires_grad))):
+        return tokens, k_shape, t_shape, x_row, k_by, v_by, t_row, dtype
+    return None
 
 
 def _check_append(qkv, k_pages, v_pages, table, positions, heads, rows, rotary, rope_base) -> None:
@@ -436,12 +450,8 @@ def compact_pages(table: torch.Tensor, pages: int) -> Tuple[torch.Tensor, torch.
     numbers below.  Returns ``(table, src, dst, live)``: the table in the new numbers, the moves (``[pages // 2]``, -1 behind
     the last) for ``copy_pages``, and ``n`` as an int32 ``[1]``."""
     dev = table.get_device()
-    if dev < 0 or not (table.dim() == 2 and table.dtype is _I32 and table.shape[0] <= MAX_ROWS and 0 <= pages <= MAX_PAGES and
-                       (table.stride(1) == 1 or table.shape[1] <= 1) and _current_device() == dev):
-        _table("compact_pages", table)
-        if not 0 <= pages <= MAX_PAGES:
-            raise ValueError(f"compact_pages: a pool of {pages} pages (at most {MAX_PAGES})")
-        _here("compact_pages", table)
+    if dev < 0 or _compact_is_off(table, pages, dev):
+        _check_compact(table, pages)
         if dev < 0:
             return compact_pages_reference(table, pages)
     rows, width = table.shape
@@ -455,15 +465,23 @@ def compact_pages(table: torch.Tensor, pages: int) -> Tuple[torch.Tensor, torch.
     return new, src, dst, live
 
 
+def _compact_is_off(table, pages, dev) -> bool:
+    return not (table.dim() == 2 and table.dtype is _I32 and table.shape[0] <= MAX_ROWS and 0 <= pages <= MAX_PAGES and
+                (table.stride(1) == 1 or table.shape[1] <= 1) and _current_device() == dev)
+
+
+def _check_compact(table, pages) -> None:
+    _table("compact_pages", table)
+    if not 0 <= pages <= MAX_PAGES:
+        raise ValueError(f"compact_pages: a pool of {pages} pages (at most {MAX_PAGES})")
+    _here("compact_pages", table)
+
+
 def copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None:
     """In place: page ``dst[i]`` of ``pool [..., pages, kv_heads, page, head_dim]`` (contiguous; every layer's keys and values at
     once) becomes a copy of page ``src[i]``; pairs with a -1 are passed over.  A page that is copied to must be in no other pair."""
     dev, shape = pool.get_device(), pool.shape
-    if dev < 0 or not (
-            len(shape) >= 4 and pool.is_contiguous() and (pool.dtype is _BF16 or pool.dtype is _F32) and src.dim() == 1 and
-            src.dtype is _I32 and dst.dtype is _I32 and src.shape == dst.shape and src.get_device() == dev and
-            dst.get_device() == dev and (src.shape[0] <= 1 or src.stride(0) == 1 and dst.stride(0) == 1) and
-            _current_device() == dev and flash._raw_call() and not (pool.requires_grad and torch.is_grad_enabled())):
+    if dev < 0 or _copy_is_off(pool, src, dst, dev):
         _check_copy(pool, src, dst)
     pages = shape[-4]
     outer = math.prod(shape[:-4])
@@ -481,6 +499,14 @@ def copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None
         pool.data_ptr(), src.data_ptr(), dst.data_ptr(), outer, shape[-3] * shape[-2] * shape[-1] * pool.element_size(),
         src.shape[0], pages), _raw_stream(dev)), "copy_pages")
     _increment_version((pool,))
+
+
+def _copy_is_off(pool, src, dst, dev) -> bool:
+    return not (
+        pool.dim() >= 4 and pool.is_contiguous() and (pool.dtype is _BF16 or pool.dtype is _F32) and src.dim() == 1 and
+        src.dtype is _I32 and dst.dtype is _I32 and src.shape == dst.shape and src.get_device() == dev and
+        dst.get_device() == dev and (src.shape[0] <= 1 or src.stride(0) == 1 and dst.stride(0) == 1) and
+        _current_device() == dev and flash._raw_call() and not (pool.requires_grad and torch.is_grad_enabled()))
 
 
 def _check_copy(pool, src, dst) -> None:
