@@ -27,6 +27,8 @@ class PagedLayer:
         extended by, and attends: a token of every row over the row's pages, or the tokens of prompts over one another (causal).
         Returns ``[batch * n, heads * hd]``."""
         c = self.cache
+        if c.positions is None:
+            raise ValueError("PagedCache: nothing to attend with: prompts and fork extend the cache")
         if c.rows is None and (n != 1 or batch != c.table.shape[0]) or c.rows is not None and batch * n != c.positions.numel():
             raise ValueError(f"PagedCache: {batch} x {n} tokens, the cache was extended by {c.positions.numel()}")
         kw = dict(rows=c.rows, rotary_dim=0 if rope is None else rope.rotary_dim, rope_base=1.0 if rope is None else rope.base)

@@ -89,3 +89,16 @@ def test_rotary_attention_over_pages_keeps_to_its_window():
         c.fork()
         with pytest.raises(ValueError, match="RopeCache: sequence of 9 tokens"):
             m(torch.randn(1, 1, 32), cache=c.layers[0])
+
+
+def test_a_step_that_nothing_was_extended_for_is_refused():
+    c = PagedCache(1, 1, 8, 2, 8, 4)
+    step = lambda: c.layers[0].attend(torch.zeros(2, 24), 2, 1, 1)  # noqa: E731
+    with pytest.raises(ValueError, match="extend"):
+        step()
+    c.prompts([3, 2], [0, 1])
+    c.fork()
+    step()
+    c.free([1])
+    with pytest.raises(ValueError, match="extend"):
+        step()
