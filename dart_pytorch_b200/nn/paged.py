@@ -122,7 +122,10 @@ class PagedCache:
 
     def free(self, rows: Sequence[int]) -> None:
         """Ends ``rows``; pages that nobody else lists are free again."""
-        keep = [-1 if r in set(rows) else r for r in range(self.table.shape[0])]
+        count, ended = self.table.shape[0], set(rows)
+        if not all(0 <= r < count for r in ended):
+            raise ValueError(f"PagedCache: rows {list(rows)} of {count} to end")
+        keep = [-1 if r in ended else r for r in range(count)]
         self._fork(torch.tensor(keep, dtype=torch.int32, device=self.table.device), 0, self.longest)
         self.rows = self.positions = None
 

@@ -102,3 +102,14 @@ def test_a_step_that_nothing_was_extended_for_is_refused():
     c.free([1])
     with pytest.raises(ValueError, match="extend"):
         step()
+
+
+def test_rows_that_are_not_there_do_not_end():
+    c = PagedCache(1, 1, 8, 2, 8, 4)
+    c.prompts([3, 2], [0, 1])
+    for rows in ([2], [-1], [0, 5]):
+        with pytest.raises(ValueError, match="rows"):
+            c.free(rows)
+    assert c.lens.tolist() == [3, 2]
+    c.free([1, 1])
+    assert c.lens.tolist() == [3, 0]
