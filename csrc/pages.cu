@@ -587,7 +587,7 @@ extern "C" int dptb_copy_pages(const CopyArgs* args, void* stream) {
   const CopyArgs& a = *args;
   if (a.n == 0 || a.outer == 0 || a.bytes == 0) return 0;
   if (a.n < 0 || a.outer < 0 || a.outer > 65535 || a.pages < 0 || a.bytes < 0 || a.bytes > 0x7fffffff) return kErrBadShape;
-  const dim3 grid(a.n < 8 * 148 ? a.n : 8 * 148, (unsigned)a.outer);
+  const dim3 grid(min(a.n, 8 * sm_count()), (unsigned)a.outer);
   auto st = static_cast<cudaStream_t>(stream);
   auto* p = static_cast<unsigned char*>(a.pool);
   if (((reinterpret_cast<uintptr_t>(p) | (uintptr_t)a.bytes) & 15) == 0)
