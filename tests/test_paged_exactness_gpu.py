@@ -67,3 +67,24 @@ def test_sine_and_cosine_are_rounded_once(rotary, hd, base):
                          rope_base=base).double().cpu()
     for got, want in ((q[:, 0, :half], cos), (q[:, 0, half:rotary], sin), (q[:, 1, :half], -sin), (q[:, 1, half:rotary], cos)):
         assert bool(((got - want).abs() <= want.abs() * 2.0 ** -24 + p * 2.0 ** -50).all())
+
+
+@pytest.mark.parametrize("start", [0, 4000, 131000])
+@pytest.mark.parametrize("rotary,hd,base", [(64, 64, 10000.0), (128, 128, 500000.0)])
+def test_both_rotary_embeddings_agree_as_far_as_32_bits_of_an_angle_reach(start, rotary, hd, base):
+    """A contiguous cache's tokens are turned by ``ops.rope``, whose frequencies and angles are of 32 bits: the exponent of the base, at most 13.2 in
+    natural logarithms, and powf (4 steps), and their product leave an angle 13.2 + 8 + 1 half steps off, 23 * 2^-24 of itself; sines, products
+    and sums add a few."""
+    n, heads, hkv, page = 72, 2, 1, 16
+    qkv = torch.randn(n, (heads + 2 * hkv) * hd, device="cuda")
+    k, v = (torch.zeros(1, hkv, page, hd, device="cuda") for _ in range(2))
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    table = torch.zeros(1, (start + n) // page + 1, dtype=torch.int32, device="cuda")
+    positions = [start + i if i < page else -1 for i in range(n)]            # (a page of them has a place)
+    q, keys = ops.paged_append(qkv, k, v, table, ints(positions), heads, rows=ints([0] * n), rotary_dim=rotary, rope_base=base, keys=True)
+    want = ops.rope(qkv[:page, :(heads + hkv) * hd].contiguous(), start, base, rotary, heads=heads + hkv).view(page, -1, hd)
+    half = rotary // 2
+    angle = (start + torch.arange(page, device="cuda").double())[:, None] * base ** (-2.0 * torch.arange(half, device="cuda").double() / rotary)
+    x = qkv[:page, :(heads + hkv) * hd].view(page, -1, 2, half).double().abs().sum(2)
+    bound = (x * (23 * angle + 8)[:, None] * 2.0 ** -24).repeat(1, 1, 2)
+    assert bool(((torch.cat([q, keys], 1)[:page].double() - want.double()).abs() <= bound).all())
