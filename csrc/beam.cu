@@ -12,8 +12,8 @@
 // and the lanes' maxima tell where to look: the best W continuations lie with the lanes of the W largest (each counted with its beam's score),
 // and only these lanes' logits are read once more, by the value of the W-th.  That is a few hundred logits, whatever the vocabulary.
 //
-// Bound by memory for many rows, by a chain of latencies for few.  256 rows of 128256 logits in bf16, 8 beams an item, take 22 us, of which the pass is half
-// (66 MB in 9 to 11 us) and the choice in each item's last CTA the other; four rows of 50257 in fp32 9.2 us, 35 of 321 7.2.  Choosing in every warp, or in CTAs barrier
+// Bound by memory for many rows, by a chain of latencies for few.  256 rows of 128256 logits in bf16, 8 beams an item, take 22.7 us, of which the pass is half
+// (66 MB in 9 to 11 us) and the choice in each item's last CTA the other; four rows of 50257 in fp32 9.3 us, 35 of 321 7.3.  Choosing in every warp, or in CTAs barrier
 // after barrier, cost more than the pass itself: 45 and 61 us for the 256 rows.
 #include <cuda_bf16.h>
 
@@ -351,7 +351,7 @@ __device__ __noinline__ void best_of_row(const BeamArgs& a, const T* row, const 
 }
 
 // Where too many are equal, or fewer lanes than beams have anything to offer (a masked vocabulary): the best of every row first.  (64 items of 32 beams over
-// 32000 logits that are all the same: 147 us, 50 for random ones; with all K K ranked against one another it was 360.)
+// 32000 logits that are all the same: 147 us in bf16 and 157 in fp32, 52 and 64 for random ones; with all K K ranked against one another it was 360.)
 template <typename T>
 __device__ __noinline__ void best_of_rows(const BeamArgs& a, BeamShared& sh, const T* rows, const BeamPart* parts) {
   const int tid = threadIdx.x, warp = tid >> 5, K = a.beams;
@@ -617,7 +617,9 @@ beam_kernel(const __grid_constant__ BeamArgs a) {
     const int begin = list * a.chunk, end = min(a.vocab, begin + a.chunk);
     // Sums of 2^(x log2(e) - shift): `shift` is a whole number, so that sums are brought to another one exactly, and stands for shift / log2(e),
     // divided out in 64 bits, so that the rounding of log2(e) moves no sum against another.  What is left is the error of an exponential, 2^-22, and of
-    // sums of 32.  Maxima that are too large for it (masks of the type's lowest value among them) go by differences, from themselves.
+    // sums of 32 in 32 bits: 1e-7 of a logarithm, where a total of -20 is rounded to 1e-6.  (Exponentials in 64 bits, some 30 multiply-adds each, would
+    // bound the pass by far: 33 million logits in 50 us at 18e12 of them a second, where memory takes 10.)  Maxima that are too large for it (masks of the
+    // type's lowest value among them) go by differences, from themselves.
     float m = -INFINITY, shift = 0.0f;
     double s = 0.0;
     for (int i = begin; i < end; i += U * 32 * N) {
