@@ -21,16 +21,19 @@
 // have the same rounds filled element by element, by the warp that works on them.
 //
 // bf16: S^T = K Q^T and O^T = V^T P^T by mma.sync, the group's heads as the 8 columns (two tiles of them for 9 to 16 heads); the bound is
-// the cache stream, and a tcgen05 tile of 128 rows would be padding for the most part.  The weights enter as three bf16 parts, all 24 bits of them:
-// with two, 16 bits, one output in 450 of 32 sequences of 1 to 4096 keys was a step off its rounding, so one in 1100
-// (53.8 us and 53.9).  What they add up to runs on in fp32, rounded to nearest: of those outputs one in 3400 is off then, and of four sequences of 65000 to
-// 131072 keys one in 3300 instead of one in 200 (heads of 256, 16 sequences of 2048 keys: 33.4 us instead of 32.1; the others within 2 %).
+// the cache stream, and a tcgen05 tile of 128 rows would be padding for the most part.  The weights enter as three bf16 parts, all 24 bits of
+// them, and what a round's products add up to goes into the running values in fp32, rounded to nearest.  With two parts and values that ran on in the
+// instructions' own accumulators, which truncate, one output in 450 of 32 sequences of 1 to 4096 keys and one in 240 of four of 65000 to 131072 was a step
+// off its rounding; one in 3000 and 4000 is.  What that costs: nothing on the 32 sequences; 16 sequences of 4096 keys, 8 heads of 64, take 31.1 us
+// instead of 30.2, 16 of 2048, 8 heads of 256 on 4, 33.4 instead of 31.7; the four take 247 us instead of 244, and for seconds on end, at the power limit,
+// 270 instead of 256.
 // fp32: multiply-adds, 8 lanes a key; they bound groups of four heads and more.
 //
-// Device time on B200, pages of 16 tokens in random order: bf16, 32 heads of 128 on 8: four sequences of 65000 to 131072 keys 242 us (6.6 TB/s, the
-// rate of a plain copy), 32 sequences of 1 to 4096 53.5 us (5.0 TB/s; its floor is 41), 32 of 2048 52 us, one of 2048 15 us.  One sequence
-// of 65 keys, 12 heads of 64: 6.5 us.  fp32, 13 sequences of up to 1531 keys, 10 heads of 80 on 5: 17.2 us; 32 of 2048, 32 heads of 128 on 8:
-// 105 us.  Filled element by element the 32 sequences of 2048 keys take 180 us in bf16 and 186 us in fp32, the one of 65 keys 9 us.
+// Device time on B200, pages of 16 tokens in random order, middle values of several runs on several GPUs: bf16, 32 heads of 128 on 8: four sequences of
+// 65000 to 131072 keys 247 us (243 to 253; 6.5 TB/s, the rate of a plain copy), 32 sequences of 1 to 4096 53.8 us (5.0 TB/s; its floor is 41), 32 of 2048
+// 52 us, one of 2048 15 us.  One sequence of 65 keys, 12 heads of 64: 6.8 us.  fp32, 13 sequences of up to 1531 keys, 10 heads of 80 on 5: 18.5 us; 32 of
+// 2048, 32 heads of 128 on 8: 104 us.  Filled element by element the 32 sequences of 2048 keys take 180 us in bf16 and 185 us in fp32, the one of 65 keys
+// 10.5 us.
 #include <cuda_bf16.h>
 
 #include "common/host.h"
@@ -114,6 +117,7 @@ struct Cursor {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kTiny = 1.2e-38f;
+constexpr float kNoHead = 1.0e30f;      // maximum of a column without a head: its weights are zero, and products of zeros take little power
 constexpr int kMaxHeadDim = 256;
 constexpr int kAlone = 2, kSnap = 3;      // rounds of a warp that may be had for no joins across CTAs
 
@@ -146,7 +150,7 @@ struct Bf16Round {
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        m[n][e] = -INFINITY;
+        m[n][e] = n * 8 + (lane & 3) * 2 + e < count ? -INFINITY : kNoHead;
         l[n][e] = 0.0f;
       }
 #pragma unroll
@@ -210,16 +214,17 @@ struct Bf16Round {
 #pragma unroll
       for (int r = 0; r < 2 * M; ++r) {
         float rest[2] = {p[r][0], p[r][1]};
+        const float tiny[2] = {fminf(p[r][0], kTiny), fminf(p[r][1], kTiny)};
 #pragma unroll
         for (int part = 0; part < 3; ++part) {
           const uint32_t u0 = __float_as_uint(rest[0]), u1 = __float_as_uint(rest[1]);
           pp[n][r >> 1][part][r & 1] = movmatrix_trans((u0 >> 16) | (u1 & 0xffff0000u));
-          rest[0] = p[r][0] > 0.0f ? fmaxf(rest[0] - __uint_as_float(u0 & 0xffff0000u), kTiny) : 0.0f;
-          rest[1] = p[r][1] > 0.0f ? fmaxf(rest[1] - __uint_as_float(u1 & 0xffff0000u), kTiny) : 0.0f;
+          rest[0] = fmaxf(rest[0] - __uint_as_float(u0 & 0xffff0000u), tiny[0]);
+          rest[1] = fmaxf(rest[1] - __uint_as_float(u1 & 0xffff0000u), tiny[1]);
         }
       }
     }
-    // A round's products are summed on their own, the smallest parts first, and added to the running values by multiply-adds: the matrix instructions cut
+    // A round's products are summed on their own and added to the running values by multiply-adds: the matrix instructions cut
     // off what does not fit their sums, so values that ran on in them would shrink by up to 2^-24 a step (8e-6 of them after 512 rounds).
 #pragma unroll
     for (int b = 0; b < HD / 64; ++b) {
@@ -241,7 +246,7 @@ struct Bf16Round {
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int part = 2; part >= 0; --part) mma_bf16_16816(sum[n], f, pp[n][c][part][0], pp[n][c][part][1]);
+            for (int part = 0; part < 3; ++part) mma_bf16_16816(sum[n], f, pp[n][c][part][0], pp[n][c][part][1]);
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n)
